@@ -391,6 +391,118 @@ B200TBE_API int b200tbe_jagged_dense_elementwise_add(const b200tbe_jagged_shape*
                                                      const void* x_values, const void* y,
                                                      void* out, b200tbe_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Attention over jagged sequences (torch.ops.fbgemm.b200tbe_jagged_attention and its gradients). No
+ * counterpart in fbgemm_gpu's schema or in the reference.
+ *
+ * q is [total_q, heads, head_dim], k and v are [total_k, kv_heads, head_dim], each with its own row
+ * and head strides (in elements; the elements of a head lie side by side). Sequence b's queries are
+ * the rows q_offsets[b] .. q_offsets[b+1], its keys the rows k_offsets[b] .. k_offsets[b+1]; query
+ * head h reads key head h / (heads / kv_heads).
+ *     out[i] = sum_j softmax_j(scale q_i . k_j) v_j
+ * over the sequence's keys, with causal over those with j <= i + klen - qlen (i, j counted inside the
+ * sequence: the last query sees every key). A query that sees no key, and a row that belongs to no
+ * sequence, gets zeros. Sequences never see one another's rows, whatever these hold; inside a sequence
+ * keys and values have to be finite, also behind the causal mask.
+ * Offsets outside the arrays are cut to them; offsets that decrease leave results unspecified.
+ * lse, [heads][total_q] or NULL, receives the natural logarithm of each row's sum of exponentials
+ * (-infinity where no key is seen): the backward pass needs it.
+ * fp32, fp16 and bf16, head_dim 1 to 256. Sums and softmax statistics are fp32.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  float* lse;
+  const void* q_offsets;            /* [batch + 1] int64 or int32 */
+  const void* k_offsets;            /* [batch + 1] same type */
+  int64_t q_stride, q_head_stride;
+  int64_t k_stride, k_head_stride;
+  int64_t v_stride, v_head_stride;
+  int64_t out_stride, out_head_stride;
+  int64_t total_q, total_k;
+  int32_t batch;
+  int32_t heads;                    /* a multiple of kv_heads */
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;                    /* B200TBE_FP32, B200TBE_FP16 or B200TBE_BF16, for all arrays */
+  int32_t offset_bytes;             /* 8 or 4 */
+  int32_t causal;
+  float scale;
+} b200tbe_attention_params;
+
+B200TBE_API int b200tbe_jagged_attention(const b200tbe_attention_params* p, b200tbe_stream_t stream);
+
+/* The gradients of sum(out * grad_out). forward is the forward call's block: out and lse as it left
+ * them. grad_q, grad_k and grad_v receive every row (zeros where nothing reaches); a shared key head's
+ * gradient is the sum over its query heads. Results do not depend on scheduling. scratch: 16-byte
+ * aligned, b200tbe_jagged_attention_backward_scratch_bytes() long. */
+typedef struct {
+  b200tbe_attention_params forward;
+  const void* grad_out;
+  void* grad_q;
+  void* grad_k;
+  void* grad_v;
+  int64_t grad_out_stride, grad_out_head_stride;
+  int64_t grad_q_stride, grad_q_head_stride;
+  int64_t grad_k_stride, grad_k_head_stride;
+  int64_t grad_v_stride, grad_v_head_stride;
+  void* scratch;
+  size_t scratch_bytes;
+} b200tbe_attention_backward_params;
+
+B200TBE_API size_t b200tbe_jagged_attention_backward_scratch_bytes(int64_t total_q, int32_t heads);
+B200TBE_API int b200tbe_jagged_attention_backward(const b200tbe_attention_backward_params* p,
+                                                  b200tbe_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * A paged key-value cache (torch.ops.fbgemm.b200tbe_paged_cache_append and b200tbe_paged_attention).
+ * k_cache and v_cache are [num_pages, page_size, kv_heads, head_dim] with strides in elements (the
+ * elements of a head lie side by side). Position t of sequence b lies in page page_table[b][t /
+ * page_size], at place t % page_size. lengths[b] is how many positions the sequence has.
+ * Positions whose page is not in [0, num_pages), or that lie past the table's max_pages pages, take no
+ * part and set B200TBE_DEV_INDEX_OUT_OF_RANGE in the optional status word.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct {
+  void* k_cache;
+  void* v_cache;
+  const int32_t* page_table;        /* [batch][max_pages], rows page_table_stride apart */
+  const void* lengths;              /* [batch] int64 or int32 */
+  int64_t k_page_stride, k_slot_stride, k_head_stride;
+  int64_t v_page_stride, v_slot_stride, v_head_stride;
+  int64_t page_table_stride;
+  int64_t num_pages;
+  int32_t max_pages;
+  int32_t page_size;
+  int32_t batch;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;                    /* B200TBE_FP32, B200TBE_FP16 or B200TBE_BF16 */
+  int32_t length_bytes;             /* 8 or 4 */
+  int32_t* status;                  /* device word or NULL */
+} b200tbe_paged_cache;
+
+/* Writes the jagged rows k, v [total, kv_heads, head_dim] into the cache: the rows offsets[b] ..
+ * offsets[b+1] become the LAST positions of sequence b, whose lengths[b] counts them already. Rows that
+ * belong to no sequence are not written; a row before position 0 sets the status bit. Elements are
+ * moved as they are. */
+B200TBE_API int b200tbe_paged_cache_append(const b200tbe_paged_cache* cache, const void* k, const void* v,
+                                           int64_t k_stride, int64_t k_head_stride, int64_t v_stride,
+                                           int64_t v_head_stride, const void* offsets, int32_t offset_bytes,
+                                           int64_t total, b200tbe_stream_t stream);
+
+/* out[b, h] = sum over t < lengths[b] of softmax_t(scale q[b, h] . k[t]) v[t], for one query of each
+ * sequence; q and out are [batch, heads, head_dim] with strides in elements. A sequence without
+ * positions gets zeros. head_dim 1 to 256, any number of query heads for a key head. The cache's length
+ * is split over the GPU and joined in a fixed order: results depend on the data, the lengths, the batch
+ * and the kernel's grid alone. scratch: 16-byte aligned, b200tbe_paged_attention_scratch_bytes() long. */
+B200TBE_API size_t b200tbe_paged_attention_scratch_bytes(int32_t head_dim);
+B200TBE_API int b200tbe_paged_attention(const b200tbe_paged_cache* cache, const void* q, void* out,
+                                        int64_t q_stride, int64_t q_head_stride, int64_t out_stride,
+                                        int64_t out_head_stride, int32_t heads, float scale, void* scratch,
+                                        size_t scratch_bytes, b200tbe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

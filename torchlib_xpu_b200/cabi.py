@@ -85,6 +85,45 @@ class JaggedShape(ctypes.Structure):
     ]
 
 
+class AttentionParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _c_void_p), ("k", _c_void_p), ("v", _c_void_p), ("out", _c_void_p), ("lse", _c_void_p),
+        ("q_offsets", _c_void_p), ("k_offsets", _c_void_p),
+        ("q_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("k_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+        ("v_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+        ("out_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64),
+        ("total_q", ctypes.c_int64), ("total_k", ctypes.c_int64),
+        ("batch", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("offset_bytes", ctypes.c_int32),
+        ("causal", ctypes.c_int32), ("scale", ctypes.c_float),
+    ]
+
+
+class AttentionBackwardParams(ctypes.Structure):
+    _fields_ = [
+        ("forward", AttentionParams), ("grad_out", _c_void_p), ("grad_q", _c_void_p), ("grad_k", _c_void_p),
+        ("grad_v", _c_void_p),
+        ("grad_out_stride", ctypes.c_int64), ("grad_out_head_stride", ctypes.c_int64),
+        ("grad_q_stride", ctypes.c_int64), ("grad_q_head_stride", ctypes.c_int64),
+        ("grad_k_stride", ctypes.c_int64), ("grad_k_head_stride", ctypes.c_int64),
+        ("grad_v_stride", ctypes.c_int64), ("grad_v_head_stride", ctypes.c_int64),
+        ("scratch", _c_void_p), ("scratch_bytes", ctypes.c_size_t),
+    ]
+
+
+class PagedCache(ctypes.Structure):
+    _fields_ = [
+        ("k_cache", _c_void_p), ("v_cache", _c_void_p), ("page_table", _c_void_p), ("lengths", _c_void_p),
+        ("k_page_stride", ctypes.c_int64), ("k_slot_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+        ("v_page_stride", ctypes.c_int64), ("v_slot_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+        ("page_table_stride", ctypes.c_int64), ("num_pages", ctypes.c_int64), ("max_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32), ("batch", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("length_bytes", ctypes.c_int32),
+        ("status", _c_void_p),
+    ]
+
+
 # Every symbol include/b200tbe.h declares; tests check that the library exports all of them.
 EXPORTS = (
     "b200tbe_status_string", "b200tbe_abi_version", "b200tbe_forward", "b200tbe_nbit_forward",
@@ -95,7 +134,9 @@ EXPORTS = (
     "b200tbe_permute_row_starts_scratch_bytes", "b200tbe_permute_row_starts", "b200tbe_permute_rows",
     "b200tbe_quantized_row_bytes",
     "b200tbe_quantize_rows", "b200tbe_dequantize_rows", "b200tbe_nv12_to_rgb", "b200tbe_jagged_to_padded_dense", "b200tbe_dense_to_jagged",
-    "b200tbe_jagged_dense_elementwise_add",
+    "b200tbe_jagged_dense_elementwise_add", "b200tbe_jagged_attention",
+    "b200tbe_jagged_attention_backward_scratch_bytes", "b200tbe_jagged_attention_backward",
+    "b200tbe_paged_cache_append", "b200tbe_paged_attention_scratch_bytes", "b200tbe_paged_attention",
 )
 
 _lib = None
@@ -157,6 +198,18 @@ def lib() -> ctypes.CDLL:
             ctypes.POINTER(JaggedShape), _c_void_p, _c_void_p, _c_void_p]
         _lib.b200tbe_jagged_dense_elementwise_add.argtypes = [
             ctypes.POINTER(JaggedShape), _c_void_p, _c_void_p, _c_void_p, _c_void_p]
+        i64, i32 = ctypes.c_int64, ctypes.c_int32
+        _lib.b200tbe_jagged_attention.argtypes = [ctypes.POINTER(AttentionParams), _c_void_p]
+        _lib.b200tbe_jagged_attention_backward_scratch_bytes.argtypes = [i64, i32]
+        _lib.b200tbe_jagged_attention_backward_scratch_bytes.restype = ctypes.c_size_t
+        _lib.b200tbe_jagged_attention_backward.argtypes = [ctypes.POINTER(AttentionBackwardParams), _c_void_p]
+        _lib.b200tbe_paged_cache_append.argtypes = [
+            ctypes.POINTER(PagedCache), _c_void_p, _c_void_p, i64, i64, i64, i64, _c_void_p, i32, i64, _c_void_p]
+        _lib.b200tbe_paged_attention_scratch_bytes.argtypes = [i32]
+        _lib.b200tbe_paged_attention_scratch_bytes.restype = ctypes.c_size_t
+        _lib.b200tbe_paged_attention.argtypes = [
+            ctypes.POINTER(PagedCache), _c_void_p, _c_void_p, i64, i64, i64, i64, i32, ctypes.c_float, _c_void_p,
+            ctypes.c_size_t, _c_void_p]
     return _lib
 
 

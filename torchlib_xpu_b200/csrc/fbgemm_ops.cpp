@@ -23,6 +23,7 @@
 
 #include <algorithm>
 #include <array>
+#include <cmath>
 #include <iterator>
 #include <mutex>
 #include <unordered_map>
@@ -414,6 +415,231 @@ Tensor jagged_dense_elementwise_add_autograd(const Tensor& x_values, const std::
 Tensor jagged_2d_to_dense_autograd(const Tensor& values, const Tensor& offsets, int64_t max_sequence_length) {
   return JaggedToPaddedDenseFunction::apply(values, std::vector<Tensor>{offsets},
                                             std::vector<int64_t>{max_sequence_length}, 0.0);
+}
+
+// ---- attention over jagged sequences, paged cache ---------------------------------------------------
+// Operators outside fbgemm's schema, named as b200tbe_pop_device_status is. q, k and v may be slices of one
+// projection: only the elements of a head have to lie side by side.
+
+// t as the kernels read it: [rows, heads, D] with the last dimension dense.
+Tensor dense_heads(const Tensor& t) { return t.size(2) <= 1 || t.stride(2) == 1 ? t : t.contiguous(); }
+
+void check_rows(const Tensor& t, const char* name, const Tensor& like) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", is on ", t.device());
+  TORCH_CHECK(t.dim() == 3, name, " must be [rows, heads, head_dim], has ", t.dim(), " dimensions");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " must share the other tensors' dtype");
+}
+
+void check_sequence_offsets(const Tensor& t, const char* name, const Tensor& like) {
+  check_cuda_contig(t, name);
+  TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", is on ", t.device());
+  TORCH_CHECK(t.dim() == 1 && t.numel() >= 1, name, " must be a vector of at least one entry");
+  TORCH_CHECK(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, name, " must be int64 or int32");
+}
+
+b200tbe_attention_params attention_params(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets,
+                                          const Tensor& k_offsets, bool causal, double scale, const Tensor& out,
+                                          const Tensor& lse) {
+  b200tbe_attention_params p{};
+  p.q = q.data_ptr(), p.k = k.data_ptr(), p.v = v.data_ptr(), p.out = out.data_ptr();
+  p.lse = lse.defined() ? lse.data_ptr<float>() : nullptr;
+  p.q_offsets = q_offsets.data_ptr(), p.k_offsets = k_offsets.data_ptr();
+  p.q_stride = q.stride(0), p.q_head_stride = q.stride(1), p.k_stride = k.stride(0), p.k_head_stride = k.stride(1);
+  p.v_stride = v.stride(0), p.v_head_stride = v.stride(1), p.out_stride = out.stride(0), p.out_head_stride = out.stride(1);
+  p.total_q = q.size(0), p.total_k = k.size(0);
+  p.batch = static_cast<int32_t>(q_offsets.numel() - 1);
+  p.heads = static_cast<int32_t>(q.size(1)), p.kv_heads = static_cast<int32_t>(k.size(1));
+  p.head_dim = static_cast<int32_t>(q.size(2));
+  p.dtype = dtype_code(q.scalar_type());
+  p.offset_bytes = static_cast<int32_t>(q_offsets.element_size());
+  p.causal = causal;
+  p.scale = static_cast<float>(scale);
+  return p;
+}
+
+// Checks the arguments and enqueues the forward pass; lse stays undefined unless it is asked for.
+std::tuple<Tensor, Tensor> jagged_attention_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_,
+                                                    const Tensor& q_offsets, const Tensor& k_offsets, bool causal,
+                                                    double scale, bool keep_lse) {
+  TORCH_CHECK(q_.is_cuda(), "q must be a CUDA tensor");
+  TORCH_CHECK(dtype_code(q_.scalar_type()) >= 0, "supported dtypes: float32, float16, bfloat16");
+  check_rows(q_, "q", q_);
+  check_rows(k_, "k", q_);
+  check_rows(v_, "v", q_);
+  TORCH_CHECK(k_.sizes() == v_.sizes(), "k and v must have the same shape");
+  TORCH_CHECK(q_.size(2) == k_.size(2), "q and k must have the same head_dim");
+  TORCH_CHECK(q_.size(2) >= 1 && q_.size(2) <= 256, "head_dim must be 1 to 256, is ", q_.size(2));
+  TORCH_CHECK(k_.size(1) >= 1 && q_.size(1) >= 1 && q_.size(1) % k_.size(1) == 0,
+              "the number of query heads must be a multiple of the number of key heads, got ", q_.size(1), " and ", k_.size(1));
+  check_sequence_offsets(q_offsets, "q_offsets", q_);
+  check_sequence_offsets(k_offsets, "k_offsets", q_);
+  TORCH_CHECK(q_offsets.numel() == k_offsets.numel() && q_offsets.scalar_type() == k_offsets.scalar_type(),
+              "q_offsets and k_offsets must have the same length and dtype");
+  c10::cuda::CUDAGuard guard(q_.device());
+  const Tensor q = dense_heads(q_), k = dense_heads(k_), v = dense_heads(v_);
+  Tensor out = at::empty(q.sizes(), q.options());
+  Tensor lse;
+  if (keep_lse) lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  const auto p = attention_params(q, k, v, q_offsets, k_offsets, causal, scale, out, lse);
+  check_status(b200tbe_jagged_attention(&p, current_stream()), "b200tbe_jagged_attention");
+  return {out, lse};
+}
+
+double scale_or_default(c10::optional<double> scale, const Tensor& q) {
+  if (scale.has_value()) return *scale;
+  return 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(1, q.dim() > 0 ? q.size(-1) : 1)));
+}
+
+const Tensor& key_offsets(const Tensor& q, const Tensor& k, const Tensor& q_offsets, const c10::optional<Tensor>& k_offsets) {
+  if (k_offsets.has_value() && k_offsets->defined()) return *k_offsets;
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && q.size(0) == k.size(0),
+              "without k_offsets, q and k must be [rows, heads, head_dim] with the same number of rows");
+  return q_offsets;
+}
+
+Tensor jagged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets,
+                        const c10::optional<Tensor>& k_offsets, bool causal, c10::optional<double> scale) {
+  return std::get<0>(jagged_attention_forward(q, k, v, q_offsets, key_offsets(q, k, q_offsets, k_offsets), causal,
+                                              scale_or_default(scale, q), false));
+}
+
+class JaggedAttentionFunction : public torch::autograd::Function<JaggedAttentionFunction> {
+ public:
+  static Variable forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets,
+                          const Tensor& k_offsets, bool causal, double scale) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [out, lse] = jagged_attention_forward(q, k, v, q_offsets, k_offsets, causal, scale, true);
+    ctx->save_for_backward({q, k, v, q_offsets, k_offsets, out, lse});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "b200tbe_jagged_attention is differentiable once: create_graph is not supported");
+    at::AutoDispatchBelowADInplaceOrView below;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor q = dense_heads(saved[0]), k = dense_heads(saved[1]), v = dense_heads(saved[2]);
+    const Tensor &q_offsets = saved[3], &k_offsets = saved[4], &out = saved[5], &lse = saved[6];
+    c10::cuda::CUDAGuard guard(q.device());
+    const Tensor g = dense_heads(grads[0]);
+    Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
+    const int32_t heads = static_cast<int32_t>(q.size(1));
+    Tensor scratch = at::empty(
+        {static_cast<int64_t>(b200tbe_jagged_attention_backward_scratch_bytes(q.size(0), heads))}, q.options().dtype(at::kByte));
+    b200tbe_attention_backward_params p{};
+    p.forward = attention_params(q, k, v, q_offsets, k_offsets, ctx->saved_data["causal"].toBool(),
+                                 ctx->saved_data["scale"].toDouble(), out, lse);
+    p.grad_out = g.data_ptr(), p.grad_q = dq.data_ptr(), p.grad_k = dk.data_ptr(), p.grad_v = dv.data_ptr();
+    p.grad_out_stride = g.stride(0), p.grad_out_head_stride = g.stride(1);
+    p.grad_q_stride = dq.stride(0), p.grad_q_head_stride = dq.stride(1);
+    p.grad_k_stride = dk.stride(0), p.grad_k_head_stride = dk.stride(1);
+    p.grad_v_stride = dv.stride(0), p.grad_v_head_stride = dv.stride(1);
+    p.scratch = scratch.data_ptr(), p.scratch_bytes = static_cast<size_t>(scratch.numel());
+    check_status(b200tbe_jagged_attention_backward(&p, current_stream()), "b200tbe_jagged_attention backward");
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor jagged_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets,
+                                 const c10::optional<Tensor>& k_offsets, bool causal, c10::optional<double> scale) {
+  const Tensor& ko = key_offsets(q, k, q_offsets, k_offsets);
+  if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad())) {
+    at::AutoDispatchBelowADInplaceOrView guard;   // nothing to keep for a backward pass
+    return std::get<0>(jagged_attention_forward(q, k, v, q_offsets, ko, causal, scale_or_default(scale, q), false));
+  }
+  return JaggedAttentionFunction::apply(q, k, v, q_offsets, ko, causal, scale_or_default(scale, q));
+}
+
+// The device's status word, unless this call is captured into a graph before the word exists: its memory
+// would belong to the graph.
+int32_t* status_word_of(const at::Device& device, Tensor* keep) {
+  static std::mutex mu;
+  static std::unordered_map<int, bool> made;
+  std::lock_guard<std::mutex> lock(mu);
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  TORCH_CHECK(cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream().stream(), &capturing) == cudaSuccess,
+              "the stream's capture status could not be read");
+  if (!made[device.index()]) {
+    if (capturing != cudaStreamCaptureStatusNone) return nullptr;
+    made[device.index()] = true;
+  }
+  *keep = device_status(device);
+  return keep->data_ptr<int32_t>();
+}
+
+b200tbe_paged_cache paged_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table, const Tensor& lengths) {
+  TORCH_CHECK(k_cache.is_cuda(), "k_cache must be a CUDA tensor");
+  for (const auto& [t, name] : {std::pair<const Tensor&, const char*>{k_cache, "k_cache"}, {v_cache, "v_cache"}}) {
+    TORCH_CHECK(t.device() == k_cache.device(), name, " must be on ", k_cache.device(), ", is on ", t.device());
+    TORCH_CHECK(t.dim() == 4, name, " must be [num_pages, page_size, kv_heads, head_dim]");
+    TORCH_CHECK(t.size(3) <= 1 || t.stride(3) == 1, name, ": the elements of a head must lie side by side");
+  }
+  TORCH_CHECK(dtype_code(k_cache.scalar_type()) >= 0 && k_cache.scalar_type() == v_cache.scalar_type(),
+              "k_cache and v_cache must share a dtype: float32, float16 or bfloat16");
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), "k_cache and v_cache must have the same shape");
+  TORCH_CHECK(k_cache.size(1) >= 1 && k_cache.size(2) >= 1, "page_size and kv_heads must be at least 1");
+  TORCH_CHECK(k_cache.size(3) >= 1 && k_cache.size(3) <= 256, "head_dim must be 1 to 256, is ", k_cache.size(3));
+  TORCH_CHECK(page_table.is_cuda() && page_table.device() == k_cache.device(), "page_table must be on ", k_cache.device());
+  TORCH_CHECK(page_table.dim() == 2 && page_table.scalar_type() == at::kInt, "page_table must be an int32 [batch, pages] matrix");
+  TORCH_CHECK(page_table.size(1) <= 1 || page_table.stride(1) == 1, "the rows of page_table must be dense");
+  check_cuda_contig(lengths, "lengths");
+  TORCH_CHECK(lengths.device() == k_cache.device(), "lengths must be on ", k_cache.device());
+  TORCH_CHECK(lengths.scalar_type() == at::kLong || lengths.scalar_type() == at::kInt, "lengths must be int64 or int32");
+  TORCH_CHECK(lengths.dim() == 1 && lengths.size(0) == page_table.size(0), "lengths and page_table must have the same batch");
+  TORCH_CHECK(k_cache.size(1) <= 0x7fffffff && page_table.size(0) <= 0x7fffffff && page_table.size(1) <= 0x7fffffff,
+              "page_size, batch and pages must fit 32 bits");
+  b200tbe_paged_cache c{};
+  c.k_cache = k_cache.data_ptr(), c.v_cache = v_cache.data_ptr();
+  c.page_table = page_table.data_ptr<int32_t>(), c.lengths = lengths.data_ptr();
+  c.k_page_stride = k_cache.stride(0), c.k_slot_stride = k_cache.stride(1), c.k_head_stride = k_cache.stride(2);
+  c.v_page_stride = v_cache.stride(0), c.v_slot_stride = v_cache.stride(1), c.v_head_stride = v_cache.stride(2);
+  c.page_table_stride = page_table.stride(0), c.num_pages = k_cache.size(0);
+  c.max_pages = static_cast<int32_t>(page_table.size(1)), c.page_size = static_cast<int32_t>(k_cache.size(1));
+  c.batch = static_cast<int32_t>(page_table.size(0)), c.kv_heads = static_cast<int32_t>(k_cache.size(2));
+  c.head_dim = static_cast<int32_t>(k_cache.size(3)), c.dtype = dtype_code(k_cache.scalar_type());
+  c.length_bytes = static_cast<int32_t>(lengths.element_size());
+  return c;
+}
+
+void paged_cache_append(const Tensor& k_, const Tensor& v_, const Tensor& offsets, Tensor k_cache, Tensor v_cache,
+                        const Tensor& page_table, const Tensor& lengths) {
+  auto c = paged_cache(k_cache, v_cache, page_table, lengths);
+  check_rows(k_, "k", k_cache);
+  check_rows(v_, "v", k_cache);
+  TORCH_CHECK(k_.sizes() == v_.sizes(), "k and v must have the same shape");
+  TORCH_CHECK(k_.size(1) == c.kv_heads && k_.size(2) == c.head_dim, "k and v must have the cache's heads and head_dim");
+  check_sequence_offsets(offsets, "offsets", k_cache);
+  TORCH_CHECK(offsets.numel() == static_cast<int64_t>(c.batch) + 1, "offsets must have one entry more than the batch");
+  c10::cuda::CUDAGuard guard(k_cache.device());
+  const Tensor k = dense_heads(k_), v = dense_heads(v_);
+  Tensor status;
+  c.status = status_word_of(k_cache.device(), &status);
+  check_status(b200tbe_paged_cache_append(&c, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                                          offsets.data_ptr(), static_cast<int32_t>(offsets.element_size()), k.size(0),
+                                          current_stream()),
+               "b200tbe_paged_cache_append");
+}
+
+Tensor paged_attention(const Tensor& q_, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
+                       const Tensor& lengths, c10::optional<double> scale) {
+  auto c = paged_cache(k_cache, v_cache, page_table, lengths);
+  check_rows(q_, "q", k_cache);
+  TORCH_CHECK(q_.size(0) == c.batch && q_.size(2) == c.head_dim, "q must be [batch, heads, head_dim] of the cache's head_dim");
+  TORCH_CHECK(q_.size(1) >= 1 && q_.size(1) % c.kv_heads == 0,
+              "the number of query heads must be a multiple of the number of key heads, got ", q_.size(1), " and ", c.kv_heads);
+  c10::cuda::CUDAGuard guard(k_cache.device());
+  const Tensor q = dense_heads(q_);
+  Tensor out = at::empty(q.sizes(), q.options());
+  Tensor scratch = at::empty({static_cast<int64_t>(b200tbe_paged_attention_scratch_bytes(c.head_dim))},
+                             q.options().dtype(at::kByte));
+  Tensor status;
+  c.status = status_word_of(k_cache.device(), &status);
+  check_status(b200tbe_paged_attention(&c, q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1),
+                                       static_cast<int32_t>(q.size(1)), static_cast<float>(scale_or_default(scale, q)),
+                                       scratch.data_ptr(), static_cast<size_t>(scratch.numel()), current_stream()),
+               "b200tbe_paged_attention");
+  return out;
 }
 
 // ---- permute_2D_sparse_data -----------------------------------------------------------------------
@@ -928,6 +1154,16 @@ TORCH_LIBRARY_FRAGMENT(fbgemm, m) {
       "Tensor? indice_weights, int output_dtype=1, Tensor? lxu_cache_weights=None, "
       "Tensor? lxu_cache_locations=None, int? row_alignment=None, int? max_float8_D=0, "
       "int? fp8_exponent_bits=-1, int? fp8_exponent_bias=-1) -> Tensor");
+  // Not fbgemm_gpu operators: attention over jagged sequences, and over a paged cache.
+  m.def(
+      "b200tbe_jagged_attention(Tensor q, Tensor k, Tensor v, Tensor q_offsets, Tensor? k_offsets=None, "
+      "bool causal=False, float? scale=None) -> Tensor");
+  m.def(
+      "b200tbe_paged_cache_append(Tensor k, Tensor v, Tensor offsets, Tensor(a!) k_cache, Tensor(b!) v_cache, "
+      "Tensor page_table, Tensor lengths) -> ()");
+  m.def(
+      "b200tbe_paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor lengths, "
+      "float? scale=None) -> Tensor");
   // Not an fbgemm_gpu operator: returns, and clears, the B200TBE_DEV_* bits the lookup kernels have
   // raised on the device of `like` since the last call (0: none). Synchronises.
   m.def("b200tbe_pop_device_status(Tensor like) -> int");
@@ -948,6 +1184,9 @@ TORCH_LIBRARY_IMPL(fbgemm, CUDA, m) {
   m.impl("int_nbit_split_embedding_codegen_lookup_function",
          TORCH_FN(int_nbit_split_embedding_codegen_lookup_function));
   m.impl("b200tbe_pop_device_status", TORCH_FN(pop_device_status));
+  m.impl("b200tbe_jagged_attention", TORCH_FN(jagged_attention));
+  m.impl("b200tbe_paged_cache_append", TORCH_FN(paged_cache_append));
+  m.impl("b200tbe_paged_attention", TORCH_FN(paged_attention));
 }
 
 // The training lookups and the jagged ops carry their own autograd nodes, so they also sit on the
@@ -957,6 +1196,7 @@ TORCH_LIBRARY_IMPL(fbgemm, AutogradCUDA, m) {
   m.impl("dense_to_jagged", TORCH_FN(dense_to_jagged_autograd));
   m.impl("jagged_dense_elementwise_add", TORCH_FN(jagged_dense_elementwise_add_autograd));
   m.impl("jagged_2d_to_dense", TORCH_FN(jagged_2d_to_dense_autograd));
+  m.impl("b200tbe_jagged_attention", TORCH_FN(jagged_attention_autograd));
   m.impl("split_embedding_codegen_lookup_rowwise_adagrad_function",
          TORCH_FN(split_embedding_codegen_lookup_rowwise_adagrad_function));
   m.impl("split_embedding_codegen_lookup_sgd_function",

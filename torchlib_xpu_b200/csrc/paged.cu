@@ -1,0 +1,457 @@
+// The paged key-value cache: jagged rows appended to it, and the attention of one new token over it.
+#include "attention.cuh"
+
+namespace b200tbe {
+namespace {
+
+struct CacheDev {
+  char* k;
+  char* v;
+  const int32_t* page_table;
+  const void* lengths;
+  int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;   // elements
+  int64_t table_stride, num_pages;
+  int32_t max_pages, page_size, batch, kv_heads, D, length_bytes;
+  int32_t* status;
+};
+
+__device__ __forceinline__ void raise(const CacheDev& c) {
+  if (c.status != nullptr) atomicOr(c.status, B200TBE_DEV_INDEX_OUT_OF_RANGE);
+}
+
+__device__ __forceinline__ int64_t raw_length(const CacheDev& c, int b) {
+  return c.length_bytes == 8 ? load_index<int64_t>(c.lengths, b) : load_index<int32_t>(c.lengths, b);
+}
+
+// Positions of sequence b that its row of the page table can hold.
+__device__ __forceinline__ int length_of(const CacheDev& c, int b) {
+  const int64_t n = raw_length(c, b);
+  const int64_t most = min(static_cast<int64_t>(c.max_pages) * c.page_size, static_cast<int64_t>(0x7fffff00));
+  return n < 0 ? 0 : static_cast<int>(n > most ? most : n);
+}
+
+// ---- append ----------------------------------------------------------------------------------
+// A warp takes 32 / kShare consecutive rows: lane l finds where row l goes (a search over the offsets), then
+// the warp moves the rows' heads one after the other, 2^kVecLog bytes a lane, keys and values together.
+// Bound by HBM: every row is read once and written once.
+struct AppendDev {
+  CacheDev c;
+  const char* k;
+  const char* v;
+  int64_t k_row, k_head, v_row, v_head;   // elements
+  const void* offsets;
+  int64_t total;
+  int32_t offset_bytes, elem_bytes, rows_per_warp;
+};
+
+template <typename VecT>
+__global__ void __launch_bounds__(256) append_kernel(const AppendDev p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row0 = (static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32) * p.rows_per_warp;
+  if (row0 >= p.total) return;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(p.rows_per_warp), p.total - row0));
+  int64_t page = -1;
+  int32_t slot = 0;
+  if (lane < rows) {
+    const int64_t row = row0 + lane;
+    // the last sequence that begins at or before the row
+    int lo = 0, hi = p.c.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (clamped_offset(p.offsets, p.offset_bytes, mid, p.total) <= row) lo = mid; else hi = mid;
+    }
+    const int64_t begin = clamped_offset(p.offsets, p.offset_bytes, lo, p.total);
+    const int64_t end = clamped_offset(p.offsets, p.offset_bytes, lo + 1, p.total);
+    if (row >= begin && row < end) {
+      const int64_t at = raw_length(p.c, lo) - (end - row);
+      if (at >= 0 && at / p.c.page_size < p.c.max_pages) {
+        page = __ldg(p.c.page_table + lo * p.c.table_stride + at / p.c.page_size);
+        slot = static_cast<int32_t>(at % p.c.page_size);
+      }
+      if (page < 0 || page >= p.c.num_pages) {
+        page = -1;
+        raise(p.c);
+      }
+    }
+  }
+  const int per_head = p.c.D * p.elem_bytes / static_cast<int>(sizeof(VecT));
+  const int vecs = per_head * p.c.kv_heads;
+  const int all = vecs * rows;   // the rows of this warp as one stream of vectors
+  constexpr int kUnroll = 4;
+  for (int i0 = 0; i0 < all; i0 += 32 * kUnroll) {
+    VecT kx[kUnroll], vx[kUnroll];
+    VecT* kd[kUnroll];
+    VecT* vd[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = i0 + u * 32 + lane;
+      const int r = min(i / vecs, rows - 1);
+      const int64_t pg = __shfl_sync(kFullMask, page, r);
+      const int sl = __shfl_sync(kFullMask, slot, r);
+      kd[u] = nullptr;
+      if (i < all && pg >= 0) {
+        const int w = i - r * vecs, h = w / per_head, e = w - h * per_head;
+        const int64_t row = row0 + r;
+        kx[u] = __ldcs(reinterpret_cast<const VecT*>(p.k + (row * p.k_row + h * p.k_head) * p.elem_bytes) + e);
+        vx[u] = __ldcs(reinterpret_cast<const VecT*>(p.v + (row * p.v_row + h * p.v_head) * p.elem_bytes) + e);
+        kd[u] = reinterpret_cast<VecT*>(p.c.k + (pg * p.c.k_page + sl * p.c.k_slot + h * p.c.k_head) * p.elem_bytes) + e;
+        vd[u] = reinterpret_cast<VecT*>(p.c.v + (pg * p.c.v_page + sl * p.c.v_slot + h * p.c.v_head) * p.elem_bytes) + e;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (kd[u] != nullptr) {
+        *kd[u] = kx[u];
+        *vd[u] = vx[u];
+      }
+  }
+}
+
+// ---- one new token ---------------------------------------------------------------------------
+//   out[h] = sum_t exp(s_t - m) v_t / sum_t exp(s_t - m),   s_t = scale q[h] . k[t]
+//
+// Work is counted in tiles of kTile positions of one unit: a sequence, a key head and up to kHeads of its
+// query heads. All units' tiles in one line are cut into equal pieces, one for each CTA, so that the GPU is
+// evenly loaded whatever the lengths. A unit inside one CTA is finished there. One that a cut divides leaves
+// a piece (m, l, unnormalised sum) in each CTA's slot; a second kernel joins the pieces in their order:
+//   m = max m_i,  l = sum l_i exp(m_i - m),  out = sum o_i exp(m_i - m) / l
+constexpr int kTile = 64;
+constexpr int kHeads = 8;
+constexpr int kAnswerThreads = 128;
+constexpr int kAnswerCtas = kNumSMs * 8;
+
+// Where a CTA's piece of the line begins.
+struct Start {
+  int32_t unit, tile, tiles, ctas;   // unit, tile inside it, the unit's tiles, CTAs with work
+  int64_t at, all;                   // place in the line, the line's length
+};
+
+struct AnswerDev {
+  CacheDev c;
+  const void* q;
+  void* out;
+  int64_t q_row, q_head, o_row, o_head;
+  int32_t heads, group, chunks, units;   // chunks of kHeads query heads a key head; units a sequence
+  float scale;
+  Start* starts;     // [gridDim.x]
+  float* stats;      // [2 * gridDim.x][kHeads][2]: m, l
+  float* sums;       // [2 * gridDim.x][kHeads][D]
+};
+
+__device__ __forceinline__ int tiles_of(const CacheDev& c, int b) { return max(1, (length_of(c, b) + kTile - 1) / kTile); }
+
+// The CTA's piece [at, end) of the line, and the sequence and unit its first tile lies in. All threads.
+__device__ __forceinline__ Start find_start(const AnswerDev& p, int64_t* end) {
+  __shared__ int64_t sums[kAnswerThreads / 32];
+  __shared__ Start found;
+  const int n = p.c.batch, per = (n + kAnswerThreads - 1) / kAnswerThreads;
+  const int b0 = min(n, static_cast<int>(threadIdx.x) * per), b1 = min(n, b0 + per);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += tiles_of(p.c, b);
+  int64_t upto = mine;   // inclusive sum over the threads
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(kFullMask, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kAnswerThreads / 32; ++w) {
+    if (w < warp) before += sums[w];
+    all += sums[w];
+  }
+  all *= p.units;
+  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), all);
+  const int64_t at = blockIdx.x < ctas ? all * blockIdx.x / ctas : all;
+  *end = blockIdx.x < ctas ? all * (blockIdx.x + 1) / ctas : all;
+  int64_t first = (before + upto - mine) * p.units;
+  if (at >= first && at < first + mine * p.units) {
+    int b = b0;
+    int64_t tiles = tiles_of(p.c, b);
+    while (at >= first + tiles * p.units) {
+      first += tiles * p.units;
+      tiles = tiles_of(p.c, ++b);
+    }
+    const int64_t u = (at - first) / tiles;
+    found = Start{static_cast<int32_t>(b * p.units + u), static_cast<int32_t>(at - first - u * tiles),
+                  static_cast<int32_t>(tiles), static_cast<int32_t>(ctas), at, all};
+  }
+  __syncthreads();
+  Start s = found;
+  if (at >= *end) s = Start{-1, 0, 0, static_cast<int32_t>(ctas), at, all};
+  if (threadIdx.x == 0) p.starts[blockIdx.x] = s;
+  return s;
+}
+
+// Any type, head dimension and stride, in 32-bit arithmetic: scores by a thread for each position, sums by a
+// thread for each column.
+template <typename T, int kCols>   // columns of a thread: D <= kCols * kAnswerThreads
+__global__ void __launch_bounds__(kAnswerThreads) answer_simt_kernel(const AnswerDev p) {
+  extern __shared__ float smem[];
+  float* qs = smem;                              // [kHeads][D]
+  float* ks = qs + kHeads * p.c.D;               // [kTile][D + 1]
+  __shared__ float ps[kHeads][kTile];
+  __shared__ float top[kHeads], sum[kHeads], keep[kHeads];
+  __shared__ int64_t k_at[kTile], v_at[kTile];   // the tile's positions in the cache, -1: none
+  const int D = p.c.D, tid = threadIdx.x;
+  int64_t end;
+  Start s = find_start(p, &end);
+  int64_t at = s.at;
+  while (at < end) {
+    const int b = s.unit / p.units, u = s.unit % p.units, kv = u / p.chunks;
+    const int head0 = kv * p.group + (u % p.chunks) * kHeads;
+    const int heads = min(kHeads, (kv + 1) * p.group - head0);
+    const int len = length_of(p.c, b);
+    const int stop = static_cast<int>(min(static_cast<int64_t>(s.tiles), s.tile + (end - at)));
+    __syncthreads();
+    for (int i = tid; i < heads * D; i += kAnswerThreads) {
+      const int h = i / D, d = i % D;
+      qs[i] = to_float<T>(static_cast<const T*>(p.q)[b * p.q_row + (head0 + h) * p.q_head + d]);
+    }
+    if (tid < kHeads) top[tid] = -INFINITY, sum[tid] = 0.f;
+    if (tid == 0 && s.tile == 0 && raw_length(p.c, b) != len) raise(p.c);
+    float o[kHeads][kCols] = {};
+    for (int tile = s.tile; tile < stop; ++tile) {
+      __syncthreads();
+      if (tid < kTile) {
+        const int t = tile * kTile + tid;
+        k_at[tid] = v_at[tid] = -1;
+        if (t < len) {
+          const int64_t page = __ldg(p.c.page_table + b * p.c.table_stride + t / p.c.page_size);
+          if (page >= 0 && page < p.c.num_pages) {
+            const int64_t slot = t % p.c.page_size;
+            k_at[tid] = page * p.c.k_page + slot * p.c.k_slot + kv * p.c.k_head;
+            v_at[tid] = page * p.c.v_page + slot * p.c.v_slot + kv * p.c.v_head;
+          } else {
+            raise(p.c);
+          }
+        }
+      }
+      __syncthreads();
+      for (int i = tid; i < kTile * D; i += kAnswerThreads) {
+        const int t = i / D, d = i % D;
+        ks[t * (D + 1) + d] = k_at[t] >= 0 ? to_float<T>(reinterpret_cast<const T*>(p.c.k)[k_at[t] + d]) : 0.f;
+      }
+      __syncthreads();
+      for (int i = tid; i < kTile * heads; i += kAnswerThreads) {
+        const int t = i % kTile, h = i / kTile;
+        float x = 0.f;
+        for (int d = 0; d < D; ++d) x = fmaf(qs[h * D + d], ks[t * (D + 1) + d], x);
+        ps[h][t] = k_at[t] >= 0 ? x * p.scale : -INFINITY;
+      }
+      __syncthreads();
+      for (int h = tid / 32; h < heads; h += kAnswerThreads / 32) {
+        const int lane = tid & 31;
+        const float a = ps[h][lane], c = ps[h][lane + 32], was = top[h];
+        float m = fmaxf(was, fmaxf(a, c));
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, w));
+        const float base = m == -INFINITY ? 0.f : m;
+        const float ea = expf(a - base), ec = expf(c - base);
+        ps[h][lane] = ea;
+        ps[h][lane + 32] = ec;
+        const float add = warp_sum(ea + ec);
+        if (lane == 0) {
+          keep[h] = expf(was - base);
+          top[h] = m;
+          sum[h] = sum[h] * keep[h] + add;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        const int d = c * kAnswerThreads + tid;
+        if (d < D) {
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h)
+            if (h < heads) o[h][c] *= keep[h];
+#pragma unroll 8
+          for (int t = 0; t < kTile; ++t) {
+            const float x = v_at[t] >= 0 ? to_float<T>(reinterpret_cast<const T*>(p.c.v)[v_at[t] + d]) : 0.f;
+#pragma unroll
+            for (int h = 0; h < kHeads; ++h)
+              if (h < heads) o[h][c] = fmaf(ps[h][t], x, o[h][c]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = s.tile == 0 && stop == s.tiles;
+    const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (s.tile == 0 ? 1 : 0);
+    if (!whole && tid < heads) {
+      p.stats[(part * kHeads + tid) * 2] = top[tid];
+      p.stats[(part * kHeads + tid) * 2 + 1] = sum[tid];
+    }
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const int d = c * kAnswerThreads + tid;
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h)
+        if (h < heads && d < D) {
+          if (whole)
+            static_cast<T*>(p.out)[b * p.o_row + (head0 + h) * p.o_head + d] = from_float<T>(sum[h] == 0.f ? 0.f : o[h][c] / sum[h]);
+          else
+            p.sums[(part * kHeads + h) * D + d] = o[h][c];
+        }
+    }
+    at += stop - s.tile;
+    if (at < end) {
+      ++s.unit;
+      s.tile = 0;
+      s.tiles = tiles_of(p.c, s.unit / p.units);
+    }
+  }
+}
+
+// Block (c, h): when the cut before CTA c is the first inside a unit, the unit's head h.
+template <typename T>
+__global__ void __launch_bounds__(kAnswerThreads) join_kernel(const AnswerDev p) {
+  const int c = blockIdx.x + 1, h = blockIdx.y;
+  const Start s = p.starts[c];
+  if (s.unit < 0 || s.tile == 0) return;
+  const Start before = p.starts[c - 1];
+  if (before.unit == s.unit && before.tile > 0) return;
+  const int u = s.unit % p.units, kv = u / p.chunks, b = s.unit / p.units;
+  const int head = kv * p.group + (u % p.chunks) * kHeads + h;
+  if (head >= (kv + 1) * p.group) return;
+  // the CTA that holds the unit's last tile
+  const int last = static_cast<int>(((s.at - s.tile + s.tiles) * s.ctas - 1) / s.all);
+  // the first piece lies in its CTA's second slot, the others in the first
+  const int64_t part0 = 2 * static_cast<int64_t>(c - 1) + 1;
+  float m = p.stats[(part0 * kHeads + h) * 2];
+  for (int i = c; i <= last; ++i) m = fmaxf(m, p.stats[(2 * static_cast<int64_t>(i) * kHeads + h) * 2]);
+  const float base = m == -INFINITY ? 0.f : m;
+  for (int d = threadIdx.x; d < p.c.D; d += kAnswerThreads) {
+    float w = expf(p.stats[(part0 * kHeads + h) * 2] - base);
+    float l = w * p.stats[(part0 * kHeads + h) * 2 + 1];
+    float o = w * p.sums[(part0 * kHeads + h) * p.c.D + d];
+#pragma unroll 4
+    for (int i = c; i <= last; ++i) {
+      const int64_t part = 2 * static_cast<int64_t>(i);
+      w = expf(p.stats[(part * kHeads + h) * 2] - base);
+      l = fmaf(w, p.stats[(part * kHeads + h) * 2 + 1], l);
+      o = fmaf(w, p.sums[(part * kHeads + h) * p.c.D + d], o);
+    }
+    static_cast<T*>(p.out)[b * p.o_row + head * p.o_head + d] = from_float<T>(l == 0.f ? 0.f : o / l);
+  }
+}
+
+int elem_bytes_of(int dtype) { return dtype == B200TBE_FP32 ? 4 : 2; }
+
+int check_cache(const b200tbe_paged_cache* c) {
+  if (c == nullptr) return B200TBE_ERR_BAD_ARG;
+  if (c->dtype != B200TBE_FP32 && c->dtype != B200TBE_FP16 && c->dtype != B200TBE_BF16) return B200TBE_ERR_UNSUPPORTED;
+  if (c->head_dim < 1 || c->head_dim > 256) return B200TBE_ERR_UNSUPPORTED;
+  if (c->length_bytes != 4 && c->length_bytes != 8) return B200TBE_ERR_UNSUPPORTED;
+  if (c->batch < 0 || c->kv_heads < 1 || c->page_size < 1 || c->max_pages < 0 || c->num_pages < 0) return B200TBE_ERR_BAD_ARG;
+  if (c->batch > 0 && c->lengths == nullptr) return B200TBE_ERR_BAD_ARG;
+  if (c->batch > 0 && c->max_pages > 0 && c->page_table == nullptr) return B200TBE_ERR_BAD_ARG;
+  if (c->num_pages > 0 && (c->k_cache == nullptr || c->v_cache == nullptr)) return B200TBE_ERR_BAD_ARG;
+  return B200TBE_OK;
+}
+
+CacheDev cache_dev(const b200tbe_paged_cache* c) {
+  CacheDev d{};
+  d.k = static_cast<char*>(c->k_cache), d.v = static_cast<char*>(c->v_cache);
+  d.page_table = c->page_table, d.lengths = c->lengths;
+  d.k_page = c->k_page_stride, d.k_slot = c->k_slot_stride, d.k_head = c->k_head_stride;
+  d.v_page = c->v_page_stride, d.v_slot = c->v_slot_stride, d.v_head = c->v_head_stride;
+  d.table_stride = c->page_table_stride, d.num_pages = c->num_pages, d.max_pages = c->max_pages;
+  d.page_size = c->page_size, d.batch = c->batch, d.kv_heads = c->kv_heads, d.D = c->head_dim;
+  d.length_bytes = c->length_bytes, d.status = c->status;
+  return d;
+}
+
+template <typename VecT>
+int launch_append(const AppendDev& p, cudaStream_t stream) {
+  const int64_t warps = (p.total + p.rows_per_warp - 1) / p.rows_per_warp, blocks = (warps + 7) / 8;
+  if (blocks > 0x7fffffff) return B200TBE_ERR_TOO_LARGE;
+  append_kernel<VecT><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
+  return launch_status();
+}
+
+template <typename T>
+int launch_answer(const AnswerDev& p, int ctas, cudaStream_t stream) {
+  const int bytes = (kHeads * p.c.D + kTile * (p.c.D + 1)) * 4;
+  const auto kernel = p.c.D <= kAnswerThreads ? answer_simt_kernel<T, 1> : answer_simt_kernel<T, 2>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return B200TBE_ERR_LAUNCH;
+  kernel<<<ctas, kAnswerThreads, bytes, stream>>>(p);
+  const int st = launch_status();
+  if (st != B200TBE_OK || ctas < 2) return st;
+  join_kernel<T><<<dim3(ctas - 1, min(kHeads, p.group)), kAnswerThreads, 0, stream>>>(p);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace b200tbe
+
+using namespace b200tbe;
+
+extern "C" int b200tbe_paged_cache_append(const b200tbe_paged_cache* cache, const void* k, const void* v, int64_t k_stride,
+                                          int64_t k_head_stride, int64_t v_stride, int64_t v_head_stride,
+                                          const void* offsets, int32_t offset_bytes, int64_t total,
+                                          b200tbe_stream_t stream_) {
+  const int st = check_cache(cache);
+  if (st != B200TBE_OK) return st;
+  if (offset_bytes != 4 && offset_bytes != 8) return B200TBE_ERR_UNSUPPORTED;
+  if (total < 0) return B200TBE_ERR_BAD_ARG;
+  if (total == 0 || cache->batch == 0) return B200TBE_OK;
+  if (k == nullptr || v == nullptr || offsets == nullptr) return B200TBE_ERR_BAD_ARG;
+  AppendDev p{};
+  p.c = cache_dev(cache);
+  p.k = static_cast<const char*>(k), p.v = static_cast<const char*>(v);
+  p.k_row = k_stride, p.k_head = k_head_stride, p.v_row = v_stride, p.v_head = v_head_stride;
+  p.offsets = offsets, p.offset_bytes = offset_bytes, p.total = total;
+  p.elem_bytes = elem_bytes_of(cache->dtype);
+  if (static_cast<int64_t>(cache->head_dim) * cache->kv_heads * p.elem_bytes > (1 << 24)) return B200TBE_ERR_TOO_LARGE;
+  // rows are shared out so that a small batch still uses every SM
+  p.rows_per_warp = static_cast<int32_t>(total / (kNumSMs * 64) < 1 ? 1 : (total / (kNumSMs * 64) > 8 ? 8 : total / (kNumSMs * 64)));
+  uint64_t bits = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(p.c.k) |
+                  reinterpret_cast<uintptr_t>(p.c.v);
+  for (int64_t s : {static_cast<int64_t>(p.c.D), p.k_row, p.k_head, p.v_row, p.v_head, p.c.k_page, p.c.k_slot, p.c.k_head,
+                    p.c.v_page, p.c.v_slot, p.c.v_head})
+    bits |= static_cast<uint64_t>(s * p.elem_bytes);
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  if (bits % 16 == 0) return launch_append<uint4>(p, stream);
+  if (bits % 4 == 0) return launch_append<uint32_t>(p, stream);
+  return launch_append<uint16_t>(p, stream);
+}
+
+extern "C" size_t b200tbe_paged_attention_scratch_bytes(int32_t head_dim) {
+  if (head_dim < 1) return 0;
+  return kAnswerCtas * (sizeof(Start) + 2 * kHeads * (2 + static_cast<size_t>(head_dim)) * sizeof(float));
+}
+
+extern "C" int b200tbe_paged_attention(const b200tbe_paged_cache* cache, const void* q, void* out, int64_t q_stride,
+                                       int64_t q_head_stride, int64_t out_stride, int64_t out_head_stride, int32_t heads,
+                                       float scale, void* scratch, size_t scratch_bytes, b200tbe_stream_t stream_) {
+  const int st = check_cache(cache);
+  if (st != B200TBE_OK) return st;
+  if (heads < 1 || heads % cache->kv_heads != 0) return B200TBE_ERR_BAD_ARG;
+  if (cache->batch == 0) return B200TBE_OK;
+  if (q == nullptr || out == nullptr) return B200TBE_ERR_BAD_ARG;
+  if (scratch == nullptr || scratch_bytes < b200tbe_paged_attention_scratch_bytes(cache->head_dim) || !aligned_to(scratch, 16))
+    return B200TBE_ERR_SCRATCH;
+  AnswerDev p{};
+  p.c = cache_dev(cache);
+  p.q = q, p.out = out;
+  p.q_row = q_stride, p.q_head = q_head_stride, p.o_row = out_stride, p.o_head = out_head_stride;
+  p.heads = heads, p.group = heads / cache->kv_heads, p.chunks = (p.group + kHeads - 1) / kHeads;
+  p.units = cache->kv_heads * p.chunks;
+  if (static_cast<int64_t>(p.units) * cache->batch > 0x7fffffff) return B200TBE_ERR_TOO_LARGE;
+  p.scale = scale;
+  p.starts = static_cast<Start*>(scratch);
+  p.stats = reinterpret_cast<float*>(p.starts + kAnswerCtas);
+  p.sums = p.stats + 2 * kAnswerCtas * kHeads * 2;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  // as many CTAs as the cache could give tiles to
+  const int64_t most = (static_cast<int64_t>(cache->max_pages) * cache->page_size + kTile - 1) / kTile;
+  const int64_t tiles = static_cast<int64_t>(p.units) * cache->batch * (most < 1 ? 1 : most);
+  const int ctas = static_cast<int>(tiles < kAnswerCtas ? tiles : kAnswerCtas);
+  if (cache->dtype == B200TBE_FP32) return launch_answer<float>(p, ctas, stream);
+  if (cache->dtype == B200TBE_FP16) return launch_answer<__half>(p, ctas, stream);
+  return launch_answer<__nv_bfloat16>(p, ctas, stream);
+}
