@@ -66,8 +66,8 @@ typedef enum { B200TBE_OPT_SGD = 0, B200TBE_OPT_ROWWISE_ADAGRAD = 1 } b200tbe_op
  * (in smaller batches such a bag only moves lookups of its table to other bags of the table). */
 #define B200TBE_DEV_OFFSETS_NOT_MONOTONE 2
 #define B200TBE_DEV_UNSUPPORTED_SHAPE 4 /* a table's row is not whole 16-byte vectors */
-#define B200TBE_DEV_WAIT_TIMEOUT 8      /* reserved: a bounded wait inside a kernel gave up (no kernel of
-                                           this version waits on anything but its own loads) */
+#define B200TBE_DEV_WAIT_TIMEOUT 8      /* a bounded wait inside a kernel gave up: its results are not valid (no
+                                           kernel waits on anything but its own block's copies and products) */
 
 #define B200TBE_MAX_DESTS 16
 #define B200TBE_MAX_JAGGED_DIMS 4
@@ -430,6 +430,7 @@ typedef struct {
   int32_t offset_bytes;             /* 8 or 4 */
   int32_t causal;
   float scale;
+  int32_t* status;                  /* device word or NULL: B200TBE_DEV_WAIT_TIMEOUT */
 } b200tbe_attention_params;
 
 B200TBE_API int b200tbe_jagged_attention(const b200tbe_attention_params* p, b200tbe_stream_t stream);

@@ -96,7 +96,7 @@ class AttentionParams(ctypes.Structure):
         ("total_q", ctypes.c_int64), ("total_k", ctypes.c_int64),
         ("batch", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
         ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("offset_bytes", ctypes.c_int32),
-        ("causal", ctypes.c_int32), ("scale", ctypes.c_float),
+        ("causal", ctypes.c_int32), ("scale", ctypes.c_float), ("status", _c_void_p),
     ]
 
 

@@ -43,7 +43,12 @@ extern "C" int b200tbe_jagged_attention(const b200tbe_attention_params* p, b200t
   if (st != B200TBE_OK) return st;
   if (p->total_q == 0) return B200TBE_OK;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  return attention_forward_simt(device_params(p), p->dtype, stream);
+  const AttnDev d = device_params(p);
+  if (attention_forward_fits(d, p->dtype)) {
+    const int tc = attention_forward_tc(d, p->dtype, p->status, stream);
+    if (tc != B200TBE_ERR_UNSUPPORTED) return tc;
+  }
+  return attention_forward_simt(d, p->dtype, stream);
 }
 
 extern "C" size_t b200tbe_jagged_attention_backward_scratch_bytes(int64_t total_q, int32_t heads) {

@@ -30,6 +30,10 @@ struct AttnDev {
 
 int attention_forward_simt(const AttnDev& p, int dtype, cudaStream_t stream);
 int attention_backward_simt(const AttnDev& p, int dtype, cudaStream_t stream);
+// Tensor-core kernels: whether they take these arguments, and the launches. B200TBE_ERR_UNSUPPORTED from a
+// launch (nothing was enqueued): the driver made no tensor map of them, the 32-bit kernels take over.
+bool attention_forward_fits(const AttnDev& p, int dtype);
+int attention_forward_tc(const AttnDev& p, int dtype, int32_t* status, cudaStream_t stream);
 int attention_delta(const AttnDev& p, int dtype, cudaStream_t stream);
 
 // One sequence's rows on both sides, or a stretch of rows that no sequence owns (klen 0).

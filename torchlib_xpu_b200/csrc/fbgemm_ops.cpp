@@ -438,6 +438,23 @@ void check_sequence_offsets(const Tensor& t, const char* name, const Tensor& lik
   TORCH_CHECK(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, name, " must be int64 or int32");
 }
 
+// The device's status word, unless this call is captured into a graph before the word exists: its memory
+// would belong to the graph.
+int32_t* status_word_of(const at::Device& device, Tensor* keep) {
+  static std::mutex mu;
+  static std::unordered_map<int, bool> made;
+  std::lock_guard<std::mutex> lock(mu);
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  TORCH_CHECK(cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream().stream(), &capturing) == cudaSuccess,
+              "the stream's capture status could not be read");
+  if (!made[device.index()]) {
+    if (capturing != cudaStreamCaptureStatusNone) return nullptr;
+    made[device.index()] = true;
+  }
+  *keep = device_status(device);
+  return keep->data_ptr<int32_t>();
+}
+
 b200tbe_attention_params attention_params(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets,
                                           const Tensor& k_offsets, bool causal, double scale, const Tensor& out,
                                           const Tensor& lse) {
@@ -455,6 +472,8 @@ b200tbe_attention_params attention_params(const Tensor& q, const Tensor& k, cons
   p.offset_bytes = static_cast<int32_t>(q_offsets.element_size());
   p.causal = causal;
   p.scale = static_cast<float>(scale);
+  Tensor word;   // kept by the library
+  p.status = status_word_of(q.device(), &word);
   return p;
 }
 
@@ -549,23 +568,6 @@ Tensor jagged_attention_autograd(const Tensor& q, const Tensor& k, const Tensor&
     return std::get<0>(jagged_attention_forward(q, k, v, q_offsets, ko, causal, scale_or_default(scale, q), false));
   }
   return JaggedAttentionFunction::apply(q, k, v, q_offsets, ko, causal, scale_or_default(scale, q));
-}
-
-// The device's status word, unless this call is captured into a graph before the word exists: its memory
-// would belong to the graph.
-int32_t* status_word_of(const at::Device& device, Tensor* keep) {
-  static std::mutex mu;
-  static std::unordered_map<int, bool> made;
-  std::lock_guard<std::mutex> lock(mu);
-  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-  TORCH_CHECK(cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream().stream(), &capturing) == cudaSuccess,
-              "the stream's capture status could not be read");
-  if (!made[device.index()]) {
-    if (capturing != cudaStreamCaptureStatusNone) return nullptr;
-    made[device.index()] = true;
-  }
-  *keep = device_status(device);
-  return keep->data_ptr<int32_t>();
 }
 
 b200tbe_paged_cache paged_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table, const Tensor& lengths) {
