@@ -453,7 +453,8 @@ typedef struct {
   size_t scratch_bytes;
 } b200tbe_attention_backward_params;
 
-B200TBE_API size_t b200tbe_jagged_attention_backward_scratch_bytes(int64_t total_q, int32_t heads);
+B200TBE_API size_t b200tbe_jagged_attention_backward_scratch_bytes(int64_t total_q, int64_t total_k, int32_t batch,
+                                                                    int32_t heads);
 B200TBE_API int b200tbe_jagged_attention_backward(const b200tbe_attention_backward_params* p,
                                                   b200tbe_stream_t stream);
 

@@ -60,10 +60,10 @@ def test_attention_backward_refuses():
     assert status(lse=None) == BAD_ARG
     assert status(scratch=None) == SCRATCH
     assert status(scratch=AT + 8) == SCRATCH
-    need = lib.b200tbe_jagged_attention_backward_scratch_bytes(10, 4)
+    need = lib.b200tbe_jagged_attention_backward_scratch_bytes(10, 10, 1, 4)
     assert need >= 10 * 4 * 4
     assert status(scratch_bytes=need - 1) == SCRATCH
-    assert lib.b200tbe_jagged_attention_backward_scratch_bytes(0, 4) == 0
+    assert lib.b200tbe_jagged_attention_backward_scratch_bytes(10, 10, 1, 0) == 0
 
 
 def test_nothing_to_do():

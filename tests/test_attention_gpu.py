@@ -367,7 +367,7 @@ def test_c_abi_with_strided_output():
     b.grad_out_stride, b.grad_out_head_stride = H * D, D
     b.grad_q_stride = b.grad_k_stride = b.grad_v_stride = 4 * H * D
     b.grad_q_head_stride = b.grad_k_head_stride = b.grad_v_head_stride = D
-    need = cabi.lib().b200tbe_jagged_attention_backward_scratch_bytes(n, H)
+    need = cabi.lib().b200tbe_jagged_attention_backward_scratch_bytes(n, n, 2, H)
     scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
     b.scratch, b.scratch_bytes = scratch.data_ptr(), need - 1
     assert cabi.lib().b200tbe_jagged_attention_backward(ctypes.byref(b), stream) == -2

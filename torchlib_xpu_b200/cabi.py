@@ -200,7 +200,7 @@ def lib() -> ctypes.CDLL:
             ctypes.POINTER(JaggedShape), _c_void_p, _c_void_p, _c_void_p, _c_void_p]
         i64, i32 = ctypes.c_int64, ctypes.c_int32
         _lib.b200tbe_jagged_attention.argtypes = [ctypes.POINTER(AttentionParams), _c_void_p]
-        _lib.b200tbe_jagged_attention_backward_scratch_bytes.argtypes = [i64, i32]
+        _lib.b200tbe_jagged_attention_backward_scratch_bytes.argtypes = [i64, i64, i32, i32]
         _lib.b200tbe_jagged_attention_backward_scratch_bytes.restype = ctypes.c_size_t
         _lib.b200tbe_jagged_attention_backward.argtypes = [ctypes.POINTER(AttentionBackwardParams), _c_void_p]
         _lib.b200tbe_paged_cache_append.argtypes = [

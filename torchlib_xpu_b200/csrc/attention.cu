@@ -51,9 +51,31 @@ extern "C" int b200tbe_jagged_attention(const b200tbe_attention_params* p, b200t
   return attention_forward_simt(d, p->dtype, stream);
 }
 
-extern "C" size_t b200tbe_jagged_attention_backward_scratch_bytes(int64_t total_q, int32_t heads) {
-  if (total_q <= 0 || heads <= 0) return 0;
-  return static_cast<size_t>(total_q) * heads * sizeof(float);
+namespace {
+
+size_t rounded(size_t n) { return (n + 15) / 16 * 16; }
+
+// delta, then the tickets and counts, then the two lists
+struct BackwardScratch {
+  size_t delta, words, q_tiles, k_tiles;
+  size_t total() const { return delta + words + q_tiles + k_tiles; }
+};
+
+BackwardScratch scratch_of(int64_t total_q, int64_t total_k, int64_t batch, int64_t heads) {
+  BackwardScratch s;
+  s.delta = rounded(static_cast<size_t>(total_q) * heads * sizeof(float));
+  s.words = 16;
+  s.q_tiles = rounded(static_cast<size_t>(tile_slots<128>(total_q, batch)) * sizeof(int2));
+  s.k_tiles = rounded(static_cast<size_t>(tile_slots<128>(total_k, batch)) * sizeof(int2));
+  return s;
+}
+
+}  // namespace
+
+extern "C" size_t b200tbe_jagged_attention_backward_scratch_bytes(int64_t total_q, int64_t total_k, int32_t batch,
+                                                                  int32_t heads) {
+  if (total_q < 0 || total_k < 0 || batch < 0 || heads <= 0) return 0;
+  return scratch_of(total_q, total_k, batch, heads).total();
 }
 
 extern "C" int b200tbe_jagged_attention_backward(const b200tbe_attention_backward_params* p, b200tbe_stream_t stream_) {
@@ -63,14 +85,27 @@ extern "C" int b200tbe_jagged_attention_backward(const b200tbe_attention_backwar
   if (st != B200TBE_OK) return st;
   if (f->total_q > 0 && (p->grad_out == nullptr || f->lse == nullptr || p->grad_q == nullptr)) return B200TBE_ERR_BAD_ARG;
   if (f->total_k > 0 && (p->grad_k == nullptr || p->grad_v == nullptr)) return B200TBE_ERR_BAD_ARG;
-  const size_t need = b200tbe_jagged_attention_backward_scratch_bytes(f->total_q, f->heads);
-  if (need > 0 && (p->scratch == nullptr || p->scratch_bytes < need || !aligned_to(p->scratch, 16))) return B200TBE_ERR_SCRATCH;
+  const BackwardScratch s = scratch_of(f->total_q, f->total_k, f->batch, f->heads);
+  if (p->scratch == nullptr || p->scratch_bytes < s.total() || !aligned_to(p->scratch, 16)) return B200TBE_ERR_SCRATCH;
+  if (f->total_q == 0 && f->total_k == 0) return B200TBE_OK;
   AttnDev d = device_params(f);
   d.grad = p->grad_out, d.dq = p->grad_q, d.dk = p->grad_k, d.dv = p->grad_v, d.delta = static_cast<float*>(p->scratch);
   d.g_row = p->grad_out_stride, d.g_head = p->grad_out_head_stride, d.dq_row = p->grad_q_stride, d.dq_head = p->grad_q_head_stride;
   d.dk_row = p->grad_k_stride, d.dk_head = p->grad_k_head_stride, d.dv_row = p->grad_v_stride, d.dv_head = p->grad_v_head_stride;
+  char* at = static_cast<char*>(p->scratch) + s.delta;
+  BackwardPlan plan;
+  plan.tickets = reinterpret_cast<int32_t*>(at);
+  plan.counts = plan.tickets + 2;
+  plan.q_tiles = reinterpret_cast<int2*>(at + s.words);
+  plan.k_tiles = reinterpret_cast<int2*>(at + s.words + s.q_tiles);
+  plan.q_room = static_cast<int32_t>(tile_slots<128>(f->total_q, f->batch));
+  plan.k_room = static_cast<int32_t>(tile_slots<128>(f->total_k, f->batch));
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  st = attention_delta(d, f->dtype, stream);
+  st = attention_delta(d, plan, f->dtype, stream);
   if (st != B200TBE_OK) return st;
+  if (attention_backward_fits(d, f->dtype)) {
+    const int tc = attention_backward_tc(d, plan, f->dtype, f->status, stream);
+    if (tc != B200TBE_ERR_UNSUPPORTED) return tc;
+  }
   return attention_backward_simt(d, f->dtype, stream);
 }

@@ -28,13 +28,25 @@ struct AttnDev {
   int64_t g_row, g_head, dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
 };
 
+// The tiles of 128 rows of a backward pass, as the delta kernel lists them in the caller's scratch: (stretch,
+// tile inside it), of queries and of keys. The tickets say how many of them (times heads) are taken.
+struct BackwardPlan {
+  int32_t* tickets;   // [2]
+  int32_t* counts;    // [2]
+  int2* q_tiles;
+  int2* k_tiles;
+  int32_t q_room, k_room;
+};
+
 int attention_forward_simt(const AttnDev& p, int dtype, cudaStream_t stream);
 int attention_backward_simt(const AttnDev& p, int dtype, cudaStream_t stream);
 // Tensor-core kernels: whether they take these arguments, and the launches. B200TBE_ERR_UNSUPPORTED from a
 // launch (nothing was enqueued): the driver made no tensor map of them, the 32-bit kernels take over.
 bool attention_forward_fits(const AttnDev& p, int dtype);
 int attention_forward_tc(const AttnDev& p, int dtype, int32_t* status, cudaStream_t stream);
-int attention_delta(const AttnDev& p, int dtype, cudaStream_t stream);
+bool attention_backward_fits(const AttnDev& p, int dtype);
+int attention_backward_tc(const AttnDev& p, const BackwardPlan& plan, int dtype, int32_t* status, cudaStream_t stream);
+int attention_delta(const AttnDev& p, const BackwardPlan& plan, int dtype, cudaStream_t stream);
 
 // One sequence's rows on both sides, or a stretch of rows that no sequence owns (klen 0).
 struct SeqRange {

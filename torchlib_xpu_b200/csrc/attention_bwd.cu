@@ -1,0 +1,621 @@
+// Gradients of the jagged attention on the tensor cores: fp16 and bf16, head dimensions that are multiples of 8
+// up to 128.
+//
+//   P = exp2(c S - lse log2 e),  dP = dO v^T,  dS = P (dP - delta),  c = scale log2 e
+//   dQ = scale dS k                     (a CTA walks the keys of 128 queries)
+//   dV = P^T dO,  dK = scale dS^T q     (a CTA walks the queries of 128 keys, of all heads that share them)
+//
+// Two kernels, so that no sum crosses a CTA and the results do not depend on scheduling: S and dP are computed
+// twice (7 products instead of 5), and nothing is added in memory. Scores and dP come into tensor memory
+// with a row for each thread pair; two warpgroups take half of the columns each; P and dS go back into tensor
+// memory, rounded to the operands' type, as the left operand of the next product. P and dS are rounded because
+// the tensor cores multiply 16-bit operands; they are summed in fp32.
+// The CTAs take the tiles of a list that the delta kernel leaves, one after the other.
+#include "attention.cuh"
+#include "tcgen05.cuh"
+
+namespace b200tbe {
+namespace {
+
+constexpr int kRows = 128;   // queries of a tile, keys of a tile
+constexpr int kThreads = 384;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct BwdDev {
+  AttnDev a;
+  BackwardPlan plan;
+  int32_t* status;
+};
+
+template <int kDP>
+struct Layout {
+  static constexpr int kTileBytes = kRows * kDP * 2;
+  static constexpr int kSmem = 6 * kTileBytes + 1024;   // two tiles that stay, two stages of two that come
+  static constexpr int kBuffers = kDP == 64 ? 2 : 1;    // of the keys' kernel: tensor memory for scores ahead
+};
+
+struct DqBarriers {
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], dp_full, loaded, ds_full, done;
+};
+struct DkvBarriers {
+  uint64_t kv_full, q_full[2], q_empty[2], s_full[2], dp_full, loaded, p_full, ds_full, stat_full[2], stat_empty[2], done;
+};
+
+// What a tile's CTA knows.
+struct Item {
+  int64_t begin, other;
+  int first, len, other_len, head;
+};
+
+// The next tile of the list: one thread takes a ticket for the CTA. false: none are left.
+template <int kHeadsOf>   // 0: tiles of queries, 1: of keys
+__device__ __forceinline__ bool next_item(const BwdDev& p, int* ticket, Item* item) {
+  const AttnDev& a = p.a;
+  if (threadIdx.x == 0) *ticket = atomicAdd(p.plan.tickets + kHeadsOf, 1);
+  __syncthreads();
+  const int heads = kHeadsOf == 0 ? a.heads : a.kv_heads;
+  const int t = *ticket;
+  if (t / heads >= p.plan.counts[kHeadsOf]) return false;
+  const int2 at = (kHeadsOf == 0 ? p.plan.q_tiles : p.plan.k_tiles)[t / heads];
+  item->head = t % heads;
+  item->first = at.y * kRows;
+  const void* mine = kHeadsOf == 0 ? a.q_offsets : a.k_offsets;
+  const void* others = kHeadsOf == 0 ? a.k_offsets : a.q_offsets;
+  const int64_t total = kHeadsOf == 0 ? a.total_q : a.total_k;
+  item->begin = stretch_bound(mine, a.offset_bytes, a.batch, total, at.x);
+  item->len = static_cast<int>(stretch_bound(mine, a.offset_bytes, a.batch, total, at.x + 1) - item->begin);
+  other_rows(others, a.offset_bytes, a.batch, kHeadsOf == 0 ? a.total_k : a.total_q, at.x, &item->other, &item->other_len);
+  return true;
+}
+
+// Zero rows [rows, next multiple of 16) of a tile in shared memory: rows of other sequences, which a zero weight
+// would not cancel if they held NaN. By a whole warp.
+template <int kDP>
+__device__ __forceinline__ void zero_tail(uint8_t* tile, int rows) {
+  const int count = (16 - rows % 16) % 16;
+  for (int i = threadIdx.x % 32; i < count * (kDP / 64) * 8; i += 32) {
+    const int x = i / (count * 8), rest = i % (count * 8);
+    *reinterpret_cast<uint4*>(tile + x * kRows * 128 + rows * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_async_smem();
+  __syncwarp();
+}
+
+template <int kDP>
+__device__ __forceinline__ void load_tile(uint8_t* tile, const CUtensorMap* map, int head, int row, uint64_t* bar) {
+  for (int x = 0; x < kDP / 64; ++x) tma_load_3d(tile + x * kRows * 128, map, x * 64, head, row, bar);
+}
+
+// d[128][n] (+)= a b^T over the head dimension, both operands rows of it
+__device__ __forceinline__ void product_over_d(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, int steps) {
+  for (int t = 0; t < steps; ++t) {
+    const uint32_t off = (t / 4) * kRows * 128 + (t % 4) * 32;
+    mma_ss(d, smem_desc(a + off, 16), smem_desc(b + off, 16), desc, t > 0);
+  }
+}
+
+// d[128][D] (+)= w x: w in tensor memory (two 16-bit weights a column), x rows of the head dimension
+__device__ __forceinline__ void product_over_rows(uint32_t d, uint32_t w, uint32_t x, uint32_t desc, int steps, bool add) {
+  for (int t = 0; t < steps; ++t) mma_ts(d, w + t * 8, smem_desc(x + t * 2048, kRows * 128), desc, add || t > 0);
+}
+
+// A row of the accumulator in tensor memory, times f, to memory.
+template <bool kBf16, int kDP>
+__device__ __forceinline__ void store_row(void* out, uint32_t at, int D, float f, bool computed, bool inside) {
+#pragma unroll 1
+  for (int i = 0; i < kDP / 32; ++i) {
+    uint32_t o[32];
+    if (computed) {
+      tmem_ld32(o, at + i * 32);
+      tmem_wait_ld();
+    }
+    if (inside) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        if (i * 32 + e < D) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (computed) {
+            v.x = pack2<kBf16>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f);
+            v.y = pack2<kBf16>(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
+            v.z = pack2<kBf16>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f);
+            v.w = pack2<kBf16>(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f);
+          }
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + i * 32 + e) = v;
+        }
+      }
+    }
+  }
+}
+
+// After a wait gave up: report it, and let what is in flight land before its memory is given back.
+__device__ __forceinline__ void report(const int* dead, int32_t* status) {
+  if (*dead) {
+    if (threadIdx.x == 0 && status != nullptr) atomicOr(status, B200TBE_DEV_WAIT_TIMEOUT);
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  }
+}
+
+// Tensor memory: scores in two buffers (dS takes the place of the scores it comes from), dP, dQ.
+template <bool kBf16, int kDP>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_dq_kernel(const BwdDev p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                        const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap g_map) {
+  using L = Layout<kDP>;
+  extern __shared__ uint8_t raw[];
+  __shared__ DqBarriers bars;
+  __shared__ uint32_t tmem_base;
+  __shared__ int dead_word, ticket;
+  const AttnDev& a = p.a;
+  uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* gs = qs + L::kTileBytes;
+  uint8_t* ks = gs + L::kTileBytes;
+  uint8_t* vs = ks + 2 * L::kTileBytes;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) dead_word = 0;
+  if (warp == 8) tmem_alloc(&tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base, dp_at = tmem + 256, dq_at = tmem + 384;
+  volatile int* dead = &dead_word;
+
+  Item it;
+  if (warp >= 8) {
+    give_registers<80>();
+    while (!*dead && next_item<0>(p, &ticket, &it)) {
+      const int kv = it.head / a.group, shift = it.other_len - it.len, klen = it.other_len;
+      const int sees = a.causal ? min(klen, min(it.len, it.first + kRows) + shift) : klen;
+      const int n = sees > 0 ? (sees + kRows - 1) / kRows : 0;
+      __syncthreads();   // the barriers are set up
+      if (warp == 9) {
+        // ---- copies ----
+        if (lane == 0 && n > 0) {
+          mbar_expect(&bars.q_full, 2 * L::kTileBytes);
+          load_tile<kDP>(qs, &q_map, it.head, static_cast<int>(it.begin) + it.first, &bars.q_full);
+          load_tile<kDP>(gs, &g_map, it.head, static_cast<int>(it.begin) + it.first, &bars.q_full);
+          for (int j = 0; j < n; ++j) {
+            const int st = j & 1, row = static_cast<int>(it.other) + j * kRows;
+            const uint32_t before = (j / 2 - 1) & 1;
+            if (j >= 2 && !mbar_wait(&bars.k_empty[st], before, dead)) break;
+            mbar_expect(&bars.k_full[st], L::kTileBytes);
+            load_tile<kDP>(ks + st * L::kTileBytes, &k_map, kv, row, &bars.k_full[st]);
+            if (j >= 2 && !mbar_wait(&bars.v_empty[st], before, dead)) break;
+            mbar_expect(&bars.v_full[st], L::kTileBytes);
+            load_tile<kDP>(vs + st * L::kTileBytes, &v_map, kv, row, &bars.v_full[st]);
+          }
+        }
+      } else if (warp == 8 && n > 0) {
+        // ---- matrix instructions ----
+        const int d_steps = (a.D + 15) / 16;
+        const uint32_t q_at = smem_addr(qs), g_at = smem_addr(gs);
+        const uint32_t dq_desc = mma_desc(kBf16, kRows, (a.D + 15) & ~15, false, true);
+        auto keys_of = [&](int j) { return min(kRows, klen - j * kRows); };
+        auto scores = [&](int j) {   // whole warp
+          const bool ok = warp_wait(&bars.k_full[j & 1], (j / 2) & 1, dead);
+          if (!ok) return false;
+          const int keys = keys_of(j);
+          if (keys % 16 != 0) zero_tail<kDP>(ks + (j & 1) * L::kTileBytes, keys);
+          if (lane == 0) {
+            product_over_d(tmem + (j & 1) * kRows, q_at, smem_addr(ks + (j & 1) * L::kTileBytes),
+                           mma_desc(kBf16, kRows, (keys + 15) & ~15, false, false), d_steps);
+            mma_commit(&bars.s_full[j & 1]);
+          }
+          __syncwarp();
+          return true;
+        };
+        auto d_weights = [&](int j) {
+          const bool ok = warp_wait(&bars.v_full[j & 1], (j / 2) & 1, dead);
+          if (!ok) return false;
+          if (lane == 0) {
+            product_over_d(dp_at, g_at, smem_addr(vs + (j & 1) * L::kTileBytes),
+                           mma_desc(kBf16, kRows, (keys_of(j) + 15) & ~15, false, false), d_steps);
+            mma_commit(&bars.dp_full);
+            if (j + 2 < n) mma_commit(&bars.v_empty[j & 1]);
+          }
+          __syncwarp();
+          return true;
+        };
+        bool alive = warp_wait(&bars.q_full, 0, dead) && scores(0) && d_weights(0);
+        for (int j = 0; alive && j < n; ++j) {
+          if (j + 1 < n) {
+            alive = scores(j + 1) && warp_wait(&bars.loaded, j & 1, dead);
+            tc_fence_after();
+            alive = alive && d_weights(j + 1);
+          }
+          alive = alive && warp_wait(&bars.ds_full, j & 1, dead);
+          tc_fence_after();
+          if (alive && lane == 0) {
+            product_over_rows(dq_at, tmem + (j & 1) * kRows, smem_addr(ks + (j & 1) * L::kTileBytes), dq_desc,
+                              (keys_of(j) + 15) / 16, j > 0);
+            if (j + 2 < n) mma_commit(&bars.k_empty[j & 1]);
+            if (j + 1 == n) mma_commit(&bars.done);
+          }
+          __syncwarp();
+        }
+      }
+      __syncthreads();
+      tc_fence_after();
+    }
+  } else {
+    take_registers<208>();
+    for (bool fresh = true; !*dead && next_item<0>(p, &ticket, &it); fresh = false) {
+      const int shift = it.other_len - it.len, klen = it.other_len;
+      const int sees = a.causal ? min(klen, min(it.len, it.first + kRows) + shift) : klen;
+      const int n = sees > 0 ? (sees + kRows - 1) / kRows : 0;
+      if (threadIdx.x == 0) {
+        if (!fresh) mbar_forget(&bars);
+        mbar_init(&bars.q_full, 1);
+        for (int i = 0; i < 2; ++i) {
+          mbar_init(&bars.k_full[i], 1);
+          mbar_init(&bars.k_empty[i], 1);
+          mbar_init(&bars.v_full[i], 1);
+          mbar_init(&bars.v_empty[i], 1);
+          mbar_init(&bars.s_full[i], 1);
+        }
+        mbar_init(&bars.dp_full, 1);
+        mbar_init(&bars.loaded, 256);
+        mbar_init(&bars.ds_full, 256);
+        mbar_init(&bars.done, 1);
+        fence_barrier_init();
+      }
+      __syncthreads();
+      // ---- weights: a row and half of the columns a thread ----
+      const int half = warp / 4, local = (warp % 4) * 32 + lane, row = it.first + local;
+      const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+      const int limit = row >= it.len ? 0 : (a.causal ? min(klen, row + shift + 1) : klen);
+      float lse2 = 0.f, delta = 0.f;
+      if (row < it.len) {
+        lse2 = a.lse[it.head * a.total_q + it.begin + row] * kLog2e;
+        delta = a.delta[it.head * a.total_q + it.begin + row];
+        if (lse2 == -INFINITY) lse2 = INFINITY;
+      }
+      const float c = a.scale * kLog2e;
+      bool alive = true;
+      for (int j = 0; j < n; ++j) {
+        alive = warp_wait(&bars.s_full[j & 1], (j / 2) & 1, dead) && warp_wait(&bars.dp_full, j & 1, dead);
+        if (!alive) break;
+        tc_fence_after();
+        const uint32_t s_at = tmem + lanes + (j & 1) * kRows;
+        const int chunks = max(0, min(2, (klen - j * kRows - half * 64 + 31) / 32));
+        const int left = limit - j * kRows - half * 64;
+        uint32_t s[2][32], dp[2][32];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (i < chunks) {
+            tmem_ld32(s[i], s_at + half * 64 + i * 32);
+            tmem_ld32(dp[i], dp_at + lanes + half * 64 + i * 32);
+          }
+        tmem_wait_ld();
+        tc_fence_before();
+        mbar_arrive(&bars.loaded);
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (i < chunks) {
+            const bool cut = __any_sync(kFullMask, left < i * 32 + 32);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float d0 = fast_exp2(fmaf(__uint_as_float(s[i][e]), c, -lse2)) * (__uint_as_float(dp[i][e]) - delta);
+              float d1 = fast_exp2(fmaf(__uint_as_float(s[i][e + 1]), c, -lse2)) * (__uint_as_float(dp[i][e + 1]) - delta);
+              if (cut) {
+                d0 = i * 32 + e < left ? d0 : 0.f;
+                d1 = i * 32 + e + 1 < left ? d1 : 0.f;
+              }
+              w[i * 16 + e / 2] = pack2<kBf16>(d0, d1);
+            }
+          }
+        // the other warpgroup's scores are overwritten: it has to have them
+        alive = warp_wait(&bars.loaded, j & 1, dead);
+        if (!alive) break;
+        tc_fence_after();
+        if (chunks > 0) tmem_st32(s_at + half * 32, w);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bars.ds_full);
+      }
+      if (alive && n > 0) alive = warp_wait(&bars.done, 0, dead);
+      tc_fence_after();
+      if (half == 0)
+        store_row<kBf16, kDP>(static_cast<uint16_t*>(a.dq) + (it.begin + row) * a.dq_row + it.head * a.dq_head, dq_at + lanes,
+                              a.D, a.scale, alive && n > 0, row < it.len);
+      tc_fence_before();
+      __syncthreads();
+      tc_fence_after();
+    }
+  }
+  report(&dead_word, p.status);
+  __syncthreads();
+  if (warp == 8) tmem_free(tmem, 512);
+}
+
+// Tensor memory: scores (transposed: a key a row) in one buffer or two, dP, dV, dK. P takes the place of the
+// first half of the scores' columns, dS of the second.
+template <bool kBf16, int kDP>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_dkv_kernel(const BwdDev p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                         const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap g_map) {
+  using L = Layout<kDP>;
+  constexpr int kB = L::kBuffers;
+  extern __shared__ uint8_t raw[];
+  __shared__ DkvBarriers bars;
+  __shared__ uint32_t tmem_base;
+  __shared__ int dead_word, ticket;
+  __shared__ __align__(16) float stats[2][2][kRows];   // [stage][lse log2 e, delta][query]
+  const AttnDev& a = p.a;
+  uint8_t* ks = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* vs = ks + L::kTileBytes;
+  uint8_t* qs = vs + L::kTileBytes;
+  uint8_t* gs = qs + 2 * L::kTileBytes;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) dead_word = 0;
+  if (warp == 8) tmem_alloc(&tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base, dp_at = tmem + kB * kRows, dv_at = dp_at + kRows, dk_at = dv_at + kDP;
+  volatile int* dead = &dead_word;
+
+  Item it;
+  if (warp >= 8) {
+    give_registers<80>();
+    while (!*dead && next_item<1>(p, &ticket, &it)) {
+      const int shift = it.len - it.other_len, qlen = it.other_len, head0 = it.head * a.group;
+      const int from = a.causal ? max(0, it.first - shift) / kRows : 0;   // first tile with a query that sees a key of this one
+      const int per_head = max(0, (qlen + kRows - 1) / kRows - from), n = per_head * a.group;
+      __syncthreads();   // the barriers are set up
+      if (warp == 9) {
+        // ---- copies ----
+        if (lane == 0 && n > 0) {
+          mbar_expect(&bars.kv_full, 2 * L::kTileBytes);
+          load_tile<kDP>(ks, &k_map, it.head, static_cast<int>(it.begin) + it.first, &bars.kv_full);
+          load_tile<kDP>(vs, &v_map, it.head, static_cast<int>(it.begin) + it.first, &bars.kv_full);
+          for (int j = 0; j < n; ++j) {
+            const int st = j & 1, row = static_cast<int>(it.other) + (from + j % per_head) * kRows, head = head0 + j / per_head;
+            if (j >= 2 && !mbar_wait(&bars.q_empty[st], (j / 2 - 1) & 1, dead)) break;
+            mbar_expect(&bars.q_full[st], 2 * L::kTileBytes);
+            load_tile<kDP>(qs + st * L::kTileBytes, &q_map, head, row, &bars.q_full[st]);
+            load_tile<kDP>(gs + st * L::kTileBytes, &g_map, head, row, &bars.q_full[st]);
+          }
+        }
+      } else if (warp == 10) {
+        // ---- the queries' log-sums and deltas ----
+        for (int j = 0; j < n; ++j) {
+          const int st = j & 1, i0 = (from + j % per_head) * kRows, head = head0 + j / per_head;
+          if (j >= 2 && !warp_wait(&bars.stat_empty[st], (j / 2 - 1) & 1, dead)) break;
+          for (int e = lane; e < kRows; e += 32) {
+            const bool in = i0 + e < qlen;
+            const int64_t at = head * a.total_q + it.other + i0 + e;
+            const float lse2 = in ? a.lse[at] * kLog2e : INFINITY;
+            stats[st][0][e] = lse2 == -INFINITY ? INFINITY : lse2;
+            stats[st][1][e] = in ? a.delta[at] : 0.f;
+          }
+          mbar_arrive(&bars.stat_full[st]);
+        }
+      } else if (warp == 8 && n > 0) {
+        // ---- matrix instructions ----
+        const int d_steps = (a.D + 15) / 16;
+        const uint32_t k_at = smem_addr(ks), v_at = smem_addr(vs);
+        const uint32_t out_desc = mma_desc(kBf16, kRows, (a.D + 15) & ~15, false, true);
+        auto rows_of = [&](int j) { return min(kRows, qlen - (from + j % per_head) * kRows); };
+        auto ready = [&](int j) {
+          const bool ok = warp_wait(&bars.q_full[j & 1], (j / 2) & 1, dead);
+          if (ok && rows_of(j) % 16 != 0) {
+            zero_tail<kDP>(qs + (j & 1) * L::kTileBytes, rows_of(j));
+            zero_tail<kDP>(gs + (j & 1) * L::kTileBytes, rows_of(j));
+          }
+          return ok;
+        };
+        auto scores = [&](int j) {
+          if (lane == 0) {
+            product_over_d(tmem + (j % kB) * kRows, k_at, smem_addr(qs + (j & 1) * L::kTileBytes),
+                           mma_desc(kBf16, kRows, (rows_of(j) + 15) & ~15, false, false), d_steps);
+            mma_commit(&bars.s_full[j % kB]);
+          }
+          __syncwarp();
+        };
+        auto d_weights = [&](int j) {
+          if (lane == 0) {
+            product_over_d(dp_at, v_at, smem_addr(gs + (j & 1) * L::kTileBytes),
+                           mma_desc(kBf16, kRows, (rows_of(j) + 15) & ~15, false, false), d_steps);
+            mma_commit(&bars.dp_full);
+          }
+          __syncwarp();
+        };
+        bool alive = warp_wait(&bars.kv_full, 0, dead) && ready(0);
+        if (alive) {
+          scores(0);
+          d_weights(0);
+        }
+        for (int j = 0; alive && j < n; ++j) {
+          const bool more = j + 1 < n;
+          const uint32_t s_at = tmem + (j % kB) * kRows;
+          const int steps = (rows_of(j) + 15) / 16;
+          if (more) {
+            alive = ready(j + 1);
+            if (!alive) break;
+            if (kB == 2) scores(j + 1);
+            alive = warp_wait(&bars.loaded, j & 1, dead);
+            if (!alive) break;
+            tc_fence_after();
+            d_weights(j + 1);
+          }
+          alive = warp_wait(&bars.p_full, j & 1, dead);
+          if (!alive) break;
+          tc_fence_after();
+          if (lane == 0) product_over_rows(dv_at, s_at, smem_addr(gs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
+          __syncwarp();
+          alive = warp_wait(&bars.ds_full, j & 1, dead);
+          if (!alive) break;
+          tc_fence_after();
+          if (lane == 0) {
+            product_over_rows(dk_at, s_at + 64, smem_addr(qs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
+            if (j + 2 < n) mma_commit(&bars.q_empty[j & 1]);
+            if (!more) mma_commit(&bars.done);
+          }
+          __syncwarp();
+          if (kB == 1 && more) scores(j + 1);
+        }
+      }
+      __syncthreads();
+      tc_fence_after();
+    }
+  } else {
+    take_registers<208>();
+    for (bool fresh = true; !*dead && next_item<1>(p, &ticket, &it); fresh = false) {
+      const int shift = it.len - it.other_len, qlen = it.other_len;
+      const int from = a.causal ? max(0, it.first - shift) / kRows : 0;   // first tile with a query that sees a key of this one
+      const int per_head = max(0, (qlen + kRows - 1) / kRows - from), n = per_head * a.group;
+      if (threadIdx.x == 0) {
+        if (!fresh) mbar_forget(&bars);
+        mbar_init(&bars.kv_full, 1);
+        for (int i = 0; i < 2; ++i) {
+          mbar_init(&bars.q_full[i], 1);
+          mbar_init(&bars.q_empty[i], 1);
+          mbar_init(&bars.s_full[i], 1);
+          mbar_init(&bars.stat_full[i], 32);
+          mbar_init(&bars.stat_empty[i], 256);
+        }
+        mbar_init(&bars.dp_full, 1);
+        mbar_init(&bars.loaded, 256);
+        mbar_init(&bars.p_full, 256);
+        mbar_init(&bars.ds_full, 256);
+        mbar_init(&bars.done, 1);
+        fence_barrier_init();
+      }
+      __syncthreads();
+      // ---- weights: a key and half of the queries a thread ----
+      const int half = warp / 4, local = (warp % 4) * 32 + lane, key = it.first + local;
+      const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+      const float c = a.scale * kLog2e;
+      bool alive = true;
+      for (int j = 0; j < n; ++j) {
+        const int st = j & 1, i0 = (from + j % per_head) * kRows + half * 64;
+        alive = warp_wait(&bars.stat_full[st], (j / 2) & 1, dead) && warp_wait(&bars.s_full[j % kB], (j / kB) & 1, dead) &&
+                warp_wait(&bars.dp_full, j & 1, dead);
+        if (!alive) break;
+        tc_fence_after();
+        const uint32_t s_at = tmem + lanes + (j % kB) * kRows;
+        const int chunks = max(0, min(2, (qlen - i0 + 31) / 32));
+        // columns [low, high) are queries of the sequence that see the key
+        const int low = a.causal ? key - shift - i0 : 0, high = qlen - i0;
+        uint32_t s[2][32], dp[2][32];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (i < chunks) {
+            tmem_ld32(s[i], s_at + half * 64 + i * 32);
+            tmem_ld32(dp[i], dp_at + lanes + half * 64 + i * 32);
+          }
+        tmem_wait_ld();
+        tc_fence_before();
+        mbar_arrive(&bars.loaded);
+        const bool cut = __any_sync(kFullMask, low > 0 || high < 64);
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (i < chunks) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 m = *reinterpret_cast<const float4*>(&stats[st][0][half * 64 + i * 32 + e]);
+              float x[4] = {fmaf(__uint_as_float(s[i][e]), c, -m.x), fmaf(__uint_as_float(s[i][e + 1]), c, -m.y),
+                            fmaf(__uint_as_float(s[i][e + 2]), c, -m.z), fmaf(__uint_as_float(s[i][e + 3]), c, -m.w)};
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                x[u] = fast_exp2(x[u]);
+                if (cut && (i * 32 + e + u < low || i * 32 + e + u >= high)) x[u] = 0.f;
+                s[i][e + u] = __float_as_uint(x[u]);
+              }
+              w[i * 16 + e / 2] = pack2<kBf16>(x[0], x[1]);
+              w[i * 16 + e / 2 + 1] = pack2<kBf16>(x[2], x[3]);
+            }
+          }
+        // the other warpgroup's scores are overwritten: it has to have them
+        alive = warp_wait(&bars.loaded, j & 1, dead);
+        if (!alive) break;
+        tc_fence_after();
+        if (chunks > 0) tmem_st32(s_at + half * 32, w);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bars.p_full);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (i < chunks) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 d = *reinterpret_cast<const float4*>(&stats[st][1][half * 64 + i * 32 + e]);
+              float x[4] = {__uint_as_float(s[i][e]) * (__uint_as_float(dp[i][e]) - d.x),
+                            __uint_as_float(s[i][e + 1]) * (__uint_as_float(dp[i][e + 1]) - d.y),
+                            __uint_as_float(s[i][e + 2]) * (__uint_as_float(dp[i][e + 2]) - d.z),
+                            __uint_as_float(s[i][e + 3]) * (__uint_as_float(dp[i][e + 3]) - d.w)};
+              if (cut) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                  if (i * 32 + e + u < low || i * 32 + e + u >= high) x[u] = 0.f;
+              }
+              w[i * 16 + e / 2] = pack2<kBf16>(x[0], x[1]);
+              w[i * 16 + e / 2 + 1] = pack2<kBf16>(x[2], x[3]);
+            }
+          }
+        if (chunks > 0) tmem_st32(s_at + 64 + half * 32, w);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bars.ds_full);
+        mbar_arrive(&bars.stat_empty[st]);
+      }
+      if (alive && n > 0) alive = warp_wait(&bars.done, 0, dead);
+      tc_fence_after();
+      if (half == 0)
+        store_row<kBf16, kDP>(static_cast<uint16_t*>(a.dv) + (it.begin + key) * a.dv_row + it.head * a.dv_head, dv_at + lanes,
+                              a.D, 1.f, alive && n > 0, key < it.len);
+      else
+        store_row<kBf16, kDP>(static_cast<uint16_t*>(a.dk) + (it.begin + key) * a.dk_row + it.head * a.dk_head, dk_at + lanes,
+                              a.D, a.scale, alive && n > 0, key < it.len);
+      tc_fence_before();
+      __syncthreads();
+      tc_fence_after();
+    }
+  }
+  report(&dead_word, p.status);
+  __syncthreads();
+  if (warp == 8) tmem_free(tmem, 512);
+}
+
+template <bool kBf16, int kDP>
+int launch(const BwdDev& p, cudaStream_t stream) {
+  using L = Layout<kDP>;
+  const AttnDev& a = p.a;
+  CUtensorMap q, k, v, g;
+  if (!rows_map(&q, kBf16, a.q, a.total_q, a.heads, a.D, a.q_row, a.q_head, kRows) ||
+      !rows_map(&k, kBf16, a.k, a.total_k, a.kv_heads, a.D, a.k_row, a.k_head, kRows) ||
+      !rows_map(&v, kBf16, a.v, a.total_k, a.kv_heads, a.D, a.v_row, a.v_head, kRows) ||
+      !rows_map(&g, kBf16, a.grad, a.total_q, a.heads, a.D, a.g_row, a.g_head, kRows))
+    return B200TBE_ERR_UNSUPPORTED;
+  const int64_t q_tiles = tile_slots<kRows>(a.total_q, a.batch) * a.heads;
+  const int64_t k_tiles = tile_slots<kRows>(a.total_k, a.batch) * a.kv_heads;
+  if (q_tiles > 0x7fffff00 || k_tiles > 0x7fffff00) return B200TBE_ERR_UNSUPPORTED;   // tickets are 32-bit
+  const auto dq = attention_dq_kernel<kBf16, kDP>;
+  const auto dkv = attention_dkv_kernel<kBf16, kDP>;
+  if (cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess ||
+      cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess)
+    return B200TBE_ERR_LAUNCH;
+  dkv<<<static_cast<unsigned>(k_tiles < kNumSMs ? k_tiles : kNumSMs), kThreads, L::kSmem, stream>>>(p, q, k, v, g);
+  const int st = launch_status();
+  if (st != B200TBE_OK) return st;
+  dq<<<static_cast<unsigned>(q_tiles < kNumSMs ? q_tiles : kNumSMs), kThreads, L::kSmem, stream>>>(p, q, k, v, g);
+  return launch_status();
+}
+
+}  // namespace
+
+bool attention_backward_fits(const AttnDev& a, int dtype) {
+  return attention_forward_fits(a, dtype) && a.total_q > 0 && mappable(a.grad, a.total_q, a.heads, a.g_row, a.g_head) &&
+         aligned_to(a.dq, 16) && aligned_to(a.dk, 16) && aligned_to(a.dv, 16) && a.dq_row % 8 == 0 && a.dq_head % 8 == 0 &&
+         a.dk_row % 8 == 0 && a.dk_head % 8 == 0 && a.dv_row % 8 == 0 && a.dv_head % 8 == 0;
+}
+
+int attention_backward_tc(const AttnDev& a, const BackwardPlan& plan, int dtype, int32_t* status, cudaStream_t stream) {
+  const BwdDev p{a, plan, status};
+  if (dtype == B200TBE_BF16) return a.D <= 64 ? launch<true, 64>(p, stream) : launch<true, 128>(p, stream);
+  return a.D <= 64 ? launch<false, 64>(p, stream) : launch<false, 128>(p, stream);
+}
+
+}  // namespace b200tbe

@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
 #pragma unroll
         for (int s = 0; s < kNQ; ++s)
           if (n[s] > 0) scores(s, 0);
-        mma_commit(&bars.k_empty[0]);
+        if (L::kStages < most) mma_commit(&bars.k_empty[0]);
       }
     }
     const uint32_t pv_desc = mma_desc(kBf16, kRows, (a.D + 15) & ~15, false, true);
@@ -188,8 +188,8 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
         }
       }
       if (alive && lane == 0) {
-        mma_commit(&bars.v_empty[st]);
-        if (j + 1 < most) mma_commit(&bars.k_empty[next]);
+        if (j + L::kStages < most) mma_commit(&bars.v_empty[st]);
+        if (j + 1 + L::kStages < most) mma_commit(&bars.k_empty[next]);
       }
       __syncwarp();
     }

@@ -179,21 +179,6 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const AttnDev p) {
   }
 }
 
-// delta[head][row] = sum over d of dO * O: one warp per row and head.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) delta_kernel(const AttnDev p) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + threadIdx.x / 32;
-  if (at >= p.total_q * p.heads) return;
-  const int64_t row = at / p.heads;
-  const int head = static_cast<int>(at % p.heads);
-  const T* g = static_cast<const T*>(p.grad) + row * p.g_row + head * p.g_head;
-  const T* o = static_cast<const T*>(p.out) + row * p.o_row + head * p.o_head;
-  float s = 0.f;
-  for (int d = threadIdx.x % 32; d < p.D; d += 32) s = fmaf(to_float<T>(g[d]), to_float<T>(o[d]), s);
-  s = warp_sum(s);
-  if (threadIdx.x % 32 == 0) p.delta[head * p.total_q + row] = s;
-}
-
 // P and dS of a tile (rows: ty, keys: tx) from its scores and dP. What lies past the lengths or behind the
 // mask is zero, whatever the rows there hold.
 template <int kDP>
@@ -373,27 +358,12 @@ int backward_of(const AttnDev& p, cudaStream_t stream) {
   return backward_as<T, 256>(p, stream);
 }
 
-template <typename T>
-int delta_of(const AttnDev& p, cudaStream_t stream) {
-  const int64_t blocks = (p.total_q * p.heads + kThreads / 32 - 1) / (kThreads / 32);
-  if (blocks > 0x7fffffff) return B200TBE_ERR_TOO_LARGE;
-  if (blocks == 0) return B200TBE_OK;
-  delta_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p);
-  return launch_status();
-}
-
 }  // namespace
 
 int attention_forward_simt(const AttnDev& p, int dtype, cudaStream_t stream) {
   if (dtype == B200TBE_FP32) return forward_of<float>(p, stream);
   if (dtype == B200TBE_FP16) return forward_of<__half>(p, stream);
   return forward_of<__nv_bfloat16>(p, stream);
-}
-
-int attention_delta(const AttnDev& p, int dtype, cudaStream_t stream) {
-  if (dtype == B200TBE_FP32) return delta_of<float>(p, stream);
-  if (dtype == B200TBE_FP16) return delta_of<__half>(p, stream);
-  return delta_of<__nv_bfloat16>(p, stream);
 }
 
 int attention_backward_simt(const AttnDev& p, int dtype, cudaStream_t stream) {

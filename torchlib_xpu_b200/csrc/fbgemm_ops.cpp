@@ -545,7 +545,9 @@ class JaggedAttentionFunction : public torch::autograd::Function<JaggedAttention
     Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
     const int32_t heads = static_cast<int32_t>(q.size(1));
     Tensor scratch = at::empty(
-        {static_cast<int64_t>(b200tbe_jagged_attention_backward_scratch_bytes(q.size(0), heads))}, q.options().dtype(at::kByte));
+        {static_cast<int64_t>(b200tbe_jagged_attention_backward_scratch_bytes(
+            q.size(0), k.size(0), static_cast<int32_t>(q_offsets.numel() - 1), heads))},
+        q.options().dtype(at::kByte));
     b200tbe_attention_backward_params p{};
     p.forward = attention_params(q, k, v, q_offsets, k_offsets, ctx->saved_data["causal"].toBool(),
                                  ctx->saved_data["scale"].toDouble(), out, lse);

@@ -14,6 +14,13 @@ __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
 }
 
+// Every barrier of a block of them: the memory may be initialised again.
+template <typename Barriers>
+__device__ __forceinline__ void mbar_forget(Barriers* bars) {
+  for (unsigned i = 0; i < sizeof(Barriers) / 8; ++i)
+    asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_addr(reinterpret_cast<uint64_t*>(bars) + i)) : "memory");
+}
+
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
@@ -154,7 +161,8 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "l"(b), "r"(desc), "r"(static_cast<uint32_t>(add))
       : "memory");
 }
-// arrives once all matrix instructions that this thread has issued are done
+// Arrives once all matrix instructions that this thread has issued are done. Some thread has to wait for it: an
+// arrival nobody waits for could come after the barrier's memory has been given to something else.
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
