@@ -1,5 +1,6 @@
 // The paged key-value cache: jagged rows appended to it, and the attention of one new token over it.
 #include "attention.cuh"
+#include "tcgen05.cuh"
 
 namespace b200tbe {
 namespace {
@@ -132,7 +133,7 @@ struct AnswerDev {
   void* out;
   int64_t q_row, q_head, o_row, o_head;
   int32_t heads, group, chunks, units;   // chunks of kHeads query heads a key head; units a sequence
-  float scale;
+  float scale_log2;   // scale log2 e: scores, maxima and log-sums are in powers of two
   Start* starts;     // [gridDim.x]
   float* stats;      // [2 * gridDim.x][kHeads][2]: m, l
   float* sums;       // [2 * gridDim.x][kHeads][D]
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(kAnswerThreads) answer_simt_kernel(const Answe
         const int t = i % kTile, h = i / kTile;
         float x = 0.f;
         for (int d = 0; d < D; ++d) x = fmaf(qs[h * D + d], ks[t * (D + 1) + d], x);
-        ps[h][t] = k_at[t] >= 0 ? x * p.scale : -INFINITY;
+        ps[h][t] = k_at[t] >= 0 ? x * p.scale_log2 : -INFINITY;
       }
       __syncthreads();
       for (int h = tid / 32; h < heads; h += kAnswerThreads / 32) {
@@ -250,12 +251,12 @@ __global__ void __launch_bounds__(kAnswerThreads) answer_simt_kernel(const Answe
 #pragma unroll
         for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, w));
         const float base = m == -INFINITY ? 0.f : m;
-        const float ea = expf(a - base), ec = expf(c - base);
+        const float ea = exp2f(a - base), ec = exp2f(c - base);
         ps[h][lane] = ea;
         ps[h][lane + 32] = ec;
         const float add = warp_sum(ea + ec);
         if (lane == 0) {
-          keep[h] = expf(was - base);
+          keep[h] = exp2f(was - base);
           top[h] = m;
           sum[h] = sum[h] * keep[h] + add;
         }
@@ -306,6 +307,205 @@ __global__ void __launch_bounds__(kAnswerThreads) answer_simt_kernel(const Answe
   }
 }
 
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// d[16][8] += a[16][16] b[16][8], fp32 sums
+template <bool kBf16>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (kBf16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16-bit types, head dimensions that are multiples of 8 up to kDP. A warp takes 16 positions of a tile:
+//   S^T [16 positions][8 heads] = k q^T,   O^T [D][8 heads] += v^T P^T
+// by warp-level matrix instructions; the cache is read 16 bytes a lane straight into their registers. That works
+// because the order of an inner dimension is free as long as both operands share it: for S^T, lane (g, t) of
+// a row of four takes elements 8 (t + 4c) .. + 7 of position g's key, and of head g's query; for O^T it takes
+// elements 8 (g + 8c) .. + 7 of the values of positions 2t, 2t + 1, 2t + 8, 2t + 9, whose pairs two byte permutes
+// put side by side. Warps meet only at the end of a unit. Bound by HBM: 2 D bytes of keys and values for
+// 4 D products a head; the products of 8 heads cost a tenth of the time the bytes take. As in the forward pass
+// over whole sequences the maximum in use only follows when it has grown by 2^8.
+template <bool kBf16, int kDP>
+__global__ void __launch_bounds__(kAnswerThreads, kDP == 64 ? 4 : 3) answer_mma_kernel(const AnswerDev p) {
+  constexpr int kKC = kDP / 32, kVC = kDP / 64;   // 16-byte loads of a lane for a key, for a value
+  __shared__ float sums[kAnswerThreads / 32][kHeads][kDP + 4];
+  __shared__ float stats[kAnswerThreads / 32][kHeads][2];
+  const int D = p.c.D, tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = lane / 4, t = lane % 4;
+  int64_t end;
+  Start s = find_start(p, &end);
+  int64_t at = s.at;
+  while (at < end) {
+    const int b = s.unit / p.units, u = s.unit % p.units, kv = u / p.chunks;
+    const int head0 = kv * p.group + (u % p.chunks) * kHeads;
+    const int heads = min(kHeads, (kv + 1) * p.group - head0);
+    const int len = length_of(p.c, b);
+    const int stop = static_cast<int>(min(static_cast<int64_t>(s.tiles), s.tile + (end - at)));
+    if (tid == 0 && s.tile == 0 && raw_length(p.c, b) != len) raise(p.c);
+    const uint16_t* kc = reinterpret_cast<const uint16_t*>(p.c.k) + kv * p.c.k_head;
+    const uint16_t* vc = reinterpret_cast<const uint16_t*>(p.c.v) + kv * p.c.v_head;
+    uint4 q[kKC];
+#pragma unroll
+    for (int c = 0; c < kKC; ++c) {
+      const int d = 8 * (t + 4 * c);
+      q[c] = make_uint4(0, 0, 0, 0);
+      if (g < heads && d < D)
+        q[c] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + b * p.q_row + (head0 + g) * p.q_head + d);
+    }
+    // the page and the place in it of position lane % 16 of this warp's share of a tile; page -1: takes no part
+    auto locate = [&](int tile, int* slot) {
+      const int x = tile * kTile + warp * 16 + (lane & 15);
+      int page = -1;
+      *slot = 0;
+      if (tile < stop && x < len) {
+        const int n = x / p.c.page_size;
+        *slot = x - n * p.c.page_size;
+        page = __ldg(p.c.page_table + b * p.c.table_stride + n);
+        if (page < 0 || page >= p.c.num_pages) {
+          page = -1;
+          raise(p.c);
+        }
+      }
+      return page;
+    };
+    uint4 k[2][kKC], v[4][kVC];
+    bool ok[2];
+    auto load_keys = [&](int page, int slot) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int pg = __shfl_sync(kFullMask, page, g + 8 * i), sl = __shfl_sync(kFullMask, slot, g + 8 * i);
+        ok[i] = pg >= 0;
+        const uint16_t* row = kc + pg * p.c.k_page + sl * p.c.k_slot + 8 * t;
+#pragma unroll
+        for (int c = 0; c < kKC; ++c) k[i][c] = ok[i] && 8 * (t + 4 * c) < D ? ldg_stream16(row + 32 * c) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto load_values = [&](int page, int slot) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int x = 2 * t + (i & 1) + 8 * (i / 2);
+        const int pg = __shfl_sync(kFullMask, page, x), sl = __shfl_sync(kFullMask, slot, x);
+        const uint16_t* row = vc + pg * p.c.v_page + sl * p.c.v_slot + 8 * g;
+#pragma unroll
+        for (int c = 0; c < kVC; ++c) v[i][c] = pg >= 0 && 8 * (g + 8 * c) < D ? ldg_stream16(row + 64 * c) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    float o[kVC * 4][4] = {};
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};   // of heads 2t and 2t + 1
+    int slot, next_slot;
+    int page = locate(s.tile, &slot);
+    load_keys(page, slot);
+    load_values(page, slot);
+    int next_page = locate(s.tile + 1, &next_slot);
+    for (int tile = s.tile; tile < stop; ++tile) {
+      float x[4] = {};
+#pragma unroll
+      for (int c = 0; c < kKC; ++c) {
+        mma16816<kBf16>(x, k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, q[c].x, q[c].y);
+        mma16816<kBf16>(x, k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, q[c].z, q[c].w);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = ok[i / 2] ? x[i] * p.scale_log2 : -INFINITY;
+      if (tile + 1 < stop) load_keys(next_page, next_slot);
+      const float most[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+      if (__any_sync(kFullMask, most[0] > top[0] + 8.f || most[1] > top[1] + 8.f)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float m = fmaxf(top[i], most[i]);
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, w));
+          const float keep = m == -INFINITY ? 1.f : fast_exp2(top[i] - m);
+          top[i] = m;
+          sum[i] *= keep;
+#pragma unroll
+          for (int r = 0; r < kVC * 4; ++r) {
+            o[r][i] *= keep;
+            o[r][2 + i] *= keep;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = fast_exp2(x[i] - (top[i & 1] == -INFINITY ? 0.f : top[i & 1]));
+        sum[i & 1] += x[i];
+      }
+      const uint32_t p0 = transpose8x8(pack2<kBf16>(x[0], x[1])), p1 = transpose8x8(pack2<kBf16>(x[2], x[3]));
+#pragma unroll
+      for (int c = 0; c < kVC; ++c) {
+        const uint32_t a[4][4] = {{v[0][c].x, v[0][c].y, v[0][c].z, v[0][c].w}, {v[1][c].x, v[1][c].y, v[1][c].z, v[1][c].w},
+                                  {v[2][c].x, v[2][c].y, v[2][c].z, v[2][c].w}, {v[3][c].x, v[3][c].y, v[3][c].z, v[3][c].w}};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          mma16816<kBf16>(o[c * 4 + r], __byte_perm(a[0][r], a[1][r], 0x5410), __byte_perm(a[0][r], a[1][r], 0x7632),
+                          __byte_perm(a[2][r], a[3][r], 0x5410), __byte_perm(a[2][r], a[3][r], 0x7632), p0, p1);
+      }
+      if (tile + 1 < stop) {
+        load_values(next_page, next_slot);
+        next_page = locate(tile + 2, &next_slot);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int w = 4; w < 32; w <<= 1) sum[i] += __shfl_xor_sync(kFullMask, sum[i], w);
+    __syncthreads();   // the last unit's sums have been read
+    if (g < 2) {
+      stats[warp][2 * t + g][0] = g == 0 ? top[0] : top[1];
+      stats[warp][2 * t + g][1] = g == 0 ? sum[0] : sum[1];
+    }
+#pragma unroll
+    for (int c = 0; c < kVC; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *reinterpret_cast<float2*>(&sums[warp][2 * t + i][8 * (g + 8 * c) + 2 * r]) = make_float2(o[c * 4 + r][i], o[c * 4 + r][2 + i]);
+    __syncthreads();
+    const bool whole = s.tile == 0 && stop == s.tiles;
+    const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (s.tile == 0 ? 1 : 0);
+    for (int i = tid; i < heads * D; i += kAnswerThreads) {
+      const int h = i / D, d = i - h * D;
+      float m = stats[0][h][0];
+#pragma unroll
+      for (int w = 1; w < kAnswerThreads / 32; ++w) m = fmaxf(m, stats[w][h][0]);
+      const float base = m == -INFINITY ? 0.f : m;
+      float l = 0.f, x = 0.f;
+#pragma unroll
+      for (int w = 0; w < kAnswerThreads / 32; ++w) {
+        const float f = fast_exp2(stats[w][h][0] - base);
+        l = fmaf(f, stats[w][h][1], l);
+        x = fmaf(f, sums[w][h][d], x);
+      }
+      if (whole) {
+        const uint32_t y = pack2<kBf16>(l == 0.f ? 0.f : x / l, 0.f);
+        static_cast<uint16_t*>(p.out)[b * p.o_row + (head0 + h) * p.o_head + d] = static_cast<uint16_t>(y);
+      } else {
+        p.sums[(part * kHeads + h) * D + d] = x;
+        if (d == 0) {
+          p.stats[(part * kHeads + h) * 2] = m;
+          p.stats[(part * kHeads + h) * 2 + 1] = l;
+        }
+      }
+    }
+    at += stop - s.tile;
+    if (at < end) {
+      ++s.unit;
+      s.tile = 0;
+      s.tiles = tiles_of(p.c, s.unit / p.units);
+    }
+  }
+}
+
 // Block (c, h): when the cut before CTA c is the first inside a unit, the unit's head h.
 template <typename T>
 __global__ void __launch_bounds__(kAnswerThreads) join_kernel(const AnswerDev p) {
@@ -325,13 +525,13 @@ __global__ void __launch_bounds__(kAnswerThreads) join_kernel(const AnswerDev p)
   for (int i = c; i <= last; ++i) m = fmaxf(m, p.stats[(2 * static_cast<int64_t>(i) * kHeads + h) * 2]);
   const float base = m == -INFINITY ? 0.f : m;
   for (int d = threadIdx.x; d < p.c.D; d += kAnswerThreads) {
-    float w = expf(p.stats[(part0 * kHeads + h) * 2] - base);
+    float w = exp2f(p.stats[(part0 * kHeads + h) * 2] - base);
     float l = w * p.stats[(part0 * kHeads + h) * 2 + 1];
     float o = w * p.sums[(part0 * kHeads + h) * p.c.D + d];
 #pragma unroll 4
     for (int i = c; i <= last; ++i) {
       const int64_t part = 2 * static_cast<int64_t>(i);
-      w = expf(p.stats[(part * kHeads + h) * 2] - base);
+      w = exp2f(p.stats[(part * kHeads + h) * 2] - base);
       l = fmaf(w, p.stats[(part * kHeads + h) * 2 + 1], l);
       o = fmaf(w, p.sums[(part * kHeads + h) * p.c.D + d], o);
     }
@@ -374,15 +574,39 @@ int launch_append(const AppendDev& p, cudaStream_t stream) {
 }
 
 template <typename T>
+int join(const AnswerDev& p, int ctas, cudaStream_t stream) {
+  if (ctas < 2) return B200TBE_OK;
+  join_kernel<T><<<dim3(ctas - 1, min(kHeads, p.group)), kAnswerThreads, 0, stream>>>(p);
+  return launch_status();
+}
+
+// 16-byte reads of everything, and a head dimension that the registers hold
+bool answer_fits_mma(const AnswerDev& p) {
+  uint64_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.c.k) | reinterpret_cast<uintptr_t>(p.c.v);
+  for (int64_t x : {static_cast<int64_t>(p.c.D), p.q_row, p.q_head, p.c.k_page, p.c.k_slot, p.c.k_head, p.c.v_page, p.c.v_slot,
+                    p.c.v_head})
+    bits |= static_cast<uint64_t>(x * 2);
+  return bits % 16 == 0 && p.c.D <= 128;
+}
+
+template <typename T, bool kBf16>
+int launch_answer_mma(const AnswerDev& p, int ctas, cudaStream_t stream) {
+  if (p.c.D <= 64)
+    answer_mma_kernel<kBf16, 64><<<ctas, kAnswerThreads, 0, stream>>>(p);
+  else
+    answer_mma_kernel<kBf16, 128><<<ctas, kAnswerThreads, 0, stream>>>(p);
+  const int st = launch_status();
+  return st != B200TBE_OK ? st : join<T>(p, ctas, stream);
+}
+
+template <typename T>
 int launch_answer(const AnswerDev& p, int ctas, cudaStream_t stream) {
   const int bytes = (kHeads * p.c.D + kTile * (p.c.D + 1)) * 4;
   const auto kernel = p.c.D <= kAnswerThreads ? answer_simt_kernel<T, 1> : answer_simt_kernel<T, 2>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return B200TBE_ERR_LAUNCH;
   kernel<<<ctas, kAnswerThreads, bytes, stream>>>(p);
   const int st = launch_status();
-  if (st != B200TBE_OK || ctas < 2) return st;
-  join_kernel<T><<<dim3(ctas - 1, min(kHeads, p.group)), kAnswerThreads, 0, stream>>>(p);
-  return launch_status();
+  return st != B200TBE_OK ? st : join<T>(p, ctas, stream);
 }
 
 }  // namespace
@@ -442,7 +666,7 @@ extern "C" int b200tbe_paged_attention(const b200tbe_paged_cache* cache, const v
   p.heads = heads, p.group = heads / cache->kv_heads, p.chunks = (p.group + kHeads - 1) / kHeads;
   p.units = cache->kv_heads * p.chunks;
   if (static_cast<int64_t>(p.units) * cache->batch > 0x7fffffff) return B200TBE_ERR_TOO_LARGE;
-  p.scale = scale;
+  p.scale_log2 = scale * 1.4426950408889634f;
   p.starts = static_cast<Start*>(scratch);
   p.stats = reinterpret_cast<float*>(p.starts + kAnswerCtas);
   p.sums = p.stats + 2 * kAnswerCtas * kHeads * 2;
@@ -450,6 +674,12 @@ extern "C" int b200tbe_paged_attention(const b200tbe_paged_cache* cache, const v
   // as many CTAs as the cache could give tiles to
   const int64_t most = (static_cast<int64_t>(cache->max_pages) * cache->page_size + kTile - 1) / kTile;
   const int64_t tiles = static_cast<int64_t>(p.units) * cache->batch * (most < 1 ? 1 : most);
+  if (cache->dtype != B200TBE_FP32 && answer_fits_mma(p)) {
+    const int most_ctas = kNumSMs * (p.c.D <= 64 ? 4 : 3);
+    const int ctas = static_cast<int>(tiles < most_ctas ? tiles : most_ctas);
+    return cache->dtype == B200TBE_FP16 ? launch_answer_mma<__half, false>(p, ctas, stream)
+                                        : launch_answer_mma<__nv_bfloat16, true>(p, ctas, stream);
+  }
   const int ctas = static_cast<int>(tiles < kAnswerCtas ? tiles : kAnswerCtas);
   if (cache->dtype == B200TBE_FP32) return launch_answer<float>(p, ctas, stream);
   if (cache->dtype == B200TBE_FP16) return launch_answer<__half>(p, ctas, stream);
