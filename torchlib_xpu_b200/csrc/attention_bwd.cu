@@ -8,7 +8,7 @@
 // Two kernels, so that no sum crosses a CTA and the results do not depend on scheduling: S and dP are computed
 // twice (7 products instead of 5), and nothing is added in memory. Scores and dP come into tensor memory
 // with a row for each thread pair; two warpgroups take half of the columns each; P and dS go back into tensor
-// memory, rounded to the operands' type, as the left operand of the next product. P and dS are rounded because
+// memory, each in its own columns' place, rounded to the operands' type, as the left operand of the next product. P and dS are rounded because
 // the tensor cores multiply 16-bit operands; they are summed in fp32.
 // The CTAs take the tiles of a list that the delta kernel leaves, one after the other.
 #include "attention.cuh"
@@ -31,14 +31,13 @@ template <int kDP>
 struct Layout {
   static constexpr int kTileBytes = kRows * kDP * 2;
   static constexpr int kSmem = 6 * kTileBytes + 1024;   // two tiles that stay, two stages of two that come
-  static constexpr int kBuffers = kDP == 64 ? 2 : 1;    // of the keys' kernel: tensor memory for scores ahead
 };
 
 struct DqBarriers {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], dp_full, loaded, ds_full, done;
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full, dp_full, s_loaded, ds_full, done;
 };
 struct DkvBarriers {
-  uint64_t kv_full, q_full[2], q_empty[2], s_full[2], dp_full, loaded, p_full, ds_full, stat_full[2], stat_empty[2], done;
+  uint64_t kv_full, q_full[2], q_empty[2], s_full, dp_full, p_full, ds_full, stat_full[2], stat_empty[2], done;
 };
 
 // What a tile's CTA knows.
@@ -94,9 +93,11 @@ __device__ __forceinline__ void product_over_d(uint32_t d, uint32_t a, uint32_t 
   }
 }
 
-// d[128][D] (+)= w x: w in tensor memory (two 16-bit weights a column), x rows of the head dimension
+// d[128][D] (+)= w x: w in tensor memory (two 16-bit weights a column, 64 in the first 32 columns, 64 from column
+// 64 on), x rows of the head dimension
 __device__ __forceinline__ void product_over_rows(uint32_t d, uint32_t w, uint32_t x, uint32_t desc, int steps, bool add) {
-  for (int t = 0; t < steps; ++t) mma_ts(d, w + t * 8, smem_desc(x + t * 2048, kRows * 128), desc, add || t > 0);
+  for (int t = 0; t < steps; ++t)
+    mma_ts(d, w + t * 8 + (t >= 4 ? 32 : 0), smem_desc(x + t * 2048, kRows * 128), desc, add || t > 0);
 }
 
 // A row of the accumulator in tensor memory, times f, to memory.
@@ -127,6 +128,23 @@ __device__ __forceinline__ void store_row(void* out, uint32_t at, int D, float f
   }
 }
 
+__device__ __forceinline__ uint64_t as_pair(const uint32_t (&x)[32], int e) {
+  return pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+}
+
+// x = exp2(x c + m) in place, two and two
+__device__ __forceinline__ void exponentials4(uint32_t (&x)[32], int e, uint64_t c, uint64_t m0, uint64_t m1) {
+  const float2 a = unpair(fma2(as_pair(x, e), c, m0)), b = unpair(fma2(as_pair(x, e + 2), c, m1));
+  x[e] = __float_as_uint(fast_exp2(a.x));
+  x[e + 1] = __float_as_uint(fast_exp2(a.y));
+  x[e + 2] = __float_as_uint(fast_exp2(b.x));
+  x[e + 3] = __float_as_uint(fast_exp2(b.y));
+}
+__device__ __forceinline__ void exponentials(uint32_t (&x)[32], uint64_t c, uint64_t m) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 4) exponentials4(x, e, c, m, m);
+}
+
 // After a wait gave up: report it, and let what is in flight land before its memory is given back.
 __device__ __forceinline__ void report(const int* dead, int32_t* status) {
   if (*dead) {
@@ -135,7 +153,8 @@ __device__ __forceinline__ void report(const int* dead, int32_t* status) {
   }
 }
 
-// Tensor memory: scores in two buffers (dS takes the place of the scores it comes from), dP, dQ.
+// Tensor memory: scores, dP (dS takes its place), dQ. The scores of the next keys are computed as soon as these are
+// in registers, under the arithmetic on dP; dQ and the next dP under the exponentials.
 template <bool kBf16, int kDP>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_dq_kernel(const BwdDev p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
@@ -156,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_base, dp_at = tmem + 256, dq_at = tmem + 384;
+  const uint32_t tmem = tmem_base, dp_at = tmem + kRows, dq_at = tmem + 2 * kRows;
   volatile int* dead = &dead_word;
 
   Item it;
@@ -195,10 +214,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) return false;
           const int keys = keys_of(j);
           if (keys % 16 != 0) zero_tail<kDP>(ks + (j & 1) * L::kTileBytes, keys);
+          if (j > 0 && !warp_wait(&bars.s_loaded, (j - 1) & 1, dead)) return false;
+          tc_fence_after();
           if (lane == 0) {
-            product_over_d(tmem + (j & 1) * kRows, q_at, smem_addr(ks + (j & 1) * L::kTileBytes),
+            product_over_d(tmem, q_at, smem_addr(ks + (j & 1) * L::kTileBytes),
                            mma_desc(kBf16, kRows, (keys + 15) & ~15, false, false), d_steps);
-            mma_commit(&bars.s_full[j & 1]);
+            mma_commit(&bars.s_full);
           }
           __syncwarp();
           return true;
@@ -217,20 +238,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         bool alive = warp_wait(&bars.q_full, 0, dead) && scores(0) && d_weights(0);
         for (int j = 0; alive && j < n; ++j) {
-          if (j + 1 < n) {
-            alive = scores(j + 1) && warp_wait(&bars.loaded, j & 1, dead);
-            tc_fence_after();
-            alive = alive && d_weights(j + 1);
-          }
+          if (j + 1 < n) alive = scores(j + 1);
           alive = alive && warp_wait(&bars.ds_full, j & 1, dead);
           tc_fence_after();
           if (alive && lane == 0) {
-            product_over_rows(dq_at, tmem + (j & 1) * kRows, smem_addr(ks + (j & 1) * L::kTileBytes), dq_desc,
-                              (keys_of(j) + 15) / 16, j > 0);
+            product_over_rows(dq_at, dp_at, smem_addr(ks + (j & 1) * L::kTileBytes), dq_desc, (keys_of(j) + 15) / 16, j > 0);
             if (j + 2 < n) mma_commit(&bars.k_empty[j & 1]);
             if (j + 1 == n) mma_commit(&bars.done);
           }
           __syncwarp();
+          if (j + 1 < n) alive = alive && d_weights(j + 1);
         }
       }
       __syncthreads();
@@ -250,10 +267,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_init(&bars.k_empty[i], 1);
           mbar_init(&bars.v_full[i], 1);
           mbar_init(&bars.v_empty[i], 1);
-          mbar_init(&bars.s_full[i], 1);
         }
+        mbar_init(&bars.s_full, 1);
         mbar_init(&bars.dp_full, 1);
-        mbar_init(&bars.loaded, 256);
+        mbar_init(&bars.s_loaded, 256);
         mbar_init(&bars.ds_full, 256);
         mbar_init(&bars.done, 1);
         fence_barrier_init();
@@ -270,45 +287,46 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lse2 == -INFINITY) lse2 = INFINITY;
       }
       const float c = a.scale * kLog2e;
+      const uint64_t c2 = pair(c, c), minus_delta = pair(-delta, -delta);
+      const uint32_t s_at = tmem + lanes + half * 64, ds_at = dp_at + lanes + half * 64;
       bool alive = true;
       for (int j = 0; j < n; ++j) {
-        alive = warp_wait(&bars.s_full[j & 1], (j / 2) & 1, dead) && warp_wait(&bars.dp_full, j & 1, dead);
+        alive = warp_wait(&bars.s_full, j & 1, dead);
         if (!alive) break;
         tc_fence_after();
-        const uint32_t s_at = tmem + lanes + (j & 1) * kRows;
         const int chunks = max(0, min(2, (klen - j * kRows - half * 64 + 31) / 32));
         const int left = limit - j * kRows - half * 64;
-        uint32_t s[2][32], dp[2][32];
+        uint32_t s[2][32];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          if (i < chunks) {
-            tmem_ld32(s[i], s_at + half * 64 + i * 32);
-            tmem_ld32(dp[i], dp_at + lanes + half * 64 + i * 32);
-          }
+          if (i < chunks) tmem_ld32(s[i], s_at + i * 32);
         tmem_wait_ld();
         tc_fence_before();
-        mbar_arrive(&bars.loaded);
-        uint32_t w[32];
+        mbar_arrive(&bars.s_loaded);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (i < chunks) exponentials(s[i], c2, pair(-lse2, -lse2));
+        alive = warp_wait(&bars.dp_full, j & 1, dead);
+        if (!alive) break;
+        tc_fence_after();
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           if (i < chunks) {
+            uint32_t dp[32], w[16];
+            tmem_ld32(dp, ds_at + i * 32);
+            tmem_wait_ld();
             const bool cut = __any_sync(kFullMask, left < i * 32 + 32);
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              float d0 = fast_exp2(fmaf(__uint_as_float(s[i][e]), c, -lse2)) * (__uint_as_float(dp[i][e]) - delta);
-              float d1 = fast_exp2(fmaf(__uint_as_float(s[i][e + 1]), c, -lse2)) * (__uint_as_float(dp[i][e + 1]) - delta);
+              float2 d = unpair(mul2(as_pair(s[i], e), add2(as_pair(dp, e), minus_delta)));
               if (cut) {
-                d0 = i * 32 + e < left ? d0 : 0.f;
-                d1 = i * 32 + e + 1 < left ? d1 : 0.f;
+                d.x = i * 32 + e < left ? d.x : 0.f;
+                d.y = i * 32 + e + 1 < left ? d.y : 0.f;
               }
-              w[i * 16 + e / 2] = pack2<kBf16>(d0, d1);
+              w[e / 2] = pack2<kBf16>(d.x, d.y);
             }
+            tmem_st16(ds_at + i * 16, w);
           }
-        // the other warpgroup's scores are overwritten: it has to have them
-        alive = warp_wait(&bars.loaded, j & 1, dead);
-        if (!alive) break;
-        tc_fence_after();
-        if (chunks > 0) tmem_st32(s_at + half * 32, w);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&bars.ds_full);
@@ -328,14 +346,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 8) tmem_free(tmem, 512);
 }
 
-// Tensor memory: scores (transposed: a key a row) in one buffer or two, dP, dV, dK. P takes the place of the
-// first half of the scores' columns, dS of the second.
+// Tensor memory: scores (transposed: a key a row; P takes their place), dP (dS takes its place), dV, dK. dV and
+// the next scores are computed under the arithmetic on dP, dK and the next dP under the exponentials.
 template <bool kBf16, int kDP>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_dkv_kernel(const BwdDev p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                          const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap g_map) {
   using L = Layout<kDP>;
-  constexpr int kB = L::kBuffers;
   extern __shared__ uint8_t raw[];
   __shared__ DkvBarriers bars;
   __shared__ uint32_t tmem_base;
@@ -352,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_base, dp_at = tmem + kB * kRows, dv_at = dp_at + kRows, dk_at = dv_at + kDP;
+  const uint32_t tmem = tmem_base, dp_at = tmem + kRows, dv_at = dp_at + kRows, dk_at = dv_at + kDP;
   volatile int* dead = &dead_word;
 
   Item it;
@@ -407,9 +424,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         auto scores = [&](int j) {
           if (lane == 0) {
-            product_over_d(tmem + (j % kB) * kRows, k_at, smem_addr(qs + (j & 1) * L::kTileBytes),
+            product_over_d(tmem, k_at, smem_addr(qs + (j & 1) * L::kTileBytes),
                            mma_desc(kBf16, kRows, (rows_of(j) + 15) & ~15, false, false), d_steps);
-            mma_commit(&bars.s_full[j % kB]);
+            mma_commit(&bars.s_full);
           }
           __syncwarp();
         };
@@ -428,32 +445,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int j = 0; alive && j < n; ++j) {
           const bool more = j + 1 < n;
-          const uint32_t s_at = tmem + (j % kB) * kRows;
           const int steps = (rows_of(j) + 15) / 16;
-          if (more) {
-            alive = ready(j + 1);
-            if (!alive) break;
-            if (kB == 2) scores(j + 1);
-            alive = warp_wait(&bars.loaded, j & 1, dead);
-            if (!alive) break;
-            tc_fence_after();
-            d_weights(j + 1);
-          }
-          alive = warp_wait(&bars.p_full, j & 1, dead);
+          alive = (!more || ready(j + 1)) && warp_wait(&bars.p_full, j & 1, dead);
           if (!alive) break;
           tc_fence_after();
-          if (lane == 0) product_over_rows(dv_at, s_at, smem_addr(gs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
+          if (lane == 0) product_over_rows(dv_at, tmem, smem_addr(gs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
           __syncwarp();
+          if (more) scores(j + 1);
           alive = warp_wait(&bars.ds_full, j & 1, dead);
           if (!alive) break;
           tc_fence_after();
           if (lane == 0) {
-            product_over_rows(dk_at, s_at + 64, smem_addr(qs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
+            product_over_rows(dk_at, dp_at, smem_addr(qs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
             if (j + 2 < n) mma_commit(&bars.q_empty[j & 1]);
             if (!more) mma_commit(&bars.done);
           }
           __syncwarp();
-          if (kB == 1 && more) scores(j + 1);
+          if (more) d_weights(j + 1);
         }
       }
       __syncthreads();
@@ -471,12 +479,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 2; ++i) {
           mbar_init(&bars.q_full[i], 1);
           mbar_init(&bars.q_empty[i], 1);
-          mbar_init(&bars.s_full[i], 1);
           mbar_init(&bars.stat_full[i], 32);
           mbar_init(&bars.stat_empty[i], 256);
         }
+        mbar_init(&bars.s_full, 1);
         mbar_init(&bars.dp_full, 1);
-        mbar_init(&bars.loaded, 256);
         mbar_init(&bars.p_full, 256);
         mbar_init(&bars.ds_full, 256);
         mbar_init(&bars.done, 1);
@@ -486,76 +493,72 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- weights: a key and half of the queries a thread ----
       const int half = warp / 4, local = (warp % 4) * 32 + lane, key = it.first + local;
       const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
-      const float c = a.scale * kLog2e;
+      const uint64_t c2 = pair(a.scale * kLog2e, a.scale * kLog2e);
+      const uint32_t s_at = tmem + lanes + half * 64, ds_at = dp_at + lanes + half * 64;
       bool alive = true;
       for (int j = 0; j < n; ++j) {
         const int st = j & 1, i0 = (from + j % per_head) * kRows + half * 64;
-        alive = warp_wait(&bars.stat_full[st], (j / 2) & 1, dead) && warp_wait(&bars.s_full[j % kB], (j / kB) & 1, dead) &&
-                warp_wait(&bars.dp_full, j & 1, dead);
+        alive = warp_wait(&bars.stat_full[st], (j / 2) & 1, dead) && warp_wait(&bars.s_full, j & 1, dead);
         if (!alive) break;
         tc_fence_after();
-        const uint32_t s_at = tmem + lanes + (j % kB) * kRows;
         const int chunks = max(0, min(2, (qlen - i0 + 31) / 32));
         // columns [low, high) are queries of the sequence that see the key
         const int low = a.causal ? key - shift - i0 : 0, high = qlen - i0;
-        uint32_t s[2][32], dp[2][32];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (i < chunks) {
-            tmem_ld32(s[i], s_at + half * 64 + i * 32);
-            tmem_ld32(dp[i], dp_at + lanes + half * 64 + i * 32);
-          }
-        tmem_wait_ld();
-        tc_fence_before();
-        mbar_arrive(&bars.loaded);
         const bool cut = __any_sync(kFullMask, low > 0 || high < 64);
-        uint32_t w[32];
+        uint32_t s[2][32];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (i < chunks) tmem_ld32(s[i], s_at + i * 32);
+        tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           if (i < chunks) {
+            uint32_t w[16];
+            const float* m = &stats[st][0][half * 64 + i * 32];
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-              const float4 m = *reinterpret_cast<const float4*>(&stats[st][0][half * 64 + i * 32 + e]);
-              float x[4] = {fmaf(__uint_as_float(s[i][e]), c, -m.x), fmaf(__uint_as_float(s[i][e + 1]), c, -m.y),
-                            fmaf(__uint_as_float(s[i][e + 2]), c, -m.z), fmaf(__uint_as_float(s[i][e + 3]), c, -m.w)};
-#pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                x[u] = fast_exp2(x[u]);
-                if (cut && (i * 32 + e + u < low || i * 32 + e + u >= high)) x[u] = 0.f;
-                s[i][e + u] = __float_as_uint(x[u]);
-              }
-              w[i * 16 + e / 2] = pack2<kBf16>(x[0], x[1]);
-              w[i * 16 + e / 2 + 1] = pack2<kBf16>(x[2], x[3]);
+              const float4 x = *reinterpret_cast<const float4*>(m + e);
+              exponentials4(s[i], e, c2, pair(-x.x, -x.y), pair(-x.z, -x.w));
             }
+            if (cut) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (i * 32 + e < low || i * 32 + e >= high) s[i][e] = 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) w[e / 2] = pack2<kBf16>(__uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
+            tmem_st16(s_at + i * 16, w);
           }
-        // the other warpgroup's scores are overwritten: it has to have them
-        alive = warp_wait(&bars.loaded, j & 1, dead);
-        if (!alive) break;
-        tc_fence_after();
-        if (chunks > 0) tmem_st32(s_at + half * 32, w);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&bars.p_full);
+        alive = warp_wait(&bars.dp_full, j & 1, dead);
+        if (!alive) break;
+        tc_fence_after();
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           if (i < chunks) {
+            uint32_t dp[32], w[16];
+            tmem_ld32(dp, ds_at + i * 32);
+            tmem_wait_ld();
+            const float* m = &stats[st][1][half * 64 + i * 32];
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-              const float4 d = *reinterpret_cast<const float4*>(&stats[st][1][half * 64 + i * 32 + e]);
-              float x[4] = {__uint_as_float(s[i][e]) * (__uint_as_float(dp[i][e]) - d.x),
-                            __uint_as_float(s[i][e + 1]) * (__uint_as_float(dp[i][e + 1]) - d.y),
-                            __uint_as_float(s[i][e + 2]) * (__uint_as_float(dp[i][e + 2]) - d.z),
-                            __uint_as_float(s[i][e + 3]) * (__uint_as_float(dp[i][e + 3]) - d.w)};
+              const float4 d = *reinterpret_cast<const float4*>(m + e);
+              float2 x = unpair(mul2(as_pair(s[i], e), add2(as_pair(dp, e), pair(-d.x, -d.y))));
+              float2 y = unpair(mul2(as_pair(s[i], e + 2), add2(as_pair(dp, e + 2), pair(-d.z, -d.w))));
               if (cut) {
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                  if (i * 32 + e + u < low || i * 32 + e + u >= high) x[u] = 0.f;
+                const int at = i * 32 + e;
+                x.x = at < low || at >= high ? 0.f : x.x;
+                x.y = at + 1 < low || at + 1 >= high ? 0.f : x.y;
+                y.x = at + 2 < low || at + 2 >= high ? 0.f : y.x;
+                y.y = at + 3 < low || at + 3 >= high ? 0.f : y.y;
               }
-              w[i * 16 + e / 2] = pack2<kBf16>(x[0], x[1]);
-              w[i * 16 + e / 2 + 1] = pack2<kBf16>(x[2], x[3]);
+              w[e / 2] = pack2<kBf16>(x.x, x.y);
+              w[e / 2 + 1] = pack2<kBf16>(y.x, y.y);
             }
+            tmem_st16(ds_at + i * 16, w);
           }
-        if (chunks > 0) tmem_st32(s_at + 64 + half * 32, w);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&bars.ds_full);

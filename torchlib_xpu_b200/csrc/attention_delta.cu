@@ -8,13 +8,27 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRows = 128;   // of a tile
 
+// How much work a tile of the stretch is, coarsely.
+__device__ __forceinline__ int weight_class(int64_t rows) { return rows >= 2048 ? 2 : rows >= 512 ? 1 : 0; }
+
 // Both lists by one CTA: the stretches' tiles are counted, summed up to each stretch, and written by its warp.
-// Later tiles of queries see more keys, and earlier keys are seen by more queries: those come first.
+// The tiles are taken in the list's order, so the long sequences' come first; within a sequence later queries see
+// more keys, and earlier keys are seen by more queries: those come first.
 __device__ __forceinline__ void list_tiles(const AttnDev& p, const BackwardPlan& plan) {
   __shared__ int64_t warp_sums[kThreads / 32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  __shared__ int present;
+  if (threadIdx.x == 0) present = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.batch + 2; i += kThreads) {
+    const int c = weight_class(stretch_bound(p.q_offsets, p.offset_bytes, p.batch, p.total_q, i + 1) -
+                               stretch_bound(p.q_offsets, p.offset_bytes, p.batch, p.total_q, i));
+    if (c > 0) atomicOr(&present, 1 << c);
+  }
+  __syncthreads();
   int64_t base = 0;   // tiles of queries in the low half, of keys in the high half
-  for (int s0 = 0; s0 < p.batch + 2; s0 += kThreads) {
+  for (int c = 2; c >= 0; --c)
+  for (int s0 = 0; (c == 0 || (present >> c & 1)) &&  s0 < p.batch + 2; s0 += kThreads) {
     const int i = s0 + threadIdx.x;
     int64_t mine = 0;
     if (i < p.batch + 2) {
@@ -22,7 +36,7 @@ __device__ __forceinline__ void list_tiles(const AttnDev& p, const BackwardPlan&
                         stretch_bound(p.q_offsets, p.offset_bytes, p.batch, p.total_q, i);
       const int64_t k = stretch_bound(p.k_offsets, p.offset_bytes, p.batch, p.total_k, i + 1) -
                         stretch_bound(p.k_offsets, p.offset_bytes, p.batch, p.total_k, i);
-      mine = max(static_cast<int64_t>(0), (q + kRows - 1) / kRows) + (max(static_cast<int64_t>(0), (k + kRows - 1) / kRows) << 32);
+      if (weight_class(q) == c) mine = max(static_cast<int64_t>(0), (q + kRows - 1) / kRows) + (max(static_cast<int64_t>(0), (k + kRows - 1) / kRows) << 32);
     }
     int64_t upto = mine;
 #pragma unroll
@@ -69,10 +83,11 @@ __global__ void __launch_bounds__(kThreads) delta_kernel(const AttnDev p, const 
   struct __align__(sizeof(T) * kElems) Vec {
     T x[kElems];
   };
-  const int64_t at = (static_cast<int64_t>(blockIdx.x - 1) * kThreads + threadIdx.x) / kLanes;
+  const int64_t at = static_cast<int64_t>(blockIdx.x - 1) * (kThreads / kLanes) + threadIdx.x / kLanes;
   const bool in = at < p.total_q * p.heads;
-  const int64_t row = in ? at / p.heads : 0;
-  const int head = in ? static_cast<int>(at % p.heads) : 0;
+  // 64-bit divisions would cost more than the rest
+  const int64_t row = !in ? 0 : at >> 32 == 0 ? static_cast<uint32_t>(at) / static_cast<uint32_t>(p.heads) : at / p.heads;
+  const int head = in ? static_cast<int>(at - row * p.heads) : 0;
   const T* g = static_cast<const T*>(p.grad) + row * p.g_row + head * p.g_head;
   const T* o = static_cast<const T*>(p.out) + row * p.o_row + head * p.o_head;
   float s = 0.f;
