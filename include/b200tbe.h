@@ -431,7 +431,12 @@ typedef struct {
   int32_t causal;
   float scale;
   int32_t* status;                  /* device word or NULL: B200TBE_DEV_WAIT_TIMEOUT */
+  void* scratch;                    /* of the forward pass, 16-byte aligned, or NULL: batches of short sequences
+                                       are slower without it */
+  size_t scratch_bytes;             /* b200tbe_jagged_attention_scratch_bytes() */
 } b200tbe_attention_params;
+
+B200TBE_API size_t b200tbe_jagged_attention_scratch_bytes(int64_t total_q, int32_t batch);
 
 B200TBE_API int b200tbe_jagged_attention(const b200tbe_attention_params* p, b200tbe_stream_t stream);
 

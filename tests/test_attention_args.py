@@ -66,6 +66,15 @@ def test_attention_backward_refuses():
     assert lib.b200tbe_jagged_attention_backward_scratch_bytes(10, 10, 1, 0) == 0
 
 
+def test_forward_scratch():
+    lib = cabi.lib()
+    need = lib.b200tbe_jagged_attention_scratch_bytes(10, 1)
+    assert need > 0 and lib.b200tbe_jagged_attention_scratch_bytes(-1, 1) == 0
+    for at, n in ((AT + 8, need), (AT, need - 1)):
+        p = _attention(scratch=at, scratch_bytes=n)
+        assert lib.b200tbe_jagged_attention(ctypes.byref(p), None) == SCRATCH
+
+
 def test_nothing_to_do():
     lib = cabi.lib()
     p = _attention(total_q=0, q=None, out=None)

@@ -97,6 +97,7 @@ class AttentionParams(ctypes.Structure):
         ("batch", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
         ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("offset_bytes", ctypes.c_int32),
         ("causal", ctypes.c_int32), ("scale", ctypes.c_float), ("status", _c_void_p),
+        ("scratch", _c_void_p), ("scratch_bytes", ctypes.c_size_t),
     ]
 
 
@@ -135,7 +136,7 @@ EXPORTS = (
     "b200tbe_quantized_row_bytes",
     "b200tbe_quantize_rows", "b200tbe_dequantize_rows", "b200tbe_nv12_to_rgb", "b200tbe_jagged_to_padded_dense", "b200tbe_dense_to_jagged",
     "b200tbe_jagged_dense_elementwise_add", "b200tbe_jagged_attention",
-    "b200tbe_jagged_attention_backward_scratch_bytes", "b200tbe_jagged_attention_backward",
+    "b200tbe_jagged_attention_scratch_bytes", "b200tbe_jagged_attention_backward_scratch_bytes", "b200tbe_jagged_attention_backward",
     "b200tbe_paged_cache_append", "b200tbe_paged_attention_scratch_bytes", "b200tbe_paged_attention",
 )
 
@@ -200,6 +201,8 @@ def lib() -> ctypes.CDLL:
             ctypes.POINTER(JaggedShape), _c_void_p, _c_void_p, _c_void_p, _c_void_p]
         i64, i32 = ctypes.c_int64, ctypes.c_int32
         _lib.b200tbe_jagged_attention.argtypes = [ctypes.POINTER(AttentionParams), _c_void_p]
+        _lib.b200tbe_jagged_attention_scratch_bytes.argtypes = [i64, i32]
+        _lib.b200tbe_jagged_attention_scratch_bytes.restype = ctypes.c_size_t
         _lib.b200tbe_jagged_attention_backward_scratch_bytes.argtypes = [i64, i64, i32, i32]
         _lib.b200tbe_jagged_attention_backward_scratch_bytes.restype = ctypes.c_size_t
         _lib.b200tbe_jagged_attention_backward.argtypes = [ctypes.POINTER(AttentionBackwardParams), _c_void_p]

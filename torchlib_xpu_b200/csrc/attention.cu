@@ -33,36 +33,16 @@ AttnDev device_params(const b200tbe_attention_params* p) {
   return d;
 }
 
-}  // namespace
-}  // namespace b200tbe
-
-using namespace b200tbe;
-
-extern "C" int b200tbe_jagged_attention(const b200tbe_attention_params* p, b200tbe_stream_t stream_) {
-  const int st = check_forward(p);
-  if (st != B200TBE_OK) return st;
-  if (p->total_q == 0) return B200TBE_OK;
-  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  const AttnDev d = device_params(p);
-  if (attention_forward_fits(d, p->dtype)) {
-    const int tc = attention_forward_tc(d, p->dtype, p->status, stream);
-    if (tc != B200TBE_ERR_UNSUPPORTED) return tc;
-  }
-  return attention_forward_simt(d, p->dtype, stream);
-}
-
-namespace {
-
 size_t rounded(size_t n) { return (n + 15) / 16 * 16; }
 
-// delta, then the tickets and counts, then the two lists
-struct BackwardScratch {
+// delta, then the list's tickets and counts, then the two lists
+struct Scratch {
   size_t delta, words, q_tiles, k_tiles;
   size_t total() const { return delta + words + q_tiles + k_tiles; }
 };
 
-BackwardScratch scratch_of(int64_t total_q, int64_t total_k, int64_t batch, int64_t heads) {
-  BackwardScratch s;
+Scratch backward_scratch(int64_t total_q, int64_t total_k, int64_t batch, int64_t heads) {
+  Scratch s;
   s.delta = rounded(static_cast<size_t>(total_q) * heads * sizeof(float));
   s.words = 16;
   s.q_tiles = rounded(static_cast<size_t>(tile_slots<128>(total_q, batch)) * sizeof(int2));
@@ -70,12 +50,68 @@ BackwardScratch scratch_of(int64_t total_q, int64_t total_k, int64_t batch, int6
   return s;
 }
 
+TileList list_at(char* at, const Scratch& s, int64_t total_q, int64_t total_k, int64_t batch) {
+  TileList list;
+  list.tickets = reinterpret_cast<int32_t*>(at);
+  list.counts = list.tickets + 2;
+  list.q_tiles = reinterpret_cast<int2*>(at + s.words);
+  list.k_tiles = reinterpret_cast<int2*>(at + s.words + s.q_tiles);
+  list.q_room = static_cast<int32_t>(tile_slots<128>(total_q, batch));
+  list.k_room = static_cast<int32_t>(tile_slots<128>(total_k, batch));
+  return list;
+}
+
+// Batches whose sequences are at most 128 long on average go through the short sequences' kernels first. There
+// the general kernels' CTAs, one or two an SM, would each spend most of a sequence's time waiting: 4096 sequences
+// of 0 to 128 positions, 4 heads of 64, forward 514 us without, and the table of measurements has what it is with.
+bool mostly_short(const AttnDev& d) {
+  return d.batch > 0 && d.total_q <= static_cast<int64_t>(d.batch) * 128 && d.total_k <= static_cast<int64_t>(d.batch) * 128;
+}
+// ... and here nothing can be longer.
+bool all_short(const AttnDev& d) { return d.total_q <= 128 && d.total_k <= 128; }
+
 }  // namespace
+}  // namespace b200tbe
+
+using namespace b200tbe;
+
+extern "C" size_t b200tbe_jagged_attention_scratch_bytes(int64_t total_q, int32_t batch) {
+  if (total_q < 0 || batch < 0) return 0;
+  const Scratch s = backward_scratch(total_q, 0, batch, 0);
+  return s.words + s.q_tiles;
+}
+
+extern "C" int b200tbe_jagged_attention(const b200tbe_attention_params* p, b200tbe_stream_t stream_) {
+  const int st = check_forward(p);
+  if (st != B200TBE_OK) return st;
+  if (p->scratch != nullptr && (!aligned_to(p->scratch, 16) ||
+                                p->scratch_bytes < b200tbe_jagged_attention_scratch_bytes(p->total_q, p->batch)))
+    return B200TBE_ERR_SCRATCH;
+  if (p->total_q == 0) return B200TBE_OK;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  const AttnDev d = device_params(p);
+  if (attention_forward_fits(d, p->dtype)) {
+    const TileList* rest = nullptr;
+    TileList list;
+    int tc = B200TBE_ERR_UNSUPPORTED;
+    if (p->scratch != nullptr && mostly_short(d)) {
+      list = list_at(static_cast<char*>(p->scratch), backward_scratch(d.total_q, 0, d.batch, 0), d.total_q, 0, d.batch);
+      if (!all_short(d) && cudaMemsetAsync(p->scratch, 0, 16, stream) != cudaSuccess) return B200TBE_ERR_LAUNCH;
+      tc = attention_short_forward(d, list, p->dtype, p->status, stream);
+      if (tc == B200TBE_OK && all_short(d)) return tc;
+      if (tc == B200TBE_OK) rest = &list;
+      if (tc != B200TBE_OK && tc != B200TBE_ERR_UNSUPPORTED) return tc;
+    }
+    tc = attention_forward_tc(d, rest, p->dtype, p->status, stream);
+    if (tc != B200TBE_ERR_UNSUPPORTED) return tc;
+  }
+  return attention_forward_simt(d, p->dtype, stream);
+}
 
 extern "C" size_t b200tbe_jagged_attention_backward_scratch_bytes(int64_t total_q, int64_t total_k, int32_t batch,
                                                                   int32_t heads) {
   if (total_q < 0 || total_k < 0 || batch < 0 || heads <= 0) return 0;
-  return scratch_of(total_q, total_k, batch, heads).total();
+  return backward_scratch(total_q, total_k, batch, heads).total();
 }
 
 extern "C" int b200tbe_jagged_attention_backward(const b200tbe_attention_backward_params* p, b200tbe_stream_t stream_) {
@@ -85,27 +121,33 @@ extern "C" int b200tbe_jagged_attention_backward(const b200tbe_attention_backwar
   if (st != B200TBE_OK) return st;
   if (f->total_q > 0 && (p->grad_out == nullptr || f->lse == nullptr || p->grad_q == nullptr)) return B200TBE_ERR_BAD_ARG;
   if (f->total_k > 0 && (p->grad_k == nullptr || p->grad_v == nullptr)) return B200TBE_ERR_BAD_ARG;
-  const BackwardScratch s = scratch_of(f->total_q, f->total_k, f->batch, f->heads);
+  const Scratch s = backward_scratch(f->total_q, f->total_k, f->batch, f->heads);
   if (p->scratch == nullptr || p->scratch_bytes < s.total() || !aligned_to(p->scratch, 16)) return B200TBE_ERR_SCRATCH;
   if (f->total_q == 0 && f->total_k == 0) return B200TBE_OK;
   AttnDev d = device_params(f);
   d.grad = p->grad_out, d.dq = p->grad_q, d.dk = p->grad_k, d.dv = p->grad_v, d.delta = static_cast<float*>(p->scratch);
   d.g_row = p->grad_out_stride, d.g_head = p->grad_out_head_stride, d.dq_row = p->grad_q_stride, d.dq_head = p->grad_q_head_stride;
   d.dk_row = p->grad_k_stride, d.dk_head = p->grad_k_head_stride, d.dv_row = p->grad_v_stride, d.dv_head = p->grad_v_head_stride;
-  char* at = static_cast<char*>(p->scratch) + s.delta;
-  BackwardPlan plan;
-  plan.tickets = reinterpret_cast<int32_t*>(at);
-  plan.counts = plan.tickets + 2;
-  plan.q_tiles = reinterpret_cast<int2*>(at + s.words);
-  plan.k_tiles = reinterpret_cast<int2*>(at + s.words + s.q_tiles);
-  plan.q_room = static_cast<int32_t>(tile_slots<128>(f->total_q, f->batch));
-  plan.k_room = static_cast<int32_t>(tile_slots<128>(f->total_k, f->batch));
+  const TileList list = list_at(static_cast<char*>(p->scratch) + s.delta, s, f->total_q, f->total_k, f->batch);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  st = attention_delta(d, plan, f->dtype, stream);
+  const bool fits = attention_backward_fits(d, f->dtype);
+  bool listed = false;   // by the short sequences' kernel
+  if (fits && mostly_short(d)) {
+    if (!all_short(d) && cudaMemsetAsync(list.tickets, 0, 16, stream) != cudaSuccess) return B200TBE_ERR_LAUNCH;
+    st = attention_short_backward(d, list, f->dtype, f->status, stream);
+    if (st == B200TBE_OK && all_short(d)) return st;
+    if (st != B200TBE_OK && st != B200TBE_ERR_UNSUPPORTED) return st;
+    listed = st == B200TBE_OK;
+  }
+  st = listed ? attention_delta_listed(d, list, f->dtype, stream) : attention_delta(d, list, f->dtype, stream);
   if (st != B200TBE_OK) return st;
-  if (attention_backward_fits(d, f->dtype)) {
-    const int tc = attention_backward_tc(d, plan, f->dtype, f->status, stream);
-    if (tc != B200TBE_ERR_UNSUPPORTED) return tc;
+  if (fits) {
+    st = attention_backward_tc(d, list, f->dtype, f->status, stream);
+    if (st != B200TBE_ERR_UNSUPPORTED) return st;
+    if (listed) {   // the 32-bit kernels take every row
+      st = attention_delta(d, list, f->dtype, stream);
+      if (st != B200TBE_OK) return st;
+    }
   }
   return attention_backward_simt(d, f->dtype, stream);
 }

@@ -28,9 +28,10 @@ struct AttnDev {
   int64_t g_row, g_head, dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
 };
 
-// The tiles of 128 rows of a backward pass, as the delta kernel lists them in the caller's scratch: (stretch,
-// tile inside it), of queries and of keys. The tickets say how many of them (times heads) are taken.
-struct BackwardPlan {
+// Tiles of 128 rows, of queries and of keys, listed in the caller's scratch as (stretch, tile inside it) by the delta
+// kernel (all of them) or by the short sequences' kernels (what they leave). The tickets say how many of them (times
+// heads) are taken.
+struct TileList {
   int32_t* tickets;   // [2]
   int32_t* counts;    // [2]
   int2* q_tiles;
@@ -43,10 +44,14 @@ int attention_backward_simt(const AttnDev& p, int dtype, cudaStream_t stream);
 // Tensor-core kernels: whether they take these arguments, and the launches. B200TBE_ERR_UNSUPPORTED from a
 // launch (nothing was enqueued): the driver made no tensor map of them, the 32-bit kernels take over.
 bool attention_forward_fits(const AttnDev& p, int dtype);
-int attention_forward_tc(const AttnDev& p, int dtype, int32_t* status, cudaStream_t stream);
+int attention_forward_tc(const AttnDev& p, const TileList* list, int dtype, int32_t* status, cudaStream_t stream);
+// Sequences of at most 128 queries and keys; the others' tiles go on the list (whose words are zero before).
+int attention_short_forward(const AttnDev& p, const TileList& list, int dtype, int32_t* status, cudaStream_t stream);
+int attention_short_backward(const AttnDev& p, const TileList& list, int dtype, int32_t* status, cudaStream_t stream);
+int attention_delta_listed(const AttnDev& p, const TileList& list, int dtype, cudaStream_t stream);
 bool attention_backward_fits(const AttnDev& p, int dtype);
-int attention_backward_tc(const AttnDev& p, const BackwardPlan& plan, int dtype, int32_t* status, cudaStream_t stream);
-int attention_delta(const AttnDev& p, const BackwardPlan& plan, int dtype, cudaStream_t stream);
+int attention_backward_tc(const AttnDev& p, const TileList& plan, int dtype, int32_t* status, cudaStream_t stream);
+int attention_delta(const AttnDev& p, const TileList& plan, int dtype, cudaStream_t stream);
 
 // One sequence's rows on both sides, or a stretch of rows that no sequence owns (klen 0).
 struct SeqRange {

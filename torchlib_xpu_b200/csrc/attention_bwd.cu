@@ -10,7 +10,7 @@
 // with a row for each thread pair; two warpgroups take half of the columns each; P and dS go back into tensor
 // memory, each in its own columns' place, rounded to the operands' type, as the left operand of the next product. P and dS are rounded because
 // the tensor cores multiply 16-bit operands; they are summed in fp32.
-// The CTAs take the tiles of a list that the delta kernel leaves, one after the other.
+// The CTAs take the tiles of a list, which an earlier kernel of the pass leaves, one after the other.
 #include "attention.cuh"
 #include "tcgen05.cuh"
 
@@ -23,7 +23,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct BwdDev {
   AttnDev a;
-  BackwardPlan plan;
+  TileList plan;
   int32_t* status;
 };
 
@@ -54,7 +54,7 @@ __device__ __forceinline__ bool next_item(const BwdDev& p, int* ticket, Item* it
   __syncthreads();
   const int heads = kHeadsOf == 0 ? a.heads : a.kv_heads;
   const int t = *ticket;
-  if (t / heads >= p.plan.counts[kHeadsOf]) return false;
+  if (t / heads >= min(p.plan.counts[kHeadsOf], kHeadsOf == 0 ? p.plan.q_room : p.plan.k_room)) return false;
   const int2 at = (kHeadsOf == 0 ? p.plan.q_tiles : p.plan.k_tiles)[t / heads];
   item->head = t % heads;
   item->first = at.y * kRows;
@@ -128,13 +128,9 @@ __device__ __forceinline__ void store_row(void* out, uint32_t at, int D, float f
   }
 }
 
-__device__ __forceinline__ uint64_t as_pair(const uint32_t (&x)[32], int e) {
-  return pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-}
-
 // x = exp2(x c + m) in place, two and two
 __device__ __forceinline__ void exponentials4(uint32_t (&x)[32], int e, uint64_t c, uint64_t m0, uint64_t m1) {
-  const float2 a = unpair(fma2(as_pair(x, e), c, m0)), b = unpair(fma2(as_pair(x, e + 2), c, m1));
+  const float2 a = unpair(fma2(as_pair(&x[e]), c, m0)), b = unpair(fma2(as_pair(&x[e + 2]), c, m1));
   x[e] = __float_as_uint(fast_exp2(a.x));
   x[e + 1] = __float_as_uint(fast_exp2(a.y));
   x[e + 2] = __float_as_uint(fast_exp2(b.x));
@@ -318,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool cut = __any_sync(kFullMask, left < i * 32 + 32);
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              float2 d = unpair(mul2(as_pair(s[i], e), add2(as_pair(dp, e), minus_delta)));
+              float2 d = unpair(mul2(as_pair(&s[i][e]), add2(as_pair(&dp[e]), minus_delta)));
               if (cut) {
                 d.x = i * 32 + e < left ? d.x : 0.f;
                 d.y = i * 32 + e + 1 < left ? d.y : 0.f;
@@ -545,8 +541,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
               const float4 d = *reinterpret_cast<const float4*>(m + e);
-              float2 x = unpair(mul2(as_pair(s[i], e), add2(as_pair(dp, e), pair(-d.x, -d.y))));
-              float2 y = unpair(mul2(as_pair(s[i], e + 2), add2(as_pair(dp, e + 2), pair(-d.z, -d.w))));
+              float2 x = unpair(mul2(as_pair(&s[i][e]), add2(as_pair(&dp[e]), pair(-d.x, -d.y))));
+              float2 y = unpair(mul2(as_pair(&s[i][e + 2]), add2(as_pair(&dp[e + 2]), pair(-d.z, -d.w))));
               if (cut) {
                 const int at = i * 32 + e;
                 x.x = at < low || at >= high ? 0.f : x.x;
@@ -615,7 +611,7 @@ bool attention_backward_fits(const AttnDev& a, int dtype) {
          a.dk_row % 8 == 0 && a.dk_head % 8 == 0 && a.dv_row % 8 == 0 && a.dv_head % 8 == 0;
 }
 
-int attention_backward_tc(const AttnDev& a, const BackwardPlan& plan, int dtype, int32_t* status, cudaStream_t stream) {
+int attention_backward_tc(const AttnDev& a, const TileList& plan, int dtype, int32_t* status, cudaStream_t stream) {
   const BwdDev p{a, plan, status};
   if (dtype == B200TBE_BF16) return a.D <= 64 ? launch<true, 64>(p, stream) : launch<true, 128>(p, stream);
   return a.D <= 64 ? launch<false, 64>(p, stream) : launch<false, 128>(p, stream);

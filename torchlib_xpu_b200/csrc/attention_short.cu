@@ -1,0 +1,525 @@
+// Jagged attention of sequences with at most 128 queries and 128 keys, forward and backward, on the tensor cores:
+// fp16 and bf16, head dimensions that are multiples of 8 up to 128.
+//
+// A batch of short sequences is bound by the chain of each of them (copy, product, softmax, product, store: some
+// microseconds) and by HBM, not by the tensor cores. So a CTA takes one sequence and head from beginning to end
+// without roles or pipelines, and small enough that several share an SM and hide one another's chain: the forward
+// pass takes 128 columns of tensor memory (P and O lie where the scores were), the backward pass 256. With all of a
+// row's keys in one tile the backward pass is one kernel of five products, not two of seven, and needs neither the
+// forward pass's output nor a kernel for delta: delta = rowsum(P dP), which equals rowsum(dO O).
+// What is longer is put on the list of tiles that the general kernels take afterwards.
+#include "attention.cuh"
+#include "tcgen05.cuh"
+
+namespace b200tbe {
+namespace {
+
+constexpr int kRows = 128;   // queries and keys at most
+constexpr int kBox = 32;     // rows a tensor copy brings
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct ShortDev {
+  AttnDev a;
+  TileList plan;
+  int32_t* status;
+};
+
+struct Sequence {
+  int64_t q0, k0;
+  int q, k;
+  bool gap;   // rows of no sequence: they see nothing, and nothing sees them
+};
+
+// The sequence of this CTA. false: it is not a short one; its tiles are on the list (by the first head's CTA), or
+// there is nothing to do.
+__device__ __forceinline__ bool sequence_of(const ShortDev& p, int stretch, bool first_head, bool list_keys, Sequence* s) {
+  const AttnDev& a = p.a;
+  s->q0 = stretch_bound(a.q_offsets, a.offset_bytes, a.batch, a.total_q, stretch);
+  s->k0 = stretch_bound(a.k_offsets, a.offset_bytes, a.batch, a.total_k, stretch);
+  const int64_t q = max(static_cast<int64_t>(0), stretch_bound(a.q_offsets, a.offset_bytes, a.batch, a.total_q, stretch + 1) - s->q0);
+  const int64_t k = max(static_cast<int64_t>(0), stretch_bound(a.k_offsets, a.offset_bytes, a.batch, a.total_k, stretch + 1) - s->k0);
+  s->q = static_cast<int>(q);
+  s->k = static_cast<int>(k);
+  s->gap = stretch < 1 || stretch > a.batch;
+  if (q <= kRows && k <= kRows) return q > 0 || k > 0;
+  if (!first_head) return false;
+  __shared__ int at;
+  for (int side = 0; side < (list_keys ? 2 : 1); ++side) {
+    const int n = static_cast<int>(((side == 0 ? q : k) + kRows - 1) / kRows);
+    if (n == 0) continue;
+    if (threadIdx.x == 0) at = atomicAdd(p.plan.counts + side, n);
+    __syncthreads();
+    const int room = side == 0 ? p.plan.q_room : p.plan.k_room;
+    int2* list = side == 0 ? p.plan.q_tiles : p.plan.k_tiles;
+    for (int t = threadIdx.x; t < n; t += blockDim.x)
+      if (at + t < room) list[at + t] = make_int2(stretch, side == 0 ? n - 1 - t : t);
+    __syncthreads();
+  }
+  return false;
+}
+
+// rows [0, rows) of a head in boxes of kBox rows; returns the bytes that will arrive
+template <int kDP>
+__device__ __forceinline__ uint32_t load_rows(uint8_t* tile, const CUtensorMap* map, int head, int64_t row, int rows, uint64_t* bar) {
+  uint32_t bytes = 0;
+  for (int r = 0; r < rows; r += kBox)
+    for (int x = 0; x < kDP / 64; ++x) {
+      tma_load_3d(tile + x * kRows * 128 + r * 128, map, x * 64, head, static_cast<int>(row) + r, bar);
+      bytes += kBox * 128;
+    }
+  return bytes;
+}
+
+// Rows [rows, next multiple of 16) become zero: other sequences' rows, whose zero weights would not cancel NaN.
+template <int kDP>
+__device__ __forceinline__ void zero_tail(uint8_t* tile, int rows) {
+  const int count = (16 - rows % 16) % 16;
+  for (int i = threadIdx.x; i < count * (kDP / 64) * 8; i += blockDim.x) {
+    const int x = i / (count * 8), rest = i % (count * 8);
+    *reinterpret_cast<uint4*>(tile + x * kRows * 128 + rows * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+__device__ __forceinline__ uint32_t up16(int n) { return static_cast<uint32_t>(n + 15) & ~15u; }
+
+// 32 columns of an accumulator row, times f, to memory (those below D)
+template <bool kBf16>
+__device__ __forceinline__ void store_columns(uint16_t* out, const uint32_t (&o)[32], int from, int D, float f) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 8)
+    if (from + e < D) {
+      uint4 v;
+      v.x = pack2<kBf16>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f);
+      v.y = pack2<kBf16>(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
+      v.z = pack2<kBf16>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f);
+      v.w = pack2<kBf16>(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f);
+      *reinterpret_cast<uint4*>(out + from + e) = v;
+    }
+}
+
+__device__ __forceinline__ void store_zeros(uint16_t* out, int from, int to, int D) {
+  for (int e = from; e < to && e < D; e += 8) *reinterpret_cast<uint4*>(out + e) = make_uint4(0, 0, 0, 0);
+}
+
+// A wait gave up: report it, and let what is in flight land before its memory is given back.
+__device__ __forceinline__ void report(const int* dead, int32_t* status) {
+  if (*dead) {
+    if (threadIdx.x == 0 && status != nullptr) atomicOr(status, B200TBE_DEV_WAIT_TIMEOUT);
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  }
+}
+
+template <int kDP>
+struct Forward {
+  static constexpr int kTileBytes = kRows * kDP * 2;
+  static constexpr int kSmem = 3 * kTileBytes + 1024;
+  static constexpr int kColumns = kDP == 64 ? 128 : 256;
+  static constexpr int kCtas = kDP == 64 ? 4 : 2;
+};
+
+template <bool kBf16, int kDP>
+__global__ void __launch_bounds__(128, Forward<kDP>::kCtas)
+    attention_short_fwd_kernel(const ShortDev p, const __grid_constant__ CUtensorMap q_map,
+                               const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+  using L = Forward<kDP>;
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t full, s_full, o_full;
+  __shared__ uint32_t tmem_base;
+  __shared__ int dead_word;
+  const AttnDev& a = p.a;
+  const int head = blockIdx.x % a.heads, stretch = blockIdx.x / a.heads, kv = head / a.group;
+  Sequence s;
+  if (!sequence_of(p, stretch, head == 0, false, &s) || s.q == 0) return;
+  if (s.gap) s.k = 0;
+  uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* ks = qs + L::kTileBytes;
+  uint8_t* vs = ks + L::kTileBytes;
+  const int warp = threadIdx.x / 32, row = threadIdx.x;
+  volatile int* dead = &dead_word;
+  if (threadIdx.x == 0) {
+    mbar_init(&full, 1);
+    mbar_init(&s_full, 1);
+    mbar_init(&o_full, 1);
+    dead_word = 0;
+    fence_barrier_init();
+    if (s.k > 0) {
+      const int q_rows = (s.q + kBox - 1) / kBox * kBox, k_rows = (s.k + kBox - 1) / kBox * kBox;
+      mbar_expect(&full, (q_rows + 2 * k_rows) * kDP * 2);
+      load_rows<kDP>(qs, &q_map, head, s.q0, s.q, &full);
+      load_rows<kDP>(ks, &k_map, kv, s.k0, s.k, &full);
+      load_rows<kDP>(vs, &v_map, kv, s.k0, s.k, &full);
+    }
+  }
+  if (warp == 0) {
+    __syncwarp();
+    tmem_alloc(&tmem_base, L::kColumns);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base, lanes = static_cast<uint32_t>(warp * 32) << 16;
+  const uint32_t s_at = tmem + lanes, o_at = tmem + lanes + 64;
+  const int shift = s.k - s.q;
+  const int limit = row >= s.q ? 0 : (a.causal ? min(s.k, row + shift + 1) : s.k);
+  uint16_t* out = static_cast<uint16_t*>(a.out) + (s.q0 + row) * a.o_row + head * a.o_head;
+  float base = 0.f, sum = 0.f;
+  if (s.k > 0) {
+    warp_wait(&full, 0, dead);
+    if (s.k % 16 != 0) {
+      zero_tail<kDP>(vs, s.k);
+      fence_async_smem();
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+      const uint32_t desc = mma_desc(kBf16, kRows, up16(s.k), false, false), q_at = smem_addr(qs), k_at = smem_addr(ks);
+      for (int d = 0; d < (a.D + 15) / 16; ++d) {
+        const uint32_t off = (d / 4) * kRows * 128 + (d % 4) * 32;
+        mma_ss(tmem, smem_desc(q_at + off, 16), smem_desc(k_at + off, 16), desc, d > 0);
+      }
+      mma_commit(&s_full);
+    }
+    __syncwarp();
+    const float c = a.scale * kLog2e;
+    const int chunks = (s.k + 31) / 32;
+    warp_wait(&s_full, 0, dead);
+    tc_fence_after();
+    float m = -INFINITY;
+    for (int i = 0; i < chunks; ++i) {
+      uint32_t x[32];
+      tmem_ld32(x, s_at + i * 32);
+      tmem_wait_ld();
+      const int left = limit - i * 32;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) m = e < left ? fmaxf(m, __uint_as_float(x[e])) : m;
+    }
+    base = m == -INFINITY ? 0.f : m * c;
+    // a chunk's weights go to columns that its own scores or earlier ones had
+    for (int i = 0; i < chunks; ++i) {
+      uint32_t x[32], w[16];
+      tmem_ld32(x, s_at + i * 32);
+      tmem_wait_ld();
+      const int left = limit - i * 32;
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        float p0 = fast_exp2(fmaf(__uint_as_float(x[e]), c, -base)), p1 = fast_exp2(fmaf(__uint_as_float(x[e + 1]), c, -base));
+        p0 = e < left ? p0 : 0.f;
+        p1 = e + 1 < left ? p1 : 0.f;
+        sum += p0 + p1;
+        w[e / 2] = pack2<kBf16>(p0, p1);
+      }
+      tmem_st16(s_at + i * 16, w);
+    }
+    tmem_wait_st();
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      tc_fence_after();
+      const uint32_t desc = mma_desc(kBf16, kRows, up16(a.D), false, true), v_at = smem_addr(vs);
+      for (int t = 0; t < (s.k + 15) / 16; ++t)
+        mma_ts(tmem + 64, tmem + t * 8, smem_desc(v_at + t * 2048, kRows * 128), desc, t > 0);
+      mma_commit(&o_full);
+    }
+    __syncwarp();
+    warp_wait(&o_full, 0, dead);
+    tc_fence_after();
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 1
+    for (int i = 0; i < kDP; i += 32) {
+      uint32_t o[32];
+      tmem_ld32(o, o_at + i);
+      tmem_wait_ld();
+      if (row < s.q) {
+        if (sum == 0.f)
+          store_zeros(out, i, i + 32, a.D);
+        else
+          store_columns<kBf16>(out, o, i, a.D, inv);
+      }
+    }
+    tc_fence_before();
+  } else if (row < s.q) {
+    store_zeros(out, 0, kDP, a.D);
+  }
+  if (a.lse != nullptr && row < s.q)
+    a.lse[head * a.total_q + s.q0 + row] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
+  __syncthreads();
+  report(&dead_word, p.status);
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_free(tmem, L::kColumns);
+}
+
+// Backward. Shared memory: q, dO, k, v, and over v (not read after dP) first P, then dS, as [query][key] in two
+// halves of 64 keys, which the matrix instructions read either way: rows of keys for dQ = dS k, columns of queries for
+// dV = P^T dO and dK = dS^T q. dV is computed under the arithmetic on dP.
+// Tensor memory: scores, dP, and the gradients: in their place when the key head has one query head (kAlone), in
+// columns of their own when several heads' are summed.
+template <int kDP, bool kAlone>
+struct Backward {
+  static constexpr int kTileBytes = kRows * kDP * 2;
+  static constexpr int kWeightBytes = kRows * kRows * 2;
+  static constexpr int kSmem = 3 * kTileBytes + kWeightBytes + 1024;
+  static constexpr int kColumns = kDP == 64 && kAlone ? 256 : 512;
+  static constexpr int kCtas = kDP == 64 && kAlone ? 2 : 1;
+};
+
+template <bool kBf16, int kDP, bool kAlone>
+__global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
+    attention_short_bwd_kernel(const ShortDev p, const __grid_constant__ CUtensorMap q_map,
+                               const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                               const __grid_constant__ CUtensorMap g_map) {
+  using L = Backward<kDP, kAlone>;
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t kv_full, q_full, s_full, v_done, d_full;
+  __shared__ uint32_t tmem_base;
+  __shared__ int dead_word;
+  __shared__ float halves[2][kRows];
+  const AttnDev& a = p.a;
+  const int kv = blockIdx.x % a.kv_heads, stretch = blockIdx.x / a.kv_heads;
+  Sequence s;
+  if (!sequence_of(p, stretch, kv == 0, true, &s)) return;
+  uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* gs = qs + L::kTileBytes;
+  uint8_t* ks = gs + L::kTileBytes;
+  uint8_t* vs = ks + L::kTileBytes;
+  uint8_t* ps = vs;
+  const int warp = threadIdx.x / 32, half = warp / 4, row = threadIdx.x % 128;
+  volatile int* dead = &dead_word;
+  const bool work = s.q > 0 && s.k > 0 && !s.gap;
+  if (threadIdx.x == 0) {
+    mbar_init(&kv_full, 1);
+    mbar_init(&q_full, 1);
+    mbar_init(&s_full, 1);
+    mbar_init(&v_done, 1);
+    mbar_init(&d_full, 1);
+    dead_word = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    __syncwarp();
+    tmem_alloc(&tmem_base, L::kColumns);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base, lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+  const uint32_t dp = tmem + kRows, dv = kAlone && kDP == 64 ? tmem : tmem + 2 * kRows, dk = dv + kDP;
+  const uint32_t dq = kAlone && kDP == 64 ? tmem + 2 * kDP : tmem;
+  const uint32_t s_at = tmem + lanes + half * 64, dp_at = dp + lanes + half * 64;
+  const int shift = s.k - s.q, d_steps = (a.D + 15) / 16;
+  const int limit = row >= s.q ? 0 : (a.causal ? min(s.k, row + shift + 1) : s.k);
+  const int left = limit - half * 64;
+  const int chunks = max(0, min(2, (s.k - half * 64 + 31) / 32));
+  const int q_rows = (s.q + kBox - 1) / kBox * kBox, k_rows = (s.k + kBox - 1) / kBox * kBox;
+  const uint64_t c2 = pair(a.scale * kLog2e, a.scale * kLog2e);
+
+  for (int g = 0; g < a.group; ++g) {
+    const int head = kv * a.group + g;
+    uint16_t* dq_row = static_cast<uint16_t*>(a.dq) + (s.q0 + row) * a.dq_row + head * a.dq_head;
+    if (!work) {
+      if (half == 0 && row < s.q) store_zeros(dq_row, 0, kDP, a.D);
+      continue;
+    }
+    if (threadIdx.x == 0) {
+      mbar_expect(&kv_full, (g == 0 ? 2 : 1) * k_rows * kDP * 2);
+      if (g == 0) load_rows<kDP>(ks, &k_map, kv, s.k0, s.k, &kv_full);
+      load_rows<kDP>(vs, &v_map, kv, s.k0, s.k, &kv_full);   // again for each head: weights took its place
+      mbar_expect(&q_full, 2 * q_rows * kDP * 2);
+      load_rows<kDP>(qs, &q_map, head, s.q0, s.q, &q_full);
+      load_rows<kDP>(gs, &g_map, head, s.q0, s.q, &q_full);
+    }
+    __syncwarp();
+    float lse2 = 0.f;
+    if (row < s.q) {
+      lse2 = a.lse[head * a.total_q + s.q0 + row] * kLog2e;
+      if (lse2 == -INFINITY) lse2 = INFINITY;
+    }
+    warp_wait(&kv_full, g & 1, dead);
+    warp_wait(&q_full, g & 1, dead);
+    if (s.k % 16 != 0 || s.q % 16 != 0) {
+      zero_tail<kDP>(ks, s.k);
+      zero_tail<kDP>(qs, s.q);
+      zero_tail<kDP>(gs, s.q);
+      fence_async_smem();
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+      const uint32_t desc = mma_desc(kBf16, kRows, up16(s.k), false, false);
+      for (int d = 0; d < d_steps; ++d) {
+        const uint32_t off = (d / 4) * kRows * 128 + (d % 4) * 32;
+        mma_ss(tmem, smem_desc(smem_addr(qs) + off, 16), smem_desc(smem_addr(ks) + off, 16), desc, d > 0);
+      }
+      for (int d = 0; d < d_steps; ++d) {
+        const uint32_t off = (d / 4) * kRows * 128 + (d % 4) * 32;
+        mma_ss(dp, smem_desc(smem_addr(gs) + off, 16), smem_desc(smem_addr(vs) + off, 16), desc, d > 0);
+      }
+      mma_commit(&s_full);
+    }
+    __syncwarp();
+    warp_wait(&s_full, g & 1, dead);
+    tc_fence_after();
+    // ---- P, and the row's part of delta ----
+    float w[2][32];
+    float part[2] = {0.f, 0.f};
+    // a row of 64 keys is 128 bytes, its 16-byte pieces exchanged by the row's number, as the copies do it
+    uint8_t* p_row = ps + half * kRows * 128 + row * 128;
+    auto put = [&](int i) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 8)
+        *reinterpret_cast<uint4*>(p_row + (((i * 32 + e) / 8) ^ (row % 8)) * 16) =
+            make_uint4(pack2<kBf16>(w[i][e], w[i][e + 1]), pack2<kBf16>(w[i][e + 2], w[i][e + 3]),
+                       pack2<kBf16>(w[i][e + 4], w[i][e + 5]), pack2<kBf16>(w[i][e + 6], w[i][e + 7]));
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (i < chunks) {
+        uint32_t x[32];
+        tmem_ld32(x, s_at + i * 32);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float2 y = unpair(fma2(pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), c2, pair(-lse2, -lse2)));
+          w[i][e] = i * 32 + e < left ? fast_exp2(y.x) : 0.f;
+          w[i][e + 1] = i * 32 + e + 1 < left ? fast_exp2(y.y) : 0.f;
+        }
+        tmem_ld32(x, dp_at + i * 32);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) part[e & 1] += i * 32 + e < left ? w[i][e] * __uint_as_float(x[e]) : 0.f;
+      }
+    halves[half][row] = part[0] + part[1];
+    __syncthreads();   // also: all of dP is computed, so v may be written over
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (i < chunks) put(i);
+    fence_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    const uint32_t desc = mma_desc(kBf16, kRows, up16(a.D), true, true);
+    if (threadIdx.x == 0) {
+      tc_fence_after();
+      for (int t = 0; t < (s.q + 15) / 16; ++t)
+        mma_ss(dv, smem_desc(smem_addr(ps) + t * 2048, kRows * 128), smem_desc(smem_addr(gs) + t * 2048, kRows * 128), desc,
+               g > 0 || t > 0);
+      mma_commit(&v_done);
+    }
+    __syncwarp();
+    // ---- dS ----
+    const float delta = halves[0][row] + halves[1][row];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (i < chunks) {
+        uint32_t x[32];
+        tmem_ld32(x, dp_at + i * 32);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) w[i][e] = i * 32 + e < left ? w[i][e] * (__uint_as_float(x[e]) - delta) : 0.f;
+      }
+    warp_wait(&v_done, g & 1, dead);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (i < chunks) put(i);
+    fence_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      tc_fence_after();
+      for (int t = 0; t < (s.q + 15) / 16; ++t)
+        mma_ss(dk, smem_desc(smem_addr(ps) + t * 2048, kRows * 128), smem_desc(smem_addr(qs) + t * 2048, kRows * 128), desc,
+               g > 0 || t > 0);
+      const uint32_t dq_desc = mma_desc(kBf16, kRows, up16(a.D), false, true);
+      for (int t = 0; t < (s.k + 15) / 16; ++t)
+        mma_ss(dq, smem_desc(smem_addr(ps) + (t / 4) * kRows * 128 + (t % 4) * 32, 16),
+               smem_desc(smem_addr(ks) + t * 2048, kRows * 128), dq_desc, t > 0);
+      mma_commit(&d_full);
+    }
+    __syncwarp();
+    warp_wait(&d_full, g & 1, dead);
+    tc_fence_after();
+#pragma unroll 1
+    for (int i = half * kDP / 2; i < (half + 1) * kDP / 2; i += 32) {
+      uint32_t o[32];
+      tmem_ld32(o, dq + lanes + i);
+      tmem_wait_ld();
+      if (row < s.q) store_columns<kBf16>(dq_row, o, i, a.D, a.scale);
+    }
+    tc_fence_before();
+    __syncthreads();   // before the next head's copies and products
+    tc_fence_after();
+  }
+  uint16_t* out = half == 0 ? static_cast<uint16_t*>(a.dv) + (s.k0 + row) * a.dv_row + kv * a.dv_head
+                            : static_cast<uint16_t*>(a.dk) + (s.k0 + row) * a.dk_row + kv * a.dk_head;
+  if (work) {
+#pragma unroll 1
+    for (int i = 0; i < kDP; i += 32) {
+      uint32_t o[32];
+      tmem_ld32(o, (half == 0 ? dv : dk) + lanes + i);
+      tmem_wait_ld();
+      if (row < s.k) store_columns<kBf16>(out, o, i, a.D, half == 0 ? 1.f : a.scale);
+    }
+  } else if (row < s.k) {
+    store_zeros(out, 0, kDP, a.D);
+  }
+  tc_fence_before();
+  __syncthreads();
+  report(&dead_word, p.status);
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_free(tmem, L::kColumns);
+}
+
+template <bool kBf16, int kDP>
+int launch_forward(const ShortDev& p, cudaStream_t stream) {
+  using L = Forward<kDP>;
+  const AttnDev& a = p.a;
+  CUtensorMap q, k, v;
+  if (!rows_map(&q, kBf16, a.q, a.total_q, a.heads, a.D, a.q_row, a.q_head, kBox) ||
+      !rows_map(&k, kBf16, a.k, a.total_k, a.kv_heads, a.D, a.k_row, a.k_head, kBox) ||
+      !rows_map(&v, kBf16, a.v, a.total_k, a.kv_heads, a.D, a.v_row, a.v_head, kBox))
+    return B200TBE_ERR_UNSUPPORTED;
+  const int64_t blocks = (static_cast<int64_t>(a.batch) + 2) * a.heads;
+  if (blocks > 0x7fffffff) return B200TBE_ERR_UNSUPPORTED;
+  const auto kernel = attention_short_fwd_kernel<kBf16, kDP>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess) return B200TBE_ERR_LAUNCH;
+  kernel<<<static_cast<unsigned>(blocks), 128, L::kSmem, stream>>>(p, q, k, v);
+  return launch_status();
+}
+
+template <bool kBf16, int kDP, bool kAlone>
+int launch_backward(const ShortDev& p, cudaStream_t stream) {
+  using L = Backward<kDP, kAlone>;
+  const AttnDev& a = p.a;
+  CUtensorMap q, k, v, g;
+  if (!rows_map(&q, kBf16, a.q, a.total_q, a.heads, a.D, a.q_row, a.q_head, kBox) ||
+      !rows_map(&k, kBf16, a.k, a.total_k, a.kv_heads, a.D, a.k_row, a.k_head, kBox) ||
+      !rows_map(&v, kBf16, a.v, a.total_k, a.kv_heads, a.D, a.v_row, a.v_head, kBox) ||
+      !rows_map(&g, kBf16, a.grad, a.total_q, a.heads, a.D, a.g_row, a.g_head, kBox))
+    return B200TBE_ERR_UNSUPPORTED;
+  const int64_t blocks = (static_cast<int64_t>(a.batch) + 2) * a.kv_heads;
+  if (blocks > 0x7fffffff) return B200TBE_ERR_UNSUPPORTED;
+  const auto kernel = attention_short_bwd_kernel<kBf16, kDP, kAlone>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess) return B200TBE_ERR_LAUNCH;
+  kernel<<<static_cast<unsigned>(blocks), 256, L::kSmem, stream>>>(p, q, k, v, g);
+  return launch_status();
+}
+
+template <bool kBf16>
+int backward_of(const ShortDev& p, cudaStream_t stream) {
+  if (p.a.D <= 64)
+    return p.a.group == 1 ? launch_backward<kBf16, 64, true>(p, stream) : launch_backward<kBf16, 64, false>(p, stream);
+  return launch_backward<kBf16, 128, false>(p, stream);
+}
+
+}  // namespace
+
+int attention_short_forward(const AttnDev& a, const TileList& plan, int dtype, int32_t* status, cudaStream_t stream) {
+  const ShortDev p{a, plan, status};
+  if (dtype == B200TBE_BF16) return a.D <= 64 ? launch_forward<true, 64>(p, stream) : launch_forward<true, 128>(p, stream);
+  return a.D <= 64 ? launch_forward<false, 64>(p, stream) : launch_forward<false, 128>(p, stream);
+}
+
+int attention_short_backward(const AttnDev& a, const TileList& plan, int dtype, int32_t* status, cudaStream_t stream) {
+  const ShortDev p{a, plan, status};
+  return dtype == B200TBE_BF16 ? backward_of<true>(p, stream) : backward_of<false>(p, stream);
+}
+
+}  // namespace b200tbe

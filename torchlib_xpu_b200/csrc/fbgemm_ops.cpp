@@ -500,7 +500,13 @@ std::tuple<Tensor, Tensor> jagged_attention_forward(const Tensor& q_, const Tens
   Tensor out = at::empty(q.sizes(), q.options());
   Tensor lse;
   if (keep_lse) lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
-  const auto p = attention_params(q, k, v, q_offsets, k_offsets, causal, scale, out, lse);
+  auto p = attention_params(q, k, v, q_offsets, k_offsets, causal, scale, out, lse);
+  Tensor scratch;
+  if (p.dtype != B200TBE_FP32) {
+    scratch = at::empty({static_cast<int64_t>(b200tbe_jagged_attention_scratch_bytes(p.total_q, p.batch))},
+                        q.options().dtype(at::kByte));
+    p.scratch = scratch.data_ptr(), p.scratch_bytes = static_cast<size_t>(scratch.numel());
+  }
   check_status(b200tbe_jagged_attention(&p, current_stream()), "b200tbe_jagged_attention");
   return {out, lse};
 }

@@ -124,6 +124,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) 
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t (&r)[16], uint32_t at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at));
+}
+
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
@@ -183,6 +191,9 @@ __device__ __forceinline__ float2 unpair(uint64_t x) {
   float2 r;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
   return r;
+}
+__device__ __forceinline__ uint64_t as_pair(const uint32_t* x) {
+  return pair(__uint_as_float(x[0]), __uint_as_float(x[1]));
 }
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
