@@ -85,21 +85,6 @@ __device__ __forceinline__ void load_tile(uint8_t* tile, const CUtensorMap* map,
   for (int x = 0; x < kDP / 64; ++x) tma_load_3d(tile + x * kRows * 128, map, x * 64, head, row, bar);
 }
 
-// d[128][n] (+)= a b^T over the head dimension, both operands rows of it
-__device__ __forceinline__ void product_over_d(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, int steps) {
-  for (int t = 0; t < steps; ++t) {
-    const uint32_t off = (t / 4) * kRows * 128 + (t % 4) * 32;
-    mma_ss(d, smem_desc(a + off, 16), smem_desc(b + off, 16), desc, t > 0);
-  }
-}
-
-// d[128][D] (+)= w x: w in tensor memory (two 16-bit weights a column, 64 in the first 32 columns, 64 from column
-// 64 on), x rows of the head dimension
-__device__ __forceinline__ void product_over_rows(uint32_t d, uint32_t w, uint32_t x, uint32_t desc, int steps, bool add) {
-  for (int t = 0; t < steps; ++t)
-    mma_ts(d, w + t * 8 + (t >= 4 ? 32 : 0), smem_desc(x + t * 2048, kRows * 128), desc, add || t > 0);
-}
-
 // A row of the accumulator in tensor memory, times f, to memory.
 template <bool kBf16, int kDP>
 __device__ __forceinline__ void store_row(void* out, uint32_t at, int D, float f, bool computed, bool inside) {
@@ -212,8 +197,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (keys % 16 != 0) zero_tail<kDP>(ks + (j & 1) * L::kTileBytes, keys);
           if (j > 0 && !warp_wait(&bars.s_loaded, (j - 1) & 1, dead)) return false;
           tc_fence_after();
-          if (lane == 0) {
-            product_over_d(tmem, q_at, smem_addr(ks + (j & 1) * L::kTileBytes),
+          if (elect_one()) {
+            mma_along_k<kDP / 16, kRows>(tmem, q_at, smem_addr(ks + (j & 1) * L::kTileBytes),
                            mma_desc(kBf16, kRows, (keys + 15) & ~15, false, false), d_steps);
             mma_commit(&bars.s_full);
           }
@@ -223,8 +208,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto d_weights = [&](int j) {
           const bool ok = warp_wait(&bars.v_full[j & 1], (j / 2) & 1, dead);
           if (!ok) return false;
-          if (lane == 0) {
-            product_over_d(dp_at, g_at, smem_addr(vs + (j & 1) * L::kTileBytes),
+          if (elect_one()) {
+            mma_along_k<kDP / 16, kRows>(dp_at, g_at, smem_addr(vs + (j & 1) * L::kTileBytes),
                            mma_desc(kBf16, kRows, (keys_of(j) + 15) & ~15, false, false), d_steps);
             mma_commit(&bars.dp_full);
             if (j + 2 < n) mma_commit(&bars.v_empty[j & 1]);
@@ -237,8 +222,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j + 1 < n) alive = scores(j + 1);
           alive = alive && warp_wait(&bars.ds_full, j & 1, dead);
           tc_fence_after();
-          if (alive && lane == 0) {
-            product_over_rows(dq_at, dp_at, smem_addr(ks + (j & 1) * L::kTileBytes), dq_desc, (keys_of(j) + 15) / 16, j > 0);
+          if (alive && elect_one()) {
+            mma_over_rows<32>(dq_at, dp_at, smem_addr(ks + (j & 1) * L::kTileBytes), dq_desc, (keys_of(j) + 15) / 16, j > 0);
             if (j + 2 < n) mma_commit(&bars.k_empty[j & 1]);
             if (j + 1 == n) mma_commit(&bars.done);
           }
@@ -419,16 +404,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           return ok;
         };
         auto scores = [&](int j) {
-          if (lane == 0) {
-            product_over_d(tmem, k_at, smem_addr(qs + (j & 1) * L::kTileBytes),
+          if (elect_one()) {
+            mma_along_k<kDP / 16, kRows>(tmem, k_at, smem_addr(qs + (j & 1) * L::kTileBytes),
                            mma_desc(kBf16, kRows, (rows_of(j) + 15) & ~15, false, false), d_steps);
             mma_commit(&bars.s_full);
           }
           __syncwarp();
         };
         auto d_weights = [&](int j) {
-          if (lane == 0) {
-            product_over_d(dp_at, v_at, smem_addr(gs + (j & 1) * L::kTileBytes),
+          if (elect_one()) {
+            mma_along_k<kDP / 16, kRows>(dp_at, v_at, smem_addr(gs + (j & 1) * L::kTileBytes),
                            mma_desc(kBf16, kRows, (rows_of(j) + 15) & ~15, false, false), d_steps);
             mma_commit(&bars.dp_full);
           }
@@ -445,14 +430,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           alive = (!more || ready(j + 1)) && warp_wait(&bars.p_full, j & 1, dead);
           if (!alive) break;
           tc_fence_after();
-          if (lane == 0) product_over_rows(dv_at, tmem, smem_addr(gs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
+          if (elect_one()) mma_over_rows<32>(dv_at, tmem, smem_addr(gs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
           __syncwarp();
           if (more) scores(j + 1);
           alive = warp_wait(&bars.ds_full, j & 1, dead);
           if (!alive) break;
           tc_fence_after();
-          if (lane == 0) {
-            product_over_rows(dk_at, dp_at, smem_addr(qs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
+          if (elect_one()) {
+            mma_over_rows<32>(dk_at, dp_at, smem_addr(qs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
             if (j + 2 < n) mma_commit(&bars.q_empty[j & 1]);
             if (!more) mma_commit(&bars.done);
           }

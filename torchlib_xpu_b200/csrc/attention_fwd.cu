@@ -170,15 +170,12 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
           const int keys = min(kRows, (klen - j * kRows + 15) & ~15);
           const uint32_t desc = mma_desc(kBf16, kRows, keys, false, false);
           const uint32_t q_at = smem_addr(qs + s * L::kTileBytes), k_at = smem_addr(ks + (j % L::kStages) * L::kTileBytes);
-          for (int d = 0; d < d_steps; ++d) {
-            const uint32_t off = (d / 4) * kRows * 128 + (d % 4) * 32;
-            mma_ss(tmem + s * kRows, smem_desc(q_at + off, 16), smem_desc(k_at + off, 16), desc, d > 0);
-          }
+          mma_along_k<kDP / 16, kRows>(tmem + s * kRows, q_at, k_at, desc, d_steps);
           mma_commit(&bars.b.s_full[s]);
         };
         if (alive && most > 0) {
           alive = warp_wait(&bars.b.k_full[0], 0, dead);
-          if (alive && lane == 0) {
+          if (alive && elect_one()) {
 #pragma unroll
             for (int s = 0; s < kNQ; ++s)
               if (n[s] > 0) scores(s, 0);
@@ -207,19 +204,17 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
             if (j < n[s]) {
               alive = alive && warp_wait(&bars.b.p_full[s], j & 1, dead);
               tc_fence_after();
-              if (alive && lane == 0) {
-                for (int t = 0; t < steps; ++t)
-                  mma_ts(tmem + kNQ * kRows + s * kDP, tmem + s * kRows + 64 + t * 8, smem_desc(v_at + t * 2048, kRows * 128), pv_desc,
-                         j > 0 || t > 0);
+              if (alive && elect_one()) {
+                mma_over_rows<0>(tmem + kNQ * kRows + s * kDP, tmem + s * kRows + 64, v_at, pv_desc, steps, j > 0);
                 if (j + 1 == n[s]) mma_commit(&bars.b.o_full[s]);
               }
             }
             if (j + 1 < n[s]) {
               alive = alive && warp_wait(&bars.b.k_full[next], ((j + 1) / L::kStages) & 1, dead);
-              if (alive && lane == 0) scores(s, j + 1);
+              if (alive && elect_one()) scores(s, j + 1);
             }
           }
-          if (alive && lane == 0) {
+          if (alive && elect_one()) {
             if (j + L::kStages < most) mma_commit(&bars.b.v_empty[st]);
             if (j + 1 + L::kStages < most) mma_commit(&bars.b.k_empty[next]);
           }

@@ -170,12 +170,9 @@ __global__ void __launch_bounds__(128, Forward<kDP>::kCtas)
       fence_async_smem();
       __syncthreads();
     }
-    if (threadIdx.x == 0) {
-      const uint32_t desc = mma_desc(kBf16, kRows, up16(s.k), false, false), q_at = smem_addr(qs), k_at = smem_addr(ks);
-      for (int d = 0; d < (a.D + 15) / 16; ++d) {
-        const uint32_t off = (d / 4) * kRows * 128 + (d % 4) * 32;
-        mma_ss(tmem, smem_desc(q_at + off, 16), smem_desc(k_at + off, 16), desc, d > 0);
-      }
+    if (warp == 0 && elect_one()) {
+      mma_along_k<kDP / 16, kRows>(tmem, smem_addr(qs), smem_addr(ks), mma_desc(kBf16, kRows, up16(s.k), false, false),
+                                   (a.D + 15) / 16);
       mma_commit(&s_full);
     }
     __syncwarp();
@@ -212,11 +209,9 @@ __global__ void __launch_bounds__(128, Forward<kDP>::kCtas)
     tmem_wait_st();
     tc_fence_before();
     __syncthreads();
-    if (threadIdx.x == 0) {
-      tc_fence_after();
-      const uint32_t desc = mma_desc(kBf16, kRows, up16(a.D), false, true), v_at = smem_addr(vs);
-      for (int t = 0; t < (s.k + 15) / 16; ++t)
-        mma_ts(tmem + 64, tmem + t * 8, smem_desc(v_at + t * 2048, kRows * 128), desc, t > 0);
+    tc_fence_after();
+    if (warp == 0 && elect_one()) {
+      mma_over_rows<0>(tmem + 64, tmem, smem_addr(vs), mma_desc(kBf16, kRows, up16(a.D), false, true), (s.k + 15) / 16, false);
       mma_commit(&o_full);
     }
     __syncwarp();
@@ -261,6 +256,14 @@ struct Backward {
   static constexpr int kColumns = kDP == 64 && kAlone ? 256 : 512;
   static constexpr int kCtas = kDP == 64 && kAlone ? 2 : 1;
 };
+
+// d[key][.] (+)= sum over queries of w[query][key] x[query][.], 16 queries a step
+__device__ __forceinline__ void transposed(uint32_t d, uint32_t w, uint32_t x, uint32_t desc, int steps, bool add) {
+  const uint64_t w0 = smem_desc(w, kRows * 128), x0 = smem_desc(x, kRows * 128);
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+    if (t < steps) mma_ss(d, w0 + t * (2048 >> 4), x0 + t * (2048 >> 4), desc, t > 0 || add);
+}
 
 template <bool kBf16, int kDP, bool kAlone>
 __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
@@ -342,16 +345,10 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
       fence_async_smem();
       __syncthreads();
     }
-    if (threadIdx.x == 0) {
+    if (warp == 0 && elect_one()) {
       const uint32_t desc = mma_desc(kBf16, kRows, up16(s.k), false, false);
-      for (int d = 0; d < d_steps; ++d) {
-        const uint32_t off = (d / 4) * kRows * 128 + (d % 4) * 32;
-        mma_ss(tmem, smem_desc(smem_addr(qs) + off, 16), smem_desc(smem_addr(ks) + off, 16), desc, d > 0);
-      }
-      for (int d = 0; d < d_steps; ++d) {
-        const uint32_t off = (d / 4) * kRows * 128 + (d % 4) * 32;
-        mma_ss(dp, smem_desc(smem_addr(gs) + off, 16), smem_desc(smem_addr(vs) + off, 16), desc, d > 0);
-      }
+      mma_along_k<kDP / 16, kRows>(tmem, smem_addr(qs), smem_addr(ks), desc, d_steps);
+      mma_along_k<kDP / 16, kRows>(dp, smem_addr(gs), smem_addr(vs), desc, d_steps);
       mma_commit(&s_full);
     }
     __syncwarp();
@@ -395,11 +392,10 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
     tc_fence_before();
     __syncthreads();
     const uint32_t desc = mma_desc(kBf16, kRows, up16(a.D), true, true);
-    if (threadIdx.x == 0) {
-      tc_fence_after();
-      for (int t = 0; t < (s.q + 15) / 16; ++t)
-        mma_ss(dv, smem_desc(smem_addr(ps) + t * 2048, kRows * 128), smem_desc(smem_addr(gs) + t * 2048, kRows * 128), desc,
-               g > 0 || t > 0);
+    const int q_steps = (s.q + 15) / 16;
+    tc_fence_after();
+    if (warp == 0 && elect_one()) {
+      transposed(dv, smem_addr(ps), smem_addr(gs), desc, q_steps, g > 0);
       mma_commit(&v_done);
     }
     __syncwarp();
@@ -421,15 +417,15 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
     fence_async_smem();
     tc_fence_before();
     __syncthreads();
-    if (threadIdx.x == 0) {
-      tc_fence_after();
-      for (int t = 0; t < (s.q + 15) / 16; ++t)
-        mma_ss(dk, smem_desc(smem_addr(ps) + t * 2048, kRows * 128), smem_desc(smem_addr(qs) + t * 2048, kRows * 128), desc,
-               g > 0 || t > 0);
+    tc_fence_after();
+    if (warp == 0 && elect_one()) {
+      transposed(dk, smem_addr(ps), smem_addr(qs), desc, q_steps, g > 0);
       const uint32_t dq_desc = mma_desc(kBf16, kRows, up16(a.D), false, true);
-      for (int t = 0; t < (s.k + 15) / 16; ++t)
-        mma_ss(dq, smem_desc(smem_addr(ps) + (t / 4) * kRows * 128 + (t % 4) * 32, 16),
-               smem_desc(smem_addr(ks) + t * 2048, kRows * 128), dq_desc, t > 0);
+      const uint64_t w0 = smem_desc(smem_addr(ps), 16), x0 = smem_desc(smem_addr(ks), kRows * 128);
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        if (t < (s.k + 15) / 16)
+          mma_ss(dq, w0 + (((t / 4) * kRows * 128 + (t % 4) * 32) >> 4), x0 + t * (2048 >> 4), dq_desc, t > 0);
       mma_commit(&d_full);
     }
     __syncwarp();

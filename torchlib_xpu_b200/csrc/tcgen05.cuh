@@ -150,6 +150,15 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
          (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// One thread of a warp that is together here; the same one each time. (The compiler keeps what follows in uniform
+// registers, where the matrix instruction wants its operands: with a lane number instead, moving them there took
+// longer than the instructions themselves.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+  return one != 0;
+}
+
 // fp32 accumulators, both operands bf16 or both fp16
 __device__ __forceinline__ constexpr uint32_t mma_desc(bool bf16, int m, int n, bool a_mn_major, bool b_mn_major) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn_major ? 1u : 0u) << 15) |
@@ -169,6 +178,28 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "l"(b), "r"(desc), "r"(static_cast<uint32_t>(add))
       : "memory");
 }
+// d[128][n] (+)= a b^T over up to kMost x 16 elements of k, both operands along k: rows of 64 elements in tiles of
+// `rows` x 128 bytes. Unrolled, so that a step costs two additions beside the instruction.
+template <int kMost, int kRowsOfTile>
+__device__ __forceinline__ void mma_along_k(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, int steps) {
+  const uint64_t a0 = smem_desc(a, 16), b0 = smem_desc(b, 16);
+#pragma unroll
+  for (int t = 0; t < kMost; ++t) {
+    const uint64_t off = ((t / 4) * kRowsOfTile * 128 + (t % 4) * 32) >> 4;
+    if (t < steps) mma_ss(d, a0 + off, b0 + off, desc, t > 0);
+  }
+}
+
+// d[128][n] (+)= w x over up to 128 rows of x, 16 a step: w in tensor memory, two 16-bit elements a column, the second
+// 64 of them kSkip columns further on; x in tiles of 128 rows, n along the row.
+template <int kSkip>
+__device__ __forceinline__ void mma_over_rows(uint32_t d, uint32_t w, uint32_t x, uint32_t desc, int steps, bool add) {
+  const uint64_t x0 = smem_desc(x, 128 * 128);
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+    if (t < steps) mma_ts(d, w + t * 8 + (t >= 4 ? kSkip : 0), x0 + t * (2048 >> 4), desc, t > 0 || add);
+}
+
 // Arrives once all matrix instructions that this thread has issued are done. Some thread has to wait for it: an
 // arrival nobody waits for could come after the barrier's memory has been given to something else.
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
