@@ -414,7 +414,9 @@ int launch(const FwdDev& p, int64_t slots, cudaStream_t stream) {
   if (blocks > 0x7fffff00) return p.listed ? B200TBE_ERR_UNSUPPORTED : B200TBE_ERR_TOO_LARGE;
   if (p.listed && blocks > kNumSMs * L::kCtas) blocks = kNumSMs * L::kCtas;
   const auto kernel = attention_fwd_kernel<kBf16, kDP, kNQ>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess) return B200TBE_ERR_LAUNCH;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess)
+    return B200TBE_ERR_LAUNCH;
   kernel<<<static_cast<unsigned>(blocks), L::kThreads, L::kSmem, stream>>>(p, q, k, v);
   return launch_status();
 }
