@@ -89,7 +89,7 @@ __device__ __forceinline__ void load_tile(uint8_t* tile, const CUtensorMap* map,
 template <bool kBf16, int kDP>
 __device__ __forceinline__ void store_row(void* out, uint32_t at, int D, float f, bool computed, bool inside) {
 #pragma unroll 1
-  for (int i = 0; i < kDP / 32; ++i) {
+  for (int i = 0; i < kDP / 32 && __any_sync(kFullMask, inside); ++i) {
     uint32_t o[32];
     if (computed) {
       tmem_ld32(o, at + i * 32);
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         alive = warp_wait(&bars.s_full, j & 1, dead);
         if (!alive) break;
         tc_fence_after();
-        const int chunks = max(0, min(2, (klen - j * kRows - half * 64 + 31) / 32));
+        const int chunks = row - lane < it.len ? max(0, min(2, (klen - j * kRows - half * 64 + 31) / 32)) : 0;
         const int left = limit - j * kRows - half * 64;
         uint32_t s[2][32];
 #pragma unroll
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         alive = warp_wait(&bars.stat_full[st], (j / 2) & 1, dead) && warp_wait(&bars.s_full, j & 1, dead);
         if (!alive) break;
         tc_fence_after();
-        const int chunks = max(0, min(2, (qlen - i0 + 31) / 32));
+        const int chunks = key - lane < it.len ? max(0, min(2, (qlen - i0 + 31) / 32)) : 0;
         // columns [low, high) are queries of the sequence that see the key
         const int low = a.causal ? key - shift - i0 : 0, high = qlen - i0;
         const bool cut = __any_sync(kFullMask, low > 0 || high < 64);

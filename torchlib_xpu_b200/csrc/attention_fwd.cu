@@ -270,7 +270,8 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
         if (!alive) break;
         tc_fence_after();
         const int left = limit - j * kRows;                        // of this tile, for this row
-        const int chunks = min(4, (klen - j * kRows + 31) / 32);   // 32 columns each, of the tile
+        // 32 columns each, of the tile; a warp whose rows are all behind the last computes nothing
+        const int chunks = row - lane < qlen ? min(4, (klen - j * kRows + 31) / 32) : 0;
         const bool cut = __any_sync(kFullMask, left < kRows);
         // The scores of the columns [32 from, 32 (from + kN)) into registers, masked; returns their maximum.
         auto fetch = [&](auto& x, int from) {

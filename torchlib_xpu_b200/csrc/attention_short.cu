@@ -184,7 +184,9 @@ __global__ void __launch_bounds__(128, Forward<kDP>::kCtas)
   }
   for (uint32_t phase = 0; item < items; phase ^= 1) {
     const int next = next_work(item + gridDim.x, &n), head = item % a.heads;
-    warp_wait(&qk_full, phase, dead);
+    // Only this warp: the next copies may complete before another one has looked, and a barrier two phases on looks
+    // as it did before. (The other barriers' next phases come after a __syncthreads() behind every warp's wait.)
+    if (warp == 0) warp_wait(&qk_full, phase, dead);
     if (warp == 0 && elect_one()) {
       mma_along_k<kDP / 16, kRows>(tmem, smem_addr(qs), smem_addr(ks), mma_desc(kBf16, kRows, up16(s.k), false, false),
                                    (a.D + 15) / 16);
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(128, Forward<kDP>::kCtas)
     __syncwarp();
     const int shift = s.k - s.q;
     const int limit = row >= s.q ? 0 : (a.causal ? min(s.k, row + shift + 1) : s.k);
-    const int chunks = (s.k + 31) / 32;
+    const int chunks = warp * 32 < s.q ? (s.k + 31) / 32 : 0;   // a warp whose rows are all behind the last computes nothing
     float sum = 0.f;
     warp_wait(&s_full, phase, dead);
     tc_fence_after();
@@ -253,8 +255,10 @@ __global__ void __launch_bounds__(128, Forward<kDP>::kCtas)
     tc_fence_after();
     if (next < items && threadIdx.x == 0) copy_v(next, n);
     uint32_t o[kDP / 32][32];
+    if (warp * 32 < s.q) {
 #pragma unroll
-    for (int i = 0; i < kDP / 32; ++i) tmem_ld32(o[i], o_at + i * 32);
+      for (int i = 0; i < kDP / 32; ++i) tmem_ld32(o[i], o_at + i * 32);
+    }
     tmem_wait_ld();
     tc_fence_before();
     const int failed = __syncthreads_or(*dead);   // also: the next scores may come
@@ -388,7 +392,8 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
     const int shift = s.k - s.q, q_steps = (s.q + 15) / 16;
     const int limit = row >= s.q ? 0 : (a.causal ? min(s.k, row + shift + 1) : s.k);
     const int left = limit - half * 64;
-    const int chunks = max(0, min(2, (s.k - half * 64 + 31) / 32));
+    // a warp whose rows are all behind the last computes nothing
+    const int chunks = warp % 4 * 32 < s.q ? max(0, min(2, (s.k - half * 64 + 31) / 32)) : 0;
     for (int g = 0; g < a.group; ++g, phase ^= 1) {
       const int head = kv * a.group + g;
       float lse2 = 0.f;
@@ -513,7 +518,7 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
       }
       __syncwarp();
 #pragma unroll 1
-      for (int i = half * kDP / 2; i < (half + 1) * kDP / 2; i += 32) {
+      for (int i = half * kDP / 2; i < (half + 1) * kDP / 2 && warp % 4 * 32 < s.q; i += 32) {
         uint32_t o[32];
         tmem_ld32(o, dq + lanes + i);
         tmem_wait_ld();
@@ -521,7 +526,7 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
       }
       if (g + 1 == a.group) {
 #pragma unroll 1
-        for (int i = 0; i < kDP; i += 32) {
+        for (int i = 0; i < kDP && warp % 4 * 32 < s.k; i += 32) {
           uint32_t o[32];
           tmem_ld32(o, (half == 0 ? dv : dk) + lanes + i);
           tmem_wait_ld();
