@@ -82,35 +82,23 @@ __device__ __forceinline__ void zero_tail(uint8_t* tile, int rows) {
 
 template <int kDP>
 __device__ __forceinline__ void load_tile(uint8_t* tile, const CUtensorMap* map, int head, int row, uint64_t* bar) {
-  for (int x = 0; x < kDP / 64; ++x) tma_load_3d(tile + x * kRows * 128, map, x * 64, head, row, bar);
+  for (int x = 0; x < kDP / 64; ++x) tma_load_3d(smem_addr(tile) + x * kRows * 128, map, x * 64, head, row, bar);
 }
 
-// A row of the accumulator in tensor memory, times f, to memory.
+// A warp's accumulator rows in tensor memory, times f, to memory: `rows` of them.
 template <bool kBf16, int kDP>
-__device__ __forceinline__ void store_row(void* out, uint32_t at, int D, float f, bool computed, bool inside) {
+__device__ __forceinline__ void store_rows(uint8_t* stage, uint16_t* out, int64_t stride, uint32_t at, int D, float f,
+                                           bool computed, int rows) {
 #pragma unroll 1
-  for (int i = 0; i < kDP / 32 && __any_sync(kFullMask, inside); ++i) {
+  for (int i = 0; i < kDP && rows > 0; i += 32) {
     uint32_t o[32];
     if (computed) {
-      tmem_ld32(o, at + i * 32);
+      tmem_ld32(o, at + i);
       tmem_wait_ld();
     }
-    if (inside) {
-#pragma unroll
-      for (int e = 0; e < 32; e += 8) {
-        if (i * 32 + e < D) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (computed) {
-            v.x = pack2<kBf16>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f);
-            v.y = pack2<kBf16>(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
-            v.z = pack2<kBf16>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f);
-            v.w = pack2<kBf16>(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f);
-          }
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + i * 32 + e) = v;
-        }
-      }
-    }
+    store_columns<kBf16>(stage, o, f, !computed, out, stride, rows, i, D);
   }
+  fence_async_smem();
 }
 
 // x = exp2(x c + m) in place, two and two
@@ -315,8 +303,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (alive && n > 0) alive = warp_wait(&bars.done, 0, dead);
       tc_fence_after();
       if (half == 0)
-        store_row<kBf16, kDP>(static_cast<uint16_t*>(a.dq) + (it.begin + row) * a.dq_row + it.head * a.dq_head, dq_at + lanes,
-                              a.D, a.scale, alive && n > 0, row < it.len);
+        store_rows<kBf16, kDP>(qs + warp * 2048, static_cast<uint16_t*>(a.dq) + (it.begin + row - lane) * a.dq_row + it.head * a.dq_head,
+                               a.dq_row, dq_at + lanes, a.D, a.scale, n > 0, it.len - row + lane);
       tc_fence_before();
       __syncthreads();
       tc_fence_after();
@@ -548,11 +536,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (alive && n > 0) alive = warp_wait(&bars.done, 0, dead);
       tc_fence_after();
       if (half == 0)
-        store_row<kBf16, kDP>(static_cast<uint16_t*>(a.dv) + (it.begin + key) * a.dv_row + it.head * a.dv_head, dv_at + lanes,
-                              a.D, 1.f, alive && n > 0, key < it.len);
+        store_rows<kBf16, kDP>(ks + warp * 2048, static_cast<uint16_t*>(a.dv) + (it.begin + key - lane) * a.dv_row + it.head * a.dv_head,
+                               a.dv_row, dv_at + lanes, a.D, 1.f, n > 0, it.len - key + lane);
       else
-        store_row<kBf16, kDP>(static_cast<uint16_t*>(a.dk) + (it.begin + key) * a.dk_row + it.head * a.dk_head, dk_at + lanes,
-                              a.D, a.scale, alive && n > 0, key < it.len);
+        store_rows<kBf16, kDP>(ks + warp * 2048, static_cast<uint16_t*>(a.dk) + (it.begin + key - lane) * a.dk_row + it.head * a.dk_head,
+                               a.dk_row, dk_at + lanes, a.D, a.scale, n > 0, it.len - key + lane);
       tc_fence_before();
       __syncthreads();
       tc_fence_after();

@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
           mbar_expect(&bars.b.q_full, kNQ * L::kTileBytes);
           for (int s = 0; s < kNQ; ++s)
             for (int x = 0; x < kDP / 64; ++x)
-              tma_load_3d(qs + s * L::kTileBytes + x * kRows * 128, &q_map, x * 64, head + (pair_heads ? s : 0),
+              tma_load_3d(smem_addr(qs) + s * L::kTileBytes + x * kRows * 128, &q_map, x * 64, head + (pair_heads ? s : 0),
                           static_cast<int>(begin) + row0 + (pair_heads ? 0 : s * kRows), &bars.b.q_full);
           for (int j = 0; j < most; ++j) {
             const int st = j % L::kStages;
@@ -152,12 +152,12 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
             if (j >= L::kStages && !mbar_wait(&bars.b.k_empty[st], before, dead)) break;
             mbar_expect(&bars.b.k_full[st], L::kTileBytes);
             for (int x = 0; x < kDP / 64; ++x)
-              tma_load_3d(ks + st * L::kTileBytes + x * kRows * 128, &k_map, x * 64, kv, static_cast<int>(k0) + j * kRows,
+              tma_load_3d(smem_addr(ks) + st * L::kTileBytes + x * kRows * 128, &k_map, x * 64, kv, static_cast<int>(k0) + j * kRows,
                           &bars.b.k_full[st]);
             if (j >= L::kStages && !mbar_wait(&bars.b.v_empty[st], before, dead)) break;
             mbar_expect(&bars.b.v_full[st], L::kTileBytes);
             for (int x = 0; x < kDP / 64; ++x)
-              tma_load_3d(vs + st * L::kTileBytes + x * kRows * 128, &v_map, x * 64, kv, static_cast<int>(k0) + j * kRows,
+              tma_load_3d(smem_addr(vs) + st * L::kTileBytes + x * kRows * 128, &v_map, x * 64, kv, static_cast<int>(k0) + j * kRows,
                           &bars.b.v_full[st]);
           }
         }
@@ -359,32 +359,22 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
       // ---- result ----
       if (alive && tiles > 0) alive = warp_wait(&bars.b.o_full[s], 0, dead);
       tc_fence_after();
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
       const int h = head + (pair_heads ? s : 0);
-      uint16_t* out = static_cast<uint16_t*>(a.out) + (begin + row) * a.o_row + h * a.o_head;
+      if (tiles == 0 && most > 0) warp_wait(&bars.b.q_full, 0, dead);
+      if (row - lane < qlen) {   // through the queries' place: they have come, and all products with them are done
+        uint16_t* out = static_cast<uint16_t*>(a.out) + (begin + row - lane) * a.o_row + h * a.o_head;
 #pragma unroll 1
-      for (int i = 0; i < kDP / 32; ++i) {
-        uint32_t o[32];
-        if (alive && tiles > 0) {
-          tmem_ld32(o, o_at + i * 32);
-          tmem_wait_ld();
-        }
-        if (row < qlen) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            if (i * 32 + e < a.D) {
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (sum != 0.f) {
-                v.x = pack2<kBf16>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-                v.y = pack2<kBf16>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-                v.z = pack2<kBf16>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-                v.w = pack2<kBf16>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-              }
-              *reinterpret_cast<uint4*>(out + i * 32 + e) = v;
-            }
+        for (int i = 0; i < kDP; i += 32) {
+          uint32_t o[32];
+          if (tiles > 0) {
+            tmem_ld32(o, o_at + i);
+            tmem_wait_ld();
           }
+          store_columns<kBf16>(qs + s * L::kTileBytes + warp % 4 * 2048, o, 1.f / sum, sum == 0.f || tiles == 0, out, a.o_row,
+                               qlen - row + lane, i, a.D);
         }
       }
+      fence_async_smem();
       if (a.lse != nullptr && row < qlen)
         a.lse[h * a.total_q + begin + row] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
       tc_fence_before();

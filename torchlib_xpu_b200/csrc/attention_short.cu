@@ -15,7 +15,7 @@ namespace b200tbe {
 namespace {
 
 constexpr int kRows = 128;   // queries and keys at most
-constexpr int kBox = 32;     // rows a tensor copy brings
+constexpr int kBox = 64;     // rows a tensor copy brings: fewer copies to issue than with 32, fewer rows than with 128
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct ShortDev {
@@ -24,82 +24,105 @@ struct ShortDev {
   int32_t* status;
 };
 
-struct Sequence {
-  int64_t q0, k0;
-  int q, k;
-  bool gap;   // rows of no sequence: they see nothing, and nothing sees them
+// A sequence and head: its rows, or q < 0 when there are no more.
+struct Job {
+  int q0, k0, q, k, head;
 };
 
-// The sequence of this CTA. false: it is not a short one; its tiles are on the list (by the first head's CTA), or
-// there is nothing to do.
-__device__ __forceinline__ bool sequence_of(const ShortDev& p, int stretch, bool first_head, bool list_keys, Sequence* s) {
-  const AttnDev& a = p.a;
-  s->q0 = stretch_bound(a.q_offsets, a.offset_bytes, a.batch, a.total_q, stretch);
-  s->k0 = stretch_bound(a.k_offsets, a.offset_bytes, a.batch, a.total_k, stretch);
-  const int64_t q = max(static_cast<int64_t>(0), stretch_bound(a.q_offsets, a.offset_bytes, a.batch, a.total_q, stretch + 1) - s->q0);
-  const int64_t k = max(static_cast<int64_t>(0), stretch_bound(a.k_offsets, a.offset_bytes, a.batch, a.total_k, stretch + 1) - s->k0);
-  s->q = static_cast<int>(q);
-  s->k = static_cast<int>(k);
-  s->gap = stretch < 1 || stretch > a.batch;
-  if (q <= kRows && k <= kRows) return q > 0 || k > 0;
-  if (!first_head) return false;
-  __shared__ int at;
-  for (int side = 0; side < (list_keys ? 2 : 1); ++side) {
-    const int n = static_cast<int>(((side == 0 ? q : k) + kRows - 1) / kRows);
-    if (n == 0) continue;
-    if (threadIdx.x == 0) at = atomicAdd(p.plan.counts + side, n);
-    __syncthreads();
-    const int room = side == 0 ? p.plan.q_room : p.plan.k_room;
-    int2* list = side == 0 ? p.plan.q_tiles : p.plan.k_tiles;
-    for (int t = threadIdx.x; t < n; t += blockDim.x)
-      if (at + t < room) list[at + t] = make_int2(stretch, side == 0 ? n - 1 - t : t);
-    __syncthreads();
-  }
-  return false;
-}
+// The jobs of a CTA, found by one of its warps (which has the fewest rows to compute): sequence after sequence, with
+// the offsets of the next one read ahead. What is not a short sequence's goes on the list of tiles on the way (by
+// its first head's finder), and rows that nothing reaches get their zeros.
+template <bool kBackward>
+struct Finder {
+  const ShortDev& p;
+  int stretch, head, step, head_step, heads;
+  int qa, qb, ka, kb;
 
-// rows [0, rows) of a head in boxes of kBox rows; returns the bytes that will arrive
-template <int kDP>
-__device__ __forceinline__ uint32_t load_rows(uint8_t* tile, const CUtensorMap* map, int head, int64_t row, int rows, uint64_t* bar) {
-  uint32_t bytes = 0;
-  for (int r = 0; r < rows; r += kBox)
-    for (int x = 0; x < kDP / 64; ++x) {
-      tma_load_3d(tile + x * kRows * 128 + r * 128, map, x * 64, head, static_cast<int>(row) + r, bar);
-      bytes += kBox * 128;
+  __device__ __forceinline__ Finder(const ShortDev& p_) : p(p_) {
+    heads = kBackward ? p.a.kv_heads : p.a.heads;
+    stretch = blockIdx.x / heads;
+    head = blockIdx.x - stretch * heads;
+    step = gridDim.x / heads;
+    head_step = gridDim.x - step * heads;
+    read();
+  }
+  __device__ __forceinline__ void read() {
+    const AttnDev& a = p.a;
+    qa = static_cast<int>(stretch_bound(a.q_offsets, a.offset_bytes, a.batch, a.total_q, stretch));
+    qb = static_cast<int>(stretch_bound(a.q_offsets, a.offset_bytes, a.batch, a.total_q, stretch + 1));
+    ka = static_cast<int>(stretch_bound(a.k_offsets, a.offset_bytes, a.batch, a.total_k, stretch));
+    kb = static_cast<int>(stretch_bound(a.k_offsets, a.offset_bytes, a.batch, a.total_k, stretch + 1));
+  }
+  __device__ __forceinline__ void list(int of, int side, int n) {
+    const int lane = threadIdx.x % 32, room = side == 0 ? p.plan.q_room : p.plan.k_room;
+    int2* tiles = side == 0 ? p.plan.q_tiles : p.plan.k_tiles;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(p.plan.counts + side, n);
+    at = __shfl_sync(kFullMask, at, 0);
+    for (int t = lane; t < n && at + t < room; t += 32) tiles[at + t] = make_int2(of, side == 0 ? n - 1 - t : t);
+  }
+  __device__ __forceinline__ void zeros(void* base, int64_t row, int64_t stride, int rows) {
+    const int vecs = p.a.D / 8;
+    for (int i = threadIdx.x % 32; i < rows * vecs; i += 32)
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + row + i / vecs * stride + i % vecs * 8) = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ Job next() {
+    const AttnDev& a = p.a;
+    for (;;) {
+      if (stretch > a.batch + 1) return Job{0, 0, -1, 0, 0};
+      const Job job{qa, ka, max(0, qb - qa), max(0, kb - ka), head};
+      const int of = stretch;
+      head += head_step;
+      stretch += step + (head >= heads ? 1 : 0);
+      if (head >= heads) head -= heads;
+      if (stretch <= a.batch + 1) read();
+      const bool gap = of < 1 || of > a.batch;   // rows of no sequence: they see nothing, and nothing sees them
+      if (job.q > kRows || job.k > kRows) {
+        if (job.head == 0) {
+          list(of, 0, (job.q + kRows - 1) / kRows);
+          if (kBackward) list(of, 1, (job.k + kRows - 1) / kRows);
+        }
+        continue;
+      }
+      if (!gap && job.q > 0 && job.k > 0) return job;
+      if constexpr (kBackward) {
+        for (int g = 0; g < a.group; ++g)
+          zeros(a.dq, job.q0 * a.dq_row + (job.head * a.group + g) * a.dq_head, a.dq_row, job.q);
+        zeros(a.dk, job.k0 * a.dk_row + job.head * a.dk_head, a.dk_row, job.k);
+        zeros(a.dv, job.k0 * a.dv_row + job.head * a.dv_head, a.dv_row, job.k);
+      } else {
+        zeros(a.out, job.q0 * a.o_row + job.head * a.o_head, a.o_row, job.q);
+        if (a.lse != nullptr)
+          for (int i = threadIdx.x % 32; i < job.q; i += 32) a.lse[job.head * a.total_q + job.q0 + i] = -INFINITY;
+      }
     }
-  return bytes;
+  }
+};
+
+// rows [0, rows) of a head in boxes of kBox rows
+template <int kDP>
+__device__ __forceinline__ void load_rows(uint32_t tile, const CUtensorMap* map, int head, int row, int rows, uint64_t* bar) {
+#pragma unroll
+  for (int r = 0; r < kRows; r += kBox)
+    if (r < rows) {
+#pragma unroll
+      for (int x = 0; x < kDP / 64; ++x) tma_load_3d(tile + x * kRows * 128 + r * 128, map, x * 64, head, row + r, bar);
+    }
 }
+__device__ __forceinline__ int boxed(int rows) { return (rows + kBox - 1) / kBox * kBox; }
 
 // Rows [rows, next multiple of 16) become zero: other sequences' rows, whose zero weights would not cancel NaN.
+// By a whole warp.
 template <int kDP>
 __device__ __forceinline__ void zero_tail(uint8_t* tile, int rows) {
   const int count = (16 - rows % 16) % 16;
-  for (int i = threadIdx.x; i < count * (kDP / 64) * 8; i += blockDim.x) {
-    const int x = i / (count * 8), rest = i % (count * 8);
-    *reinterpret_cast<uint4*>(tile + x * kRows * 128 + rows * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
-  }
+  for (int i = threadIdx.x % 32; i < count * 8; i += 32)
+#pragma unroll
+    for (int x = 0; x < kDP / 64; ++x)
+      *reinterpret_cast<uint4*>(tile + x * kRows * 128 + rows * 128 + i * 16) = make_uint4(0, 0, 0, 0);
 }
 
 __device__ __forceinline__ uint32_t up16(int n) { return static_cast<uint32_t>(n + 15) & ~15u; }
-
-// 32 columns of an accumulator row, times f, to memory (those below D)
-template <bool kBf16>
-__device__ __forceinline__ void store_columns(uint16_t* out, const uint32_t (&o)[32], int from, int D, float f) {
-#pragma unroll
-  for (int e = 0; e < 32; e += 8)
-    if (from + e < D) {
-      uint4 v;
-      v.x = pack2<kBf16>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f);
-      v.y = pack2<kBf16>(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
-      v.z = pack2<kBf16>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f);
-      v.w = pack2<kBf16>(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f);
-      *reinterpret_cast<uint4*>(out + from + e) = v;
-    }
-}
-
-__device__ __forceinline__ void store_zeros(uint16_t* out, int from, int to, int D) {
-  for (int e = from; e < to && e < D; e += 8) *reinterpret_cast<uint4*>(out + e) = make_uint4(0, 0, 0, 0);
-}
 
 // A wait gave up: report it, and let what is in flight land before its memory is given back.
 __device__ __forceinline__ void report(const int* dead, int32_t* status) {
@@ -117,8 +140,8 @@ struct Forward {
   static constexpr int kCtas = kDP == 64 ? 4 : 2;
 };
 
-// A CTA's items are blockIdx.x, blockIdx.x + gridDim.x, ...: the next one's copies are under way while this one's
-// softmax and products run.
+// A CTA takes jobs as long as there are some; the next one's copies are under way while this one's softmax and products
+// run. Warp 0 issues the products, warp 3 finds the jobs and issues the copies.
 template <bool kBf16, int kDP>
 __global__ void __launch_bounds__(128, Forward<kDP>::kCtas)
     attention_short_fwd_kernel(const ShortDev p, const __grid_constant__ CUtensorMap q_map,
@@ -126,13 +149,14 @@ __global__ void __launch_bounds__(128, Forward<kDP>::kCtas)
   using L = Forward<kDP>;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t qk_full, v_full, s_full, o_full;
+  __shared__ Job jobs[2];
   __shared__ uint32_t tmem_base;
   __shared__ int dead_word;
   const AttnDev& a = p.a;
   uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* ks = qs + L::kTileBytes;
-  uint8_t* vs = ks + L::kTileBytes;
-  const int warp = threadIdx.x / 32, row = threadIdx.x, items = (a.batch + 2) * a.heads;
+  uint8_t* vs = qs + 2 * L::kTileBytes;
+  const uint32_t q_at = smem_addr(qs), k_at = q_at + L::kTileBytes, v_at = k_at + L::kTileBytes;
+  const int warp = __shfl_sync(kFullMask, threadIdx.x / 32, 0), row = threadIdx.x;
   volatile int* dead = &dead_word;
   if (threadIdx.x == 0) {
     mbar_init(&qk_full, 1);
@@ -152,133 +176,151 @@ __global__ void __launch_bounds__(128, Forward<kDP>::kCtas)
   const uint32_t tmem = tmem_base, lanes = static_cast<uint32_t>(warp * 32) << 16;
   const uint32_t s_at = tmem + lanes, o_at = tmem + lanes + 64;
   const float c = a.scale * kLog2e;
+  const uint64_t c2 = pair(c, c);
 
-  // the first item from `i` on with products to compute; those without any get their zeros on the way
-  auto next_work = [&](int i, Sequence* s) {
-    for (; i < items; i += gridDim.x) {
-      const int stretch = i / a.heads, head = i - stretch * a.heads;
-      if (!sequence_of(p, stretch, head == 0, false, s) || s->q == 0) continue;
-      if (!s->gap && s->k > 0) break;
-      if (row < s->q) {
-        store_zeros(static_cast<uint16_t*>(a.out) + (s->q0 + row) * a.o_row + head * a.o_head, 0, kDP, a.D);
-        if (a.lse != nullptr) a.lse[head * a.total_q + s->q0 + row] = -INFINITY;
-      }
-    }
-    return i;
+  auto copy_qk = [&](const Job& s) {
+    mbar_expect(&qk_full, (boxed(s.q) + boxed(s.k)) * kDP * 2);
+    load_rows<kDP>(q_at, &q_map, s.head, s.q0, s.q, &qk_full);
+    load_rows<kDP>(k_at, &k_map, s.head / a.group, s.k0, s.k, &qk_full);
   };
-  auto copy_qk = [&](int i, const Sequence& s) {
-    const int head = i % a.heads;
-    mbar_expect(&qk_full, ((s.q + kBox - 1) / kBox + (s.k + kBox - 1) / kBox) * kBox * kDP * 2);
-    load_rows<kDP>(qs, &q_map, head, s.q0, s.q, &qk_full);
-    load_rows<kDP>(ks, &k_map, head / a.group, s.k0, s.k, &qk_full);
+  auto copy_v = [&](const Job& s) {
+    mbar_expect(&v_full, boxed(s.k) * kDP * 2);
+    load_rows<kDP>(v_at, &v_map, s.head / a.group, s.k0, s.k, &v_full);
   };
-  auto copy_v = [&](int i, const Sequence& s) {
-    mbar_expect(&v_full, (s.k + kBox - 1) / kBox * kBox * kDP * 2);
-    load_rows<kDP>(vs, &v_map, i % a.heads / a.group, s.k0, s.k, &v_full);
-  };
-  Sequence s, n;
-  int item = next_work(blockIdx.x, &s);
-  if (item < items && threadIdx.x == 0) {
-    copy_qk(item, s);
-    copy_v(item, s);
-  }
-  for (uint32_t phase = 0; item < items; phase ^= 1) {
-    const int next = next_work(item + gridDim.x, &n), head = item % a.heads;
-    // Only this warp: the next copies may complete before another one has looked, and a barrier two phases on looks
-    // as it did before. (The other barriers' next phases come after a __syncthreads() behind every warp's wait.)
-    if (warp == 0) warp_wait(&qk_full, phase, dead);
-    if (warp == 0 && elect_one()) {
-      mma_along_k<kDP / 16, kRows>(tmem, smem_addr(qs), smem_addr(ks), mma_desc(kBf16, kRows, up16(s.k), false, false),
-                                   (a.D + 15) / 16);
-      mma_commit(&s_full);
+  Finder<false> finder(p);
+  Job n{0, 0, -1, 0, 0};
+  if (warp == 3) {
+    n = finder.next();
+    if (n.q > 0 && elect_one()) {
+      copy_qk(n);
+      copy_v(n);
     }
     __syncwarp();
-    const int shift = s.k - s.q;
-    const int limit = row >= s.q ? 0 : (a.causal ? min(s.k, row + shift + 1) : s.k);
-    const int chunks = warp * 32 < s.q ? (s.k + 31) / 32 : 0;   // a warp whose rows are all behind the last computes nothing
-    float sum = 0.f;
+    if (row == 96) jobs[0] = n;
+  }
+  __syncthreads();
+  for (int turn = 0, failed = 0; !failed; ++turn) {
+    const Job s = jobs[turn & 1];
+    if (s.q < 0) break;
+    const uint32_t phase = turn & 1;
+    if (warp == 0) {
+      // Only this warp waits for these copies: the next ones may complete before another warp has looked, and a
+      // barrier two phases on looks as it did before. (The other barriers' next phases come after a __syncthreads()
+      // behind every warp's wait.)
+      warp_wait(&qk_full, phase, dead);
+      if (elect_one()) {
+        mma_along_k<kDP / 16, kRows>(tmem, q_at, k_at, mma_desc(kBf16, kRows, up16(s.k), false, false), (a.D + 15) / 16);
+        mma_commit(&s_full);
+      }
+      __syncwarp();
+    } else if (warp == 3) {
+      n = finder.next();
+      if (row == 96) jobs[(turn + 1) & 1] = n;
+    }
     warp_wait(&s_full, phase, dead);
     tc_fence_after();
-    if (next < items && threadIdx.x == 0) copy_qk(next, n);
-    float m = -INFINITY;
-    for (int i = 0; i < chunks; ++i) {
-      uint32_t x[32];
-      tmem_ld32(x, s_at + i * 32);
-      tmem_wait_ld();
-      const int left = limit - i * 32;
-      if (__all_sync(kFullMask, left >= 32)) {
+    if (warp == 3) {
+      if (n.q > 0 && elect_one()) copy_qk(n);
+      __syncwarp();
+    }
+    float sum = 0.f, base = 0.f;
+    if (warp * 32 < s.q) {   // a warp whose rows are all behind the last computes nothing
+      const int chunks = (s.k + 31) / 32;
+      const int limit = row >= s.q ? 0 : (a.causal ? min(s.k, row + s.k - s.q + 1) : s.k);
+      auto largest = [&](uint32_t (&x)[32], int i, float m) {   // of chunk i, whose masked scores become -infinity
+        if (__any_sync(kFullMask, limit < i * 32 + 32)) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (i * 32 + e >= limit) x[e] = 0xff800000u;
+        }
 #pragma unroll
         for (int e = 0; e < 32; e += 2) m = max3(m, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-      } else {
+        return m;
+      };
+      // a chunk's weights go to columns that its own scores or earlier ones had
+      auto weigh = [&](const uint32_t (&x)[32], int i) {
+        uint32_t w[16];
+        uint64_t add = 0;
+        const uint64_t minus = pair(-base, -base);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) m = e < left ? fmaxf(m, __uint_as_float(x[e])) : m;
+        for (int e = 0; e < 32; e += 2) {
+          const float2 y = unpair(fma2(as_pair(&x[e]), c2, minus));
+          const float p0 = fast_exp2(y.x), p1 = fast_exp2(y.y);
+          add = add2(add, pair(p0, p1));
+          w[e / 2] = pack2<kBf16>(p0, p1);
+        }
+        sum += unpair(add).x + unpair(add).y;
+        tmem_st16(s_at + i * 16, w);
+      };
+      uint32_t x[2][32];
+      float m = -INFINITY;
+      if (chunks > 2) {   // the second half's maximum first; its scores are read again when the first half is done
+        tmem_ld32(x[0], s_at + 64);
+        if (chunks > 3) tmem_ld32(x[1], s_at + 96);
+        tmem_wait_ld();
+        m = largest(x[0], 2, m);
+        if (chunks > 3) m = largest(x[1], 3, m);
       }
-    }
-    const float base = m == -INFINITY ? 0.f : m * c;
-    // a chunk's weights go to columns that its own scores or earlier ones had
-    for (int i = 0; i < chunks; ++i) {
-      uint32_t x[32], w[16];
-      tmem_ld32(x, s_at + i * 32);
+      tmem_ld32(x[0], s_at);
+      if (chunks > 1) tmem_ld32(x[1], s_at + 32);
       tmem_wait_ld();
-      const int left = limit - i * 32;
-      uint64_t add = 0;
-      if (__any_sync(kFullMask, left < 32)) {
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-          if (e >= left) x[e] = 0xff800000u;
+      m = largest(x[0], 0, m);
+      if (chunks > 1) m = largest(x[1], 1, m);
+      base = m == -INFINITY ? 0.f : m * c;
+      weigh(x[0], 0);
+      if (chunks > 1) weigh(x[1], 1);
+      if (chunks > 2) {
+        tmem_ld32(x[0], s_at + 64);
+        if (chunks > 3) tmem_ld32(x[1], s_at + 96);
+        tmem_wait_ld();
+        largest(x[0], 2, m);
+        weigh(x[0], 2);
+        if (chunks > 3) {
+          largest(x[1], 3, m);
+          weigh(x[1], 3);
+        }
       }
-#pragma unroll
-      for (int e = 0; e < 32; e += 2) {
-        const float2 y = unpair(fma2(as_pair(&x[e]), pair(c, c), pair(-base, -base)));
-        const float p0 = fast_exp2(y.x), p1 = fast_exp2(y.y);
-        add = add2(add, pair(p0, p1));
-        w[e / 2] = pack2<kBf16>(p0, p1);
-      }
-      sum += unpair(add).x + unpair(add).y;
-      tmem_st16(s_at + i * 16, w);
-    }
-    tmem_wait_st();
-    warp_wait(&v_full, phase, dead);
-    if (s.k % 16 != 0) {
-      zero_tail<kDP>(vs, s.k);
-      fence_async_smem();
+      tmem_wait_st();
     }
     tc_fence_before();
     __syncthreads();
-    tc_fence_after();
-    if (warp == 0 && elect_one()) {
-      mma_over_rows<0>(tmem + 64, tmem, smem_addr(vs), mma_desc(kBf16, kRows, up16(a.D), false, true), (s.k + 15) / 16, false);
-      mma_commit(&o_full);
+    if (warp == 0) {
+      warp_wait(&v_full, phase, dead);
+      if (s.k % 16 != 0) {
+        zero_tail<kDP>(vs, s.k);
+        fence_async_smem();
+        __syncwarp();
+      }
+      tc_fence_after();
+      if (elect_one()) {
+        mma_over_rows<0>(tmem + 64, tmem, v_at, mma_desc(kBf16, kRows, up16(a.D), false, true), (s.k + 15) / 16, false);
+        mma_commit(&o_full);
+      }
+      __syncwarp();
     }
-    __syncwarp();
     warp_wait(&o_full, phase, dead);
     tc_fence_after();
-    if (next < items && threadIdx.x == 0) copy_v(next, n);
-    uint32_t o[kDP / 32][32];
-    if (warp * 32 < s.q) {
+    if (warp * 32 < s.q) {   // through v's place, which has been read
+      uint32_t o[kDP / 32][32];
 #pragma unroll
       for (int i = 0; i < kDP / 32; ++i) tmem_ld32(o[i], o_at + i * 32);
-    }
-    tmem_wait_ld();
-    tc_fence_before();
-    const int failed = __syncthreads_or(*dead);   // also: the next scores may come
-    tc_fence_after();
-    if (row < s.q) {
+      tmem_wait_ld();
+      uint16_t* out = static_cast<uint16_t*>(a.out) + (s.q0 + warp * 32) * a.o_row + s.head * a.o_head;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      uint16_t* out = static_cast<uint16_t*>(a.out) + (s.q0 + row) * a.o_row + head * a.o_head;
 #pragma unroll
-      for (int i = 0; i < kDP / 32; ++i) {
-        if (sum == 0.f)
-          store_zeros(out, i * 32, i * 32 + 32, a.D);
-        else
-          store_columns<kBf16>(out, o[i], i * 32, a.D, inv);
-      }
-      if (a.lse != nullptr)
-        a.lse[head * a.total_q + s.q0 + row] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
+      for (int i = 0; i < kDP / 32; ++i)
+        store_columns<kBf16>(vs + warp * 2048, o[i], inv, sum == 0.f, out, a.o_row, s.q - warp * 32, i * 32, a.D);
+      if (a.lse != nullptr && row < s.q)
+        a.lse[s.head * a.total_q + s.q0 + row] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
     }
-    if (failed) break;
-    item = next;
-    s = n;
+    fence_async_smem();
+    tc_fence_before();
+    failed = __syncthreads_or(*dead);
+    tc_fence_after();
+    if (warp == 3) {
+      if (n.q > 0 && !failed && elect_one()) copy_v(n);
+      __syncwarp();
+    }
   }
   __syncthreads();
   report(&dead_word, p.status);
@@ -296,7 +338,9 @@ template <int kDP, bool kAlone>
 struct Backward {
   static constexpr int kTileBytes = kRows * kDP * 2;
   static constexpr int kWeightBytes = kRows * kRows * 2;
-  static constexpr int kSmem = 3 * kTileBytes + kWeightBytes + 1024;
+  // the results' way out, 2 KB a warp: with 64 columns the half of the weights' place that v does not share
+  static constexpr int kStage = kDP == 64 ? kRows * 128 : kWeightBytes;
+  static constexpr int kSmem = 3 * kTileBytes + kWeightBytes + (kDP == 64 ? 0 : 8 * 2048) + 1024;
   static constexpr int kColumns = kDP == 64 && kAlone ? 256 : 512;
   static constexpr int kCtas = kDP == 64 && kAlone ? 2 : 1;
 };
@@ -316,22 +360,21 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
                                const __grid_constant__ CUtensorMap g_map) {
   using L = Backward<kDP, kAlone>;
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t kv_full, q_full, s_full, v_done, d_full;
+  __shared__ uint64_t full, s_full, v_done, d_full;
+  __shared__ Job jobs[2];
   __shared__ uint32_t tmem_base;
   __shared__ int dead_word;
   __shared__ float halves[2][kRows];
   const AttnDev& a = p.a;
-  const int items = (a.batch + 2) * a.kv_heads;
   uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* gs = qs + L::kTileBytes;
   uint8_t* ks = gs + L::kTileBytes;
-  uint8_t* vs = ks + L::kTileBytes;
-  uint8_t* ps = vs;
-  const int warp = threadIdx.x / 32, half = warp / 4, row = threadIdx.x % 128;
+  uint8_t* ps = ks + L::kTileBytes;   // and v
+  const uint32_t q_at = smem_addr(qs), g_at = smem_addr(gs), k_at = smem_addr(ks), v_at = smem_addr(ps), p_at = v_at;
+  const int warp = __shfl_sync(kFullMask, threadIdx.x / 32, 0), half = warp / 4, row = threadIdx.x % 128;
   volatile int* dead = &dead_word;
   if (threadIdx.x == 0) {
-    mbar_init(&kv_full, 1);
-    mbar_init(&q_full, 1);
+    mbar_init(&full, 1);
     mbar_init(&s_full, 1);
     mbar_init(&v_done, 1);
     mbar_init(&d_full, 1);
@@ -351,76 +394,66 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
   const uint32_t s_at = tmem + lanes + half * 64, dp_at = dp + lanes + half * 64;
   const int d_steps = (a.D + 15) / 16;
   const uint64_t c2 = pair(a.scale * kLog2e, a.scale * kLog2e);
-  const uint32_t desc = mma_desc(kBf16, kRows, up16(a.D), true, true);
+  uint8_t* stage = ps + L::kStage + warp * 2048;
 
-  auto dq_row = [&](const Sequence& s, int head) {
-    return static_cast<uint16_t*>(a.dq) + (s.q0 + row) * a.dq_row + head * a.dq_head;
+  auto copy = [&](const Job& s, int g) {
+    const int head = s.head * a.group + g;
+    mbar_expect(&full, ((g == 0 ? 2 : 1) * boxed(s.k) + 2 * boxed(s.q)) * kDP * 2);
+    load_rows<kDP>(q_at, &q_map, head, s.q0, s.q, &full);
+    if (g == 0) load_rows<kDP>(k_at, &k_map, s.head, s.k0, s.k, &full);
+    load_rows<kDP>(g_at, &g_map, head, s.q0, s.q, &full);
+    load_rows<kDP>(v_at, &v_map, s.head, s.k0, s.k, &full);   // again for each head: weights took its place
   };
-  auto dkv_row = [&](const Sequence& s, int kv) {
-    return half == 0 ? static_cast<uint16_t*>(a.dv) + (s.k0 + row) * a.dv_row + kv * a.dv_head
-                     : static_cast<uint16_t*>(a.dk) + (s.k0 + row) * a.dk_row + kv * a.dk_head;
-  };
-  // the first item from `i` on with products to compute; those without any get their zeros on the way
-  auto next_work = [&](int i, Sequence* s) {
-    for (; i < items; i += gridDim.x) {
-      const int stretch = i / a.kv_heads, kv = i - stretch * a.kv_heads;
-      if (!sequence_of(p, stretch, kv == 0, true, s)) continue;
-      if (!s->gap && s->q > 0 && s->k > 0) break;
-      if (row < s->q && half == 0)
-        for (int g = 0; g < a.group; ++g) store_zeros(dq_row(*s, kv * a.group + g), 0, kDP, a.D);
-      if (row < s->k) store_zeros(dkv_row(*s, kv), 0, kDP, a.D);
-    }
-    return i;
-  };
-  // the tiles of head g of an item
-  auto copy = [&](int i, const Sequence& s, int g) {
-    const int kv = i % a.kv_heads, head = kv * a.group + g, q_rows = (s.q + kBox - 1) / kBox * kBox;
-    mbar_expect(&kv_full, (g == 0 ? 2 : 1) * ((s.k + kBox - 1) / kBox * kBox) * kDP * 2);
-    if (g == 0) load_rows<kDP>(ks, &k_map, kv, s.k0, s.k, &kv_full);
-    load_rows<kDP>(vs, &v_map, kv, s.k0, s.k, &kv_full);   // again for each head: weights took its place
-    mbar_expect(&q_full, 2 * q_rows * kDP * 2);
-    load_rows<kDP>(qs, &q_map, head, s.q0, s.q, &q_full);
-    load_rows<kDP>(gs, &g_map, head, s.q0, s.q, &q_full);
-  };
-  Sequence s, n;
-  int item = next_work(blockIdx.x, &s);
-  if (item < items && threadIdx.x == 0) copy(item, s, 0);
+  Finder<true> finder(p);
+  Job n{0, 0, -1, 0, 0};
+  if (warp == 7) {
+    n = finder.next();
+    if (n.q > 0 && elect_one()) copy(n, 0);
+    __syncwarp();
+    if (row == 127) jobs[0] = n;
+  }
+  __syncthreads();
   uint32_t phase = 0;
-  int failed = 0;
-  while (item < items && !failed) {
-    const int next = next_work(item + gridDim.x, &n), kv = item % a.kv_heads;
-    const int shift = s.k - s.q, q_steps = (s.q + 15) / 16;
-    const int limit = row >= s.q ? 0 : (a.causal ? min(s.k, row + shift + 1) : s.k);
+  for (int turn = 0, failed = 0; !failed; ++turn) {
+    const Job s = jobs[turn & 1];
+    if (s.q < 0) break;
+    const int q_steps = (s.q + 15) / 16;
+    const int limit = row >= s.q ? 0 : (a.causal ? min(s.k, row + s.k - s.q + 1) : s.k);
     const int left = limit - half * 64;
     // a warp whose rows are all behind the last computes nothing
-    const int chunks = warp % 4 * 32 < s.q ? max(0, min(2, (s.k - half * 64 + 31) / 32)) : 0;
+    const bool rows_here = warp % 4 * 32 < s.q, keys_here = warp % 4 * 32 < s.k;
+    const int chunks = rows_here ? max(0, min(2, (s.k - half * 64 + 31) / 32)) : 0;
     for (int g = 0; g < a.group; ++g, phase ^= 1) {
-      const int head = kv * a.group + g;
+      const int head = s.head * a.group + g;
       float lse2 = 0.f;
       if (row < s.q) {
         lse2 = a.lse[head * a.total_q + s.q0 + row] * kLog2e;
         if (lse2 == -INFINITY) lse2 = INFINITY;
       }
-      warp_wait(&kv_full, phase, dead);
-      warp_wait(&q_full, phase, dead);
-      if (s.k % 16 != 0 || s.q % 16 != 0) {
-        zero_tail<kDP>(ks, s.k);
-        zero_tail<kDP>(qs, s.q);
-        zero_tail<kDP>(gs, s.q);
-        fence_async_smem();
-        __syncthreads();
+      if (warp == 0) {
+        warp_wait(&full, phase, dead);
+        if (s.k % 16 != 0 || s.q % 16 != 0) {
+          zero_tail<kDP>(ks, s.k);
+          zero_tail<kDP>(qs, s.q);
+          zero_tail<kDP>(gs, s.q);
+          fence_async_smem();
+          __syncwarp();
+        }
+        if (elect_one()) {
+          const uint32_t s_desc = mma_desc(kBf16, kRows, up16(s.k), false, false);
+          mma_along_k<kDP / 16, kRows>(tmem, q_at, k_at, s_desc, d_steps);
+          mma_along_k<kDP / 16, kRows>(dp, g_at, v_at, s_desc, d_steps);
+          mma_commit(&s_full);
+        }
+        __syncwarp();
+      } else if (warp == 7 && g == 0) {
+        n = finder.next();
+        if (row == 127) jobs[(turn + 1) & 1] = n;
       }
-      if (warp == 0 && elect_one()) {
-        const uint32_t s_desc = mma_desc(kBf16, kRows, up16(s.k), false, false);
-        mma_along_k<kDP / 16, kRows>(tmem, smem_addr(qs), smem_addr(ks), s_desc, d_steps);
-        mma_along_k<kDP / 16, kRows>(dp, smem_addr(gs), smem_addr(vs), s_desc, d_steps);
-        mma_commit(&s_full);
-      }
-      __syncwarp();
       warp_wait(&s_full, phase, dead);
       tc_fence_after();
       // ---- P, and the row's part of delta ----
-      uint32_t w[2][32];
+      uint32_t w[2][32], x[32];
       uint64_t part = 0;
       // a row of 64 keys is 128 bytes, its 16-byte pieces exchanged by the row's number, as the copies do it
       uint8_t* p_row = ps + half * kRows * 128 + row * 128;
@@ -433,16 +466,16 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
           *reinterpret_cast<uint4*>(p_row + (((i * 32 + e) / 8) ^ (row % 8)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
         }
       };
+      const uint64_t minus = pair(-lse2, -lse2);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (i < chunks) {
-          uint32_t x[32];
           tmem_ld32(w[i], s_at + i * 32);
           tmem_ld32(x, dp_at + i * 32);
           tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float2 y = unpair(fma2(as_pair(&w[i][e]), c2, pair(-lse2, -lse2)));
+            const float2 y = unpair(fma2(as_pair(&w[i][e]), c2, minus));
             w[i][e] = __float_as_uint(fast_exp2(y.x));
             w[i][e + 1] = __float_as_uint(fast_exp2(y.y));
           }
@@ -453,27 +486,26 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
           }
 #pragma unroll
           for (int e = 0; e < 32; e += 2) part = fma2(as_pair(&w[i][e]), as_pair(&x[e]), part);
+          put(i);   // v, whose place it is, has been read
         }
       halves[half][row] = unpair(part).x + unpair(part).y;
-      tc_fence_before();
-      __syncthreads();   // also: all of dP is computed, so v may be written over
-      tc_fence_after();
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (i < chunks) put(i);
       fence_async_smem();
+      tc_fence_before();
       __syncthreads();
-      if (warp == 0 && elect_one()) {
-        transposed(dv, smem_addr(ps), smem_addr(gs), desc, q_steps, g > 0);
-        mma_commit(&v_done);
+      if (warp == 0) {
+        tc_fence_after();
+        if (elect_one()) {
+          transposed(dv, p_at, g_at, mma_desc(kBf16, kRows, up16(a.D), true, true), q_steps, g > 0);
+          mma_commit(&v_done);
+        }
+        __syncwarp();
       }
-      __syncwarp();
       // ---- dS ----
       const float delta = halves[0][row] + halves[1][row];
+      const uint64_t minus_delta = pair(-delta, -delta);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (i < chunks) {
-          uint32_t x[32];
           tmem_ld32(x, dp_at + i * 32);
           tmem_wait_ld();
           if (__any_sync(kFullMask, left < i * 32 + 32)) {
@@ -483,7 +515,7 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
           }
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float2 y = unpair(mul2(as_pair(&w[i][e]), add2(as_pair(&x[e]), pair(-delta, -delta))));
+            const float2 y = unpair(mul2(as_pair(&w[i][e]), add2(as_pair(&x[e]), minus_delta)));
             w[i][e] = __float_as_uint(y.x);
             w[i][e + 1] = __float_as_uint(y.y);
           }
@@ -495,51 +527,57 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
       fence_async_smem();
       tc_fence_before();
       __syncthreads();
-      tc_fence_after();
-      if (warp == 0 && elect_one()) {
-        transposed(dk, smem_addr(ps), smem_addr(qs), desc, q_steps, g > 0);
-        const uint32_t dq_desc = mma_desc(kBf16, kRows, up16(a.D), false, true);
-        const uint64_t w0 = smem_desc(smem_addr(ps), 16), x0 = smem_desc(smem_addr(ks), kRows * 128);
+      if (warp == 0) {
+        tc_fence_after();
+        if (elect_one()) {
+          transposed(dk, p_at, q_at, mma_desc(kBf16, kRows, up16(a.D), true, true), q_steps, g > 0);
+          const uint32_t dq_desc = mma_desc(kBf16, kRows, up16(a.D), false, true);
+          const uint64_t w0 = smem_desc(p_at, 16), x0 = smem_desc(k_at, kRows * 128);
 #pragma unroll
-        for (int t = 0; t < 8; ++t)
-          if (t < (s.k + 15) / 16)
-            mma_ss(dq, w0 + (((t / 4) * kRows * 128 + (t % 4) * 32) >> 4), x0 + t * (2048 >> 4), dq_desc, t > 0);
-        mma_commit(&d_full);
+          for (int t = 0; t < 8; ++t)
+            if (t < (s.k + 15) / 16)
+              mma_ss(dq, w0 + (((t / 4) * kRows * 128 + (t % 4) * 32) >> 4), x0 + t * (2048 >> 4), dq_desc, t > 0);
+          mma_commit(&d_full);
+        }
+        __syncwarp();
       }
-      __syncwarp();
       warp_wait(&d_full, phase, dead);
       tc_fence_after();
       // the tiles have been read: the next ones' copies go under this one's stores
-      if (threadIdx.x == 0) {
-        if (g + 1 < a.group)
-          copy(item, s, g + 1);
-        else if (next < items)
-          copy(next, n, 0);
+      if (warp == 7) {
+        if (g + 1 < a.group) {
+          if (elect_one()) copy(s, g + 1);
+        } else if (n.q > 0) {
+          if (elect_one()) copy(n, 0);
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      if (rows_here) {
+        uint16_t* out = static_cast<uint16_t*>(a.dq) + (s.q0 + warp % 4 * 32) * a.dq_row + head * a.dq_head;
 #pragma unroll 1
-      for (int i = half * kDP / 2; i < (half + 1) * kDP / 2 && warp % 4 * 32 < s.q; i += 32) {
-        uint32_t o[32];
-        tmem_ld32(o, dq + lanes + i);
-        tmem_wait_ld();
-        if (row < s.q) store_columns<kBf16>(dq_row(s, head), o, i, a.D, a.scale);
-      }
-      if (g + 1 == a.group) {
-#pragma unroll 1
-        for (int i = 0; i < kDP && warp % 4 * 32 < s.k; i += 32) {
-          uint32_t o[32];
-          tmem_ld32(o, (half == 0 ? dv : dk) + lanes + i);
+        for (int i = half * kDP / 2; i < (half + 1) * kDP / 2; i += 32) {
+          tmem_ld32(x, dq + lanes + i);
           tmem_wait_ld();
-          if (row < s.k) store_columns<kBf16>(dkv_row(s, kv), o, i, a.D, half == 0 ? 1.f : a.scale);
+          store_columns<kBf16>(stage, x, a.scale, false, out, a.dq_row, s.q - warp % 4 * 32, i, a.D);
         }
       }
+      if (g + 1 == a.group && keys_here) {
+        const int64_t stride = half == 0 ? a.dv_row : a.dk_row;
+        uint16_t* out = static_cast<uint16_t*>(half == 0 ? a.dv : a.dk) + (s.k0 + warp % 4 * 32) * stride +
+                        s.head * (half == 0 ? a.dv_head : a.dk_head);
+#pragma unroll 1
+        for (int i = 0; i < kDP; i += 32) {
+          tmem_ld32(x, (half == 0 ? dv : dk) + lanes + i);
+          tmem_wait_ld();
+          store_columns<kBf16>(stage, x, half == 0 ? 1.f : a.scale, false, out, stride, s.k - warp % 4 * 32, i, a.D);
+        }
+      }
+      fence_async_smem();
       tc_fence_before();
       failed = __syncthreads_or(*dead);   // before the next head's products
       tc_fence_after();
       if (failed) break;
     }
-    item = next;
-    s = n;
   }
   __syncthreads();
   report(&dead_word, p.status);

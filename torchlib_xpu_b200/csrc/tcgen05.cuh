@@ -74,17 +74,13 @@ __device__ __forceinline__ void fence_barrier_init() { asm volatile("fence.mbarr
 // shared-memory writes of this thread, before asynchronous units read them
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          smem_addr(dst)),
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
       : "memory");
 }
 
-__device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-}
 
 // Tensor memory: 128 lanes x 512 columns of 32 bits a SM. A whole warp allocates and frees.
 __device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t columns) {
@@ -255,6 +251,32 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   else
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// 32 columns of a warp's 32 accumulator rows (a row a lane), times f, rounded, to memory: columns [col, col + 32) of the
+// rows out, out + stride, ...; `rows` of them, columns below D. Through 2 KB of shared memory of the warp's own, so
+// that an instruction writes eight rows' 64 bytes; 16 bytes a lane in 32 rows took most of a short sequence's time.
+template <bool kBf16>
+__device__ __forceinline__ void store_columns(uint8_t* stage, const uint32_t (&o)[32], float f, bool zero, uint16_t* out,
+                                              int64_t stride, int rows, int col, int D) {
+  const int lane = threadIdx.x % 32;
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 32; e += 8) {
+    uint32_t y[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      y[u] = zero ? 0u : pack2<kBf16>(__uint_as_float(o[e + 2 * u]) * f, __uint_as_float(o[e + 2 * u + 1]) * f);
+    *reinterpret_cast<uint4*>(stage + lane * 64 + ((e / 8) ^ (lane / 2 % 4)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+  }
+  __syncwarp();
+  const int first = lane / 4, c = lane % 4;
+  out += first * stride + col + c * 8;
+  rows = col + c * 8 < D ? rows - first : 0;
+  const uint8_t* from = stage + first * 64 + (c ^ (first / 2 % 4)) * 16;   // the same piece in every eighth row
+#pragma unroll
+  for (int i = 0; i < 4; ++i, out += 8 * stride)
+    if (i * 8 < rows) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(from + i * 512);
 }
 
 // A tensor map over [rows][heads][D] of 16-bit elements, in boxes of 64 columns of one head x `box_rows` rows.
