@@ -150,6 +150,11 @@ def test_bad_pages_take_no_part_and_are_reported():
         ref.assert_within(out[b:b + 1], one["o"], one["o_off"], "sequence %d" % b)
     answer(q.cuda(), k.cuda(), v.cuda(), table.cuda(), long)
     assert pop(out) == 1
+    for value in (-1, pages, -(1 << 31), (1 << 31) - 1):
+        one_bad = table.clone()
+        one_bad[2, 1] = value
+        answer(q.cuda(), k.cuda(), v.cuda(), one_bad.cuda(), torch.tensor(lengths, device="cuda"))
+        assert pop(out) == 1
     all_bad = torch.full_like(table, pages + 3)
     got = answer(q.cuda(), k.cuda(), v.cuda(), all_bad.cuda(), torch.tensor(lengths, device="cuda"))
     assert (got == 0).all() and pop(out) == 1

@@ -327,21 +327,48 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Copies 16 bytes to shared memory without waiting for them; zeros where `on` is false.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+
+template <int kDP>
+struct Ring {
+  static constexpr int kKC = kDP / 32, kVC = kDP / 64;      // 16-byte pieces of a lane for a key, for a value
+  static constexpr int kPieces = 2 * kKC + 4 * kVC;         // of a lane for a step
+  static constexpr int kStages = kDP == 64 ? 4 : 3;
+  static constexpr int kCtas = kDP == 64 ? 3 : 2;           // per SM
+  static constexpr int kStep = kPieces * 512;
+  static constexpr int kBytes = kAnswerThreads / 32 * kStages * kStep;
+  static constexpr int kSumRow = kDP + 4;
+  static_assert(kBytes >= kAnswerThreads / 32 * kHeads * kSumRow * 4, "the warps' sums take the ring's place");
+};
+
 // 16-bit types, head dimensions that are multiples of 8 up to kDP. A warp takes 16 positions of a tile:
 //   S^T [16 positions][8 heads] = k q^T,   O^T [D][8 heads] += v^T P^T
-// by warp-level matrix instructions; the cache is read 16 bytes a lane straight into their registers. That works
-// because the order of an inner dimension is free as long as both operands share it: for S^T, lane (g, t) of
-// a row of four takes elements 8 (t + 4c) .. + 7 of position g's key, and of head g's query; for O^T it takes
-// elements 8 (g + 8c) .. + 7 of the values of positions 2t, 2t + 1, 2t + 8, 2t + 9, whose pairs two byte permutes
-// put side by side. Warps meet only at the end of a unit. Bound by HBM: 2 D bytes of keys and values for
-// 4 D products a head; the products of 8 heads cost a tenth of the time the bytes take. As in the forward pass
-// over whole sequences the maximum in use only follows when it has grown by 2^8.
+// by warp-level matrix instructions. The order of an inner dimension is free as long as both operands share it, so
+// a lane's fragments can be whole 16-byte pieces of rows: for S^T, lane (g, t) of a row of four takes elements
+// 8 (t + 4c) .. + 7 of position g's key, and of head g's query; for O^T it takes elements 8 (g + 8c) .. + 7 of the
+// values of positions 2t, 2t + 1, 2t + 8, 2t + 9, whose pairs two byte permutes put side by side. Every lane copies
+// its own pieces into its own places of a ring in shared memory, some steps ahead: no lane waits for another, there
+// are no bank conflicts, and the bytes on their way are bounded by shared memory (192 KB an SM), not by registers.
+// (Pieces loaded into registers one step ahead: 4.5 TB/s and 237 us on 64 sequences of 1 to 8191 positions, 32
+// heads of 128 over 8 key heads.) Warps meet only at the end of a unit. Bound by HBM: 2 D bytes of keys and values for
+// 4 D products a head; the products of 8 heads cost a tenth of the time the bytes take. As in the forward pass over
+// whole sequences the maximum in use only follows when it has grown by 2^8.
 template <bool kBf16, int kDP>
-__global__ void __launch_bounds__(kAnswerThreads, kDP == 64 ? 4 : 3) answer_mma_kernel(const AnswerDev p) {
-  constexpr int kKC = kDP / 32, kVC = kDP / 64;   // 16-byte loads of a lane for a key, for a value
-  __shared__ float sums[kAnswerThreads / 32][kHeads][kDP + 4];
+__global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_kernel(const AnswerDev p) {
+  using R = Ring<kDP>;
+  constexpr int kKC = R::kKC, kVC = R::kVC, kStages = R::kStages;
+  extern __shared__ uint4 ring[];
   __shared__ float stats[kAnswerThreads / 32][kHeads][2];
+  float* sums = reinterpret_cast<float*>(ring);   // [warp][head][kSumRow]
   const int D = p.c.D, tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = lane / 4, t = lane % 4;
+  const uint4* mine = ring + warp * kStages * R::kPieces * 32 + lane;
+  const uint32_t mine_at = smem_addr(mine);
   int64_t end;
   Start s = find_start(p, &end);
   int64_t at = s.at;
@@ -362,61 +389,80 @@ __global__ void __launch_bounds__(kAnswerThreads, kDP == 64 ? 4 : 3) answer_mma_
       if (g < heads && d < D)
         q[c] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + b * p.q_row + (head0 + g) * p.q_head + d);
     }
-    // the page and the place in it of position lane % 16 of this warp's share of a tile; page -1: takes no part
-    auto locate = [&](int tile, int* slot) {
+    // the page and the place in it of position lane % 16 of this warp's share of a tile; place -1: behind the last
+    int page, slot;
+    auto locate = [&](int tile) {
       const int x = tile * kTile + warp * 16 + (lane & 15);
-      int page = -1;
-      *slot = 0;
+      page = -1;
+      slot = -1;
       if (tile < stop && x < len) {
         const int n = x / p.c.page_size;
-        *slot = x - n * p.c.page_size;
+        slot = x - n * p.c.page_size;
         page = __ldg(p.c.page_table + b * p.c.table_stride + n);
-        if (page < 0 || page >= p.c.num_pages) {
-          page = -1;
-          raise(p.c);
-        }
       }
-      return page;
     };
-    uint4 k[2][kKC], v[4][kVC];
-    bool ok[2];
-    auto load_keys = [&](int page, int slot) {
+    uint32_t part = 0;   // which of positions g and g + 8 take part, two bits a step, the newest lowest
+    auto copy = [&](int stage) {   // the step that was located last
+      if (slot >= 0 && (page < 0 || page >= p.c.num_pages)) {
+        page = -1;
+        raise(p.c);
+      }
+      const uint32_t to = mine_at + stage * R::kStep;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int pg = __shfl_sync(kFullMask, page, g + 8 * i), sl = __shfl_sync(kFullMask, slot, g + 8 * i);
-        ok[i] = pg >= 0;
-        const uint16_t* row = kc + pg * p.c.k_page + sl * p.c.k_slot + 8 * t;
+        const bool in = pg >= 0;
+        part = part << 1 | (in ? 1u : 0u);
+        const uint16_t* row = in ? kc + pg * p.c.k_page + sl * p.c.k_slot + 8 * t : kc;
 #pragma unroll
-        for (int c = 0; c < kKC; ++c) k[i][c] = ok[i] && 8 * (t + 4 * c) < D ? ldg_stream16(row + 32 * c) : make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < kKC; ++c) {
+          const bool on = in && 8 * (t + 4 * c) < D;
+          copy16(to + (i * kKC + c) * 512, on ? row + 32 * c : kc, on);
+        }
       }
-    };
-    auto load_values = [&](int page, int slot) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int x = 2 * t + (i & 1) + 8 * (i / 2);
         const int pg = __shfl_sync(kFullMask, page, x), sl = __shfl_sync(kFullMask, slot, x);
-        const uint16_t* row = vc + pg * p.c.v_page + sl * p.c.v_slot + 8 * g;
+        const bool in = pg >= 0;
+        const uint16_t* row = in ? vc + pg * p.c.v_page + sl * p.c.v_slot + 8 * g : vc;
 #pragma unroll
-        for (int c = 0; c < kVC; ++c) v[i][c] = pg >= 0 && 8 * (g + 8 * c) < D ? ldg_stream16(row + 64 * c) : make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < kVC; ++c) {
+          const bool on = in && 8 * (g + 8 * c) < D;
+          copy16(to + (2 * kKC + i * kVC + c) * 512, on ? row + 64 * c : vc, on);
+        }
       }
     };
     float o[kVC * 4][4] = {};
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};   // of heads 2t and 2t + 1
-    int slot, next_slot;
-    int page = locate(s.tile, &slot);
-    load_keys(page, slot);
-    load_values(page, slot);
-    int next_page = locate(s.tile + 1, &next_slot);
+    __syncthreads();   // the last unit's sums, which lie in the ring, have been read
+    locate(s.tile);
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (s.tile + i < stop) copy(i); else part <<= 2;
+      copies_commit();
+      locate(s.tile + i + 1);
+    }
+    int stage = 0;
     for (int tile = s.tile; tile < stop; ++tile) {
+      copies_wait<kStages - 2>();
+      {
+        const int next = stage == 0 ? kStages - 1 : stage - 1;   // (stage + kStages - 1) % kStages
+        if (tile + kStages - 1 < stop) copy(next); else part <<= 2;
+        copies_commit();
+        locate(tile + kStages);
+      }
+      const uint4* from = mine + stage * (R::kStep / 16);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
       float x[4] = {};
 #pragma unroll
       for (int c = 0; c < kKC; ++c) {
-        mma16816<kBf16>(x, k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, q[c].x, q[c].y);
-        mma16816<kBf16>(x, k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, q[c].z, q[c].w);
+        const uint4 k0 = from[c * 32], k1 = from[(kKC + c) * 32];
+        mma16816<kBf16>(x, k0.x, k1.x, k0.y, k1.y, q[c].x, q[c].y);
+        mma16816<kBf16>(x, k0.z, k1.z, k0.w, k1.w, q[c].z, q[c].w);
       }
+      const uint32_t in = part >> (2 * (kStages - 1));   // of this step: position g in bit 1, g + 8 in bit 0
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = ok[i / 2] ? x[i] * p.scale_log2 : -INFINITY;
-      if (tile + 1 < stop) load_keys(next_page, next_slot);
+      for (int i = 0; i < 4; ++i) x[i] = (in >> (1 - i / 2) & 1) != 0 ? x[i] * p.scale_log2 : -INFINITY;
       const float most[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
       if (__any_sync(kFullMask, most[0] > top[0] + 8.f || most[1] > top[1] + 8.f)) {
 #pragma unroll
@@ -442,23 +488,24 @@ __global__ void __launch_bounds__(kAnswerThreads, kDP == 64 ? 4 : 3) answer_mma_
       const uint32_t p0 = transpose8x8(pack2<kBf16>(x[0], x[1])), p1 = transpose8x8(pack2<kBf16>(x[2], x[3]));
 #pragma unroll
       for (int c = 0; c < kVC; ++c) {
-        const uint32_t a[4][4] = {{v[0][c].x, v[0][c].y, v[0][c].z, v[0][c].w}, {v[1][c].x, v[1][c].y, v[1][c].z, v[1][c].w},
-                                  {v[2][c].x, v[2][c].y, v[2][c].z, v[2][c].w}, {v[3][c].x, v[3][c].y, v[3][c].z, v[3][c].w}};
+        uint32_t a[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 v = from[(2 * kKC + i * kVC + c) * 32];
+          a[i][0] = v.x, a[i][1] = v.y, a[i][2] = v.z, a[i][3] = v.w;
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           mma16816<kBf16>(o[c * 4 + r], __byte_perm(a[0][r], a[1][r], 0x5410), __byte_perm(a[0][r], a[1][r], 0x7632),
                           __byte_perm(a[2][r], a[3][r], 0x5410), __byte_perm(a[2][r], a[3][r], 0x7632), p0, p1);
       }
-      if (tile + 1 < stop) {
-        load_values(next_page, next_slot);
-        next_page = locate(tile + 2, &next_slot);
-      }
     }
+    copies_wait<0>();
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int w = 4; w < 32; w <<= 1) sum[i] += __shfl_xor_sync(kFullMask, sum[i], w);
-    __syncthreads();   // the last unit's sums have been read
+    __syncthreads();   // every warp is done with its part of the ring
     if (g < 2) {
       stats[warp][2 * t + g][0] = g == 0 ? top[0] : top[1];
       stats[warp][2 * t + g][1] = g == 0 ? sum[0] : sum[1];
@@ -469,10 +516,11 @@ __global__ void __launch_bounds__(kAnswerThreads, kDP == 64 ? 4 : 3) answer_mma_
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          *reinterpret_cast<float2*>(&sums[warp][2 * t + i][8 * (g + 8 * c) + 2 * r]) = make_float2(o[c * 4 + r][i], o[c * 4 + r][2 + i]);
+          *reinterpret_cast<float2*>(&sums[(warp * kHeads + 2 * t + i) * R::kSumRow + 8 * (g + 8 * c) + 2 * r]) =
+              make_float2(o[c * 4 + r][i], o[c * 4 + r][2 + i]);
     __syncthreads();
     const bool whole = s.tile == 0 && stop == s.tiles;
-    const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (s.tile == 0 ? 1 : 0);
+    const int64_t slot_of = 2 * static_cast<int64_t>(blockIdx.x) + (s.tile == 0 ? 1 : 0);
     for (int i = tid; i < heads * D; i += kAnswerThreads) {
       const int h = i / D, d = i - h * D;
       float m = stats[0][h][0];
@@ -484,16 +532,16 @@ __global__ void __launch_bounds__(kAnswerThreads, kDP == 64 ? 4 : 3) answer_mma_
       for (int w = 0; w < kAnswerThreads / 32; ++w) {
         const float f = fast_exp2(stats[w][h][0] - base);
         l = fmaf(f, stats[w][h][1], l);
-        x = fmaf(f, sums[w][h][d], x);
+        x = fmaf(f, sums[(w * kHeads + h) * R::kSumRow + d], x);
       }
       if (whole) {
         const uint32_t y = pack2<kBf16>(l == 0.f ? 0.f : x / l, 0.f);
         static_cast<uint16_t*>(p.out)[b * p.o_row + (head0 + h) * p.o_head + d] = static_cast<uint16_t>(y);
       } else {
-        p.sums[(part * kHeads + h) * D + d] = x;
+        p.sums[(slot_of * kHeads + h) * D + d] = x;
         if (d == 0) {
-          p.stats[(part * kHeads + h) * 2] = m;
-          p.stats[(part * kHeads + h) * 2 + 1] = l;
+          p.stats[(slot_of * kHeads + h) * 2] = m;
+          p.stats[(slot_of * kHeads + h) * 2 + 1] = l;
         }
       }
     }
@@ -589,12 +637,15 @@ bool answer_fits_mma(const AnswerDev& p) {
   return bits % 16 == 0 && p.c.D <= 128;
 }
 
-template <typename T, bool kBf16>
-int launch_answer_mma(const AnswerDev& p, int ctas, cudaStream_t stream) {
-  if (p.c.D <= 64)
-    answer_mma_kernel<kBf16, 64><<<ctas, kAnswerThreads, 0, stream>>>(p);
-  else
-    answer_mma_kernel<kBf16, 128><<<ctas, kAnswerThreads, 0, stream>>>(p);
+template <typename T, bool kBf16, int kDP>
+int launch_answer_mma(const AnswerDev& p, int64_t tiles, cudaStream_t stream) {
+  using R = Ring<kDP>;
+  const auto kernel = answer_mma_kernel<kBf16, kDP>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes) != cudaSuccess ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess)
+    return B200TBE_ERR_LAUNCH;
+  const int ctas = static_cast<int>(tiles < kNumSMs * R::kCtas ? tiles : kNumSMs * R::kCtas);
+  kernel<<<ctas, kAnswerThreads, R::kBytes, stream>>>(p);
   const int st = launch_status();
   return st != B200TBE_OK ? st : join<T>(p, ctas, stream);
 }
@@ -675,10 +726,10 @@ extern "C" int b200tbe_paged_attention(const b200tbe_paged_cache* cache, const v
   const int64_t most = (static_cast<int64_t>(cache->max_pages) * cache->page_size + kTile - 1) / kTile;
   const int64_t tiles = static_cast<int64_t>(p.units) * cache->batch * (most < 1 ? 1 : most);
   if (cache->dtype != B200TBE_FP32 && answer_fits_mma(p)) {
-    const int most_ctas = kNumSMs * (p.c.D <= 64 ? 4 : 3);
-    const int ctas = static_cast<int>(tiles < most_ctas ? tiles : most_ctas);
-    return cache->dtype == B200TBE_FP16 ? launch_answer_mma<__half, false>(p, ctas, stream)
-                                        : launch_answer_mma<__nv_bfloat16, true>(p, ctas, stream);
+    if (cache->dtype == B200TBE_FP16)
+      return p.c.D <= 64 ? launch_answer_mma<__half, false, 64>(p, tiles, stream) : launch_answer_mma<__half, false, 128>(p, tiles, stream);
+    return p.c.D <= 64 ? launch_answer_mma<__nv_bfloat16, true, 64>(p, tiles, stream)
+                       : launch_answer_mma<__nv_bfloat16, true, 128>(p, tiles, stream);
   }
   const int ctas = static_cast<int>(tiles < kAnswerCtas ? tiles : kAnswerCtas);
   if (cache->dtype == B200TBE_FP32) return launch_answer<float>(p, ctas, stream);
