@@ -112,19 +112,21 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendDev p) {
 //   out[h] = sum_t exp(s_t - m) v_t / sum_t exp(s_t - m),   s_t = scale q[h] . k[t]
 //
 // Work is counted in tiles of kTile positions of one unit: a sequence, a key head and up to kHeads of its
-// query heads. All units' tiles in one line are cut into equal pieces, one for each CTA, so that the GPU is
-// evenly loaded whatever the lengths. A unit inside one CTA is finished there. One that a cut divides leaves
+// query heads. All units in one line, each as long as its tiles and kUnitCost more (what beginning and ending one
+// takes), are cut into equal pieces, one for each CTA, so that the GPU is evenly loaded whatever the lengths.
+// (Without the unit's own cost the CTAs that got the short sequences of a mixed batch were the last by a third.) A unit inside one CTA is finished there. One that a cut divides leaves
 // a piece (m, l, unnormalised sum) in each CTA's slot; a second kernel joins the pieces in their order:
 //   m = max m_i,  l = sum l_i exp(m_i - m),  out = sum o_i exp(m_i - m) / l
 constexpr int kTile = 64;
 constexpr int kHeads = 8;
+constexpr int kUnitCost = 2;
 constexpr int kAnswerThreads = 128;
 constexpr int kAnswerCtas = kNumSMs * 8;
 
 // Where a CTA's piece of the line begins.
 struct Start {
   int32_t unit, tile, tiles, ctas;   // unit, tile inside it, the unit's tiles, CTAs with work
-  int64_t at, all;                   // place in the line, the line's length
+  int64_t first, all;                // the unit's first place in the line, the line's length
 };
 
 struct AnswerDev {
@@ -132,7 +134,7 @@ struct AnswerDev {
   const void* q;
   void* out;
   int64_t q_row, q_head, o_row, o_head;
-  int32_t heads, group, chunks, units;   // chunks of kHeads query heads a key head; units a sequence
+  int32_t heads, group, per, chunks, units;   // chunks of `per` query heads a key head; units a sequence
   float scale_log2;   // scale log2 e: scores, maxima and log-sums are in powers of two
   Start* starts;     // [gridDim.x]
   float* stats;      // [2 * gridDim.x][kHeads][2]: m, l
@@ -141,14 +143,14 @@ struct AnswerDev {
 
 __device__ __forceinline__ int tiles_of(const CacheDev& c, int b) { return max(1, (length_of(c, b) + kTile - 1) / kTile); }
 
-// The CTA's piece [at, end) of the line, and the sequence and unit its first tile lies in. All threads.
+// Where the CTA's piece of the line begins, and its end. All threads.
 __device__ __forceinline__ Start find_start(const AnswerDev& p, int64_t* end) {
   __shared__ int64_t sums[kAnswerThreads / 32];
   __shared__ Start found;
   const int n = p.c.batch, per = (n + kAnswerThreads - 1) / kAnswerThreads;
   const int b0 = min(n, static_cast<int>(threadIdx.x) * per), b1 = min(n, b0 + per);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += tiles_of(p.c, b);
+  int64_t mine = 0;   // of these sequences' units of one kind
+  for (int b = b0; b < b1; ++b) mine += tiles_of(p.c, b) + kUnitCost;
   int64_t upto = mine;   // inclusive sum over the threads
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
 #pragma unroll
@@ -172,17 +174,18 @@ __device__ __forceinline__ Start find_start(const AnswerDev& p, int64_t* end) {
   if (at >= first && at < first + mine * p.units) {
     int b = b0;
     int64_t tiles = tiles_of(p.c, b);
-    while (at >= first + tiles * p.units) {
-      first += tiles * p.units;
+    while (at >= first + (tiles + kUnitCost) * p.units) {
+      first += (tiles + kUnitCost) * p.units;
       tiles = tiles_of(p.c, ++b);
     }
-    const int64_t u = (at - first) / tiles;
-    found = Start{static_cast<int32_t>(b * p.units + u), static_cast<int32_t>(at - first - u * tiles),
-                  static_cast<int32_t>(tiles), static_cast<int32_t>(ctas), at, all};
+    const int64_t u = (at - first) / (tiles + kUnitCost);
+    first += u * (tiles + kUnitCost);
+    found = Start{static_cast<int32_t>(b * p.units + u), static_cast<int32_t>(max(static_cast<int64_t>(0), at - first - kUnitCost)),
+                  static_cast<int32_t>(tiles), static_cast<int32_t>(ctas), first, all};
   }
   __syncthreads();
   Start s = found;
-  if (at >= *end) s = Start{-1, 0, 0, static_cast<int32_t>(ctas), at, all};
+  if (at >= *end) s = Start{-1, 0, 0, static_cast<int32_t>(ctas), at, all};   // no piece
   if (threadIdx.x == 0) p.starts[blockIdx.x] = s;
   return s;
 }
@@ -200,13 +203,15 @@ __global__ void __launch_bounds__(kAnswerThreads) answer_simt_kernel(const Answe
   const int D = p.c.D, tid = threadIdx.x;
   int64_t end;
   Start s = find_start(p, &end);
-  int64_t at = s.at;
-  while (at < end) {
+  for (; s.first < end; s.first += s.tiles + kUnitCost, ++s.unit, s.tile = 0) {
+    if (s.unit >= p.units * p.c.batch) break;
+    s.tiles = tiles_of(p.c, s.unit / p.units);
+    const int stop = static_cast<int>(min(static_cast<int64_t>(s.tiles), end - s.first - kUnitCost));
+    if (stop <= s.tile) continue;
     const int b = s.unit / p.units, u = s.unit % p.units, kv = u / p.chunks;
-    const int head0 = kv * p.group + (u % p.chunks) * kHeads;
-    const int heads = min(kHeads, (kv + 1) * p.group - head0);
+    const int head0 = kv * p.group + (u % p.chunks) * p.per;
+    const int heads = min(p.per, (kv + 1) * p.group - head0);
     const int len = length_of(p.c, b);
-    const int stop = static_cast<int>(min(static_cast<int64_t>(s.tiles), s.tile + (end - at)));
     __syncthreads();
     for (int i = tid; i < heads * D; i += kAnswerThreads) {
       const int h = i / D, d = i % D;
@@ -298,12 +303,6 @@ __global__ void __launch_bounds__(kAnswerThreads) answer_simt_kernel(const Answe
             p.sums[(part * kHeads + h) * D + d] = o[h][c];
         }
     }
-    at += stop - s.tile;
-    if (at < end) {
-      ++s.unit;
-      s.tile = 0;
-      s.tiles = tiles_of(p.c, s.unit / p.units);
-    }
   }
 }
 
@@ -371,13 +370,15 @@ __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_k
   const uint32_t mine_at = smem_addr(mine);
   int64_t end;
   Start s = find_start(p, &end);
-  int64_t at = s.at;
-  while (at < end) {
+  for (; s.first < end; s.first += s.tiles + kUnitCost, ++s.unit, s.tile = 0) {
+    if (s.unit >= p.units * p.c.batch) break;
+    s.tiles = tiles_of(p.c, s.unit / p.units);
+    const int stop = static_cast<int>(min(static_cast<int64_t>(s.tiles), end - s.first - kUnitCost));
+    if (stop <= s.tile) continue;
     const int b = s.unit / p.units, u = s.unit % p.units, kv = u / p.chunks;
-    const int head0 = kv * p.group + (u % p.chunks) * kHeads;
-    const int heads = min(kHeads, (kv + 1) * p.group - head0);
+    const int head0 = kv * p.group + (u % p.chunks) * p.per;
+    const int heads = min(p.per, (kv + 1) * p.group - head0);
     const int len = length_of(p.c, b);
-    const int stop = static_cast<int>(min(static_cast<int64_t>(s.tiles), s.tile + (end - at)));
     if (tid == 0 && s.tile == 0 && raw_length(p.c, b) != len) raise(p.c);
     const uint16_t* kc = reinterpret_cast<const uint16_t*>(p.c.k) + kv * p.c.k_head;
     const uint16_t* vc = reinterpret_cast<const uint16_t*>(p.c.v) + kv * p.c.v_head;
@@ -545,11 +546,225 @@ __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_k
         }
       }
     }
-    at += stop - s.tile;
-    if (at < end) {
-      ++s.unit;
-      s.tile = 0;
-      s.tiles = tiles_of(p.c, s.unit / p.units);
+  }
+}
+
+// fp32, head dimensions that are multiples of 4 up to kDP, up to kH query heads of a key head. Eight lanes share a
+// position, a warp takes four positions at once and 4 kPos a step; a lane has elements 4 (t + 8c) .. + 3 of its
+// positions' keys and values, of the heads' queries (in shared memory) and of their sums. Scores are summed over the
+// eight lanes by shuffles, the warp's four groups of lanes are summed at the end of a unit. The ring is as above.
+// Bound by HBM as long as a key head has few query heads: 2 D FMAs a head and position against 8 D bytes.
+template <int kDP>
+struct RingF {
+  static constexpr int kC = kDP / 32;                 // 16-byte pieces of a lane for a key or a value
+  static constexpr int kPos = kDP == 64 ? 4 : 2;      // positions of a lane in a step
+  static constexpr int kH = kDP == 64 ? 8 : 4;
+  static constexpr int kPieces = 2 * kPos * kC;
+  static constexpr int kStep = kPieces * 512;         // 8 KB
+  static constexpr int kStages = 3, kCtas = 2;
+  static constexpr int kSteps = 4 / kPos;             // of a tile
+  static constexpr int kBytes = kAnswerThreads / 32 * kStages * kStep;
+  static_assert(kBytes >= kAnswerThreads / 32 * kH * kDP * 4, "the warps' sums take the ring's place");
+};
+
+template <int kDP>
+__global__ void __launch_bounds__(kAnswerThreads, RingF<kDP>::kCtas) answer_fma_kernel(const AnswerDev p) {
+  using R = RingF<kDP>;
+  constexpr int kC = R::kC, kPos = R::kPos, kH = R::kH, kStages = R::kStages;
+  extern __shared__ uint4 ring[];
+  __shared__ float stats[kAnswerThreads / 32][kH][2];
+  __shared__ __align__(16) float qs[kH][kDP];
+  float* sums = reinterpret_cast<float*>(ring);   // [warp][head][kDP]
+  const int D = p.c.D, tid = threadIdx.x, lane = tid & 31, warp = tid / 32, group = lane / 8, t = lane % 8;
+  const uint4* mine = ring + warp * kStages * R::kPieces * 32 + lane;
+  const uint32_t mine_at = smem_addr(mine);
+  int64_t end;
+  Start s = find_start(p, &end);
+  for (; s.first < end; s.first += s.tiles + kUnitCost, ++s.unit, s.tile = 0) {
+    if (s.unit >= p.units * p.c.batch) break;
+    s.tiles = tiles_of(p.c, s.unit / p.units);
+    const int stop = static_cast<int>(min(static_cast<int64_t>(s.tiles), end - s.first - kUnitCost));
+    if (stop <= s.tile) continue;
+    const int b = s.unit / p.units, u = s.unit % p.units, kv = u / p.chunks;
+    const int head0 = kv * p.group + (u % p.chunks) * p.per;
+    const int heads = min(p.per, (kv + 1) * p.group - head0);
+    const int len = length_of(p.c, b);
+    if (tid == 0 && s.tile == 0 && raw_length(p.c, b) != len) raise(p.c);
+    const float* kc = reinterpret_cast<const float*>(p.c.k) + kv * p.c.k_head;
+    const float* vc = reinterpret_cast<const float*>(p.c.v) + kv * p.c.v_head;
+    __syncthreads();   // the last unit's queries, and its sums, which lie in the ring, have been read
+    for (int i = tid; i < kH * kDP; i += kAnswerThreads) {
+      const int h = i / kDP, d = i % kDP;
+      qs[h][d] = h < heads && d < D ? static_cast<const float*>(p.q)[b * p.q_row + (head0 + h) * p.q_head + d] : 0.f;
+    }
+    __syncthreads();
+    const int first_step = s.tile * R::kSteps, last_step = stop * R::kSteps;
+    // the page and the place in it of position lane % (4 kPos) of this warp's share of a step; place -1: behind the last
+    int page, slot;
+    auto locate = [&](int step) {
+      const int x = step / R::kSteps * kTile + warp * 16 + step % R::kSteps * 4 * kPos + lane % (4 * kPos);
+      page = -1;
+      slot = -1;
+      if (step < last_step && x < len) {
+        const int n = x / p.c.page_size;
+        slot = x - n * p.c.page_size;
+        page = __ldg(p.c.page_table + b * p.c.table_stride + n);
+      }
+    };
+    uint32_t part = 0;   // which of the lane's positions take part, kPos bits a step, the newest lowest
+    auto copy = [&](int stage) {   // the step that was located last
+      if (slot >= 0 && (page < 0 || page >= p.c.num_pages)) {
+        page = -1;
+        raise(p.c);
+      }
+      const uint32_t to = mine_at + stage * R::kStep;
+#pragma unroll
+      for (int i = 0; i < kPos; ++i) {
+        const int pg = __shfl_sync(kFullMask, page, i * 4 + group), sl = __shfl_sync(kFullMask, slot, i * 4 + group);
+        const bool in = pg >= 0;
+        part = part << 1 | (in ? 1u : 0u);
+        const float* kr = in ? kc + pg * p.c.k_page + sl * p.c.k_slot + 4 * t : kc;
+        const float* vr = in ? vc + pg * p.c.v_page + sl * p.c.v_slot + 4 * t : vc;
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+          const bool on = in && 4 * (t + 8 * c) < D;
+          copy16(to + (i * kC + c) * 512, on ? kr + 32 * c : kc, on);
+          copy16(to + ((kPos + i) * kC + c) * 512, on ? vr + 32 * c : vc, on);
+        }
+      }
+    };
+    float o[kH][kC][4] = {};
+    float top[kH], sum[kH];
+#pragma unroll
+    for (int h = 0; h < kH; ++h) top[h] = -INFINITY, sum[h] = 0.f;
+    locate(first_step);
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (first_step + i < last_step) copy(i); else part <<= kPos;
+      copies_commit();
+      locate(first_step + i + 1);
+    }
+    int stage = 0;
+    for (int step = first_step; step < last_step; ++step) {
+      copies_wait<kStages - 2>();
+      {
+        const int next = stage == 0 ? kStages - 1 : stage - 1;   // (stage + kStages - 1) % kStages
+        if (step + kStages - 1 < last_step) copy(next); else part <<= kPos;
+        copies_commit();
+        locate(step + kStages);
+      }
+      const uint4* from = mine + stage * (R::kStep / 16);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      const uint32_t in = part >> (kPos * (kStages - 1));
+      float x[kH][kPos];
+#pragma unroll
+      for (int h = 0; h < kH; ++h) {
+        if (h < heads) {
+#pragma unroll
+          for (int i = 0; i < kPos; ++i) x[h][i] = 0.f;
+#pragma unroll
+          for (int c = 0; c < kC; ++c) {
+            const float4 q = *reinterpret_cast<const float4*>(&qs[h][4 * (t + 8 * c)]);
+#pragma unroll
+            for (int i = 0; i < kPos; ++i) {
+              const uint4 k = from[(i * kC + c) * 32];
+              x[h][i] = fmaf(__uint_as_float(k.x), q.x, x[h][i]);
+              x[h][i] = fmaf(__uint_as_float(k.y), q.y, x[h][i]);
+              x[h][i] = fmaf(__uint_as_float(k.z), q.z, x[h][i]);
+              x[h][i] = fmaf(__uint_as_float(k.w), q.w, x[h][i]);
+            }
+          }
+          float most = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kPos; ++i) {
+#pragma unroll
+            for (int w = 1; w < 8; w <<= 1) x[h][i] += __shfl_xor_sync(kFullMask, x[h][i], w);
+            x[h][i] = (in >> (kPos - 1 - i) & 1) != 0 ? x[h][i] * p.scale_log2 : -INFINITY;
+            most = fmaxf(most, x[h][i]);
+          }
+          if (__any_sync(kFullMask, most > top[h] + 8.f)) {
+            float m = fmaxf(top[h], most);
+            m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 16));
+            const float keep = m == -INFINITY ? 1.f : exp2f(top[h] - m);
+            top[h] = m;
+            sum[h] *= keep;
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[h][c][e] *= keep;
+          }
+          const float base = top[h] == -INFINITY ? 0.f : top[h];
+#pragma unroll
+          for (int i = 0; i < kPos; ++i) {
+            x[h][i] = exp2f(x[h][i] - base);
+            sum[h] += x[h][i];
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kPos; ++i)
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+          const uint4 v = from[((kPos + i) * kC + c) * 32];
+#pragma unroll
+          for (int h = 0; h < kH; ++h)
+            if (h < heads) {
+              o[h][c][0] = fmaf(x[h][i], __uint_as_float(v.x), o[h][c][0]);
+              o[h][c][1] = fmaf(x[h][i], __uint_as_float(v.y), o[h][c][1]);
+              o[h][c][2] = fmaf(x[h][i], __uint_as_float(v.z), o[h][c][2]);
+              o[h][c][3] = fmaf(x[h][i], __uint_as_float(v.w), o[h][c][3]);
+            }
+        }
+    }
+    copies_wait<0>();
+    __syncthreads();   // every warp is done with its part of the ring
+#pragma unroll
+    for (int h = 0; h < kH; ++h)
+      if (h < heads) {
+#pragma unroll
+        for (int w = 8; w < 32; w <<= 1) {
+          sum[h] += __shfl_xor_sync(kFullMask, sum[h], w);
+#pragma unroll
+          for (int c = 0; c < kC; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[h][c][e] += __shfl_xor_sync(kFullMask, o[h][c][e], w);
+        }
+        if (lane == 0) {
+          stats[warp][h][0] = top[h];
+          stats[warp][h][1] = sum[h];
+        }
+        if (group == 0) {
+#pragma unroll
+          for (int c = 0; c < kC; ++c)
+            *reinterpret_cast<float4*>(&sums[(warp * kH + h) * kDP + 4 * (t + 8 * c)]) =
+                make_float4(o[h][c][0], o[h][c][1], o[h][c][2], o[h][c][3]);
+        }
+      }
+    __syncthreads();
+    const bool whole = s.tile == 0 && stop == s.tiles;
+    const int64_t slot_of = 2 * static_cast<int64_t>(blockIdx.x) + (s.tile == 0 ? 1 : 0);
+    for (int i = tid; i < heads * D; i += kAnswerThreads) {
+      const int h = i / D, d = i - h * D;
+      float m = stats[0][h][0];
+#pragma unroll
+      for (int w = 1; w < kAnswerThreads / 32; ++w) m = fmaxf(m, stats[w][h][0]);
+      const float base = m == -INFINITY ? 0.f : m;
+      float l = 0.f, x = 0.f;
+#pragma unroll
+      for (int w = 0; w < kAnswerThreads / 32; ++w) {
+        const float f = exp2f(stats[w][h][0] - base);
+        l = fmaf(f, stats[w][h][1], l);
+        x = fmaf(f, sums[(w * kH + h) * kDP + d], x);
+      }
+      if (whole) {
+        static_cast<float*>(p.out)[b * p.o_row + (head0 + h) * p.o_head + d] = l == 0.f ? 0.f : x / l;
+      } else {
+        p.sums[(slot_of * kHeads + h) * D + d] = x;
+        if (d == 0) {
+          p.stats[(slot_of * kHeads + h) * 2] = m;
+          p.stats[(slot_of * kHeads + h) * 2 + 1] = l;
+        }
+      }
     }
   }
 }
@@ -563,10 +778,10 @@ __global__ void __launch_bounds__(kAnswerThreads) join_kernel(const AnswerDev p)
   const Start before = p.starts[c - 1];
   if (before.unit == s.unit && before.tile > 0) return;
   const int u = s.unit % p.units, kv = u / p.chunks, b = s.unit / p.units;
-  const int head = kv * p.group + (u % p.chunks) * kHeads + h;
+  const int head = kv * p.group + (u % p.chunks) * p.per + h;
   if (head >= (kv + 1) * p.group) return;
   // the CTA that holds the unit's last tile
-  const int last = static_cast<int>(((s.at - s.tile + s.tiles) * s.ctas - 1) / s.all);
+  const int last = static_cast<int>(((s.first + kUnitCost + s.tiles) * s.ctas - 1) / s.all);
   // the first piece lies in its CTA's second slot, the others in the first
   const int64_t part0 = 2 * static_cast<int64_t>(c - 1) + 1;
   float m = p.stats[(part0 * kHeads + h) * 2];
@@ -624,17 +839,35 @@ int launch_append(const AppendDev& p, cudaStream_t stream) {
 template <typename T>
 int join(const AnswerDev& p, int ctas, cudaStream_t stream) {
   if (ctas < 2) return B200TBE_OK;
-  join_kernel<T><<<dim3(ctas - 1, min(kHeads, p.group)), kAnswerThreads, 0, stream>>>(p);
+  join_kernel<T><<<dim3(ctas - 1, min(p.per, p.group)), kAnswerThreads, 0, stream>>>(p);
   return launch_status();
 }
 
 // 16-byte reads of everything, and a head dimension that the registers hold
-bool answer_fits_mma(const AnswerDev& p) {
+bool answer_in_pieces(const AnswerDev& p, int elem_bytes) {
   uint64_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.c.k) | reinterpret_cast<uintptr_t>(p.c.v);
   for (int64_t x : {static_cast<int64_t>(p.c.D), p.q_row, p.q_head, p.c.k_page, p.c.k_slot, p.c.k_head, p.c.v_page, p.c.v_slot,
                     p.c.v_head})
-    bits |= static_cast<uint64_t>(x * 2);
+    bits |= static_cast<uint64_t>(x * elem_bytes);
   return bits % 16 == 0 && p.c.D <= 128;
+}
+
+template <int kDP>
+int launch_answer_fma(AnswerDev p, int64_t most, cudaStream_t stream) {
+  using R = RingF<kDP>;
+  const auto kernel = answer_fma_kernel<kDP>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes) != cudaSuccess ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess)
+    return B200TBE_ERR_LAUNCH;
+  p.per = R::kH;
+  p.chunks = (p.group + p.per - 1) / p.per;
+  p.units = p.c.kv_heads * p.chunks;
+  if (static_cast<int64_t>(p.units) * p.c.batch > 0x7fffffff) return B200TBE_ERR_TOO_LARGE;
+  const int64_t tiles = static_cast<int64_t>(p.units) * p.c.batch * (most + kUnitCost);
+  const int ctas = static_cast<int>(tiles < kNumSMs * R::kCtas ? tiles : kNumSMs * R::kCtas);
+  kernel<<<ctas, kAnswerThreads, R::kBytes, stream>>>(p);
+  const int st = launch_status();
+  return st != B200TBE_OK ? st : join<float>(p, ctas, stream);
 }
 
 template <typename T, bool kBf16, int kDP>
@@ -714,7 +947,7 @@ extern "C" int b200tbe_paged_attention(const b200tbe_paged_cache* cache, const v
   p.c = cache_dev(cache);
   p.q = q, p.out = out;
   p.q_row = q_stride, p.q_head = q_head_stride, p.o_row = out_stride, p.o_head = out_head_stride;
-  p.heads = heads, p.group = heads / cache->kv_heads, p.chunks = (p.group + kHeads - 1) / kHeads;
+  p.heads = heads, p.group = heads / cache->kv_heads, p.per = kHeads, p.chunks = (p.group + kHeads - 1) / kHeads;
   p.units = cache->kv_heads * p.chunks;
   if (static_cast<int64_t>(p.units) * cache->batch > 0x7fffffff) return B200TBE_ERR_TOO_LARGE;
   p.scale_log2 = scale * 1.4426950408889634f;
@@ -723,9 +956,12 @@ extern "C" int b200tbe_paged_attention(const b200tbe_paged_cache* cache, const v
   p.sums = p.stats + 2 * kAnswerCtas * kHeads * 2;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   // as many CTAs as the cache could give tiles to
-  const int64_t most = (static_cast<int64_t>(cache->max_pages) * cache->page_size + kTile - 1) / kTile;
-  const int64_t tiles = static_cast<int64_t>(p.units) * cache->batch * (most < 1 ? 1 : most);
-  if (cache->dtype != B200TBE_FP32 && answer_fits_mma(p)) {
+  int64_t most = (static_cast<int64_t>(cache->max_pages) * cache->page_size + kTile - 1) / kTile;
+  if (most < 1) most = 1;
+  const int64_t tiles = static_cast<int64_t>(p.units) * cache->batch * (most + kUnitCost);
+  if (cache->dtype == B200TBE_FP32 && answer_in_pieces(p, 4))
+    return p.c.D <= 64 ? launch_answer_fma<64>(p, most, stream) : launch_answer_fma<128>(p, most, stream);
+  if (cache->dtype != B200TBE_FP32 && answer_in_pieces(p, 2)) {
     if (cache->dtype == B200TBE_FP16)
       return p.c.D <= 64 ? launch_answer_mma<__half, false, 64>(p, tiles, stream) : launch_answer_mma<__half, false, 128>(p, tiles, stream);
     return p.c.D <= 64 ? launch_answer_mma<__nv_bfloat16, true, 64>(p, tiles, stream)
