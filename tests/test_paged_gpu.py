@@ -65,6 +65,10 @@ ANSWERS = [
     (FP16, [65, 66], 3, 3, 8, 16),
     (BF16, [64] * 40, 5, 1, 96, 16),
     (FP32, [9000, 10], 8, 8, 64, 32),
+    (FP32, [300, 0, 65, 4000], 6, 1, 128, 16),
+    (FP32, [129, 64], 18, 2, 100, 10),
+    (FP16, [64, 128, 192, 1, 63, 65], 3, 1, 64, 64),
+    (BF16, [1025, 700], 8, 8, 72, 48),
 ]
 
 

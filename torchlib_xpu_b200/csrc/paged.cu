@@ -337,9 +337,9 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_grou
 template <int kDP>
 struct Ring {
   static constexpr int kKC = kDP / 32, kVC = kDP / 64;      // 16-byte pieces of a lane for a key, for a value
-  static constexpr int kPieces = 2 * kKC + 4 * kVC;         // of a lane for a step
-  static constexpr int kStages = kDP == 64 ? 4 : 3;
-  static constexpr int kCtas = kDP == 64 ? 3 : 2;           // per SM
+  static constexpr int kTiles = kDP == 64 ? 2 : 1;          // of a step: independent products hide one another's latency
+  static constexpr int kPieces = kTiles * (2 * kKC + 4 * kVC);   // of a lane for a step: 8 KB a warp
+  static constexpr int kStages = 3, kCtas = 2;              // per SM
   static constexpr int kStep = kPieces * 512;
   static constexpr int kBytes = kAnswerThreads / 32 * kStages * kStep;
   static constexpr int kSumRow = kDP + 4;
@@ -361,7 +361,7 @@ struct Ring {
 template <bool kBf16, int kDP>
 __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_kernel(const AnswerDev p) {
   using R = Ring<kDP>;
-  constexpr int kKC = R::kKC, kVC = R::kVC, kStages = R::kStages;
+  constexpr int kKC = R::kKC, kVC = R::kVC, kStages = R::kStages, kTiles = R::kTiles, kEach = R::kPieces / kTiles;
   extern __shared__ uint4 ring[];
   __shared__ float stats[kAnswerThreads / 32][kHeads][2];
   float* sums = reinterpret_cast<float*>(ring);   // [warp][head][kSumRow]
@@ -390,28 +390,32 @@ __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_k
       if (g < heads && d < D)
         q[c] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + b * p.q_row + (head0 + g) * p.q_head + d);
     }
-    // the page and the place in it of position lane % 16 of this warp's share of a tile; place -1: behind the last
+    // the page and the place in it of a position of this warp's share of a step's tiles: lane % 16 of tile lane / 16;
+    // place -1: behind the last
     int page, slot;
     auto locate = [&](int tile) {
-      const int x = tile * kTile + warp * 16 + (lane & 15);
+      const int of = tile + (kTiles == 2 ? lane / 16 : 0), x = of * kTile + warp * 16 + (lane & 15);
       page = -1;
       slot = -1;
-      if (tile < stop && x < len) {
+      if (of < stop && x < len) {
         const int n = x / p.c.page_size;
         slot = x - n * p.c.page_size;
         page = __ldg(p.c.page_table + b * p.c.table_stride + n);
       }
     };
-    uint32_t part = 0;   // which of positions g and g + 8 take part, two bits a step, the newest lowest
+    uint32_t part = 0;   // which of positions g and g + 8 take part, two bits a tile, the newest lowest
     auto copy = [&](int stage) {   // the step that was located last
       if (slot >= 0 && (page < 0 || page >= p.c.num_pages)) {
         page = -1;
         raise(p.c);
       }
-      const uint32_t to = mine_at + stage * R::kStep;
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) {
+      const uint32_t to = mine_at + stage * R::kStep + j * kEach * 512;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int pg = __shfl_sync(kFullMask, page, g + 8 * i), sl = __shfl_sync(kFullMask, slot, g + 8 * i);
+        const int x = j * 16 + g + 8 * i;
+        const int pg = __shfl_sync(kFullMask, page, x), sl = __shfl_sync(kFullMask, slot, x);
         const bool in = pg >= 0;
         part = part << 1 | (in ? 1u : 0u);
         const uint16_t* row = in ? kc + pg * p.c.k_page + sl * p.c.k_slot + 8 * t : kc;
@@ -423,7 +427,7 @@ __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_k
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int x = 2 * t + (i & 1) + 8 * (i / 2);
+        const int x = j * 16 + 2 * t + (i & 1) + 8 * (i / 2);
         const int pg = __shfl_sync(kFullMask, page, x), sl = __shfl_sync(kFullMask, slot, x);
         const bool in = pg >= 0;
         const uint16_t* row = in ? vc + pg * p.c.v_page + sl * p.c.v_slot + 8 * g : vc;
@@ -433,38 +437,46 @@ __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_k
           copy16(to + (2 * kKC + i * kVC + c) * 512, on ? row + 64 * c : vc, on);
         }
       }
+      }
     };
     float o[kVC * 4][4] = {};
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};   // of heads 2t and 2t + 1
     __syncthreads();   // the last unit's sums, which lie in the ring, have been read
     locate(s.tile);
     for (int i = 0; i < kStages - 1; ++i) {
-      if (s.tile + i < stop) copy(i); else part <<= 2;
+      if (s.tile + i * kTiles < stop) copy(i); else part <<= 2 * kTiles;
       copies_commit();
-      locate(s.tile + i + 1);
+      locate(s.tile + (i + 1) * kTiles);
     }
     int stage = 0;
-    for (int tile = s.tile; tile < stop; ++tile) {
+    for (int tile = s.tile; tile < stop; tile += kTiles) {
       copies_wait<kStages - 2>();
       {
         const int next = stage == 0 ? kStages - 1 : stage - 1;   // (stage + kStages - 1) % kStages
-        if (tile + kStages - 1 < stop) copy(next); else part <<= 2;
+        if (tile + (kStages - 1) * kTiles < stop) copy(next); else part <<= 2 * kTiles;
         copies_commit();
-        locate(tile + kStages);
+        locate(tile + kStages * kTiles);
       }
       const uint4* from = mine + stage * (R::kStep / 16);
       stage = stage + 1 == kStages ? 0 : stage + 1;
-      float x[4] = {};
+      const uint32_t in = part >> (2 * kTiles * (kStages - 1));   // of this step, the last tile's position g + 8 lowest
+      float x[kTiles][4] = {};
 #pragma unroll
-      for (int c = 0; c < kKC; ++c) {
-        const uint4 k0 = from[c * 32], k1 = from[(kKC + c) * 32];
-        mma16816<kBf16>(x, k0.x, k1.x, k0.y, k1.y, q[c].x, q[c].y);
-        mma16816<kBf16>(x, k0.z, k1.z, k0.w, k1.w, q[c].z, q[c].w);
-      }
-      const uint32_t in = part >> (2 * (kStages - 1));   // of this step: position g in bit 1, g + 8 in bit 0
+      for (int c = 0; c < kKC; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = (in >> (1 - i / 2) & 1) != 0 ? x[i] * p.scale_log2 : -INFINITY;
-      const float most[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+        for (int j = 0; j < kTiles; ++j) {
+          const uint4 k0 = from[(j * kEach + c) * 32], k1 = from[(j * kEach + kKC + c) * 32];
+          mma16816<kBf16>(x[j], k0.x, k1.x, k0.y, k1.y, q[c].x, q[c].y);
+          mma16816<kBf16>(x[j], k0.z, k1.z, k0.w, k1.w, q[c].z, q[c].w);
+        }
+      float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[j][i] = (in >> (2 * (kTiles - 1 - j) + 1 - i / 2) & 1) != 0 ? x[j][i] * p.scale_log2 : -INFINITY;
+          most[i & 1] = fmaxf(most[i & 1], x[j][i]);
+        }
       if (__any_sync(kFullMask, most[0] > top[0] + 8.f || most[1] > top[1] + 8.f)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -481,25 +493,32 @@ __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_k
           }
         }
       }
+      uint32_t w[kTiles][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = fast_exp2(x[i] - (top[i & 1] == -INFINITY ? 0.f : top[i & 1]));
-        sum[i & 1] += x[i];
-      }
-      const uint32_t p0 = transpose8x8(pack2<kBf16>(x[0], x[1])), p1 = transpose8x8(pack2<kBf16>(x[2], x[3]));
-#pragma unroll
-      for (int c = 0; c < kVC; ++c) {
-        uint32_t a[4][4];
+      for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint4 v = from[(2 * kKC + i * kVC + c) * 32];
-          a[i][0] = v.x, a[i][1] = v.y, a[i][2] = v.z, a[i][3] = v.w;
+          x[j][i] = fast_exp2(x[j][i] - (top[i & 1] == -INFINITY ? 0.f : top[i & 1]));
+          sum[i & 1] += x[j][i];
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          mma16816<kBf16>(o[c * 4 + r], __byte_perm(a[0][r], a[1][r], 0x5410), __byte_perm(a[0][r], a[1][r], 0x7632),
-                          __byte_perm(a[2][r], a[3][r], 0x5410), __byte_perm(a[2][r], a[3][r], 0x7632), p0, p1);
+        w[j][0] = transpose8x8(pack2<kBf16>(x[j][0], x[j][1]));
+        w[j][1] = transpose8x8(pack2<kBf16>(x[j][2], x[j][3]));
       }
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+        for (int c = 0; c < kVC; ++c) {
+          uint32_t a[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 v = from[(j * kEach + 2 * kKC + i * kVC + c) * 32];
+            a[i][0] = v.x, a[i][1] = v.y, a[i][2] = v.z, a[i][3] = v.w;
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            mma16816<kBf16>(o[c * 4 + r], __byte_perm(a[0][r], a[1][r], 0x5410), __byte_perm(a[0][r], a[1][r], 0x7632),
+                            __byte_perm(a[2][r], a[3][r], 0x5410), __byte_perm(a[2][r], a[3][r], 0x7632), w[j][0], w[j][1]);
+        }
     }
     copies_wait<0>();
 #pragma unroll
