@@ -13,6 +13,7 @@ struct CacheDev {
   int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;   // elements
   int64_t table_stride, num_pages;
   int32_t max_pages, page_size, batch, kv_heads, D, length_bytes;
+  int32_t page_shift;   // log2 of page_size, or -1
   int32_t* status;
 };
 
@@ -30,6 +31,8 @@ __device__ __forceinline__ int length_of(const CacheDev& c, int b) {
   const int64_t most = min(static_cast<int64_t>(c.max_pages) * c.page_size, static_cast<int64_t>(0x7fffff00));
   return n < 0 ? 0 : static_cast<int>(n > most ? most : n);
 }
+
+__device__ __forceinline__ int page_of(const CacheDev& c, int x) { return c.page_shift >= 0 ? x >> c.page_shift : x / c.page_size; }
 
 // ---- append ----------------------------------------------------------------------------------
 // A warp takes 32 / kShare consecutive rows: lane l finds where row l goes (a search over the offsets), then
@@ -336,12 +339,13 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_grou
 
 template <int kDP>
 struct Ring {
-  static constexpr int kKC = kDP / 32, kVC = kDP / 64;      // 16-byte pieces of a lane for a key, for a value
+  static constexpr int kKC = kDP / 32, kVC = kDP / 64;      // 16-byte pieces of a lane's fragments of a key, of a value
+  static constexpr int kLanes = kDP / 8, kRows = 32 / kLanes;   // lanes that copy a row, rows of a copy
   static constexpr int kTiles = kDP == 64 ? 2 : 1;          // of a step: independent products hide one another's latency
-  static constexpr int kPieces = kTiles * (2 * kKC + 4 * kVC);   // of a lane for a step: 8 KB a warp
-  static constexpr int kStages = 3, kCtas = 2;              // per SM
-  static constexpr int kStep = kPieces * 512;
-  static constexpr int kBytes = kAnswerThreads / 32 * kStages * kStep;
+  static constexpr int kRegion = 16 * kLanes;               // pieces of 16 keys, or values
+  static constexpr int kStep = kTiles * 2 * kRegion;        // 8 KB a warp
+  static constexpr int kStages = 2, kCtas = 3;              // per SM
+  static constexpr int kBytes = kAnswerThreads / 32 * kStages * kStep * 16;
   static constexpr int kSumRow = kDP + 4;
   static_assert(kBytes >= kAnswerThreads / 32 * kHeads * kSumRow * 4, "the warps' sums take the ring's place");
 };
@@ -349,24 +353,27 @@ struct Ring {
 // 16-bit types, head dimensions that are multiples of 8 up to kDP. A warp takes 16 positions of a tile:
 //   S^T [16 positions][8 heads] = k q^T,   O^T [D][8 heads] += v^T P^T
 // by warp-level matrix instructions. The order of an inner dimension is free as long as both operands share it, so
-// a lane's fragments can be whole 16-byte pieces of rows: for S^T, lane (g, t) of a row of four takes elements
+// a lane's fragments are whole 16-byte pieces of rows: for S^T, lane (g, t) of a row of four takes elements
 // 8 (t + 4c) .. + 7 of position g's key, and of head g's query; for O^T it takes elements 8 (g + 8c) .. + 7 of the
-// values of positions 2t, 2t + 1, 2t + 8, 2t + 9, whose pairs two byte permutes put side by side. Every lane copies
-// its own pieces into its own places of a ring in shared memory, some steps ahead: no lane waits for another, there
-// are no bank conflicts, and the bytes on their way are bounded by shared memory (192 KB an SM), not by registers.
-// (Pieces loaded into registers one step ahead: 4.5 TB/s and 237 us on 64 sequences of 1 to 8191 positions, 32
-// heads of 128 over 8 key heads.) Warps meet only at the end of a unit. Bound by HBM: 2 D bytes of keys and values for
-// 4 D products a head; the products of 8 heads cost a tenth of the time the bytes take. As in the forward pass over
-// whole sequences the maximum in use only follows when it has grown by 2^8.
+// values of positions 2t, 2t + 1, 2t + 8, 2t + 9, whose pairs two byte permutes put side by side.
+//
+// A warp copies whole rows (16 or 8 lanes side by side) into its own part of a ring in shared memory, a step ahead.
+// Bound by HBM, and sensitive to how it is asked: 64 sequences of 1 to 8191 positions, 32 heads of 128 over 8 key
+// heads, take 219 us for the copies alone when each lane copies the pieces that it will use itself (64 bytes of a
+// row side by side), 166 us in whole rows, where the copy rate would give 164. A piece's place in its row is
+// exchanged by the row's number, differently for keys and values, so that no eight lanes meet in a bank. Warps meet
+// only at the end of a unit. As in the forward pass over whole sequences the maximum in use only follows when it has
+// grown by 2^8.
 template <bool kBf16, int kDP>
 __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_kernel(const AnswerDev p) {
   using R = Ring<kDP>;
-  constexpr int kKC = R::kKC, kVC = R::kVC, kStages = R::kStages, kTiles = R::kTiles, kEach = R::kPieces / kTiles;
+  constexpr int kKC = R::kKC, kVC = R::kVC, kStages = R::kStages, kTiles = R::kTiles, kL = R::kLanes;
   extern __shared__ uint4 ring[];
   __shared__ float stats[kAnswerThreads / 32][kHeads][2];
+  __shared__ longlong2 places[kAnswerThreads / 32][32];   // where the positions' keys and values begin
   float* sums = reinterpret_cast<float*>(ring);   // [warp][head][kSumRow]
   const int D = p.c.D, tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = lane / 4, t = lane % 4;
-  const uint4* mine = ring + warp * kStages * R::kPieces * 32 + lane;
+  const uint4* mine = ring + warp * kStages * R::kStep;
   const uint32_t mine_at = smem_addr(mine);
   int64_t end;
   Start s = find_start(p, &end);
@@ -398,74 +405,70 @@ __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_k
       page = -1;
       slot = -1;
       if (of < stop && x < len) {
-        const int n = x / p.c.page_size;
+        const int n = page_of(p.c, x);
         slot = x - n * p.c.page_size;
         page = __ldg(p.c.page_table + b * p.c.table_stride + n);
       }
     };
-    uint32_t part = 0;   // which of positions g and g + 8 take part, two bits a tile, the newest lowest
+    uint32_t part[kStages] = {};   // the lanes whose positions take part, of the steps on their way, the newest first
+    auto shift_part = [&](uint32_t newest) {
+#pragma unroll
+      for (int i = kStages - 1; i > 0; --i) part[i] = part[i - 1];
+      part[0] = newest;
+    };
     auto copy = [&](int stage) {   // the step that was located last
       if (slot >= 0 && (page < 0 || page >= p.c.num_pages)) {
         page = -1;
         raise(p.c);
       }
+      shift_part(__ballot_sync(kFullMask, page >= 0));
+      __syncwarp();   // the places, and the stage, have been read
+      places[warp][lane] = make_longlong2(page < 0 ? -1 : page * p.c.k_page + slot * p.c.k_slot,
+                                          page < 0 ? -1 : page * p.c.v_page + slot * p.c.v_slot);
+      __syncwarp();
+      const int piece = lane % kL;
+      const bool column = piece * 8 < D;
 #pragma unroll
-      for (int j = 0; j < kTiles; ++j) {
-      const uint32_t to = mine_at + stage * R::kStep + j * kEach * 512;
+      for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int x = j * 16 + g + 8 * i;
-        const int pg = __shfl_sync(kFullMask, page, x), sl = __shfl_sync(kFullMask, slot, x);
-        const bool in = pg >= 0;
-        part = part << 1 | (in ? 1u : 0u);
-        const uint16_t* row = in ? kc + pg * p.c.k_page + sl * p.c.k_slot + 8 * t : kc;
-#pragma unroll
-        for (int c = 0; c < kKC; ++c) {
-          const bool on = in && 8 * (t + 4 * c) < D;
-          copy16(to + (i * kKC + c) * 512, on ? row + 32 * c : kc, on);
+        for (int i = 0; i < 16 / R::kRows; ++i) {
+          const int row = i * R::kRows + lane / kL;
+          const longlong2 from = places[warp][j * 16 + row];
+          const bool on = from.x >= 0 && column;
+          const uint32_t to = mine_at + (stage * R::kStep + j * 2 * R::kRegion + row * kL) * 16;
+          copy16(to + (piece ^ (4 * (row & 1))) * 16, on ? kc + from.x + piece * 8 : kc, on);
+          copy16(to + (R::kRegion + (piece ^ (2 * (row / 2 % 4)))) * 16, on ? vc + from.y + piece * 8 : vc, on);
         }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int x = j * 16 + 2 * t + (i & 1) + 8 * (i / 2);
-        const int pg = __shfl_sync(kFullMask, page, x), sl = __shfl_sync(kFullMask, slot, x);
-        const bool in = pg >= 0;
-        const uint16_t* row = in ? vc + pg * p.c.v_page + sl * p.c.v_slot + 8 * g : vc;
-#pragma unroll
-        for (int c = 0; c < kVC; ++c) {
-          const bool on = in && 8 * (g + 8 * c) < D;
-          copy16(to + (2 * kKC + i * kVC + c) * 512, on ? row + 64 * c : vc, on);
-        }
-      }
-      }
     };
     float o[kVC * 4][4] = {};
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};   // of heads 2t and 2t + 1
     __syncthreads();   // the last unit's sums, which lie in the ring, have been read
     locate(s.tile);
     for (int i = 0; i < kStages - 1; ++i) {
-      if (s.tile + i * kTiles < stop) copy(i); else part <<= 2 * kTiles;
+      if (s.tile + i * kTiles < stop) copy(i); else shift_part(0);
       copies_commit();
       locate(s.tile + (i + 1) * kTiles);
     }
     int stage = 0;
     for (int tile = s.tile; tile < stop; tile += kTiles) {
-      copies_wait<kStages - 2>();
       {
-        const int next = stage == 0 ? kStages - 1 : stage - 1;   // (stage + kStages - 1) % kStages
-        if (tile + (kStages - 1) * kTiles < stop) copy(next); else part <<= 2 * kTiles;
+        const int next = stage == 0 ? kStages - 1 : stage - 1;   // (stage + kStages - 1) % kStages, read a step ago
+        if (tile + (kStages - 1) * kTiles < stop) copy(next); else shift_part(0);
         copies_commit();
         locate(tile + kStages * kTiles);
       }
-      const uint4* from = mine + stage * (R::kStep / 16);
+      copies_wait<kStages - 1>();
+      __syncwarp();   // the other lanes' copies too
+      const uint4* from = mine + stage * R::kStep;
       stage = stage + 1 == kStages ? 0 : stage + 1;
-      const uint32_t in = part >> (2 * kTiles * (kStages - 1));   // of this step, the last tile's position g + 8 lowest
+      const uint32_t in = part[kStages - 1];
       float x[kTiles][4] = {};
 #pragma unroll
       for (int c = 0; c < kKC; ++c)
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
-          const uint4 k0 = from[(j * kEach + c) * 32], k1 = from[(j * kEach + kKC + c) * 32];
+          const uint4* k = from + j * 2 * R::kRegion + g * kL + ((t + 4 * c) ^ (4 * (g & 1)));
+          const uint4 k0 = k[0], k1 = k[8 * kL];
           mma16816<kBf16>(x[j], k0.x, k1.x, k0.y, k1.y, q[c].x, q[c].y);
           mma16816<kBf16>(x[j], k0.z, k1.z, k0.w, k1.w, q[c].z, q[c].w);
         }
@@ -474,7 +477,7 @@ __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_k
       for (int j = 0; j < kTiles; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[j][i] = (in >> (2 * (kTiles - 1 - j) + 1 - i / 2) & 1) != 0 ? x[j][i] * p.scale_log2 : -INFINITY;
+          x[j][i] = (in >> (j * 16 + g + i / 2 * 8) & 1) != 0 ? x[j][i] * p.scale_log2 : -INFINITY;
           most[i & 1] = fmaxf(most[i & 1], x[j][i]);
         }
       if (__any_sync(kFullMask, most[0] > top[0] + 8.f || most[1] > top[1] + 8.f)) {
@@ -511,7 +514,7 @@ __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_k
           uint32_t a[4][4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint4 v = from[(j * kEach + 2 * kKC + i * kVC + c) * 32];
+            const uint4 v = from[j * 2 * R::kRegion + R::kRegion + (2 * t + (i & 1) + 8 * (i / 2)) * kL + ((g + 8 * c) ^ (2 * t))];
             a[i][0] = v.x, a[i][1] = v.y, a[i][2] = v.z, a[i][3] = v.w;
           }
 #pragma unroll
@@ -571,7 +574,8 @@ __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_k
 // fp32, head dimensions that are multiples of 4 up to kDP, up to kH query heads of a key head. Eight lanes share a
 // position, a warp takes four positions at once and 4 kPos a step; a lane has elements 4 (t + 8c) .. + 3 of its
 // positions' keys and values, of the heads' queries (in shared memory) and of their sums. Scores are summed over the
-// eight lanes by shuffles, the warp's four groups of lanes are summed at the end of a unit. The ring is as above.
+// eight lanes by shuffles, the warp's four groups of lanes are summed at the end of a unit. Every lane copies its own
+// pieces into its own places of the ring: eight lanes side by side are 128 bytes of a row.
 // Bound by HBM as long as a key head has few query heads: 2 D FMAs a head and position against 8 D bytes.
 template <int kDP>
 struct RingF {
@@ -580,7 +584,7 @@ struct RingF {
   static constexpr int kH = kDP == 64 ? 8 : 4;
   static constexpr int kPieces = 2 * kPos * kC;
   static constexpr int kStep = kPieces * 512;         // 8 KB
-  static constexpr int kStages = 3, kCtas = 2;
+  static constexpr int kStages = 3, kCtas = 2;   // per SM
   static constexpr int kSteps = 4 / kPos;             // of a tile
   static constexpr int kBytes = kAnswerThreads / 32 * kStages * kStep;
   static_assert(kBytes >= kAnswerThreads / 32 * kH * kDP * 4, "the warps' sums take the ring's place");
@@ -625,7 +629,7 @@ __global__ void __launch_bounds__(kAnswerThreads, RingF<kDP>::kCtas) answer_fma_
       page = -1;
       slot = -1;
       if (step < last_step && x < len) {
-        const int n = x / p.c.page_size;
+        const int n = page_of(p.c, x);
         slot = x - n * p.c.page_size;
         page = __ldg(p.c.page_table + b * p.c.table_stride + n);
       }
@@ -636,14 +640,17 @@ __global__ void __launch_bounds__(kAnswerThreads, RingF<kDP>::kCtas) answer_fma_
         page = -1;
         raise(p.c);
       }
+      // where the position's key and value begin, in elements; -1: takes no part
+      const int64_t k_at = page < 0 ? -1 : page * p.c.k_page + slot * p.c.k_slot;
+      const int64_t v_at = page < 0 ? -1 : page * p.c.v_page + slot * p.c.v_slot;
       const uint32_t to = mine_at + stage * R::kStep;
 #pragma unroll
       for (int i = 0; i < kPos; ++i) {
-        const int pg = __shfl_sync(kFullMask, page, i * 4 + group), sl = __shfl_sync(kFullMask, slot, i * 4 + group);
-        const bool in = pg >= 0;
+        const int64_t k_from = __shfl_sync(kFullMask, k_at, i * 4 + group), v_from = __shfl_sync(kFullMask, v_at, i * 4 + group);
+        const bool in = k_from >= 0;
         part = part << 1 | (in ? 1u : 0u);
-        const float* kr = in ? kc + pg * p.c.k_page + sl * p.c.k_slot + 4 * t : kc;
-        const float* vr = in ? vc + pg * p.c.v_page + sl * p.c.v_slot + 4 * t : vc;
+        const float* kr = kc + k_from + 4 * t;
+        const float* vr = vc + v_from + 4 * t;
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
           const bool on = in && 4 * (t + 8 * c) < D;
@@ -664,13 +671,13 @@ __global__ void __launch_bounds__(kAnswerThreads, RingF<kDP>::kCtas) answer_fma_
     }
     int stage = 0;
     for (int step = first_step; step < last_step; ++step) {
-      copies_wait<kStages - 2>();
       {
-        const int next = stage == 0 ? kStages - 1 : stage - 1;   // (stage + kStages - 1) % kStages
+        const int next = stage == 0 ? kStages - 1 : stage - 1;   // (stage + kStages - 1) % kStages, read a step ago
         if (step + kStages - 1 < last_step) copy(next); else part <<= kPos;
         copies_commit();
         locate(step + kStages);
       }
+      copies_wait<kStages - 1>();
       const uint4* from = mine + stage * (R::kStep / 16);
       stage = stage + 1 == kStages ? 0 : stage + 1;
       const uint32_t in = part >> (kPos * (kStages - 1));
@@ -788,36 +795,64 @@ __global__ void __launch_bounds__(kAnswerThreads, RingF<kDP>::kCtas) answer_fma_
   }
 }
 
-// Block (c, h): when the cut before CTA c is the first inside a unit, the unit's head h.
+// Block (c, h): when the cut before CTA c is the first inside a unit, the unit's head h. The pieces' weights by a thread
+// each, then their sums by as many threads a column as there are.
 template <typename T>
 __global__ void __launch_bounds__(kAnswerThreads) join_kernel(const AnswerDev p) {
-  const int c = blockIdx.x + 1, h = blockIdx.y;
+  __shared__ float weights[kAnswerCtas];
+  __shared__ float shared[kAnswerThreads / 32], sums[kAnswerThreads];
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the answers' kernel is done
+  const int c = blockIdx.x + 1, h = blockIdx.y, tid = threadIdx.x;
   const Start s = p.starts[c];
   if (s.unit < 0 || s.tile == 0) return;
   const Start before = p.starts[c - 1];
   if (before.unit == s.unit && before.tile > 0) return;
   const int u = s.unit % p.units, kv = u / p.chunks, b = s.unit / p.units;
   const int head = kv * p.group + (u % p.chunks) * p.per + h;
-  if (head >= (kv + 1) * p.group) return;
-  // the CTA that holds the unit's last tile
+  if (h >= p.per || head >= (kv + 1) * p.group) return;
+  // pieces from CTA c - 1 (in its second slot) to the one that holds the unit's last tile (in their first slots)
   const int last = static_cast<int>(((s.first + kUnitCost + s.tiles) * s.ctas - 1) / s.all);
-  // the first piece lies in its CTA's second slot, the others in the first
-  const int64_t part0 = 2 * static_cast<int64_t>(c - 1) + 1;
-  float m = p.stats[(part0 * kHeads + h) * 2];
-  for (int i = c; i <= last; ++i) m = fmaxf(m, p.stats[(2 * static_cast<int64_t>(i) * kHeads + h) * 2]);
-  const float base = m == -INFINITY ? 0.f : m;
-  for (int d = threadIdx.x; d < p.c.D; d += kAnswerThreads) {
-    float w = exp2f(p.stats[(part0 * kHeads + h) * 2] - base);
-    float l = w * p.stats[(part0 * kHeads + h) * 2 + 1];
-    float o = w * p.sums[(part0 * kHeads + h) * p.c.D + d];
-#pragma unroll 4
-    for (int i = c; i <= last; ++i) {
-      const int64_t part = 2 * static_cast<int64_t>(i);
-      w = exp2f(p.stats[(part * kHeads + h) * 2] - base);
-      l = fmaf(w, p.stats[(part * kHeads + h) * 2 + 1], l);
-      o = fmaf(w, p.sums[(part * kHeads + h) * p.c.D + d], o);
+  const int pieces = last - c + 2;
+  auto piece = [&](int i) { return (2 * static_cast<int64_t>(c - 1 + i) + (i == 0 ? 1 : 0)) * kHeads + h; };
+  auto over_block = [&](float x, bool largest) {
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) {
+      const float y = __shfl_xor_sync(kFullMask, x, w);
+      x = largest ? fmaxf(x, y) : x + y;
     }
-    static_cast<T*>(p.out)[b * p.o_row + head * p.o_head + d] = from_float<T>(l == 0.f ? 0.f : o / l);
+    __syncthreads();
+    if (tid % 32 == 0) shared[tid / 32] = x;
+    __syncthreads();
+    x = shared[0];
+#pragma unroll
+    for (int w = 1; w < kAnswerThreads / 32; ++w) x = largest ? fmaxf(x, shared[w]) : x + shared[w];
+    return x;
+  };
+  float m = -INFINITY;
+  for (int i = tid; i < pieces; i += kAnswerThreads) m = fmaxf(m, weights[i] = p.stats[piece(i) * 2]);
+  m = over_block(m, true);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  for (int i = tid; i < pieces; i += kAnswerThreads) {
+    weights[i] = exp2f(weights[i] - base);
+    l = fmaf(weights[i], p.stats[piece(i) * 2 + 1], l);
+  }
+  l = over_block(l, false);   // also: the weights are there
+  const int columns = p.c.D <= 32 ? 32 : p.c.D <= 64 ? 64 : 128, shares = kAnswerThreads / columns, share = tid / columns;
+  for (int d0 = 0; d0 < p.c.D; d0 += columns) {
+    const int d = d0 + tid % columns;
+    float o = 0.f;
+    if (d < p.c.D) {
+#pragma unroll 4
+      for (int i = share; i < pieces; i += shares) o = fmaf(weights[i], p.sums[piece(i) * p.c.D + d], o);
+    }
+    __syncthreads();
+    sums[tid] = o;
+    __syncthreads();
+    if (share == 0 && d < p.c.D) {
+      for (int w = 1; w < shares; ++w) o += sums[w * columns + tid];
+      static_cast<T*>(p.out)[b * p.o_row + head * p.o_head + d] = from_float<T>(l == 0.f ? 0.f : o / l);
+    }
   }
 }
 
@@ -844,6 +879,9 @@ CacheDev cache_dev(const b200tbe_paged_cache* c) {
   d.table_stride = c->page_table_stride, d.num_pages = c->num_pages, d.max_pages = c->max_pages;
   d.page_size = c->page_size, d.batch = c->batch, d.kv_heads = c->kv_heads, d.D = c->head_dim;
   d.length_bytes = c->length_bytes, d.status = c->status;
+  d.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (d.page_size == 1 << i) d.page_shift = i;
   return d;
 }
 
@@ -855,11 +893,20 @@ int launch_append(const AppendDev& p, cudaStream_t stream) {
   return launch_status();
 }
 
+// Launched while the answers' kernel still runs, whose results it waits for: its launch costs no time of its own.
 template <typename T>
 int join(const AnswerDev& p, int ctas, cudaStream_t stream) {
   if (ctas < 2) return B200TBE_OK;
-  join_kernel<T><<<dim3(ctas - 1, min(p.per, p.group)), kAnswerThreads, 0, stream>>>(p);
-  return launch_status();
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(ctas - 1, p.per < p.group ? p.per : p.group);
+  config.blockDim = dim3(kAnswerThreads);
+  config.stream = stream;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, join_kernel<T>, p) == cudaSuccess ? B200TBE_OK : B200TBE_ERR_LAUNCH;
 }
 
 // 16-byte reads of everything, and a head dimension that the registers hold
