@@ -577,23 +577,23 @@ __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_k
 // eight lanes by shuffles, the warp's four groups of lanes are summed at the end of a unit. Every lane copies its own
 // pieces into its own places of the ring: eight lanes side by side are 128 bytes of a row.
 // Bound by HBM as long as a key head has few query heads: 2 D FMAs a head and position against 8 D bytes.
-template <int kDP>
+template <int kDP, int kH>
 struct RingF {
   static constexpr int kC = kDP / 32;                 // 16-byte pieces of a lane for a key or a value
-  static constexpr int kPos = kDP == 64 ? 4 : 2;      // positions of a lane in a step
-  static constexpr int kH = kDP == 64 ? 8 : 4;
+  static constexpr int kPos = kDP == 64 && kH > 2 ? 4 : 2;   // positions of a lane in a step
   static constexpr int kPieces = 2 * kPos * kC;
-  static constexpr int kStep = kPieces * 512;         // 8 KB
-  static constexpr int kStages = 3, kCtas = 2;   // per SM
+  static constexpr int kStep = kPieces * 512;         // 4 or 8 KB
+  static constexpr int kStages = 3;
+  static constexpr int kCtas = kH > 2 || kDP == 128 ? 2 : 4;   // per SM: few heads leave registers for more warps
   static constexpr int kSteps = 4 / kPos;             // of a tile
   static constexpr int kBytes = kAnswerThreads / 32 * kStages * kStep;
   static_assert(kBytes >= kAnswerThreads / 32 * kH * kDP * 4, "the warps' sums take the ring's place");
 };
 
-template <int kDP>
-__global__ void __launch_bounds__(kAnswerThreads, RingF<kDP>::kCtas) answer_fma_kernel(const AnswerDev p) {
-  using R = RingF<kDP>;
-  constexpr int kC = R::kC, kPos = R::kPos, kH = R::kH, kStages = R::kStages;
+template <int kDP, int kH>
+__global__ void __launch_bounds__(kAnswerThreads, RingF<kDP, kH>::kCtas) answer_fma_kernel(const AnswerDev p) {
+  using R = RingF<kDP, kH>;
+  constexpr int kC = R::kC, kPos = R::kPos, kStages = R::kStages;
   extern __shared__ uint4 ring[];
   __shared__ float stats[kAnswerThreads / 32][kH][2];
   __shared__ __align__(16) float qs[kH][kDP];
@@ -918,14 +918,14 @@ bool answer_in_pieces(const AnswerDev& p, int elem_bytes) {
   return bits % 16 == 0 && p.c.D <= 128;
 }
 
-template <int kDP>
+template <int kDP, int kH>
 int launch_answer_fma(AnswerDev p, int64_t most, cudaStream_t stream) {
-  using R = RingF<kDP>;
-  const auto kernel = answer_fma_kernel<kDP>;
+  using R = RingF<kDP, kH>;
+  const auto kernel = answer_fma_kernel<kDP, kH>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes) != cudaSuccess ||
       cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess)
     return B200TBE_ERR_LAUNCH;
-  p.per = R::kH;
+  p.per = kH;
   p.chunks = (p.group + p.per - 1) / p.per;
   p.units = p.c.kv_heads * p.chunks;
   if (static_cast<int64_t>(p.units) * p.c.batch > 0x7fffffff) return B200TBE_ERR_TOO_LARGE;
@@ -1026,7 +1026,8 @@ extern "C" int b200tbe_paged_attention(const b200tbe_paged_cache* cache, const v
   if (most < 1) most = 1;
   const int64_t tiles = static_cast<int64_t>(p.units) * cache->batch * (most + kUnitCost);
   if (cache->dtype == B200TBE_FP32 && answer_in_pieces(p, 4))
-    return p.c.D <= 64 ? launch_answer_fma<64>(p, most, stream) : launch_answer_fma<128>(p, most, stream);
+    return p.c.D <= 64 ? (p.group <= 2 ? launch_answer_fma<64, 2>(p, most, stream) : launch_answer_fma<64, 8>(p, most, stream))
+                       : (p.group <= 2 ? launch_answer_fma<128, 2>(p, most, stream) : launch_answer_fma<128, 4>(p, most, stream));
   if (cache->dtype != B200TBE_FP32 && answer_in_pieces(p, 2)) {
     if (cache->dtype == B200TBE_FP16)
       return p.c.D <= 64 ? launch_answer_mma<__half, false, 64>(p, tiles, stream) : launch_answer_mma<__half, false, 128>(p, tiles, stream);
