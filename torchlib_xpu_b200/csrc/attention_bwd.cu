@@ -34,10 +34,10 @@ struct Layout {
 };
 
 struct DqBarriers {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full, dp_full, s_loaded, ds_full, done;
+  uint64_t q_full, a_full, k_full[3], k_empty[3], v_full, v_empty, s_full, dp_full, s_loaded, ds_full, done;
 };
 struct DkvBarriers {
-  uint64_t kv_full, q_full[2], q_empty[2], s_full, dp_full, p_full, ds_full, stat_full[2], stat_empty[2], done;
+  uint64_t kv_full, q_full[2], q_empty[2], g_full[2], g_empty[2], s_full, dp_full, p_full, ds_full, stat_full[2], stat_empty[2], done;
 };
 
 // What a tile's CTA knows.
@@ -85,6 +85,24 @@ __device__ __forceinline__ void load_tile(uint8_t* tile, const CUtensorMap* map,
   for (int x = 0; x < kDP / 64; ++x) tma_load_3d(smem_addr(tile) + x * kRows * 128, map, x * 64, head, row, bar);
 }
 
+// Row `row` of a tile in shared memory (as the tensor copies leave it) to this thread's lane of tensor memory, two
+// elements a column: a left operand.
+template <int kDP>
+__device__ __forceinline__ void copy_row(uint32_t to, const uint8_t* tile, int row) {
+#pragma unroll
+  for (int x = 0; x < kDP / 64; ++x) {
+    uint32_t r[32];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const uint4 v = *reinterpret_cast<const uint4*>(tile + x * kRows * 128 + row * 128 + (c ^ (row % 8)) * 16);
+      r[4 * c] = v.x, r[4 * c + 1] = v.y, r[4 * c + 2] = v.z, r[4 * c + 3] = v.w;
+    }
+    tmem_st32(to + x * 32, r);
+  }
+  tmem_wait_st();
+  tc_fence_before();
+}
+
 // A warp's accumulator rows in tensor memory, times f, to memory: `rows` of them.
 template <bool kBf16, int kDP>
 __device__ __forceinline__ void store_rows(uint8_t* stage, uint16_t* out, int64_t stride, uint32_t at, int D, float f,
@@ -122,8 +140,10 @@ __device__ __forceinline__ void report(const int* dead, int32_t* status) {
   }
 }
 
-// Tensor memory: scores, dP (dS takes its place), dQ. The scores of the next keys are computed as soon as these are
-// in registers, under the arithmetic on dP; dQ and the next dP under the exponentials.
+// Tensor memory: scores, dP (dS takes its place), dQ, and the queries and dO, copied there once: as left operands from
+// shared memory they would be read again for every tile of keys, and its bandwidth, not the tensor cores', would bound
+// the products. The scores of the next keys are computed as soon as these are in registers, under the arithmetic on dP;
+// dQ and the next dP under the exponentials. Keys are held until dQ and come three tiles ahead, values one.
 template <bool kBf16, int kDP>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_dq_kernel(const BwdDev p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
@@ -137,14 +157,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* gs = qs + L::kTileBytes;
   uint8_t* ks = gs + L::kTileBytes;
-  uint8_t* vs = ks + 2 * L::kTileBytes;
+  uint8_t* vs = ks + 3 * L::kTileBytes;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) dead_word = 0;
   if (warp == 8) tmem_alloc(&tmem_base, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_base, dp_at = tmem + kRows, dq_at = tmem + 2 * kRows;
+  const uint32_t tmem = tmem_base, dp_at = tmem + kRows, dq_at = tmem + 2 * kRows, q_at = dq_at + kDP, g_at = q_at + kDP / 2;
   volatile int* dead = &dead_word;
 
   Item it;
@@ -162,57 +182,55 @@ __global__ void __launch_bounds__(kThreads, 1)
           load_tile<kDP>(qs, &q_map, it.head, static_cast<int>(it.begin) + it.first, &bars.q_full);
           load_tile<kDP>(gs, &g_map, it.head, static_cast<int>(it.begin) + it.first, &bars.q_full);
           for (int j = 0; j < n; ++j) {
-            const int st = j & 1, row = static_cast<int>(it.other) + j * kRows;
-            const uint32_t before = (j / 2 - 1) & 1;
-            if (j >= 2 && !mbar_wait(&bars.k_empty[st], before, dead)) break;
+            const int st = j % 3, row = static_cast<int>(it.other) + j * kRows;
+            if (j >= 3 && !mbar_wait(&bars.k_empty[st], (j / 3 - 1) & 1, dead)) break;
             mbar_expect(&bars.k_full[st], L::kTileBytes);
             load_tile<kDP>(ks + st * L::kTileBytes, &k_map, kv, row, &bars.k_full[st]);
-            if (j >= 2 && !mbar_wait(&bars.v_empty[st], before, dead)) break;
-            mbar_expect(&bars.v_full[st], L::kTileBytes);
-            load_tile<kDP>(vs + st * L::kTileBytes, &v_map, kv, row, &bars.v_full[st]);
+            if (j >= 1 && !mbar_wait(&bars.v_empty, (j - 1) & 1, dead)) break;
+            mbar_expect(&bars.v_full, L::kTileBytes);
+            load_tile<kDP>(vs, &v_map, kv, row, &bars.v_full);
           }
         }
       } else if (warp == 8 && n > 0) {
         // ---- matrix instructions ----
         const int d_steps = (a.D + 15) / 16;
-        const uint32_t q_at = smem_addr(qs), g_at = smem_addr(gs);
         const uint32_t dq_desc = mma_desc(kBf16, kRows, (a.D + 15) & ~15, false, true);
         auto keys_of = [&](int j) { return min(kRows, klen - j * kRows); };
         auto scores = [&](int j) {   // whole warp
-          const bool ok = warp_wait(&bars.k_full[j & 1], (j / 2) & 1, dead);
-          if (!ok) return false;
-          const int keys = keys_of(j);
-          if (keys % 16 != 0) zero_tail<kDP>(ks + (j & 1) * L::kTileBytes, keys);
+          const int st = j % 3, keys = keys_of(j);
+          uint8_t* tile = ks + st * L::kTileBytes;
+          if (!warp_wait(&bars.k_full[st], (j / 3) & 1, dead)) return false;
+          if (keys % 16 != 0) zero_tail<kDP>(tile, keys);
           if (j > 0 && !warp_wait(&bars.s_loaded, (j - 1) & 1, dead)) return false;
           tc_fence_after();
           if (elect_one()) {
-            mma_along_k<kDP / 16, kRows>(tmem, q_at, smem_addr(ks + (j & 1) * L::kTileBytes),
-                           mma_desc(kBf16, kRows, (keys + 15) & ~15, false, false), d_steps);
+            mma_along_k_ts<kDP / 16, kRows>(tmem, q_at, smem_addr(tile), mma_desc(kBf16, kRows, (keys + 15) & ~15, false, false), d_steps);
             mma_commit(&bars.s_full);
           }
           __syncwarp();
           return true;
         };
         auto d_weights = [&](int j) {
-          const bool ok = warp_wait(&bars.v_full[j & 1], (j / 2) & 1, dead);
-          if (!ok) return false;
+          if (!warp_wait(&bars.v_full, j & 1, dead)) return false;
           if (elect_one()) {
-            mma_along_k<kDP / 16, kRows>(dp_at, g_at, smem_addr(vs + (j & 1) * L::kTileBytes),
-                           mma_desc(kBf16, kRows, (keys_of(j) + 15) & ~15, false, false), d_steps);
+            mma_along_k_ts<kDP / 16, kRows>(dp_at, g_at, smem_addr(vs), mma_desc(kBf16, kRows, (keys_of(j) + 15) & ~15, false, false),
+                                            d_steps);
             mma_commit(&bars.dp_full);
-            if (j + 2 < n) mma_commit(&bars.v_empty[j & 1]);
+            if (j + 1 < n) mma_commit(&bars.v_empty);
           }
           __syncwarp();
           return true;
         };
-        bool alive = warp_wait(&bars.q_full, 0, dead) && scores(0) && d_weights(0);
+        bool alive = warp_wait(&bars.a_full, 0, dead);
+        tc_fence_after();
+        alive = alive && scores(0) && d_weights(0);
         for (int j = 0; alive && j < n; ++j) {
           if (j + 1 < n) alive = scores(j + 1);
           alive = alive && warp_wait(&bars.ds_full, j & 1, dead);
           tc_fence_after();
           if (alive && elect_one()) {
-            mma_over_rows<32>(dq_at, dp_at, smem_addr(ks + (j & 1) * L::kTileBytes), dq_desc, (keys_of(j) + 15) / 16, j > 0);
-            if (j + 2 < n) mma_commit(&bars.k_empty[j & 1]);
+            mma_over_rows<32>(dq_at, dp_at, smem_addr(ks + j % 3 * L::kTileBytes), dq_desc, (keys_of(j) + 15) / 16, j > 0);
+            if (j + 3 < n) mma_commit(&bars.k_empty[j % 3]);
             if (j + 1 == n) mma_commit(&bars.done);
           }
           __syncwarp();
@@ -231,12 +249,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (threadIdx.x == 0) {
         if (!fresh) mbar_forget(&bars);
         mbar_init(&bars.q_full, 1);
-        for (int i = 0; i < 2; ++i) {
+        mbar_init(&bars.a_full, 256);
+        for (int i = 0; i < 3; ++i) {
           mbar_init(&bars.k_full[i], 1);
           mbar_init(&bars.k_empty[i], 1);
-          mbar_init(&bars.v_full[i], 1);
-          mbar_init(&bars.v_empty[i], 1);
         }
+        mbar_init(&bars.v_full, 1);
+        mbar_init(&bars.v_empty, 1);
         mbar_init(&bars.s_full, 1);
         mbar_init(&bars.dp_full, 1);
         mbar_init(&bars.s_loaded, 256);
@@ -258,8 +277,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float c = a.scale * kLog2e;
       const uint64_t c2 = pair(c, c), minus_delta = pair(-delta, -delta);
       const uint32_t s_at = tmem + lanes + half * 64, ds_at = dp_at + lanes + half * 64;
-      bool alive = true;
-      for (int j = 0; j < n; ++j) {
+      bool alive = n == 0 || warp_wait(&bars.q_full, 0, dead);
+      if (alive && n > 0) {   // the queries' rows by one warpgroup, dO's by the other
+        copy_row<kDP>((half == 0 ? q_at : g_at) + lanes, half == 0 ? qs : gs, local);
+        mbar_arrive(&bars.a_full);
+      }
+      for (int j = 0; alive && j < n; ++j) {
         alive = warp_wait(&bars.s_full, j & 1, dead);
         if (!alive) break;
         tc_fence_after();
@@ -357,10 +380,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           load_tile<kDP>(vs, &v_map, it.head, static_cast<int>(it.begin) + it.first, &bars.kv_full);
           for (int j = 0; j < n; ++j) {
             const int st = j & 1, row = static_cast<int>(it.other) + (from + j % per_head) * kRows, head = head0 + j / per_head;
+            // q, wanted first, apart from dO: both take longer than the arithmetic that hides them
             if (j >= 2 && !mbar_wait(&bars.q_empty[st], (j / 2 - 1) & 1, dead)) break;
-            mbar_expect(&bars.q_full[st], 2 * L::kTileBytes);
+            mbar_expect(&bars.q_full[st], L::kTileBytes);
             load_tile<kDP>(qs + st * L::kTileBytes, &q_map, head, row, &bars.q_full[st]);
-            load_tile<kDP>(gs + st * L::kTileBytes, &g_map, head, row, &bars.q_full[st]);
+            if (j >= 2 && !mbar_wait(&bars.g_empty[st], (j / 2 - 1) & 1, dead)) break;
+            mbar_expect(&bars.g_full[st], L::kTileBytes);
+            load_tile<kDP>(gs + st * L::kTileBytes, &g_map, head, row, &bars.g_full[st]);
           }
         }
       } else if (warp == 10) {
@@ -383,12 +409,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t k_at = smem_addr(ks), v_at = smem_addr(vs);
         const uint32_t out_desc = mma_desc(kBf16, kRows, (a.D + 15) & ~15, false, true);
         auto rows_of = [&](int j) { return min(kRows, qlen - (from + j % per_head) * kRows); };
-        auto ready = [&](int j) {
-          const bool ok = warp_wait(&bars.q_full[j & 1], (j / 2) & 1, dead);
-          if (ok && rows_of(j) % 16 != 0) {
-            zero_tail<kDP>(qs + (j & 1) * L::kTileBytes, rows_of(j));
-            zero_tail<kDP>(gs + (j & 1) * L::kTileBytes, rows_of(j));
-          }
+        auto arrived = [&](uint64_t* bar, uint8_t* tiles, int j) {
+          const bool ok = warp_wait(bar + (j & 1), (j / 2) & 1, dead);
+          if (ok && rows_of(j) % 16 != 0) zero_tail<kDP>(tiles + (j & 1) * L::kTileBytes, rows_of(j));
           return ok;
         };
         auto scores = [&](int j) {
@@ -407,21 +430,25 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
         };
-        bool alive = warp_wait(&bars.kv_full, 0, dead) && ready(0);
-        if (alive) {
-          scores(0);
-          d_weights(0);
-        }
+        bool alive = warp_wait(&bars.kv_full, 0, dead) && arrived(bars.q_full, qs, 0);
+        if (alive) scores(0);
+        alive = alive && arrived(bars.g_full, gs, 0);
+        if (alive) d_weights(0);
         for (int j = 0; alive && j < n; ++j) {
           const bool more = j + 1 < n;
           const int steps = (rows_of(j) + 15) / 16;
-          alive = (!more || ready(j + 1)) && warp_wait(&bars.p_full, j & 1, dead);
+          alive = warp_wait(&bars.p_full, j & 1, dead);
           if (!alive) break;
           tc_fence_after();
           if (elect_one()) mma_over_rows<32>(dv_at, tmem, smem_addr(gs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
+          if (elect_one() && j + 2 < n) mma_commit(&bars.g_empty[j & 1]);
           __syncwarp();
-          if (more) scores(j + 1);
-          alive = warp_wait(&bars.ds_full, j & 1, dead);
+          if (more) {
+            alive = arrived(bars.q_full, qs, j + 1);
+            if (!alive) break;
+            scores(j + 1);
+          }
+          alive = (!more || arrived(bars.g_full, gs, j + 1)) && warp_wait(&bars.ds_full, j & 1, dead);
           if (!alive) break;
           tc_fence_after();
           if (elect_one()) {
@@ -448,6 +475,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 2; ++i) {
           mbar_init(&bars.q_full[i], 1);
           mbar_init(&bars.q_empty[i], 1);
+          mbar_init(&bars.g_full[i], 1);
+          mbar_init(&bars.g_empty[i], 1);
           mbar_init(&bars.stat_full[i], 32);
           mbar_init(&bars.stat_empty[i], 256);
         }

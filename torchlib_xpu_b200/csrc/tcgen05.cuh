@@ -186,6 +186,15 @@ __device__ __forceinline__ void mma_along_k(uint32_t d, uint32_t a, uint32_t b, 
   }
 }
 
+// The same with a in tensor memory, two elements a column.
+template <int kMost, int kRowsOfTile>
+__device__ __forceinline__ void mma_along_k_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, int steps) {
+  const uint64_t b0 = smem_desc(b, 16);
+#pragma unroll
+  for (int t = 0; t < kMost; ++t)
+    if (t < steps) mma_ts(d, a + t * 8, b0 + (((t / 4) * kRowsOfTile * 128 + (t % 4) * 32) >> 4), desc, t > 0);
+}
+
 // d[128][n] (+)= w x over up to 128 rows of x, 16 a step: w in tensor memory, two 16-bit elements a column, the second
 // 64 of them kSkip columns further on; x in tiles of 128 rows, n along the row.
 template <int kSkip>
