@@ -67,6 +67,11 @@ TileList list_at(char* at, const Scratch& s, int64_t total_q, int64_t total_k, i
 bool mostly_short(const AttnDev& d) {
   return d.batch > 0 && d.total_q <= static_cast<int64_t>(d.batch) * 128 && d.total_k <= static_cast<int64_t>(d.batch) * 128;
 }
+// Several waves of tiles of sequences of different lengths: sorted first, so that the longest are not the last.
+bool listed_first(const AttnDev& d) {
+  const bool by_rows = d.group % 2 != 0 && d.total_q > static_cast<int64_t>(d.batch) * 128;   // tiles of 256, which no list has
+  return d.batch > 1 && !by_rows && (d.total_q / 128 + d.batch) * d.heads > 2 * kNumSMs;
+}
 // ... and here nothing can be longer.
 bool all_short(const AttnDev& d) { return d.total_q <= 128 && d.total_k <= 128; }
 
@@ -101,6 +106,12 @@ extern "C" int b200tbe_jagged_attention(const b200tbe_attention_params* p, b200t
       if (tc == B200TBE_OK && all_short(d)) return tc;
       if (tc == B200TBE_OK) rest = &list;
       if (tc != B200TBE_OK && tc != B200TBE_ERR_UNSUPPORTED) return tc;
+    } else if (p->scratch != nullptr && listed_first(d)) {
+      list = list_at(static_cast<char*>(p->scratch), backward_scratch(d.total_q, 0, d.batch, 0), d.total_q, 0, d.batch);
+      list.k_room = 0;
+      tc = attention_list(d, list, stream);
+      if (tc != B200TBE_OK) return tc;
+      rest = &list;
     }
     tc = attention_forward_tc(d, rest, p->dtype, p->status, stream);
     if (tc != B200TBE_ERR_UNSUPPORTED) return tc;

@@ -48,6 +48,8 @@ int attention_forward_tc(const AttnDev& p, const TileList* list, int dtype, int3
 // Sequences of at most 128 queries and keys; the others' tiles go on the list (whose words are zero before).
 int attention_short_forward(const AttnDev& p, const TileList& list, int dtype, int32_t* status, cudaStream_t stream);
 int attention_short_backward(const AttnDev& p, const TileList& list, int dtype, int32_t* status, cudaStream_t stream);
+// All tiles, the long sequences' first, as attention_delta() lists them. With k_room 0, of the queries alone.
+int attention_list(const AttnDev& p, const TileList& list, cudaStream_t stream);
 int attention_delta_listed(const AttnDev& p, const TileList& list, int dtype, cudaStream_t stream);
 bool attention_backward_fits(const AttnDev& p, int dtype);
 int attention_backward_tc(const AttnDev& p, const TileList& plan, int dtype, int32_t* status, cudaStream_t stream);

@@ -8,77 +8,68 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRows = 128;   // of a tile
 
-// How much work a tile of the stretch is, coarsely.
-__device__ __forceinline__ int weight_class(int64_t rows) { return rows >= 2048 ? 2 : rows >= 512 ? 1 : 0; }
+// How much work a tile of a stretch is, to a factor of two: by the rows of the other side.
+constexpr int kClasses = 8;
+__device__ __forceinline__ int weight_class(int64_t rows) {
+  const int64_t tiles = rows / kRows;
+  return tiles <= 0 ? 0 : min(kClasses - 1, 64 - __clzll(tiles));
+}
 
-// Both lists by one CTA: the stretches' tiles are counted, summed up to each stretch, and written by its warp.
-// The tiles are taken in the list's order, so the long sequences' come first; within a sequence later queries see
-// more keys, and earlier keys are seen by more queries: those come first.
-__device__ __forceinline__ void list_tiles(const AttnDev& p, const TileList& plan) {
-  __shared__ int64_t warp_sums[kThreads / 32];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  __shared__ int present;
-  if (threadIdx.x == 0) present = 0;
+// Both lists by one CTA: the classes' tiles are counted, then every stretch takes room in its class. The tiles are taken
+// in the list's order, so the long sequences' come first (which of two in a class does not matter: no result depends on
+// it); within a sequence later queries see more keys, and earlier keys are seen by more queries: those come first.
+__device__ __forceinline__ void list_tiles(const AttnDev& p, const TileList& list) {
+  __shared__ int next[2][kClasses];   // of queries, of keys
+  const int lane = threadIdx.x % 32;
+  auto rows_of = [&](const void* offsets, int64_t total, int i) {
+    return i >= p.batch + 2 ? static_cast<int64_t>(0)
+                            : max(static_cast<int64_t>(0), stretch_bound(offsets, p.offset_bytes, p.batch, total, i + 1) -
+                                                               stretch_bound(offsets, p.offset_bytes, p.batch, total, i));
+  };
+  if (threadIdx.x < 2 * kClasses) next[threadIdx.x / kClasses][threadIdx.x % kClasses] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < p.batch + 2; i += kThreads) {
-    const int c = weight_class(stretch_bound(p.q_offsets, p.offset_bytes, p.batch, p.total_q, i + 1) -
-                               stretch_bound(p.q_offsets, p.offset_bytes, p.batch, p.total_q, i));
-    if (c > 0) atomicOr(&present, 1 << c);
+    const int64_t q = rows_of(p.q_offsets, p.total_q, i), k = rows_of(p.k_offsets, p.total_k, i);
+    const int c = weight_class(max(q, k));
+    if (q > 0) atomicAdd(&next[0][c], static_cast<int>((q + kRows - 1) / kRows));
+    if (k > 0) atomicAdd(&next[1][c], static_cast<int>((k + kRows - 1) / kRows));
   }
   __syncthreads();
-  int64_t base = 0;   // tiles of queries in the low half, of keys in the high half
-  const int rounds = (p.batch + 2 + kThreads - 1) / kThreads;
-  for (int turn = 0; turn < 3 * rounds; ++turn) {
-    const int c = 2 - turn / rounds, s0 = turn % rounds * kThreads, i = s0 + threadIdx.x;
-    if (c > 0 && (present >> c & 1) == 0) continue;
-    int64_t mine = 0;
-    if (i < p.batch + 2) {
-      const int64_t q = stretch_bound(p.q_offsets, p.offset_bytes, p.batch, p.total_q, i + 1) -
-                        stretch_bound(p.q_offsets, p.offset_bytes, p.batch, p.total_q, i);
-      const int64_t k = stretch_bound(p.k_offsets, p.offset_bytes, p.batch, p.total_k, i + 1) -
-                        stretch_bound(p.k_offsets, p.offset_bytes, p.batch, p.total_k, i);
-      if (weight_class(q) == c)
-        mine = max(static_cast<int64_t>(0), (q + kRows - 1) / kRows) + (max(static_cast<int64_t>(0), (k + kRows - 1) / kRows) << 32);
+  if (threadIdx.x < 2) {   // where the classes begin, the heaviest first
+    int at = 0;
+    for (int c = kClasses - 1; c >= 0; --c) {
+      const int n = next[threadIdx.x][c];
+      next[threadIdx.x][c] = at;
+      at += n;
     }
-    int64_t upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(kFullMask, upto, o);
-      if (lane >= o) upto += x;
-    }
-    if (lane == 31) warp_sums[warp] = upto;
-    __syncthreads();
-    int64_t all = 0;
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) upto += warp_sums[w];
-      all += warp_sums[w];
-    }
-    const int64_t at = base + upto - mine;
-    auto write = [&](int stretch, int64_t n, int64_t to, int t0, int step) {
-      const int nq = static_cast<int>(n & 0xffffffff), nk = static_cast<int>(n >> 32);
-      const int tq = static_cast<int>(to & 0xffffffff), tk = static_cast<int>(to >> 32);
-      // offsets that decrease give more tiles than there is room for
-      for (int t = t0; t < nq; t += step)
-        if (tq + t < plan.q_room) plan.q_tiles[tq + t] = make_int2(stretch, nq - 1 - t);
-      for (int t = t0; t < nk; t += step)
-        if (tk + t < plan.k_room) plan.k_tiles[tk + t] = make_int2(stretch, t);
-    };
+    list.tickets[threadIdx.x] = 0;
+    // offsets that decrease give more tiles than there is room for
+    list.counts[threadIdx.x] = min(at, threadIdx.x == 0 ? list.q_room : list.k_room);
+  }
+  __syncthreads();
+  auto write = [&](int stretch, int nq, int nk, int tq, int tk, int first, int step) {
+    for (int t = first; t < nq; t += step)
+      if (tq + t < list.q_room) list.q_tiles[tq + t] = make_int2(stretch, nq - 1 - t);
+    for (int t = first; t < nk; t += step)
+      if (tk + t < list.k_room) list.k_tiles[tk + t] = make_int2(stretch, t);
+  };
+  for (int i0 = 0; i0 < p.batch + 2; i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    const int64_t q = rows_of(p.q_offsets, p.total_q, i), k = rows_of(p.k_offsets, p.total_k, i);
+    const int c = weight_class(max(q, k)), nq = static_cast<int>((q + kRows - 1) / kRows), nk = static_cast<int>((k + kRows - 1) / kRows);
+    const int tq = nq > 0 ? atomicAdd(&next[0][c], nq) : 0, tk = nk > 0 ? atomicAdd(&next[1][c], nk) : 0;
     // few tiles by the stretch's thread, many by its warp
-    const bool many = (mine & 0xffffffff) > 4 || (mine >> 32) > 4;
-    if (!many) write(i, mine, at, 0, 1);
+    const bool many = nq > 4 || nk > 4;
+    if (!many) write(i, nq, nk, tq, tk, 0, 1);
     for (unsigned left = __ballot_sync(kFullMask, many); left != 0; left &= left - 1) {
       const int l = __ffs(left) - 1;
-      write(s0 + warp * 32 + l, __shfl_sync(kFullMask, mine, l), __shfl_sync(kFullMask, at, l), lane, 32);
+      write(i - lane + l, __shfl_sync(kFullMask, nq, l), __shfl_sync(kFullMask, nk, l), __shfl_sync(kFullMask, tq, l),
+            __shfl_sync(kFullMask, tk, l), lane, 32);
     }
-    base += all;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) {
-    plan.tickets[0] = plan.tickets[1] = 0;
-    plan.counts[0] = min(static_cast<int>(base & 0xffffffff), plan.q_room);
-    plan.counts[1] = min(static_cast<int>(base >> 32), plan.k_room);
   }
 }
+
+__global__ void __launch_bounds__(kThreads) list_kernel(const AttnDev p, const TileList plan) { list_tiles(p, plan); }
 
 // Group of kLanes lanes for a row of one head, a vector of kElems elements each; block 0 lists the tiles.
 template <typename T, int kElems, int kLanes>
@@ -160,6 +151,11 @@ int delta_of(const AttnDev& p, const TileList& plan, cudaStream_t stream) {
 }
 
 }  // namespace
+
+int attention_list(const AttnDev& p, const TileList& list, cudaStream_t stream) {
+  list_kernel<<<1, kThreads, 0, stream>>>(p, list);
+  return launch_status();
+}
 
 int attention_delta_listed(const AttnDev& p, const TileList& list, int dtype, cudaStream_t stream) {
   // 16-byte vectors: the tensor-core kernels that use the list have checked the strides
