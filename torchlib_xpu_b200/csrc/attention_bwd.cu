@@ -7,7 +7,8 @@
 //
 // Two kernels, so that no sum crosses a CTA and the results do not depend on scheduling: S and dP are computed
 // twice (7 products instead of 5), and nothing is added in memory. Scores and dP come into tensor memory
-// with a row for each thread pair; two warpgroups take half of the columns each; P and dS go back into tensor
+// with a row for each four threads; four warpgroups take a quarter of the columns each
+// (two, with half of them each, left the exponentials waiting for one another: dK and dV 455 us, dQ 312); P and dS go back into tensor
 // memory, each in its own columns' place, rounded to the operands' type, as the left operand of the next product. P and dS are rounded because
 // the tensor cores multiply 16-bit operands; they are summed in fp32.
 // The CTAs take the tiles of a list, which an earlier kernel of the pass leaves, one after the other.
@@ -18,7 +19,11 @@ namespace b200tbe {
 namespace {
 
 constexpr int kRows = 128;   // queries of a tile, keys of a tile
-constexpr int kThreads = 384;
+constexpr int kParts = 4;                       // warpgroups that share a tile's columns, 32 each
+constexpr int kThreads = kParts * 128 + 128;
+constexpr int kIssue = kParts * 4, kCopy = kIssue + 1, kStats = kIssue + 2;   // warps
+// registers: 96 x 640 threads are launched as 104 four times and 64 a warpgroup
+constexpr int kWeightRegs = 104, kOtherRegs = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct BwdDev {
@@ -85,38 +90,30 @@ __device__ __forceinline__ void load_tile(uint8_t* tile, const CUtensorMap* map,
   for (int x = 0; x < kDP / 64; ++x) tma_load_3d(smem_addr(tile) + x * kRows * 128, map, x * 64, head, row, bar);
 }
 
-// Row `row` of a tile in shared memory (as the tensor copies leave it) to this thread's lane of tensor memory, two
-// elements a column: a left operand.
-template <int kDP>
+// 64 elements of row `row` of a tile in shared memory (as the tensor copies leave it) to this thread's lane of tensor
+// memory, two a column: a left operand.
 __device__ __forceinline__ void copy_row(uint32_t to, const uint8_t* tile, int row) {
+  uint32_t r[32];
 #pragma unroll
-  for (int x = 0; x < kDP / 64; ++x) {
-    uint32_t r[32];
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const uint4 v = *reinterpret_cast<const uint4*>(tile + x * kRows * 128 + row * 128 + (c ^ (row % 8)) * 16);
-      r[4 * c] = v.x, r[4 * c + 1] = v.y, r[4 * c + 2] = v.z, r[4 * c + 3] = v.w;
-    }
-    tmem_st32(to + x * 32, r);
+  for (int c = 0; c < 8; ++c) {
+    const uint4 v = *reinterpret_cast<const uint4*>(tile + row * 128 + (c ^ (row % 8)) * 16);
+    r[4 * c] = v.x, r[4 * c + 1] = v.y, r[4 * c + 2] = v.z, r[4 * c + 3] = v.w;
   }
+  tmem_st32(to, r);
   tmem_wait_st();
-  tc_fence_before();
 }
 
-// A warp's accumulator rows in tensor memory, times f, to memory: `rows` of them.
-template <bool kBf16, int kDP>
-__device__ __forceinline__ void store_rows(uint8_t* stage, uint16_t* out, int64_t stride, uint32_t at, int D, float f,
+// 32 columns from `col` on of a warp's accumulator rows in tensor memory, times f, to memory: `rows` of them.
+template <bool kBf16>
+__device__ __forceinline__ void store_rows(uint8_t* stage, uint16_t* out, int64_t stride, uint32_t at, int col, int D, float f,
                                            bool computed, int rows) {
-#pragma unroll 1
-  for (int i = 0; i < kDP && rows > 0; i += 32) {
-    uint32_t o[32];
-    if (computed) {
-      tmem_ld32(o, at + i);
-      tmem_wait_ld();
-    }
-    store_columns<kBf16>(stage, o, f, !computed, out, stride, rows, i, D);
+  if (rows <= 0) return;
+  uint32_t o[32];
+  if (computed) {
+    tmem_ld32(o, at + col);
+    tmem_wait_ld();
   }
-  fence_async_smem();
+  store_columns<kBf16>(stage, o, f, !computed, out, stride, rows, col, D);
 }
 
 // x = exp2(x c + m) in place, two and two
@@ -160,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* vs = ks + 3 * L::kTileBytes;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) dead_word = 0;
-  if (warp == 8) tmem_alloc(&tmem_base, 512);
+  if (warp == kIssue) tmem_alloc(&tmem_base, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -168,14 +165,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* dead = &dead_word;
 
   Item it;
-  if (warp >= 8) {
-    give_registers<80>();
+  if (warp >= kIssue) {
+    give_registers<kOtherRegs>();
     while (!*dead && next_item<0>(p, &ticket, &it)) {
       const int kv = it.head / a.group, shift = it.other_len - it.len, klen = it.other_len;
       const int sees = a.causal ? min(klen, min(it.len, it.first + kRows) + shift) : klen;
       const int n = sees > 0 ? (sees + kRows - 1) / kRows : 0;
       __syncthreads();   // the barriers are set up
-      if (warp == 9) {
+      if (warp == kCopy) {
         // ---- copies ----
         if (lane == 0 && n > 0) {
           mbar_expect(&bars.q_full, 2 * L::kTileBytes);
@@ -191,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             load_tile<kDP>(vs, &v_map, kv, row, &bars.v_full);
           }
         }
-      } else if (warp == 8 && n > 0) {
+      } else if (warp == kIssue && n > 0) {
         // ---- matrix instructions ----
         const int d_steps = (a.D + 15) / 16;
         const uint32_t dq_desc = mma_desc(kBf16, kRows, (a.D + 15) & ~15, false, true);
@@ -229,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           alive = alive && warp_wait(&bars.ds_full, j & 1, dead);
           tc_fence_after();
           if (alive && elect_one()) {
-            mma_over_rows<32>(dq_at, dp_at, smem_addr(ks + j % 3 * L::kTileBytes), dq_desc, (keys_of(j) + 15) / 16, j > 0);
+            mma_over_rows<16, 2>(dq_at, dp_at, smem_addr(ks + j % 3 * L::kTileBytes), dq_desc, (keys_of(j) + 15) / 16, j > 0);
             if (j + 3 < n) mma_commit(&bars.k_empty[j % 3]);
             if (j + 1 == n) mma_commit(&bars.done);
           }
@@ -241,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
     }
   } else {
-    take_registers<208>();
+    take_registers<kWeightRegs>();
     for (bool fresh = true; !*dead && next_item<0>(p, &ticket, &it); fresh = false) {
       const int shift = it.other_len - it.len, klen = it.other_len;
       const int sees = a.causal ? min(klen, min(it.len, it.first + kRows) + shift) : klen;
@@ -249,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (threadIdx.x == 0) {
         if (!fresh) mbar_forget(&bars);
         mbar_init(&bars.q_full, 1);
-        mbar_init(&bars.a_full, 256);
+        mbar_init(&bars.a_full, kParts * 128);
         for (int i = 0; i < 3; ++i) {
           mbar_init(&bars.k_full[i], 1);
           mbar_init(&bars.k_empty[i], 1);
@@ -258,14 +255,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&bars.v_empty, 1);
         mbar_init(&bars.s_full, 1);
         mbar_init(&bars.dp_full, 1);
-        mbar_init(&bars.s_loaded, 256);
-        mbar_init(&bars.ds_full, 256);
+        mbar_init(&bars.s_loaded, kParts * 128);
+        mbar_init(&bars.ds_full, kParts * 128);
         mbar_init(&bars.done, 1);
         fence_barrier_init();
       }
       __syncthreads();
-      // ---- weights: a row and half of the columns a thread ----
-      const int half = warp / 4, local = (warp % 4) * 32 + lane, row = it.first + local;
+      // ---- weights: a row and 32 columns a thread ----
+      const int part = warp / 4, local = (warp % 4) * 32 + lane, row = it.first + local;
       const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
       const int limit = row >= it.len ? 0 : (a.causal ? min(klen, row + shift + 1) : klen);
       float lse2 = 0.f, delta = 0.f;
@@ -276,58 +273,54 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float c = a.scale * kLog2e;
       const uint64_t c2 = pair(c, c), minus_delta = pair(-delta, -delta);
-      const uint32_t s_at = tmem + lanes + half * 64, ds_at = dp_at + lanes + half * 64;
+      const uint32_t s_at = tmem + lanes + part * 32, ds_at = dp_at + lanes + part * 32;
       bool alive = n == 0 || warp_wait(&bars.q_full, 0, dead);
-      if (alive && n > 0) {   // the queries' rows by one warpgroup, dO's by the other
-        copy_row<kDP>((half == 0 ? q_at : g_at) + lanes, half == 0 ? qs : gs, local);
+      if (alive && n > 0) {   // the queries' rows by two warpgroups, dO's by the others
+        if (part % 2 < kDP / 64) copy_row((part < 2 ? q_at : g_at) + lanes + part % 2 * 32, (part < 2 ? qs : gs) + part % 2 * kRows * 128, local);
+        tc_fence_before();
         mbar_arrive(&bars.a_full);
       }
       for (int j = 0; alive && j < n; ++j) {
         alive = warp_wait(&bars.s_full, j & 1, dead);
         if (!alive) break;
         tc_fence_after();
-        const int chunks = row - lane < it.len ? max(0, min(2, (klen - j * kRows - half * 64 + 31) / 32)) : 0;
-        const int left = limit - j * kRows - half * 64;
-        uint32_t s[2][32];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (i < chunks) tmem_ld32(s[i], s_at + i * 32);
+        const bool any = row - lane < it.len && klen - j * kRows - part * 32 > 0;   // rows and columns of the sequence here
+        const int left = limit - j * kRows - part * 32;
+        uint32_t s[32];
+        if (any) tmem_ld32(s, s_at);
         tmem_wait_ld();
         tc_fence_before();
         mbar_arrive(&bars.s_loaded);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (i < chunks) exponentials(s[i], c2, pair(-lse2, -lse2));
+        if (any) exponentials(s, c2, pair(-lse2, -lse2));
         alive = warp_wait(&bars.dp_full, j & 1, dead);
         if (!alive) break;
         tc_fence_after();
+        if (any) {
+          uint32_t dp[32], w[16];
+          tmem_ld32(dp, ds_at);
+          tmem_wait_ld();
+          const bool cut = __any_sync(kFullMask, left < 32);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (i < chunks) {
-            uint32_t dp[32], w[16];
-            tmem_ld32(dp, ds_at + i * 32);
-            tmem_wait_ld();
-            const bool cut = __any_sync(kFullMask, left < i * 32 + 32);
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              float2 d = unpair(mul2(as_pair(&s[i][e]), add2(as_pair(&dp[e]), minus_delta)));
-              if (cut) {
-                d.x = i * 32 + e < left ? d.x : 0.f;
-                d.y = i * 32 + e + 1 < left ? d.y : 0.f;
-              }
-              w[e / 2] = pack2<kBf16>(d.x, d.y);
+          for (int e = 0; e < 32; e += 2) {
+            float2 d = unpair(mul2(as_pair(&s[e]), add2(as_pair(&dp[e]), minus_delta)));
+            if (cut) {
+              d.x = e < left ? d.x : 0.f;
+              d.y = e + 1 < left ? d.y : 0.f;
             }
-            tmem_st16(ds_at + i * 16, w);
+            w[e / 2] = pack2<kBf16>(d.x, d.y);
           }
+          tmem_st16(ds_at, w);
+        }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&bars.ds_full);
       }
       if (alive && n > 0) alive = warp_wait(&bars.done, 0, dead);
       tc_fence_after();
-      if (half == 0)
-        store_rows<kBf16, kDP>(qs + warp * 2048, static_cast<uint16_t*>(a.dq) + (it.begin + row - lane) * a.dq_row + it.head * a.dq_head,
-                               a.dq_row, dq_at + lanes, a.D, a.scale, n > 0, it.len - row + lane);
+      if (part < kDP / 32)
+        store_rows<kBf16>(qs + warp * 2048, static_cast<uint16_t*>(a.dq) + (it.begin + row - lane) * a.dq_row + it.head * a.dq_head,
+                          a.dq_row, dq_at + lanes, part * 32, a.D, a.scale, n > 0, it.len - row + lane);
+      fence_async_smem();
       tc_fence_before();
       __syncthreads();
       tc_fence_after();
@@ -335,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   report(&dead_word, p.status);
   __syncthreads();
-  if (warp == 8) tmem_free(tmem, 512);
+  if (warp == kIssue) tmem_free(tmem, 512);
 }
 
 // Tensor memory: scores (transposed: a key a row; P takes their place), dP (dS takes its place), dV, dK. dV and
@@ -357,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* gs = qs + 2 * L::kTileBytes;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) dead_word = 0;
-  if (warp == 8) tmem_alloc(&tmem_base, 512);
+  if (warp == kIssue) tmem_alloc(&tmem_base, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -365,14 +358,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* dead = &dead_word;
 
   Item it;
-  if (warp >= 8) {
-    give_registers<80>();
+  if (warp >= kIssue) {
+    give_registers<kOtherRegs>();
     while (!*dead && next_item<1>(p, &ticket, &it)) {
       const int shift = it.len - it.other_len, qlen = it.other_len, head0 = it.head * a.group;
       const int from = a.causal ? max(0, it.first - shift) / kRows : 0;   // first tile with a query that sees a key of this one
       const int per_head = max(0, (qlen + kRows - 1) / kRows - from), n = per_head * a.group;
       __syncthreads();   // the barriers are set up
-      if (warp == 9) {
+      if (warp == kCopy) {
         // ---- copies ----
         if (lane == 0 && n > 0) {
           mbar_expect(&bars.kv_full, 2 * L::kTileBytes);
@@ -389,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             load_tile<kDP>(gs + st * L::kTileBytes, &g_map, head, row, &bars.g_full[st]);
           }
         }
-      } else if (warp == 10) {
+      } else if (warp == kStats) {
         // ---- the queries' log-sums and deltas ----
         for (int j = 0; j < n; ++j) {
           const int st = j & 1, i0 = (from + j % per_head) * kRows, head = head0 + j / per_head;
@@ -403,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           mbar_arrive(&bars.stat_full[st]);
         }
-      } else if (warp == 8 && n > 0) {
+      } else if (warp == kIssue && n > 0) {
         // ---- matrix instructions ----
         const int d_steps = (a.D + 15) / 16;
         const uint32_t k_at = smem_addr(ks), v_at = smem_addr(vs);
@@ -440,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           alive = warp_wait(&bars.p_full, j & 1, dead);
           if (!alive) break;
           tc_fence_after();
-          if (elect_one()) mma_over_rows<32>(dv_at, tmem, smem_addr(gs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
+          if (elect_one()) mma_over_rows<16, 2>(dv_at, tmem, smem_addr(gs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
           if (elect_one() && j + 2 < n) mma_commit(&bars.g_empty[j & 1]);
           __syncwarp();
           if (more) {
@@ -452,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!alive) break;
           tc_fence_after();
           if (elect_one()) {
-            mma_over_rows<32>(dk_at, dp_at, smem_addr(qs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
+            mma_over_rows<16, 2>(dk_at, dp_at, smem_addr(qs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
             if (j + 2 < n) mma_commit(&bars.q_empty[j & 1]);
             if (!more) mma_commit(&bars.done);
           }
@@ -464,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
     }
   } else {
-    take_registers<208>();
+    take_registers<kWeightRegs>();
     for (bool fresh = true; !*dead && next_item<1>(p, &ticket, &it); fresh = false) {
       const int shift = it.len - it.other_len, qlen = it.other_len;
       const int from = a.causal ? max(0, it.first - shift) / kRows : 0;   // first tile with a query that sees a key of this one
@@ -478,85 +471,75 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_init(&bars.g_full[i], 1);
           mbar_init(&bars.g_empty[i], 1);
           mbar_init(&bars.stat_full[i], 32);
-          mbar_init(&bars.stat_empty[i], 256);
+          mbar_init(&bars.stat_empty[i], kParts * 128);
         }
         mbar_init(&bars.s_full, 1);
         mbar_init(&bars.dp_full, 1);
-        mbar_init(&bars.p_full, 256);
-        mbar_init(&bars.ds_full, 256);
+        mbar_init(&bars.p_full, kParts * 128);
+        mbar_init(&bars.ds_full, kParts * 128);
         mbar_init(&bars.done, 1);
         fence_barrier_init();
       }
       __syncthreads();
-      // ---- weights: a key and half of the queries a thread ----
-      const int half = warp / 4, local = (warp % 4) * 32 + lane, key = it.first + local;
+      // ---- weights: a key and 32 queries a thread ----
+      const int part = warp / 4, local = (warp % 4) * 32 + lane, key = it.first + local;
       const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
       const uint64_t c2 = pair(a.scale * kLog2e, a.scale * kLog2e);
-      const uint32_t s_at = tmem + lanes + half * 64, ds_at = dp_at + lanes + half * 64;
+      const uint32_t s_at = tmem + lanes + part * 32, ds_at = dp_at + lanes + part * 32;
       bool alive = true;
       for (int j = 0; j < n; ++j) {
-        const int st = j & 1, i0 = (from + j % per_head) * kRows + half * 64;
+        const int st = j & 1, i0 = (from + j % per_head) * kRows + part * 32;
         alive = warp_wait(&bars.stat_full[st], (j / 2) & 1, dead) && warp_wait(&bars.s_full, j & 1, dead);
         if (!alive) break;
         tc_fence_after();
-        const int chunks = key - lane < it.len ? max(0, min(2, (qlen - i0 + 31) / 32)) : 0;
+        const bool any = key - lane < it.len && qlen - i0 > 0;   // rows and columns of the sequence here
         // columns [low, high) are queries of the sequence that see the key
         const int low = a.causal ? key - shift - i0 : 0, high = qlen - i0;
-        const bool cut = __any_sync(kFullMask, low > 0 || high < 64);
-        uint32_t s[2][32];
+        const bool cut = __any_sync(kFullMask, low > 0 || high < 32);
+        uint32_t s[32], w[16];
+        if (any) {
+          tmem_ld32(s, s_at);
+          tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (i < chunks) tmem_ld32(s[i], s_at + i * 32);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (i < chunks) {
-            uint32_t w[16];
-            const float* m = &stats[st][0][half * 64 + i * 32];
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const float4 x = *reinterpret_cast<const float4*>(m + e);
-              exponentials4(s[i], e, c2, pair(-x.x, -x.y), pair(-x.z, -x.w));
-            }
-            if (cut) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (i * 32 + e < low || i * 32 + e >= high) s[i][e] = 0u;
-            }
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) w[e / 2] = pack2<kBf16>(__uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
-            tmem_st16(s_at + i * 16, w);
+          for (int e = 0; e < 32; e += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(&stats[st][0][part * 32 + e]);
+            exponentials4(s, e, c2, pair(-x.x, -x.y), pair(-x.z, -x.w));
           }
+          if (cut) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (e < low || e >= high) s[e] = 0u;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) w[e / 2] = pack2<kBf16>(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+          tmem_st16(s_at, w);
+        }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&bars.p_full);
         alive = warp_wait(&bars.dp_full, j & 1, dead);
         if (!alive) break;
         tc_fence_after();
+        if (any) {
+          uint32_t dp[32];
+          tmem_ld32(dp, ds_at);
+          tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (i < chunks) {
-            uint32_t dp[32], w[16];
-            tmem_ld32(dp, ds_at + i * 32);
-            tmem_wait_ld();
-            const float* m = &stats[st][1][half * 64 + i * 32];
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const float4 d = *reinterpret_cast<const float4*>(m + e);
-              float2 x = unpair(mul2(as_pair(&s[i][e]), add2(as_pair(&dp[e]), pair(-d.x, -d.y))));
-              float2 y = unpair(mul2(as_pair(&s[i][e + 2]), add2(as_pair(&dp[e + 2]), pair(-d.z, -d.w))));
-              if (cut) {
-                const int at = i * 32 + e;
-                x.x = at < low || at >= high ? 0.f : x.x;
-                x.y = at + 1 < low || at + 1 >= high ? 0.f : x.y;
-                y.x = at + 2 < low || at + 2 >= high ? 0.f : y.x;
-                y.y = at + 3 < low || at + 3 >= high ? 0.f : y.y;
-              }
-              w[e / 2] = pack2<kBf16>(x.x, x.y);
-              w[e / 2 + 1] = pack2<kBf16>(y.x, y.y);
+          for (int e = 0; e < 32; e += 4) {
+            const float4 d = *reinterpret_cast<const float4*>(&stats[st][1][part * 32 + e]);
+            float2 x = unpair(mul2(as_pair(&s[e]), add2(as_pair(&dp[e]), pair(-d.x, -d.y))));
+            float2 y = unpair(mul2(as_pair(&s[e + 2]), add2(as_pair(&dp[e + 2]), pair(-d.z, -d.w))));
+            if (cut) {
+              x.x = e < low || e >= high ? 0.f : x.x;
+              x.y = e + 1 < low || e + 1 >= high ? 0.f : x.y;
+              y.x = e + 2 < low || e + 2 >= high ? 0.f : y.x;
+              y.y = e + 3 < low || e + 3 >= high ? 0.f : y.y;
             }
-            tmem_st16(ds_at + i * 16, w);
+            w[e / 2] = pack2<kBf16>(x.x, x.y);
+            w[e / 2 + 1] = pack2<kBf16>(y.x, y.y);
           }
+          tmem_st16(ds_at, w);
+        }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&bars.ds_full);
@@ -564,12 +547,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (alive && n > 0) alive = warp_wait(&bars.done, 0, dead);
       tc_fence_after();
-      if (half == 0)
-        store_rows<kBf16, kDP>(ks + warp * 2048, static_cast<uint16_t*>(a.dv) + (it.begin + key - lane) * a.dv_row + it.head * a.dv_head,
-                               a.dv_row, dv_at + lanes, a.D, 1.f, n > 0, it.len - key + lane);
-      else
-        store_rows<kBf16, kDP>(ks + warp * 2048, static_cast<uint16_t*>(a.dk) + (it.begin + key - lane) * a.dk_row + it.head * a.dk_head,
-                               a.dk_row, dk_at + lanes, a.D, a.scale, n > 0, it.len - key + lane);
+      const bool first = part < 2;   // dV by two warpgroups, dK by the others
+      const int64_t stride = first ? a.dv_row : a.dk_row;
+      uint16_t* out = static_cast<uint16_t*>(first ? a.dv : a.dk) + (it.begin + key - lane) * stride +
+                      it.head * (first ? a.dv_head : a.dk_head);
+#pragma unroll 1
+      for (int i = part % 2 * 32; i < kDP; i += 64)
+        store_rows<kBf16>(ks + warp * 2048, out, stride, (first ? dv_at : dk_at) + lanes, i, a.D, first ? 1.f : a.scale, n > 0,
+                          it.len - key + lane);
+      fence_async_smem();
       tc_fence_before();
       __syncthreads();
       tc_fence_after();
@@ -577,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   report(&dead_word, p.status);
   __syncthreads();
-  if (warp == 8) tmem_free(tmem, 512);
+  if (warp == kIssue) tmem_free(tmem, 512);
 }
 
 template <bool kBf16, int kDP>

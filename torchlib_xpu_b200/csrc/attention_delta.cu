@@ -49,9 +49,9 @@ __device__ __forceinline__ void list_tiles(const AttnDev& p, const TileList& lis
   __syncthreads();
   auto write = [&](int stretch, int nq, int nk, int tq, int tk, int first, int step) {
     for (int t = first; t < nq; t += step)
-      if (tq + t < list.q_room) list.q_tiles[tq + t] = make_int2(stretch, nq - 1 - t);
+      if (static_cast<unsigned>(tq + t) < static_cast<unsigned>(list.q_room)) list.q_tiles[tq + t] = make_int2(stretch, nq - 1 - t);
     for (int t = first; t < nk; t += step)
-      if (tk + t < list.k_room) list.k_tiles[tk + t] = make_int2(stretch, t);
+      if (static_cast<unsigned>(tk + t) < static_cast<unsigned>(list.k_room)) list.k_tiles[tk + t] = make_int2(stretch, t);
   };
   for (int i0 = 0; i0 < p.batch + 2; i0 += kThreads) {
     const int i = i0 + threadIdx.x;

@@ -59,7 +59,9 @@ struct Finder {
     int at = 0;
     if (lane == 0) at = atomicAdd(p.plan.counts + side, n);
     at = __shfl_sync(kFullMask, at, 0);
-    for (int t = lane; t < n && at + t < room; t += 32) tiles[at + t] = make_int2(of, side == 0 ? n - 1 - t : t);
+    // offsets that decrease give more tiles than there is room for, or than an int counts
+    for (int t = lane; t < n; t += 32)
+      if (static_cast<unsigned>(at + t) < static_cast<unsigned>(room)) tiles[at + t] = make_int2(of, side == 0 ? n - 1 - t : t);
   }
   __device__ __forceinline__ void zeros(void* base, int64_t row, int64_t stride, int rows) {
     const int vecs = p.a.D / 8;

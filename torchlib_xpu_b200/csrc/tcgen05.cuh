@@ -195,14 +195,14 @@ __device__ __forceinline__ void mma_along_k_ts(uint32_t d, uint32_t a, uint32_t 
     if (t < steps) mma_ts(d, a + t * 8, b0 + (((t / 4) * kRowsOfTile * 128 + (t % 4) * 32) >> 4), desc, t > 0);
 }
 
-// d[128][n] (+)= w x over up to 128 rows of x, 16 a step: w in tensor memory, two 16-bit elements a column, the second
-// 64 of them kSkip columns further on; x in tiles of 128 rows, n along the row.
-template <int kSkip>
+// d[128][n] (+)= w x over up to 128 rows of x, 16 a step: w in tensor memory, two 16-bit elements a column, kSkip columns
+// left out after every kRun steps' worth; x in tiles of 128 rows, n along the row.
+template <int kSkip = 0, int kRun = 8>
 __device__ __forceinline__ void mma_over_rows(uint32_t d, uint32_t w, uint32_t x, uint32_t desc, int steps, bool add) {
   const uint64_t x0 = smem_desc(x, 128 * 128);
 #pragma unroll
   for (int t = 0; t < 8; ++t)
-    if (t < steps) mma_ts(d, w + t * 8 + (t >= 4 ? kSkip : 0), x0 + t * (2048 >> 4), desc, t > 0 || add);
+    if (t < steps) mma_ts(d, w + t * 8 + t / kRun * kSkip, x0 + t * (2048 >> 4), desc, t > 0 || add);
 }
 
 // Arrives once all matrix instructions that this thread has issued are done. Some thread has to wait for it: an
