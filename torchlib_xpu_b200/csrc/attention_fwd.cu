@@ -23,17 +23,18 @@ struct FwdDev {
   AttnDev a;
   int32_t pair_heads;   // the two query tiles: 1: two heads' (one key head, same rows), 0: consecutive rows of a head
   int32_t* status;
-  // With a list of tiles of 128 queries (what the short sequences' kernel left over) the CTAs take them one after
-  // the other; without one, a CTA takes its slot's tile.
+  // The CTAs' items: the tiles of 128 queries of a list, or without one those of the slots, times heads (or pairs).
   int32_t listed;
-  TileList plan;
+  int64_t slots;
+  TileList list;
 };
 
 template <int kDP, int kNQ>
 struct Layout {
   static constexpr int kTileBytes = kRows * kDP * 2;
   static constexpr int kStages = kNQ == 1 && kDP == 128 ? 1 : 2;
-  static constexpr int kSmem = (kNQ + 2 * kStages) * kTileBytes + 1024;
+  static constexpr int kStage = 2048;   // a warp's way out for results
+  static constexpr int kSmem = (kNQ + 2 * kStages) * kTileBytes + kNQ * 4 * kStage + 1024;
   static constexpr int kThreads = kNQ * 128 + 128;
   // registers: 168 x 384 threads are launched as 208 + 208 + 80 a warpgroup, 128 x 256 as 152 + 104
   static constexpr int kSoftmaxRegs = kNQ == 1 ? 152 : 208;
@@ -43,235 +44,299 @@ struct Layout {
 };
 
 struct Barriers {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
-};
-struct Shared {
-  Barriers b;
-  uint32_t tmem;
-  int dead;
+  uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2];
 };
 
 // A CTA's queries: rows row0 .. of a stretch of qlen rows that begins at row `begin`, of one head (or two), with the
-// stretch's keys.
+// stretch's keys; n[s]: tiles of keys that the rows of query tile s see.
+template <int kNQ>
 struct Item {
-  int64_t begin, k0;
-  int row0, qlen, klen, head;
+  int begin, k0, row0, qlen, klen, head;
+  int n[kNQ], most;
 };
 
-// The item of this CTA's slot; false: it has none.
-template <bool kTwo>
-__device__ __forceinline__ bool slot_item(const FwdDev& p, bool pair_heads, int per_slot, Item* item) {
+// All items of the launch (of the list, as many as it has).
+template <int kNQ>
+__device__ __forceinline__ int64_t all_items(const FwdDev& p) {
+  const int per_slot = kNQ == 2 && p.pair_heads ? p.a.heads / 2 : p.a.heads;
+  return (p.listed ? min(p.list.counts[0], p.list.q_room) : p.slots) * static_cast<int64_t>(per_slot);
+}
+
+// Item `index`, found by a whole warp for itself. false: its slot is empty.
+template <int kNQ>
+__device__ __forceinline__ bool find_item(const FwdDev& p, int64_t index, Item<kNQ>* item) {
   const AttnDev& a = p.a;
-  const int64_t slots = gridDim.x / per_slot;
-  // later tiles of a sequence see more keys: they go first
-  const int64_t slot = a.causal ? slots - 1 - blockIdx.x / per_slot : blockIdx.x / per_slot;
+  const bool pair_heads = kNQ == 2 && p.pair_heads;
+  const int per_slot = pair_heads ? a.heads / 2 : a.heads;
+  int64_t slot = index / per_slot, begin, first, end, k0;
   int32_t stretch;
-  int64_t first, end;
-  const bool ok = kTwo && !pair_heads ? find_tile<2 * kRows>(a.q_offsets, a.offset_bytes, a.batch, a.total_q, slot, &stretch,
-                                                             &item->begin, &first, &end)
-                                      : find_tile<kRows>(a.q_offsets, a.offset_bytes, a.batch, a.total_q, slot, &stretch,
-                                                         &item->begin, &first, &end);
-  if (!ok) return false;
-  other_rows(a.k_offsets, a.offset_bytes, a.batch, a.total_k, stretch, &item->k0, &item->klen);
+  if (p.listed) {
+    const int2 at = p.list.q_tiles[slot];
+    stretch = at.x;
+    first = static_cast<int64_t>(at.y) * kRows;
+    begin = stretch_bound(a.q_offsets, a.offset_bytes, a.batch, a.total_q, stretch);
+    end = stretch_bound(a.q_offsets, a.offset_bytes, a.batch, a.total_q, stretch + 1);
+  } else {
+    if (a.causal) slot = p.slots - 1 - slot;   // later tiles of a sequence see more keys: they go first
+    const bool ok = kNQ == 2 && !pair_heads
+                        ? find_tile<2 * kRows>(a.q_offsets, a.offset_bytes, a.batch, a.total_q, slot, &stretch, &begin, &first, &end)
+                        : find_tile<kRows>(a.q_offsets, a.offset_bytes, a.batch, a.total_q, slot, &stretch, &begin, &first, &end);
+    if (!ok) return false;
+  }
+  other_rows(a.k_offsets, a.offset_bytes, a.batch, a.total_k, stretch, &k0, &item->klen);
+  item->begin = static_cast<int>(begin);
+  item->k0 = static_cast<int>(k0);
   item->row0 = static_cast<int>(first);
-  item->qlen = static_cast<int>(end - item->begin);
-  item->head = static_cast<int>(blockIdx.x % per_slot) * (pair_heads ? 2 : 1);
+  item->qlen = static_cast<int>(end - begin);
+  item->head = static_cast<int>(index % per_slot) * (pair_heads ? 2 : 1);
+  item->most = 0;
+#pragma unroll
+  for (int s = 0; s < kNQ; ++s) {
+    const int from = item->row0 + (pair_heads ? 0 : s * kRows);
+    const int sees = a.causal ? min(item->klen, min(item->qlen, from + kRows) + item->klen - item->qlen) : item->klen;
+    item->n[s] = from < item->qlen && sees > 0 ? (sees + kRows - 1) / kRows : 0;
+    item->most = max(item->most, item->n[s]);
+  }
   return true;
 }
 
-// The next item of the list: one thread takes a ticket for the CTA. false: none are left.
-__device__ __forceinline__ bool list_item(const FwdDev& p, int per_slot, bool pair_heads, int* ticket, Item* item) {
-  const AttnDev& a = p.a;
-  if (threadIdx.x == 0) *ticket = atomicAdd(p.plan.tickets, 1);
-  __syncthreads();
-  const int t = *ticket;
-  if (t / per_slot >= min(p.plan.counts[0], p.plan.q_room)) return false;
-  const int2 at = p.plan.q_tiles[t / per_slot];
-  item->begin = stretch_bound(a.q_offsets, a.offset_bytes, a.batch, a.total_q, at.x);
-  item->qlen = static_cast<int>(stretch_bound(a.q_offsets, a.offset_bytes, a.batch, a.total_q, at.x + 1) - item->begin);
-  other_rows(a.k_offsets, a.offset_bytes, a.batch, a.total_k, at.x, &item->k0, &item->klen);
-  item->row0 = at.y * kRows;
-  item->head = t % per_slot * (pair_heads ? 2 : 1);
+// The numbers of the CTA's items, handed from the warp that copies to the others, a few ahead; -1 ends them.
+struct Queue {
+  static constexpr int kRoom = 4;
+  uint64_t full[kRoom], empty[kRoom];
+  int64_t index[kRoom];
+};
+__device__ __forceinline__ bool put_item(Queue* queue, int turn, int64_t index, volatile int* dead) {
+  const int at = turn % Queue::kRoom;
+  if (turn >= Queue::kRoom && !warp_wait(&queue->empty[at], (turn / Queue::kRoom - 1) & 1, dead)) return false;
+  if (threadIdx.x % 32 == 0) {
+    queue->index[at] = index;
+    mbar_arrive(&queue->full[at]);
+  }
+  __syncwarp();
   return true;
 }
+// the turn's item, -1 after the last or when a wait gave up
+__device__ __forceinline__ int64_t take_item(Queue* queue, int turn, volatile int* dead) {
+  const int at = turn % Queue::kRoom;
+  if (!warp_wait(&queue->full[at], (turn / Queue::kRoom) & 1, dead)) return -1;
+  const int64_t index = queue->index[at];
+  __syncwarp();
+  if (threadIdx.x % 32 == 0) mbar_arrive(&queue->empty[at]);
+  return index;
+}
 
+// The CTA's items go through its roles one after the other without a common stop: while the softmax warps finish one, the
+// next one's copies and first scores are under way. So the barriers' phases run on over the items; every role counts
+// for itself what it has waited for.
 template <bool kBf16, int kDP, int kNQ>
 __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::kCtas)
     attention_fwd_kernel(const FwdDev p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-               const __grid_constant__ CUtensorMap v_map) {
+                         const __grid_constant__ CUtensorMap v_map) {
   using L = Layout<kDP, kNQ>;
+  constexpr int kSt = L::kStages;
   extern __shared__ uint8_t raw[];
-  __shared__ Shared bars;
-  __shared__ int ticket;
+  __shared__ Barriers bars;
+  __shared__ Queue queue;
+  __shared__ uint32_t tmem_base;
+  __shared__ int dead_word;
   const AttnDev& a = p.a;
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* qs = smem;
+  uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* ks = qs + kNQ * L::kTileBytes;
-  uint8_t* vs = ks + L::kStages * L::kTileBytes;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-
+  uint8_t* vs = ks + kSt * L::kTileBytes;
+  uint8_t* stage = vs + kSt * L::kTileBytes;
+  const int warp = __shfl_sync(kFullMask, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const bool pair_heads = kNQ == 2 && p.pair_heads;
-  const int per_slot = pair_heads ? a.heads / 2 : a.heads;
-  Item item;
-  if (!p.listed && !slot_item<kNQ == 2>(p, pair_heads, per_slot, &item)) return;
-  if (threadIdx.x == 0) bars.dead = 0;
-  if (warp == kNQ * 4) tmem_alloc(&bars.tmem, L::kColumns);
+  volatile int* dead = &dead_word;
+  if (threadIdx.x == 0) {
+    mbar_init(&bars.q_full, 1);
+    mbar_init(&bars.q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.k_full[i], 1);
+      mbar_init(&bars.k_empty[i], 1);
+      mbar_init(&bars.v_full[i], 1);
+      mbar_init(&bars.v_empty[i], 1);
+      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_full[i], 128);
+      mbar_init(&bars.o_full[i], 1);
+      mbar_init(&bars.o_empty[i], 128);
+    }
+    for (int i = 0; i < Queue::kRoom; ++i) {
+      mbar_init(&queue.full[i], 1);
+      mbar_init(&queue.empty[i], kNQ * 4 + 1);
+    }
+    dead_word = 0;
+    fence_barrier_init();
+  }
+  if (warp == kNQ * 4) tmem_alloc(&tmem_base, L::kColumns);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars.tmem;
-  volatile int* dead = &bars.dead;
+  const uint32_t tmem = tmem_base;
+  Item<kNQ> it;
 
   if (warp >= kNQ * 4) {
     give_registers<L::kOtherRegs>();
-    for (bool fresh = true; !*dead && (p.listed ? list_item(p, per_slot, pair_heads, &ticket, &item) : fresh); fresh = false) {
-      const int64_t begin = item.begin;
-      const int head = item.head, kv = head / a.group, klen = item.klen, qlen = item.qlen, row0 = item.row0, shift = klen - qlen;
-      const int64_t k0 = item.k0;
-      // key tiles that the streams' rows see
-      int n[kNQ];
+    if (warp == kNQ * 4 + 1) {
+      // ---- copies ----
+      bool alive = true;
+      int items = 0, tile = 0;   // with products, and their tiles of keys
+      const int64_t all = all_items<kNQ>(p);
+      for (int turn = 0; alive; ++turn) {
+        // off a list whoever is ready takes the next, so that the CTAs end together
+        int64_t index = blockIdx.x + static_cast<int64_t>(turn) * gridDim.x;
+        if (p.listed) {
+          int ticket = 0;
+          if (lane == 0) ticket = atomicAdd(p.list.tickets, 1);
+          index = __shfl_sync(kFullMask, ticket, 0);
+        }
+        if (index >= all) index = -1;
+        alive = put_item(&queue, turn, index, dead);
+        if (index < 0 || !alive) break;
+        if (!find_item(p, index, &it) || it.most == 0) continue;
+        const int kv = it.head / a.group;
+        alive = items == 0 || warp_wait(&bars.q_empty, (items - 1) & 1, dead);
+        if (alive && elect_one()) {
+          mbar_expect(&bars.q_full, kNQ * L::kTileBytes);
 #pragma unroll
-      for (int s = 0; s < kNQ; ++s) {
-        const int from = row0 + (pair_heads ? 0 : s * kRows);
-        const int sees = a.causal ? min(klen, min(qlen, from + kRows) + shift) : klen;
-        n[s] = from < qlen && sees > 0 ? (sees + kRows - 1) / kRows : 0;
-      }
-      const int most = kNQ == 2 ? max(n[0], n[kNQ - 1]) : n[0];
-      __syncthreads();   // the barriers are set up
-      if (warp == kNQ * 4 + 1) {
-        // ---- copies ----
-        if (lane == 0 && most > 0) {
-          mbar_expect(&bars.b.q_full, kNQ * L::kTileBytes);
           for (int s = 0; s < kNQ; ++s)
-            for (int x = 0; x < kDP / 64; ++x)
-              tma_load_3d(smem_addr(qs) + s * L::kTileBytes + x * kRows * 128, &q_map, x * 64, head + (pair_heads ? s : 0),
-                          static_cast<int>(begin) + row0 + (pair_heads ? 0 : s * kRows), &bars.b.q_full);
-          for (int j = 0; j < most; ++j) {
-            const int st = j % L::kStages;
-            const uint32_t before = (j / L::kStages - 1) & 1;
-            if (j >= L::kStages && !mbar_wait(&bars.b.k_empty[st], before, dead)) break;
-            mbar_expect(&bars.b.k_full[st], L::kTileBytes);
-            for (int x = 0; x < kDP / 64; ++x)
-              tma_load_3d(smem_addr(ks) + st * L::kTileBytes + x * kRows * 128, &k_map, x * 64, kv, static_cast<int>(k0) + j * kRows,
-                          &bars.b.k_full[st]);
-            if (j >= L::kStages && !mbar_wait(&bars.b.v_empty[st], before, dead)) break;
-            mbar_expect(&bars.b.v_full[st], L::kTileBytes);
-            for (int x = 0; x < kDP / 64; ++x)
-              tma_load_3d(smem_addr(vs) + st * L::kTileBytes + x * kRows * 128, &v_map, x * 64, kv, static_cast<int>(k0) + j * kRows,
-                          &bars.b.v_full[st]);
-          }
-        }
-      } else if (warp == kNQ * 4) {
-        // ---- matrix instructions ----
-        const int d_steps = (a.D + 15) / 16;
-        bool alive = most == 0 || warp_wait(&bars.b.q_full, 0, dead);
-        // scores of stream s with key tile j; keys past the sequence's end are not multiplied
-        auto scores = [&](int s, int j) {
-          const int keys = min(kRows, (klen - j * kRows + 15) & ~15);
-          const uint32_t desc = mma_desc(kBf16, kRows, keys, false, false);
-          const uint32_t q_at = smem_addr(qs + s * L::kTileBytes), k_at = smem_addr(ks + (j % L::kStages) * L::kTileBytes);
-          mma_along_k<kDP / 16, kRows>(tmem + s * kRows, q_at, k_at, desc, d_steps);
-          mma_commit(&bars.b.s_full[s]);
-        };
-        if (alive && most > 0) {
-          alive = warp_wait(&bars.b.k_full[0], 0, dead);
-          if (alive && elect_one()) {
 #pragma unroll
-            for (int s = 0; s < kNQ; ++s)
-              if (n[s] > 0) scores(s, 0);
-            if (L::kStages < most) mma_commit(&bars.b.k_empty[0]);
-          }
+            for (int x = 0; x < kDP / 64; ++x)
+              tma_load_3d(smem_addr(qs) + s * L::kTileBytes + x * kRows * 128, &q_map, x * 64, it.head + (pair_heads ? s : 0),
+                          it.begin + it.row0 + (pair_heads ? 0 : s * kRows), &bars.q_full);
         }
-        const uint32_t pv_desc = mma_desc(kBf16, kRows, (a.D + 15) & ~15, false, true);
-        for (int j = 0; alive && j < most; ++j) {
-          const int st = j % L::kStages, next = (j + 1) % L::kStages;
-          alive = warp_wait(&bars.b.v_full[st], (j / L::kStages) & 1, dead);
-          if (!alive) break;
-          const int keys = min(kRows, klen - j * kRows);
-          if (keys % 16 != 0) {
-            // rows of other sequences up to the next 16: their weights are zero, which would not cancel NaN
-            for (int i = lane; i < (16 - keys % 16) * (kDP / 64) * 8; i += 32) {
-              const int x = i / ((16 - keys % 16) * 8), rest = i % ((16 - keys % 16) * 8);
-              *reinterpret_cast<uint4*>(vs + st * L::kTileBytes + x * kRows * 128 + keys * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_async_smem();
-            __syncwarp();
-          }
-          const int steps = (keys + 15) / 16;
-          const uint32_t v_at = smem_addr(vs + st * L::kTileBytes);
-#pragma unroll
-          for (int s = 0; s < kNQ; ++s) {
-            if (j < n[s]) {
-              alive = alive && warp_wait(&bars.b.p_full[s], j & 1, dead);
-              tc_fence_after();
-              if (alive && elect_one()) {
-                mma_over_rows<0>(tmem + kNQ * kRows + s * kDP, tmem + s * kRows + 64, v_at, pv_desc, steps, j > 0);
-                if (j + 1 == n[s]) mma_commit(&bars.b.o_full[s]);
-              }
-            }
-            if (j + 1 < n[s]) {
-              alive = alive && warp_wait(&bars.b.k_full[next], ((j + 1) / L::kStages) & 1, dead);
-              if (alive && elect_one()) scores(s, j + 1);
-            }
-          }
+        __syncwarp();
+        for (int j = 0; alive && j < it.most; ++j, ++tile) {
+          const int st = tile % kSt;
+          const uint32_t before = (tile / kSt - 1) & 1;
+          alive = tile < kSt || warp_wait(&bars.k_empty[st], before, dead);
           if (alive && elect_one()) {
-            if (j + L::kStages < most) mma_commit(&bars.b.v_empty[st]);
-            if (j + 1 + L::kStages < most) mma_commit(&bars.b.k_empty[next]);
+            mbar_expect(&bars.k_full[st], L::kTileBytes);
+#pragma unroll
+            for (int x = 0; x < kDP / 64; ++x)
+              tma_load_3d(smem_addr(ks) + st * L::kTileBytes + x * kRows * 128, &k_map, x * 64, kv, it.k0 + j * kRows, &bars.k_full[st]);
+          }
+          __syncwarp();
+          alive = alive && (tile < kSt || warp_wait(&bars.v_empty[st], before, dead));
+          if (alive && elect_one()) {
+            mbar_expect(&bars.v_full[st], L::kTileBytes);
+#pragma unroll
+            for (int x = 0; x < kDP / 64; ++x)
+              tma_load_3d(smem_addr(vs) + st * L::kTileBytes + x * kRows * 128, &v_map, x * 64, kv, it.k0 + j * kRows, &bars.v_full[st]);
           }
           __syncwarp();
         }
+        ++items;
       }
-      __syncthreads();
-      tc_fence_after();
+    } else if (warp == kNQ * 4) {
+      // ---- matrix instructions ----
+      const int d_steps = (a.D + 15) / 16;
+      const uint32_t pv_desc = mma_desc(kBf16, kRows, (a.D + 15) & ~15, false, true);
+      bool alive = true;
+      int items = 0, tile = 0;                // as the copies count them; tile: the item's first
+      int weighed[kNQ] = {}, summed[kNQ] = {};   // tiles of a stream whose weights have come, its items
+      for (int turn = 0; alive; ++turn) {
+        const int64_t index = take_item(&queue, turn, dead);
+        if (index < 0) break;
+        if (!find_item(p, index, &it) || it.most == 0) continue;
+        // scores of stream s with key tile j; keys past the sequence's end are not multiplied
+        auto scores = [&](int s, int j) {
+          const int keys = min(kRows, (it.klen - j * kRows + 15) & ~15);
+          mma_along_k<kDP / 16, kRows>(tmem + s * kRows, smem_addr(qs) + s * L::kTileBytes,
+                                       smem_addr(ks) + (tile + j) % kSt * L::kTileBytes, mma_desc(kBf16, kRows, keys, false, false),
+                                       d_steps);
+          mma_commit(&bars.s_full[s]);
+        };
+        alive = warp_wait(&bars.q_full, items & 1, dead) && warp_wait(&bars.k_full[tile % kSt], (tile / kSt) & 1, dead);
+        if (alive && elect_one()) {
+#pragma unroll
+          for (int s = 0; s < kNQ; ++s)
+            if (it.n[s] > 0) scores(s, 0);
+          mma_commit(&bars.k_empty[tile % kSt]);
+          if (it.most == 1) mma_commit(&bars.q_empty);
+        }
+        __syncwarp();
+        for (int j = 0; alive && j < it.most; ++j) {
+          const int st = (tile + j) % kSt, next = (tile + j + 1) % kSt;
+          alive = warp_wait(&bars.v_full[st], ((tile + j) / kSt) & 1, dead);
+          if (!alive) break;
+          const int keys = min(kRows, it.klen - j * kRows), steps = (keys + 15) / 16;
+          if (keys % 16 != 0) {
+            // rows of other sequences up to the next 16: their weights are zero, which would not cancel NaN
+            const int count = 16 - keys % 16;
+            for (int i = lane; i < count * 8; i += 32)
+#pragma unroll
+              for (int x = 0; x < kDP / 64; ++x)
+                *reinterpret_cast<uint4*>(vs + st * L::kTileBytes + x * kRows * 128 + keys * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+            fence_async_smem();
+            __syncwarp();
+          }
+#pragma unroll
+          for (int s = 0; s < kNQ; ++s) {
+            if (j < it.n[s]) {
+              alive = alive && warp_wait(&bars.p_full[s], weighed[s]++ & 1, dead);
+              // the stream's last sums have been read
+              if (j == 0 && summed[s] > 0) alive = alive && warp_wait(&bars.o_empty[s], (summed[s] - 1) & 1, dead);
+              tc_fence_after();
+              if (alive && elect_one()) {
+                mma_over_rows(tmem + kNQ * kRows + s * kDP, tmem + s * kRows + 64, smem_addr(vs) + st * L::kTileBytes, pv_desc, steps,
+                              j > 0);
+                if (j + 1 == it.n[s]) mma_commit(&bars.o_full[s]);
+              }
+              __syncwarp();
+              if (j + 1 == it.n[s]) ++summed[s];
+            }
+            if (j + 1 < it.n[s]) {
+              alive = alive && warp_wait(&bars.k_full[next], ((tile + j + 1) / kSt) & 1, dead);
+              if (alive && elect_one()) scores(s, j + 1);
+              __syncwarp();
+            }
+          }
+          if (alive && elect_one()) {
+            mma_commit(&bars.v_empty[st]);
+            if (j + 1 < it.most) mma_commit(&bars.k_empty[next]);
+            if (j + 2 == it.most) mma_commit(&bars.q_empty);
+          }
+          __syncwarp();
+        }
+        tile += it.most;
+        ++items;
+      }
+      // arrivals that nobody else waits for any more have to come before the barriers' memory goes
+      if (alive && items > 0) {
+        warp_wait(&bars.q_empty, (items - 1) & 1, dead);
+        for (int st = 0; st < kSt && st < tile; ++st) {
+          const int uses = (tile - st + kSt - 1) / kSt;
+          warp_wait(&bars.k_empty[st], (uses - 1) & 1, dead);
+          warp_wait(&bars.v_empty[st], (uses - 1) & 1, dead);
+        }
+      }
     }
   } else {
     take_registers<L::kSoftmaxRegs>();
-    for (bool fresh = true; !*dead && (p.listed ? list_item(p, per_slot, pair_heads, &ticket, &item) : fresh); fresh = false) {
-      const int64_t begin = item.begin;
-      const int head = item.head, klen = item.klen, qlen = item.qlen, row0 = item.row0, shift = klen - qlen;
-      // key tiles that the streams' rows see
-      int n[kNQ];
-#pragma unroll
-      for (int s = 0; s < kNQ; ++s) {
-        const int from = row0 + (pair_heads ? 0 : s * kRows);
-        const int sees = a.causal ? min(klen, min(qlen, from + kRows) + shift) : klen;
-        n[s] = from < qlen && sees > 0 ? (sees + kRows - 1) / kRows : 0;
-      }
-      const int most = kNQ == 2 ? max(n[0], n[kNQ - 1]) : n[0];
-      if (threadIdx.x == 0) {
-        if (!fresh) mbar_forget(&bars.b);
-        mbar_init(&bars.b.q_full, 1);
-        for (int i = 0; i < 2; ++i) {
-          mbar_init(&bars.b.k_full[i], 1);
-          mbar_init(&bars.b.k_empty[i], 1);
-          mbar_init(&bars.b.v_full[i], 1);
-          mbar_init(&bars.b.v_empty[i], 1);
-          mbar_init(&bars.b.s_full[i], 1);
-          mbar_init(&bars.b.p_full[i], 128);
-          mbar_init(&bars.b.o_full[i], 1);
-        }
-        fence_barrier_init();
-      }
-      __syncthreads();
-      // ---- softmax: thread = row ----
-      const int s = warp / 4;
-      const int local = (warp % 4) * 32 + lane;
-      const int row = row0 + (pair_heads ? 0 : s * kRows) + local;
-      const int tiles = n[kNQ == 2 ? s : 0];
-      const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
-      const uint32_t s_at = tmem + lanes + s * kRows, o_at = tmem + lanes + kNQ * kRows + s * kDP;
-      const int limit = row >= qlen ? 0 : (a.causal ? min(klen, row + shift + 1) : klen);   // keys that the row sees
-      const float c = a.scale * 1.4426950408889634f;
+    // ---- softmax: thread = row ----
+    const int s = warp / 4;
+    const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + s * kRows, o_at = tmem + lanes + kNQ * kRows + s * kDP;
+    const float c = a.scale * 1.4426950408889634f;
+    bool alive = true;
+    int scored = 0, summed = 0;   // tiles of the stream, and its items
+    for (int turn = 0; alive; ++turn) {
+      const int64_t index = take_item(&queue, turn, dead);
+      if (index < 0) break;
+      if (!find_item(p, index, &it)) continue;
+      const int row = it.row0 + (pair_heads ? 0 : s * kRows) + (warp % 4) * 32 + lane;
+      const int tiles = it.n[kNQ == 2 ? s : 0];
+      const int limit = row >= it.qlen ? 0 : (a.causal ? min(it.klen, row + it.klen - it.qlen + 1) : it.klen);   // keys that the row sees
       float top = -INFINITY, base = 0.f;   // the maximum in use, times c
       float sum = 0.f;
-      bool alive = true;
-      for (int j = 0; j < tiles; ++j) {
-        alive = warp_wait(&bars.b.s_full[s], j & 1, dead);
+      for (int j = 0; j < tiles; ++j, ++scored) {
+        alive = warp_wait(&bars.s_full[s], scored & 1, dead);
         if (!alive) break;
         tc_fence_after();
         const int left = limit - j * kRows;                        // of this tile, for this row
         // 32 columns each, of the tile; a warp whose rows are all behind the last computes nothing
-        const int chunks = row - lane < qlen ? min(4, (klen - j * kRows + 31) / 32) : 0;
+        const int chunks = row - lane < it.qlen ? min(4, (it.klen - j * kRows + 31) / 32) : 0;
         const bool cut = __any_sync(kFullMask, left < kRows);
         // The scores of the columns [32 from, 32 (from + kN)) into registers, masked; returns their maximum.
         auto fetch = [&](auto& x, int from) {
@@ -354,35 +419,40 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
         sum += all.x + all.y;
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&bars.b.p_full[s]);
+        mbar_arrive(&bars.p_full[s]);
       }
+      if (!alive) break;
       // ---- result ----
-      if (alive && tiles > 0) alive = warp_wait(&bars.b.o_full[s], 0, dead);
-      tc_fence_after();
-      const int h = head + (pair_heads ? s : 0);
-      if (tiles == 0 && most > 0) warp_wait(&bars.b.q_full, 0, dead);
-      if (row - lane < qlen) {   // through the queries' place: they have come, and all products with them are done
-        uint16_t* out = static_cast<uint16_t*>(a.out) + (begin + row - lane) * a.o_row + h * a.o_head;
-#pragma unroll 1
-        for (int i = 0; i < kDP; i += 32) {
-          uint32_t o[32];
-          if (tiles > 0) {
-            tmem_ld32(o, o_at + i);
-            tmem_wait_ld();
-          }
-          store_columns<kBf16>(qs + s * L::kTileBytes + warp % 4 * 2048, o, 1.f / sum, sum == 0.f || tiles == 0, out, a.o_row,
-                               qlen - row + lane, i, a.D);
-        }
+      if (tiles > 0) {
+        alive = warp_wait(&bars.o_full[s], summed++ & 1, dead);
+        if (!alive) break;
+        tc_fence_after();
       }
-      fence_async_smem();
-      if (a.lse != nullptr && row < qlen)
-        a.lse[h * a.total_q + begin + row] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
-      tc_fence_before();
-      __syncthreads();
-      tc_fence_after();
+      const int h = it.head + (pair_heads ? s : 0);
+      const bool here = row - lane < it.qlen;
+      uint16_t* out = static_cast<uint16_t*>(a.out) + (it.begin + static_cast<int64_t>(row - lane)) * a.o_row + h * a.o_head;
+#pragma unroll 1
+      for (int i = 0; i < kDP; i += 32) {
+        uint32_t o[32];
+        if (here && tiles > 0) {
+          tmem_ld32(o, o_at + i);
+          tmem_wait_ld();
+        }
+        if (tiles > 0 && i + 32 == kDP) {   // the next item's sums may come
+          tc_fence_before();
+          mbar_arrive(&bars.o_empty[s]);
+        }
+        if (here)
+          store_columns<kBf16>(stage + warp * L::kStage, o, 1.f / sum, sum == 0.f || tiles == 0, out, a.o_row, it.qlen - row + lane, i,
+                               a.D);
+      }
+      if (a.lse != nullptr && row < it.qlen)
+        a.lse[h * a.total_q + it.begin + row] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
     }
+    tc_fence_before();
   }
-  if (bars.dead) {
+  __syncthreads();
+  if (dead_word) {
     // a wait gave up: report it, and let what is in flight land before the memory is given back
     if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, B200TBE_DEV_WAIT_TIMEOUT);
     for (int i = 0; i < 1000; ++i) __nanosleep(1000);
@@ -393,7 +463,7 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
 }
 
 template <bool kBf16, int kDP, int kNQ>
-int launch(const FwdDev& p, int64_t slots, cudaStream_t stream) {
+int launch(FwdDev p, cudaStream_t stream) {
   using L = Layout<kDP, kNQ>;
   const AttnDev& a = p.a;
   CUtensorMap q, k, v;
@@ -401,23 +471,20 @@ int launch(const FwdDev& p, int64_t slots, cudaStream_t stream) {
       !rows_map(&k, kBf16, a.k, a.total_k, a.kv_heads, a.D, a.k_row, a.k_head, kRows) ||
       !rows_map(&v, kBf16, a.v, a.total_k, a.kv_heads, a.D, a.v_row, a.v_head, kRows))
     return B200TBE_ERR_UNSUPPORTED;
-  int64_t blocks = slots * (p.pair_heads && kNQ == 2 ? a.heads / 2 : a.heads);
-  if (blocks > 0x7fffff00) return p.listed ? B200TBE_ERR_UNSUPPORTED : B200TBE_ERR_TOO_LARGE;
-  if (p.listed && blocks > kNumSMs * L::kCtas) blocks = kNumSMs * L::kCtas;
+  p.slots = kNQ == 2 && !p.pair_heads ? tile_slots<2 * kRows>(a.total_q, a.batch) : tile_slots<kRows>(a.total_q, a.batch);
+  const int64_t items = p.slots * (p.pair_heads && kNQ == 2 ? a.heads / 2 : a.heads), ctas = kNumSMs * L::kCtas;
   const auto kernel = attention_fwd_kernel<kBf16, kDP, kNQ>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess ||
       cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess)
     return B200TBE_ERR_LAUNCH;
-  kernel<<<static_cast<unsigned>(blocks), L::kThreads, L::kSmem, stream>>>(p, q, k, v);
+  kernel<<<static_cast<unsigned>(items < ctas ? items : ctas), L::kThreads, L::kSmem, stream>>>(p, q, k, v);
   return launch_status();
 }
 
 template <bool kBf16>
 int forward_of(const FwdDev& p, bool two, cudaStream_t stream) {
-  const AttnDev& a = p.a;
-  const int64_t slots = two && !p.pair_heads ? tile_slots<2 * kRows>(a.total_q, a.batch) : tile_slots<kRows>(a.total_q, a.batch);
-  if (a.D <= 64) return two ? launch<kBf16, 64, 2>(p, slots, stream) : launch<kBf16, 64, 1>(p, slots, stream);
-  return two ? launch<kBf16, 128, 2>(p, slots, stream) : launch<kBf16, 128, 1>(p, slots, stream);
+  if (p.a.D <= 64) return two ? launch<kBf16, 64, 2>(p, stream) : launch<kBf16, 64, 1>(p, stream);
+  return two ? launch<kBf16, 128, 2>(p, stream) : launch<kBf16, 128, 1>(p, stream);
 }
 
 }  // namespace
@@ -432,7 +499,7 @@ bool attention_forward_fits(const AttnDev& a, int dtype) {
 }
 
 int attention_forward_tc(const AttnDev& a, const TileList* list, int dtype, int32_t* status, cudaStream_t stream) {
-  FwdDev p{a, a.group % 2 == 0, status, list != nullptr, list != nullptr ? *list : TileList{}};
+  FwdDev p{a, a.group % 2 == 0, status, list != nullptr, 0, list != nullptr ? *list : TileList{}};
   // Two query tiles a CTA read keys and values once for both and keep the tensor cores busy under the softmax.
   // Sequences so short that the second tile would mostly be empty, and tiles off a list, take one tile, and two
   // CTAs a SM.
