@@ -22,8 +22,8 @@ constexpr int kRows = 128;   // queries of a tile, keys of a tile
 constexpr int kParts = 4;                       // warpgroups that share a tile's columns, 32 each
 constexpr int kThreads = kParts * 128 + 128;
 constexpr int kIssue = kParts * 4, kCopy = kIssue + 1, kStats = kIssue + 2;   // warps
-// registers: 96 x 640 threads are launched as 104 four times and 64 a warpgroup
-constexpr int kWeightRegs = 104, kOtherRegs = 64;
+// registers: 96 x 640 threads are launched as 112 four times and 32 a warpgroup
+constexpr int kWeightRegs = 112, kOtherRegs = 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct BwdDev {
@@ -35,41 +35,54 @@ struct BwdDev {
 template <int kDP>
 struct Layout {
   static constexpr int kTileBytes = kRows * kDP * 2;
-  static constexpr int kSmem = 6 * kTileBytes + 1024;   // two tiles that stay, two stages of two that come
+  static constexpr int kStage = 2048;   // a warp's way out for results
+  static constexpr int kDqSmem = 6 * kTileBytes + kParts * 4 * kStage + 1024;
+  static constexpr int kDkvSmem = 6 * kTileBytes + 8 * kStage + 1024;
 };
 
 struct DqBarriers {
-  uint64_t q_full, a_full, k_full[3], k_empty[3], v_full, v_empty, s_full, dp_full, s_loaded, ds_full, done;
+  uint64_t q_full, q_empty, a_full, k_full[3], k_empty[3], v_full, v_empty, s_full, dp_full, s_loaded, ds_full, done;
 };
 struct DkvBarriers {
-  uint64_t kv_full, q_full[2], q_empty[2], g_full[2], g_empty[2], s_full, dp_full, p_full, ds_full, stat_full[2], stat_empty[2], done;
+  uint64_t kv_full, kv_empty, q_full[2], q_empty[2], g_full[2], g_empty[2], s_full, dp_full, p_full, ds_full, stat_full[2],
+      stat_empty[2], done;
 };
 
 // What a tile's CTA knows.
 struct Item {
-  int64_t begin, other;
-  int first, len, other_len, head;
+  int begin, other, first, len, other_len, head;
 };
 
-// The next tile of the list: one thread takes a ticket for the CTA. false: none are left.
-template <int kHeadsOf>   // 0: tiles of queries, 1: of keys
-__device__ __forceinline__ bool next_item(const BwdDev& p, int* ticket, Item* item) {
+// Tile and head `index` of the list of tiles of queries (kOf 0) or of keys (1).
+template <int kOf>
+__device__ __forceinline__ Item item_at(const BwdDev& p, int64_t index) {
   const AttnDev& a = p.a;
-  if (threadIdx.x == 0) *ticket = atomicAdd(p.plan.tickets + kHeadsOf, 1);
-  __syncthreads();
-  const int heads = kHeadsOf == 0 ? a.heads : a.kv_heads;
-  const int t = *ticket;
-  if (t / heads >= min(p.plan.counts[kHeadsOf], kHeadsOf == 0 ? p.plan.q_room : p.plan.k_room)) return false;
-  const int2 at = (kHeadsOf == 0 ? p.plan.q_tiles : p.plan.k_tiles)[t / heads];
-  item->head = t % heads;
-  item->first = at.y * kRows;
-  const void* mine = kHeadsOf == 0 ? a.q_offsets : a.k_offsets;
-  const void* others = kHeadsOf == 0 ? a.k_offsets : a.q_offsets;
-  const int64_t total = kHeadsOf == 0 ? a.total_q : a.total_k;
-  item->begin = stretch_bound(mine, a.offset_bytes, a.batch, total, at.x);
-  item->len = static_cast<int>(stretch_bound(mine, a.offset_bytes, a.batch, total, at.x + 1) - item->begin);
-  other_rows(others, a.offset_bytes, a.batch, kHeadsOf == 0 ? a.total_k : a.total_q, at.x, &item->other, &item->other_len);
-  return true;
+  const int heads = kOf == 0 ? a.heads : a.kv_heads;
+  const int2 at = (kOf == 0 ? p.plan.q_tiles : p.plan.k_tiles)[index / heads];
+  const void* mine = kOf == 0 ? a.q_offsets : a.k_offsets;
+  const int64_t total = kOf == 0 ? a.total_q : a.total_k;
+  Item it;
+  int64_t other;
+  const int64_t begin = stretch_bound(mine, a.offset_bytes, a.batch, total, at.x);
+  other_rows(kOf == 0 ? a.k_offsets : a.q_offsets, a.offset_bytes, a.batch, kOf == 0 ? a.total_k : a.total_q, at.x, &other,
+             &it.other_len);
+  it.begin = static_cast<int>(begin);
+  it.other = static_cast<int>(other);
+  it.len = static_cast<int>(stretch_bound(mine, a.offset_bytes, a.batch, total, at.x + 1) - begin);
+  it.first = at.y * kRows;
+  it.head = static_cast<int>(index % heads);
+  return it;
+}
+
+// The next item nobody has taken, or -1; by a whole warp.
+template <int kOf>
+__device__ __forceinline__ int64_t ticket_of(const BwdDev& p) {
+  int ticket = 0;
+  if (threadIdx.x % 32 == 0) ticket = atomicAdd(p.plan.tickets + kOf, 1);
+  ticket = __shfl_sync(kFullMask, ticket, 0);
+  const int64_t all = static_cast<int64_t>(min(p.plan.counts[kOf], kOf == 0 ? p.plan.q_room : p.plan.k_room)) *
+                      (kOf == 0 ? p.a.heads : p.a.kv_heads);
+  return ticket < all ? ticket : -1;
 }
 
 // Zero rows [rows, next multiple of 16) of a tile in shared memory: rows of other sequences, which a zero weight
@@ -141,6 +154,9 @@ __device__ __forceinline__ void report(const int* dead, int32_t* status) {
 // shared memory they would be read again for every tile of keys, and its bandwidth, not the tensor cores', would bound
 // the products. The scores of the next keys are computed as soon as these are in registers, under the arithmetic on dP;
 // dQ and the next dP under the exponentials. Keys are held until dQ and come three tiles ahead, values one.
+//
+// In both kernels the items go through the CTA's roles without a common stop (while one is finished, the next one's copies
+// and first products are under way), so the barriers' phases run on over the items and every role counts for itself.
 template <bool kBf16, int kDP>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_dq_kernel(const BwdDev p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
@@ -148,140 +164,181 @@ __global__ void __launch_bounds__(kThreads, 1)
   using L = Layout<kDP>;
   extern __shared__ uint8_t raw[];
   __shared__ DqBarriers bars;
+  __shared__ Queue queue;
   __shared__ uint32_t tmem_base;
-  __shared__ int dead_word, ticket;
+  __shared__ int dead_word;
   const AttnDev& a = p.a;
   uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* gs = qs + L::kTileBytes;
   uint8_t* ks = gs + L::kTileBytes;
   uint8_t* vs = ks + 3 * L::kTileBytes;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (threadIdx.x == 0) dead_word = 0;
+  uint8_t* stage = vs + L::kTileBytes;
+  const int warp = __shfl_sync(kFullMask, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  volatile int* dead = &dead_word;
+  if (threadIdx.x == 0) {
+    mbar_init(&bars.q_full, 1);
+    mbar_init(&bars.q_empty, kParts * 128);
+    mbar_init(&bars.a_full, kParts * 128);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&bars.k_full[i], 1);
+      mbar_init(&bars.k_empty[i], 1);
+    }
+    mbar_init(&bars.v_full, 1);
+    mbar_init(&bars.v_empty, 1);
+    mbar_init(&bars.s_full, 1);
+    mbar_init(&bars.dp_full, 1);
+    mbar_init(&bars.s_loaded, kParts * 128);
+    mbar_init(&bars.ds_full, kParts * 128);
+    mbar_init(&bars.done, 1);
+    queue_init(&queue, kParts * 4 + 1);
+    dead_word = 0;
+    fence_barrier_init();
+  }
   if (warp == kIssue) tmem_alloc(&tmem_base, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base, dp_at = tmem + kRows, dq_at = tmem + 2 * kRows, q_at = dq_at + kDP, g_at = q_at + kDP / 2;
-  volatile int* dead = &dead_word;
+  // tiles of keys that an item's queries see
+  auto tiles_of = [&](const Item& it) {
+    const int sees = a.causal ? min(it.other_len, min(it.len, it.first + kRows) + it.other_len - it.len) : it.other_len;
+    return sees > 0 ? (sees + kRows - 1) / kRows : 0;
+  };
 
-  Item it;
   if (warp >= kIssue) {
     give_registers<kOtherRegs>();
-    while (!*dead && next_item<0>(p, &ticket, &it)) {
-      const int kv = it.head / a.group, shift = it.other_len - it.len, klen = it.other_len;
-      const int sees = a.causal ? min(klen, min(it.len, it.first + kRows) + shift) : klen;
-      const int n = sees > 0 ? (sees + kRows - 1) / kRows : 0;
-      __syncthreads();   // the barriers are set up
-      if (warp == kCopy) {
-        // ---- copies ----
-        if (lane == 0 && n > 0) {
+    if (warp == kCopy) {
+      // ---- copies ----
+      bool alive = true;
+      int items = 0, tile = 0;   // with products, and their tiles
+      for (int turn = 0; alive; ++turn) {
+        const int64_t index = ticket_of<0>(p);
+        alive = put_item(&queue, turn, index, dead);
+        if (index < 0 || !alive) break;
+        const Item it = item_at<0>(p, index);
+        const int n = tiles_of(it), kv = it.head / a.group;
+        if (n == 0) continue;
+        alive = items == 0 || warp_wait(&bars.q_empty, (items - 1) & 1, dead);
+        if (alive && elect_one()) {
           mbar_expect(&bars.q_full, 2 * L::kTileBytes);
-          load_tile<kDP>(qs, &q_map, it.head, static_cast<int>(it.begin) + it.first, &bars.q_full);
-          load_tile<kDP>(gs, &g_map, it.head, static_cast<int>(it.begin) + it.first, &bars.q_full);
-          for (int j = 0; j < n; ++j) {
-            const int st = j % 3, row = static_cast<int>(it.other) + j * kRows;
-            if (j >= 3 && !mbar_wait(&bars.k_empty[st], (j / 3 - 1) & 1, dead)) break;
+          load_tile<kDP>(qs, &q_map, it.head, it.begin + it.first, &bars.q_full);
+          load_tile<kDP>(gs, &g_map, it.head, it.begin + it.first, &bars.q_full);
+        }
+        __syncwarp();
+        for (int j = 0; alive && j < n; ++j, ++tile) {
+          const int st = tile % 3, row = it.other + j * kRows;
+          alive = tile < 3 || warp_wait(&bars.k_empty[st], (tile / 3 - 1) & 1, dead);
+          if (alive && elect_one()) {
             mbar_expect(&bars.k_full[st], L::kTileBytes);
             load_tile<kDP>(ks + st * L::kTileBytes, &k_map, kv, row, &bars.k_full[st]);
-            if (j >= 1 && !mbar_wait(&bars.v_empty, (j - 1) & 1, dead)) break;
+          }
+          __syncwarp();
+          alive = alive && (tile < 1 || warp_wait(&bars.v_empty, (tile - 1) & 1, dead));
+          if (alive && elect_one()) {
             mbar_expect(&bars.v_full, L::kTileBytes);
             load_tile<kDP>(vs, &v_map, kv, row, &bars.v_full);
           }
+          __syncwarp();
         }
-      } else if (warp == kIssue && n > 0) {
-        // ---- matrix instructions ----
-        const int d_steps = (a.D + 15) / 16;
-        const uint32_t dq_desc = mma_desc(kBf16, kRows, (a.D + 15) & ~15, false, true);
-        auto keys_of = [&](int j) { return min(kRows, klen - j * kRows); };
+        ++items;
+      }
+    } else if (warp == kIssue) {
+      // ---- matrix instructions ----
+      const int d_steps = (a.D + 15) / 16;
+      const uint32_t dq_desc = mma_desc(kBf16, kRows, (a.D + 15) & ~15, false, true);
+      bool alive = true;
+      int items = 0, tile = 0;   // tile: the item's first
+      for (int turn = 0; alive; ++turn) {
+        const int64_t index = take_item(&queue, turn, dead);
+        if (index < 0) break;
+        const Item it = item_at<0>(p, index);
+        const int n = tiles_of(it);
+        if (n == 0) continue;
+        auto keys_of = [&](int j) { return min(kRows, it.other_len - j * kRows); };
         auto scores = [&](int j) {   // whole warp
-          const int st = j % 3, keys = keys_of(j);
-          uint8_t* tile = ks + st * L::kTileBytes;
-          if (!warp_wait(&bars.k_full[st], (j / 3) & 1, dead)) return false;
-          if (keys % 16 != 0) zero_tail<kDP>(tile, keys);
-          if (j > 0 && !warp_wait(&bars.s_loaded, (j - 1) & 1, dead)) return false;
+          const int of = tile + j, keys = keys_of(j);
+          uint8_t* at = ks + of % 3 * L::kTileBytes;
+          if (!warp_wait(&bars.k_full[of % 3], (of / 3) & 1, dead)) return false;
+          if (keys % 16 != 0) zero_tail<kDP>(at, keys);
+          if (of > 0 && !warp_wait(&bars.s_loaded, (of - 1) & 1, dead)) return false;
           tc_fence_after();
           if (elect_one()) {
-            mma_along_k_ts<kDP / 16, kRows>(tmem, q_at, smem_addr(tile), mma_desc(kBf16, kRows, (keys + 15) & ~15, false, false), d_steps);
+            mma_along_k_ts<kDP / 16, kRows>(tmem, q_at, smem_addr(at), mma_desc(kBf16, kRows, (keys + 15) & ~15, false, false), d_steps);
             mma_commit(&bars.s_full);
           }
           __syncwarp();
           return true;
         };
         auto d_weights = [&](int j) {
-          if (!warp_wait(&bars.v_full, j & 1, dead)) return false;
+          if (!warp_wait(&bars.v_full, (tile + j) & 1, dead)) return false;
           if (elect_one()) {
             mma_along_k_ts<kDP / 16, kRows>(dp_at, g_at, smem_addr(vs), mma_desc(kBf16, kRows, (keys_of(j) + 15) & ~15, false, false),
                                             d_steps);
             mma_commit(&bars.dp_full);
-            if (j + 1 < n) mma_commit(&bars.v_empty);
+            mma_commit(&bars.v_empty);
           }
           __syncwarp();
           return true;
         };
-        bool alive = warp_wait(&bars.a_full, 0, dead);
+        alive = warp_wait(&bars.a_full, items & 1, dead);
         tc_fence_after();
         alive = alive && scores(0) && d_weights(0);
         for (int j = 0; alive && j < n; ++j) {
           if (j + 1 < n) alive = scores(j + 1);
-          alive = alive && warp_wait(&bars.ds_full, j & 1, dead);
+          alive = alive && warp_wait(&bars.ds_full, (tile + j) & 1, dead);
           tc_fence_after();
           if (alive && elect_one()) {
-            mma_over_rows<16, 2>(dq_at, dp_at, smem_addr(ks + j % 3 * L::kTileBytes), dq_desc, (keys_of(j) + 15) / 16, j > 0);
-            if (j + 3 < n) mma_commit(&bars.k_empty[j % 3]);
+            mma_over_rows<16, 2>(dq_at, dp_at, smem_addr(ks) + (tile + j) % 3 * L::kTileBytes, dq_desc, (keys_of(j) + 15) / 16, j > 0);
+            mma_commit(&bars.k_empty[(tile + j) % 3]);
             if (j + 1 == n) mma_commit(&bars.done);
           }
           __syncwarp();
           if (j + 1 < n) alive = alive && d_weights(j + 1);
         }
+        tile += n;
+        ++items;
       }
-      __syncthreads();
-      tc_fence_after();
+      // arrivals that nobody else waits for any more have to come before the barriers' memory goes
+      if (alive && tile > 0) {
+        warp_wait(&bars.v_empty, (tile - 1) & 1, dead);
+        for (int st = 0; st < 3 && st < tile; ++st) warp_wait(&bars.k_empty[st], ((tile - st + 2) / 3 - 1) & 1, dead);
+      }
     }
   } else {
     take_registers<kWeightRegs>();
-    for (bool fresh = true; !*dead && next_item<0>(p, &ticket, &it); fresh = false) {
-      const int shift = it.other_len - it.len, klen = it.other_len;
-      const int sees = a.causal ? min(klen, min(it.len, it.first + kRows) + shift) : klen;
-      const int n = sees > 0 ? (sees + kRows - 1) / kRows : 0;
-      if (threadIdx.x == 0) {
-        if (!fresh) mbar_forget(&bars);
-        mbar_init(&bars.q_full, 1);
-        mbar_init(&bars.a_full, kParts * 128);
-        for (int i = 0; i < 3; ++i) {
-          mbar_init(&bars.k_full[i], 1);
-          mbar_init(&bars.k_empty[i], 1);
-        }
-        mbar_init(&bars.v_full, 1);
-        mbar_init(&bars.v_empty, 1);
-        mbar_init(&bars.s_full, 1);
-        mbar_init(&bars.dp_full, 1);
-        mbar_init(&bars.s_loaded, kParts * 128);
-        mbar_init(&bars.ds_full, kParts * 128);
-        mbar_init(&bars.done, 1);
-        fence_barrier_init();
-      }
-      __syncthreads();
-      // ---- weights: a row and 32 columns a thread ----
-      const int part = warp / 4, local = (warp % 4) * 32 + lane, row = it.first + local;
-      const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
-      const int limit = row >= it.len ? 0 : (a.causal ? min(klen, row + shift + 1) : klen);
+    // ---- weights: a row and 32 columns a thread ----
+    const int part = warp / 4, local = (warp % 4) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + part * 32, ds_at = dp_at + lanes + part * 32;
+    const float c = a.scale * kLog2e;
+    const uint64_t c2 = pair(c, c);
+    bool alive = true;
+    int items = 0, tile = 0;
+    // The queries' rows by two warpgroups, dO's by the others, once the last item's products with theirs are done.
+    auto bring = [&]() {
+      if (!warp_wait(&bars.q_full, items & 1, dead)) return false;
+      if (part % 2 < kDP / 64) copy_row((part < 2 ? q_at : g_at) + lanes + part % 2 * 32, (part < 2 ? qs : gs) + part % 2 * kRows * 128, local);
+      tc_fence_before();
+      mbar_arrive(&bars.a_full);
+      mbar_arrive(&bars.q_empty);
+      return true;
+    };
+    int64_t index = take_item(&queue, 0, dead);
+    bool brought = false;
+    for (int turn = 1; index >= 0; ++turn) {
+      const Item it = item_at<0>(p, index);
+      const int n = tiles_of(it), row = it.first + local, klen = it.other_len;
+      const int limit = row >= it.len ? 0 : (a.causal ? min(klen, row + klen - it.len + 1) : klen);
       float lse2 = 0.f, delta = 0.f;
       if (row < it.len) {
         lse2 = a.lse[it.head * a.total_q + it.begin + row] * kLog2e;
         delta = a.delta[it.head * a.total_q + it.begin + row];
         if (lse2 == -INFINITY) lse2 = INFINITY;
       }
-      const float c = a.scale * kLog2e;
-      const uint64_t c2 = pair(c, c), minus_delta = pair(-delta, -delta);
-      const uint32_t s_at = tmem + lanes + part * 32, ds_at = dp_at + lanes + part * 32;
-      bool alive = n == 0 || warp_wait(&bars.q_full, 0, dead);
-      if (alive && n > 0) {   // the queries' rows by two warpgroups, dO's by the others
-        if (part % 2 < kDP / 64) copy_row((part < 2 ? q_at : g_at) + lanes + part % 2 * 32, (part < 2 ? qs : gs) + part % 2 * kRows * 128, local);
-        tc_fence_before();
-        mbar_arrive(&bars.a_full);
-      }
-      for (int j = 0; alive && j < n; ++j) {
-        alive = warp_wait(&bars.s_full, j & 1, dead);
+      const uint64_t minus_delta = pair(-delta, -delta);
+      if (n > 0 && !brought) alive = bring();
+      for (int j = 0; alive && j < n; ++j, ++tile) {
+        alive = warp_wait(&bars.s_full, tile & 1, dead);
         if (!alive) break;
         tc_fence_after();
         const bool any = row - lane < it.len && klen - j * kRows - part * 32 > 0;   // rows and columns of the sequence here
@@ -292,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         mbar_arrive(&bars.s_loaded);
         if (any) exponentials(s, c2, pair(-lse2, -lse2));
-        alive = warp_wait(&bars.dp_full, j & 1, dead);
+        alive = warp_wait(&bars.dp_full, tile & 1, dead);
         if (!alive) break;
         tc_fence_after();
         if (any) {
@@ -315,19 +372,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         mbar_arrive(&bars.ds_full);
       }
-      if (alive && n > 0) alive = warp_wait(&bars.done, 0, dead);
+      if (alive && n > 0) alive = warp_wait(&bars.done, items++ & 1, dead);
+      if (!alive) break;
       tc_fence_after();
+      // the next item's operands before this one's results, so that its first products run under the stores; dQ is
+      // written again only after the next dS, which this warp is then still to bring
+      index = take_item(&queue, turn, dead);
+      brought = index >= 0 && tiles_of(item_at<0>(p, index)) > 0;
+      if (brought) alive = bring();
+      if (!alive) break;
       if (part < kDP / 32)
-        store_rows<kBf16>(qs + warp * 2048, static_cast<uint16_t*>(a.dq) + (it.begin + row - lane) * a.dq_row + it.head * a.dq_head,
+        store_rows<kBf16>(stage + warp * L::kStage, static_cast<uint16_t*>(a.dq) + (it.begin + static_cast<int64_t>(row - lane)) * a.dq_row + it.head * a.dq_head,
                           a.dq_row, dq_at + lanes, part * 32, a.D, a.scale, n > 0, it.len - row + lane);
-      fence_async_smem();
-      tc_fence_before();
-      __syncthreads();
-      tc_fence_after();
     }
+    tc_fence_before();
   }
+  __syncthreads();
   report(&dead_word, p.status);
   __syncthreads();
+  tc_fence_after();
   if (warp == kIssue) tmem_free(tmem, 512);
 }
 
@@ -340,55 +403,101 @@ __global__ void __launch_bounds__(kThreads, 1)
   using L = Layout<kDP>;
   extern __shared__ uint8_t raw[];
   __shared__ DkvBarriers bars;
+  __shared__ Queue queue;
   __shared__ uint32_t tmem_base;
-  __shared__ int dead_word, ticket;
+  __shared__ int dead_word;
   __shared__ __align__(16) float stats[2][2][kRows];   // [stage][lse log2 e, delta][query]
   const AttnDev& a = p.a;
   uint8_t* ks = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* vs = ks + L::kTileBytes;
   uint8_t* qs = vs + L::kTileBytes;
   uint8_t* gs = qs + 2 * L::kTileBytes;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (threadIdx.x == 0) dead_word = 0;
+  uint8_t* stage = gs + 2 * L::kTileBytes;
+  const int warp = __shfl_sync(kFullMask, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  volatile int* dead = &dead_word;
+  if (threadIdx.x == 0) {
+    mbar_init(&bars.kv_full, 1);
+    mbar_init(&bars.kv_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.q_full[i], 1);
+      mbar_init(&bars.q_empty[i], 1);
+      mbar_init(&bars.g_full[i], 1);
+      mbar_init(&bars.g_empty[i], 1);
+      mbar_init(&bars.stat_full[i], 32);
+      mbar_init(&bars.stat_empty[i], kParts * 128);
+    }
+    mbar_init(&bars.s_full, 1);
+    mbar_init(&bars.dp_full, 1);
+    mbar_init(&bars.p_full, kParts * 128);
+    mbar_init(&bars.ds_full, kParts * 128);
+    mbar_init(&bars.done, 1);
+    queue_init(&queue, kParts * 4 + 2);
+    dead_word = 0;
+    fence_barrier_init();
+  }
   if (warp == kIssue) tmem_alloc(&tmem_base, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base, dp_at = tmem + kRows, dv_at = dp_at + kRows, dk_at = dv_at + kDP;
-  volatile int* dead = &dead_word;
+  // the first tile of queries with one that sees a key of the item, and how many there are from it on, of one head
+  auto from_of = [&](const Item& it) { return a.causal ? max(0, it.first - (it.len - it.other_len)) / kRows : 0; };
+  auto per_head_of = [&](const Item& it) { return max(0, (it.other_len + kRows - 1) / kRows - from_of(it)); };
 
-  Item it;
   if (warp >= kIssue) {
     give_registers<kOtherRegs>();
-    while (!*dead && next_item<1>(p, &ticket, &it)) {
-      const int shift = it.len - it.other_len, qlen = it.other_len, head0 = it.head * a.group;
-      const int from = a.causal ? max(0, it.first - shift) / kRows : 0;   // first tile with a query that sees a key of this one
-      const int per_head = max(0, (qlen + kRows - 1) / kRows - from), n = per_head * a.group;
-      __syncthreads();   // the barriers are set up
-      if (warp == kCopy) {
-        // ---- copies ----
-        if (lane == 0 && n > 0) {
+    if (warp == kCopy) {
+      // ---- copies ----
+      bool alive = true;
+      int items = 0, tile = 0;   // with products, and their tiles of queries
+      for (int turn = 0; alive; ++turn) {
+        const int64_t index = ticket_of<1>(p);
+        alive = put_item(&queue, turn, index, dead);
+        if (index < 0 || !alive) break;
+        const Item it = item_at<1>(p, index);
+        const int from = from_of(it), per_head = per_head_of(it), n = per_head * a.group;
+        if (n == 0) continue;
+        alive = items == 0 || warp_wait(&bars.kv_empty, (items - 1) & 1, dead);
+        if (alive && elect_one()) {
           mbar_expect(&bars.kv_full, 2 * L::kTileBytes);
-          load_tile<kDP>(ks, &k_map, it.head, static_cast<int>(it.begin) + it.first, &bars.kv_full);
-          load_tile<kDP>(vs, &v_map, it.head, static_cast<int>(it.begin) + it.first, &bars.kv_full);
-          for (int j = 0; j < n; ++j) {
-            const int st = j & 1, row = static_cast<int>(it.other) + (from + j % per_head) * kRows, head = head0 + j / per_head;
-            // q, wanted first, apart from dO: both take longer than the arithmetic that hides them
-            if (j >= 2 && !mbar_wait(&bars.q_empty[st], (j / 2 - 1) & 1, dead)) break;
+          load_tile<kDP>(ks, &k_map, it.head, it.begin + it.first, &bars.kv_full);
+          load_tile<kDP>(vs, &v_map, it.head, it.begin + it.first, &bars.kv_full);
+        }
+        __syncwarp();
+        for (int j = 0; alive && j < n; ++j, ++tile) {
+          const int st = tile & 1, row = it.other + (from + j % per_head) * kRows, head = it.head * a.group + j / per_head;
+          const uint32_t before = (tile / 2 - 1) & 1;
+          // q, wanted first, apart from dO: both take longer than the arithmetic that hides them
+          alive = tile < 2 || warp_wait(&bars.q_empty[st], before, dead);
+          if (alive && elect_one()) {
             mbar_expect(&bars.q_full[st], L::kTileBytes);
             load_tile<kDP>(qs + st * L::kTileBytes, &q_map, head, row, &bars.q_full[st]);
-            if (j >= 2 && !mbar_wait(&bars.g_empty[st], (j / 2 - 1) & 1, dead)) break;
+          }
+          __syncwarp();
+          alive = alive && (tile < 2 || warp_wait(&bars.g_empty[st], before, dead));
+          if (alive && elect_one()) {
             mbar_expect(&bars.g_full[st], L::kTileBytes);
             load_tile<kDP>(gs + st * L::kTileBytes, &g_map, head, row, &bars.g_full[st]);
           }
+          __syncwarp();
         }
-      } else if (warp == kStats) {
-        // ---- the queries' log-sums and deltas ----
-        for (int j = 0; j < n; ++j) {
-          const int st = j & 1, i0 = (from + j % per_head) * kRows, head = head0 + j / per_head;
-          if (j >= 2 && !warp_wait(&bars.stat_empty[st], (j / 2 - 1) & 1, dead)) break;
+        ++items;
+      }
+    } else if (warp == kStats) {
+      // ---- the queries' log-sums and deltas ----
+      bool alive = true;
+      int tile = 0;
+      for (int turn = 0; alive; ++turn) {
+        const int64_t index = take_item(&queue, turn, dead);
+        if (index < 0) break;
+        const Item it = item_at<1>(p, index);
+        const int from = from_of(it), per_head = per_head_of(it), n = per_head * a.group;
+        for (int j = 0; j < n; ++j, ++tile) {
+          const int st = tile & 1, i0 = (from + j % per_head) * kRows, head = it.head * a.group + j / per_head;
+          alive = tile < 2 || warp_wait(&bars.stat_empty[st], (tile / 2 - 1) & 1, dead);
+          if (!alive) break;
           for (int e = lane; e < kRows; e += 32) {
-            const bool in = i0 + e < qlen;
+            const bool in = i0 + e < it.other_len;
             const int64_t at = head * a.total_q + it.other + i0 + e;
             const float lse2 = in ? a.lse[at] * kLog2e : INFINITY;
             stats[st][0][e] = lse2 == -INFINITY ? INFINITY : lse2;
@@ -396,105 +505,111 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           mbar_arrive(&bars.stat_full[st]);
         }
-      } else if (warp == kIssue && n > 0) {
-        // ---- matrix instructions ----
-        const int d_steps = (a.D + 15) / 16;
-        const uint32_t k_at = smem_addr(ks), v_at = smem_addr(vs);
-        const uint32_t out_desc = mma_desc(kBf16, kRows, (a.D + 15) & ~15, false, true);
-        auto rows_of = [&](int j) { return min(kRows, qlen - (from + j % per_head) * kRows); };
+      }
+    } else if (warp == kIssue) {
+      // ---- matrix instructions ----
+      const int d_steps = (a.D + 15) / 16;
+      const uint32_t k_at = smem_addr(ks), v_at = smem_addr(vs);
+      const uint32_t out_desc = mma_desc(kBf16, kRows, (a.D + 15) & ~15, false, true);
+      bool alive = true;
+      int items = 0, tile = 0;   // tile: the item's first
+      for (int turn = 0; alive; ++turn) {
+        const int64_t index = take_item(&queue, turn, dead);
+        if (index < 0) break;
+        const Item it = item_at<1>(p, index);
+        const int from = from_of(it), per_head = per_head_of(it), n = per_head * a.group;
+        if (n == 0) continue;
+        auto rows_of = [&](int j) { return min(kRows, it.other_len - (from + j % per_head) * kRows); };
+        auto stage_of = [&](int j) { return ((tile + j) & 1) * L::kTileBytes; };
         auto arrived = [&](uint64_t* bar, uint8_t* tiles, int j) {
-          const bool ok = warp_wait(bar + (j & 1), (j / 2) & 1, dead);
-          if (ok && rows_of(j) % 16 != 0) zero_tail<kDP>(tiles + (j & 1) * L::kTileBytes, rows_of(j));
+          const bool ok = warp_wait(bar + ((tile + j) & 1), ((tile + j) / 2) & 1, dead);
+          if (ok && rows_of(j) % 16 != 0) zero_tail<kDP>(tiles + stage_of(j), rows_of(j));
           return ok;
         };
         auto scores = [&](int j) {
           if (elect_one()) {
-            mma_along_k<kDP / 16, kRows>(tmem, k_at, smem_addr(qs + (j & 1) * L::kTileBytes),
-                           mma_desc(kBf16, kRows, (rows_of(j) + 15) & ~15, false, false), d_steps);
+            mma_along_k<kDP / 16, kRows>(tmem, k_at, smem_addr(qs) + stage_of(j), mma_desc(kBf16, kRows, (rows_of(j) + 15) & ~15, false, false),
+                                         d_steps);
             mma_commit(&bars.s_full);
           }
           __syncwarp();
         };
         auto d_weights = [&](int j) {
           if (elect_one()) {
-            mma_along_k<kDP / 16, kRows>(dp_at, v_at, smem_addr(gs + (j & 1) * L::kTileBytes),
-                           mma_desc(kBf16, kRows, (rows_of(j) + 15) & ~15, false, false), d_steps);
+            mma_along_k<kDP / 16, kRows>(dp_at, v_at, smem_addr(gs) + stage_of(j), mma_desc(kBf16, kRows, (rows_of(j) + 15) & ~15, false, false),
+                                         d_steps);
             mma_commit(&bars.dp_full);
+            if (j + 1 == n) mma_commit(&bars.kv_empty);
           }
           __syncwarp();
         };
-        bool alive = warp_wait(&bars.kv_full, 0, dead) && arrived(bars.q_full, qs, 0);
+        alive = warp_wait(&bars.kv_full, items & 1, dead) && arrived(bars.q_full, qs, 0);
         if (alive) scores(0);
         alive = alive && arrived(bars.g_full, gs, 0);
         if (alive) d_weights(0);
         for (int j = 0; alive && j < n; ++j) {
           const bool more = j + 1 < n;
-          const int steps = (rows_of(j) + 15) / 16;
-          alive = warp_wait(&bars.p_full, j & 1, dead);
+          const int steps = (rows_of(j) + 15) / 16, of = tile + j;
+          alive = warp_wait(&bars.p_full, of & 1, dead);
           if (!alive) break;
           tc_fence_after();
-          if (elect_one()) mma_over_rows<16, 2>(dv_at, tmem, smem_addr(gs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
-          if (elect_one() && j + 2 < n) mma_commit(&bars.g_empty[j & 1]);
+          if (elect_one()) {
+            mma_over_rows<16, 2>(dv_at, tmem, smem_addr(gs) + stage_of(j), out_desc, steps, j > 0);
+            mma_commit(&bars.g_empty[of & 1]);
+          }
           __syncwarp();
           if (more) {
             alive = arrived(bars.q_full, qs, j + 1);
             if (!alive) break;
             scores(j + 1);
           }
-          alive = (!more || arrived(bars.g_full, gs, j + 1)) && warp_wait(&bars.ds_full, j & 1, dead);
+          alive = (!more || arrived(bars.g_full, gs, j + 1)) && warp_wait(&bars.ds_full, of & 1, dead);
           if (!alive) break;
           tc_fence_after();
           if (elect_one()) {
-            mma_over_rows<16, 2>(dk_at, dp_at, smem_addr(qs + (j & 1) * L::kTileBytes), out_desc, steps, j > 0);
-            if (j + 2 < n) mma_commit(&bars.q_empty[j & 1]);
+            mma_over_rows<16, 2>(dk_at, dp_at, smem_addr(qs) + stage_of(j), out_desc, steps, j > 0);
+            mma_commit(&bars.q_empty[of & 1]);
             if (!more) mma_commit(&bars.done);
           }
           __syncwarp();
           if (more) d_weights(j + 1);
         }
+        tile += n;
+        ++items;
       }
-      __syncthreads();
-      tc_fence_after();
+      // arrivals that nobody else waits for any more have to come before the barriers' memory goes
+      if (alive && items > 0) {
+        warp_wait(&bars.kv_empty, (items - 1) & 1, dead);
+        for (int st = 0; st < 2 && st < tile; ++st) {
+          const uint32_t last = ((tile - st + 1) / 2 - 1) & 1;
+          warp_wait(&bars.q_empty[st], last, dead);
+          warp_wait(&bars.g_empty[st], last, dead);
+        }
+      }
     }
   } else {
     take_registers<kWeightRegs>();
-    for (bool fresh = true; !*dead && next_item<1>(p, &ticket, &it); fresh = false) {
-      const int shift = it.len - it.other_len, qlen = it.other_len;
-      const int from = a.causal ? max(0, it.first - shift) / kRows : 0;   // first tile with a query that sees a key of this one
-      const int per_head = max(0, (qlen + kRows - 1) / kRows - from), n = per_head * a.group;
-      if (threadIdx.x == 0) {
-        if (!fresh) mbar_forget(&bars);
-        mbar_init(&bars.kv_full, 1);
-        for (int i = 0; i < 2; ++i) {
-          mbar_init(&bars.q_full[i], 1);
-          mbar_init(&bars.q_empty[i], 1);
-          mbar_init(&bars.g_full[i], 1);
-          mbar_init(&bars.g_empty[i], 1);
-          mbar_init(&bars.stat_full[i], 32);
-          mbar_init(&bars.stat_empty[i], kParts * 128);
-        }
-        mbar_init(&bars.s_full, 1);
-        mbar_init(&bars.dp_full, 1);
-        mbar_init(&bars.p_full, kParts * 128);
-        mbar_init(&bars.ds_full, kParts * 128);
-        mbar_init(&bars.done, 1);
-        fence_barrier_init();
-      }
-      __syncthreads();
-      // ---- weights: a key and 32 queries a thread ----
-      const int part = warp / 4, local = (warp % 4) * 32 + lane, key = it.first + local;
-      const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
-      const uint64_t c2 = pair(a.scale * kLog2e, a.scale * kLog2e);
-      const uint32_t s_at = tmem + lanes + part * 32, ds_at = dp_at + lanes + part * 32;
-      bool alive = true;
-      for (int j = 0; j < n; ++j) {
-        const int st = j & 1, i0 = (from + j % per_head) * kRows + part * 32;
-        alive = warp_wait(&bars.stat_full[st], (j / 2) & 1, dead) && warp_wait(&bars.s_full, j & 1, dead);
+    // ---- weights: a key and 32 queries a thread ----
+    const int part = warp / 4, local = (warp % 4) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + part * 32, ds_at = dp_at + lanes + part * 32;
+    const uint64_t c2 = pair(a.scale * kLog2e, a.scale * kLog2e);
+    bool alive = true;
+    int items = 0, tile = 0;
+    for (int turn = 0; alive; ++turn) {
+      const int64_t index = take_item(&queue, turn, dead);
+      if (index < 0) break;
+      const Item it = item_at<1>(p, index);
+      const int from = from_of(it), per_head = per_head_of(it), n = per_head * a.group;
+      const int key = it.first + local, shift = it.len - it.other_len;
+      for (int j = 0; j < n; ++j, ++tile) {
+        const int st = tile & 1, i0 = (from + j % per_head) * kRows + part * 32;
+        alive = warp_wait(&bars.stat_full[st], (tile / 2) & 1, dead) && warp_wait(&bars.s_full, tile & 1, dead);
         if (!alive) break;
         tc_fence_after();
-        const bool any = key - lane < it.len && qlen - i0 > 0;   // rows and columns of the sequence here
+        const bool any = key - lane < it.len && it.other_len - i0 > 0;   // rows and columns of the sequence here
         // columns [low, high) are queries of the sequence that see the key
-        const int low = a.causal ? key - shift - i0 : 0, high = qlen - i0;
+        const int low = a.causal ? key - shift - i0 : 0, high = it.other_len - i0;
         const bool cut = __any_sync(kFullMask, low > 0 || high < 32);
         uint32_t s[32], w[16];
         if (any) {
@@ -517,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&bars.p_full);
-        alive = warp_wait(&bars.dp_full, j & 1, dead);
+        alive = warp_wait(&bars.dp_full, tile & 1, dead);
         if (!alive) break;
         tc_fence_after();
         if (any) {
@@ -545,24 +660,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&bars.ds_full);
         mbar_arrive(&bars.stat_empty[st]);
       }
-      if (alive && n > 0) alive = warp_wait(&bars.done, 0, dead);
+      if (alive && n > 0) alive = warp_wait(&bars.done, items++ & 1, dead);
+      if (!alive) break;
       tc_fence_after();
-      const bool first = part < 2;   // dV by two warpgroups, dK by the others
-      const int64_t stride = first ? a.dv_row : a.dk_row;
-      uint16_t* out = static_cast<uint16_t*>(first ? a.dv : a.dk) + (it.begin + key - lane) * stride +
-                      it.head * (first ? a.dv_head : a.dk_head);
+      // dV and dK are written again only after the next P and dS, which this warp is then still to bring
+      if (part % 2 == 0) {   // dV by one warpgroup, dK by another: shared memory has no room for four ways out
+        const bool first = part == 0;
+        const int64_t stride = first ? a.dv_row : a.dk_row;
+        uint16_t* out = static_cast<uint16_t*>(first ? a.dv : a.dk) + (it.begin + static_cast<int64_t>(key - lane)) * stride +
+                        it.head * (first ? a.dv_head : a.dk_head);
 #pragma unroll 1
-      for (int i = part % 2 * 32; i < kDP; i += 64)
-        store_rows<kBf16>(ks + warp * 2048, out, stride, (first ? dv_at : dk_at) + lanes, i, a.D, first ? 1.f : a.scale, n > 0,
-                          it.len - key + lane);
-      fence_async_smem();
+        for (int i = 0; i < kDP; i += 32)
+          store_rows<kBf16>(stage + (part / 2 * 4 + warp % 4) * L::kStage, out, stride, (first ? dv_at : dk_at) + lanes, i, a.D,
+                            first ? 1.f : a.scale, n > 0, it.len - key + lane);
+      }
       tc_fence_before();
-      __syncthreads();
-      tc_fence_after();
     }
   }
+  __syncthreads();
   report(&dead_word, p.status);
   __syncthreads();
+  tc_fence_after();
   if (warp == kIssue) tmem_free(tmem, 512);
 }
 
@@ -581,13 +699,13 @@ int launch(const BwdDev& p, cudaStream_t stream) {
   if (q_tiles > 0x7fffff00 || k_tiles > 0x7fffff00) return B200TBE_ERR_UNSUPPORTED;   // tickets are 32-bit
   const auto dq = attention_dq_kernel<kBf16, kDP>;
   const auto dkv = attention_dkv_kernel<kBf16, kDP>;
-  if (cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess ||
-      cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess)
+  if (cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDqSmem) != cudaSuccess ||
+      cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDkvSmem) != cudaSuccess)
     return B200TBE_ERR_LAUNCH;
-  dkv<<<static_cast<unsigned>(k_tiles < kNumSMs ? k_tiles : kNumSMs), kThreads, L::kSmem, stream>>>(p, q, k, v, g);
+  dkv<<<static_cast<unsigned>(k_tiles < kNumSMs ? k_tiles : kNumSMs), kThreads, L::kDkvSmem, stream>>>(p, q, k, v, g);
   const int st = launch_status();
   if (st != B200TBE_OK) return st;
-  dq<<<static_cast<unsigned>(q_tiles < kNumSMs ? q_tiles : kNumSMs), kThreads, L::kSmem, stream>>>(p, q, k, v, g);
+  dq<<<static_cast<unsigned>(q_tiles < kNumSMs ? q_tiles : kNumSMs), kThreads, L::kDqSmem, stream>>>(p, q, k, v, g);
   return launch_status();
 }
 

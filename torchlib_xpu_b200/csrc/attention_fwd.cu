@@ -100,32 +100,6 @@ __device__ __forceinline__ bool find_item(const FwdDev& p, int64_t index, Item<k
   return true;
 }
 
-// The numbers of the CTA's items, handed from the warp that copies to the others, a few ahead; -1 ends them.
-struct Queue {
-  static constexpr int kRoom = 4;
-  uint64_t full[kRoom], empty[kRoom];
-  int64_t index[kRoom];
-};
-__device__ __forceinline__ bool put_item(Queue* queue, int turn, int64_t index, volatile int* dead) {
-  const int at = turn % Queue::kRoom;
-  if (turn >= Queue::kRoom && !warp_wait(&queue->empty[at], (turn / Queue::kRoom - 1) & 1, dead)) return false;
-  if (threadIdx.x % 32 == 0) {
-    queue->index[at] = index;
-    mbar_arrive(&queue->full[at]);
-  }
-  __syncwarp();
-  return true;
-}
-// the turn's item, -1 after the last or when a wait gave up
-__device__ __forceinline__ int64_t take_item(Queue* queue, int turn, volatile int* dead) {
-  const int at = turn % Queue::kRoom;
-  if (!warp_wait(&queue->full[at], (turn / Queue::kRoom) & 1, dead)) return -1;
-  const int64_t index = queue->index[at];
-  __syncwarp();
-  if (threadIdx.x % 32 == 0) mbar_arrive(&queue->empty[at]);
-  return index;
-}
-
 // The CTA's items go through its roles one after the other without a common stop: while the softmax warps finish one, the
 // next one's copies and first scores are under way. So the barriers' phases run on over the items; every role counts
 // for itself what it has waited for.
@@ -161,10 +135,7 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
       mbar_init(&bars.o_full[i], 1);
       mbar_init(&bars.o_empty[i], 128);
     }
-    for (int i = 0; i < Queue::kRoom; ++i) {
-      mbar_init(&queue.full[i], 1);
-      mbar_init(&queue.empty[i], kNQ * 4 + 1);
-    }
+    queue_init(&queue, kNQ * 4 + 1);
     dead_word = 0;
     fence_barrier_init();
   }

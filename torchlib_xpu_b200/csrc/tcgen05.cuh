@@ -14,13 +14,6 @@ __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
 }
 
-// Every barrier of a block of them: the memory may be initialised again.
-template <typename Barriers>
-__device__ __forceinline__ void mbar_forget(Barriers* bars) {
-  for (unsigned i = 0; i < sizeof(Barriers) / 8; ++i)
-    asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_addr(reinterpret_cast<uint64_t*>(bars) + i)) : "memory");
-}
-
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
@@ -260,6 +253,38 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   else
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// The numbers of the CTA's items, handed from the warp that copies to the others, a few ahead; -1 ends them.
+struct Queue {
+  static constexpr int kRoom = 4;
+  uint64_t full[kRoom], empty[kRoom];
+  int64_t index[kRoom];
+};
+__device__ __forceinline__ void queue_init(Queue* queue, int takers) {
+  for (int i = 0; i < Queue::kRoom; ++i) {
+    mbar_init(&queue->full[i], 1);
+    mbar_init(&queue->empty[i], takers);
+  }
+}
+__device__ __forceinline__ bool put_item(Queue* queue, int turn, int64_t index, volatile int* dead) {
+  const int at = turn % Queue::kRoom;
+  if (turn >= Queue::kRoom && !warp_wait(&queue->empty[at], (turn / Queue::kRoom - 1) & 1, dead)) return false;
+  if (threadIdx.x % 32 == 0) {
+    queue->index[at] = index;
+    mbar_arrive(&queue->full[at]);
+  }
+  __syncwarp();
+  return true;
+}
+// the turn's item, -1 after the last or when a wait gave up
+__device__ __forceinline__ int64_t take_item(Queue* queue, int turn, volatile int* dead) {
+  const int at = turn % Queue::kRoom;
+  if (!warp_wait(&queue->full[at], (turn / Queue::kRoom) & 1, dead)) return -1;
+  const int64_t index = queue->index[at];
+  __syncwarp();
+  if (threadIdx.x % 32 == 0) mbar_arrive(&queue->empty[at]);
+  return index;
 }
 
 // 32 columns of a warp's 32 accumulator rows (a row a lane), times f, rounded, to memory: columns [col, col + 32) of the
