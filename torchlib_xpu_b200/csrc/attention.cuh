@@ -18,6 +18,7 @@ struct AttnDev {
   int32_t batch, heads, kv_heads, group, D;
   int32_t offset_bytes;
   int32_t causal;
+  int32_t fours;   // of the 32-bit kernels: operands may be read in fours of elements
   float scale;
   // backward
   const void* grad;

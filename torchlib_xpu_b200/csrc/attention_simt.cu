@@ -27,15 +27,41 @@ struct Shape {
   static constexpr int kWeights = kT * kPad;
 };
 
-// rows [first, first + kT) of one head into dst[d][row]; rows at or past `rows` and columns past D are zero
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return *reinterpret_cast<const float4*>(p);
+  } else {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    const T* e = reinterpret_cast<const T*>(&x);
+    return make_float4(to_float<T>(e[0]), to_float<T>(e[1]), to_float<T>(e[2]), to_float<T>(e[3]));
+  }
+}
+
+// rows [first, first + kT) of one head into dst[d][row]; rows at or past `rows` and columns past D are zero. Lanes
+// take consecutive rows: the stores meet no bank twice, and what a row's other lanes want next is in L1.
 template <typename T, int kDP>
-__device__ __forceinline__ void load_transposed(float* dst, const T* src, int64_t row_stride, int first, int rows, int D) {
+__device__ __forceinline__ void load_transposed(float* dst, const T* src, int64_t row_stride, int first, int rows, int D, bool fours) {
   using S = Shape<kDP>;
+  if (fours) {   // D, strides and addresses are whole fours of elements
+    constexpr int kEach = S::kT * kDP / 4 / kThreads;
+    float4 x[kEach];
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      const int i = u * kThreads + threadIdx.x, r = i % S::kT, d = i / S::kT * 4;
+      x[u] = d < D && first + r < rows ? load4(src + static_cast<int64_t>(first + r) * row_stride + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      const int i = u * kThreads + threadIdx.x, r = i % S::kT, d = i / S::kT * 4;
+      float* to = dst + d * S::kPad + r;
+      to[0] = x[u].x, to[S::kPad] = x[u].y, to[2 * S::kPad] = x[u].z, to[3 * S::kPad] = x[u].w;
+    }
+    return;
+  }
   for (int i = threadIdx.x; i < S::kT * kDP; i += kThreads) {
-    const int d = i % kDP, r = i / kDP;
-    float x = 0.f;
-    if (d < D && first + r < rows) x = to_float<T>(src[static_cast<int64_t>(first + r) * row_stride + d]);
-    dst[d * S::kPad + r] = x;
+    const int r = i % S::kT, d = i / S::kT;
+    dst[d * S::kPad + r] = d < D && first + r < rows ? to_float<T>(src[static_cast<int64_t>(first + r) * row_stride + d]) : 0.f;
   }
 }
 
@@ -67,21 +93,53 @@ __device__ __forceinline__ void accumulate(float (&acc)[Shape<kDP>::kR][Shape<kD
                                            int tx, int ty) {
   using S = Shape<kDP>;
 #pragma unroll 2
-  for (int t = 0; t < S::kT; t += 2) {
-    float a[2][S::kR];
+  for (int t = 0; t < S::kT; t += 4) {
+    float a[4][S::kR];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < S::kR; ++i) a[u][i] = w[(t + u) * S::kPad + ty * S::kR + i];
+    for (int u = 0; u < 4; ++u) {
+      const float* from = w + (t + u) * S::kPad + ty * S::kR;
+      if constexpr (S::kR == 4)
+        *reinterpret_cast<float4*>(a[u]) = *reinterpret_cast<const float4*>(from);
+      else
+        *reinterpret_cast<float2*>(a[u]) = *reinterpret_cast<const float2*>(from);
+    }
 #pragma unroll
     for (int c = 0; c < S::kC; ++c) {
-      const float2 b = *reinterpret_cast<const float2*>(y + (c * 16 + tx) * S::kPad + t);
+      const float4 b = *reinterpret_cast<const float4*>(y + (c * 16 + tx) * S::kPad + t);
 #pragma unroll
       for (int i = 0; i < S::kR; ++i) {
         acc[i][c] = fmaf(a[0][i], b.x, acc[i][c]);
         acc[i][c] = fmaf(a[1][i], b.y, acc[i][c]);
+        acc[i][c] = fmaf(a[2][i], b.z, acc[i][c]);
+        acc[i][c] = fmaf(a[3][i], b.w, acc[i][c]);
       }
     }
+  }
+}
+
+// A thread's products to shared memory, its rows (or columns) side by side.
+template <int kDP>
+__device__ __forceinline__ void store_columns_of(float* to, const float (&x)[Shape<kDP>::kR][Shape<kDP>::kR], int tx, int ty) {
+  using S = Shape<kDP>;
+#pragma unroll
+  for (int j = 0; j < S::kR; ++j) {
+    float* at = to + (tx * S::kR + j) * S::kPad + ty * S::kR;
+    if constexpr (S::kR == 4)
+      *reinterpret_cast<float4*>(at) = make_float4(x[0][j], x[1][j], x[2][j], x[3][j]);
+    else
+      *reinterpret_cast<float2*>(at) = make_float2(x[0][j], x[1][j]);
+  }
+}
+template <int kDP>
+__device__ __forceinline__ void store_rows_of(float* to, const float (&x)[Shape<kDP>::kR][Shape<kDP>::kR], int tx, int ty) {
+  using S = Shape<kDP>;
+#pragma unroll
+  for (int i = 0; i < S::kR; ++i) {
+    float* at = to + (ty * S::kR + i) * S::kPad + tx * S::kR;
+    if constexpr (S::kR == 4)
+      *reinterpret_cast<float4*>(at) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
+    else
+      *reinterpret_cast<float2*>(at) = make_float2(x[i][0], x[i][1]);
   }
 }
 
@@ -120,7 +178,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const AttnDev p) {
   const T* v = static_cast<const T*>(p.v) + t.other * p.v_row + kv * p.v_head;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const int shift = t.other_len - t.len;   // query i sees the keys up to i + shift
-  load_transposed<T, kDP>(qs, q, p.q_row, t.first, t.len, p.D);
+  load_transposed<T, kDP>(qs, q, p.q_row, t.first, t.len, p.D, p.fours);
 
   float o[S::kR][S::kC] = {};
   float top[S::kR], sum[S::kR];
@@ -129,8 +187,8 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const AttnDev p) {
   const int last = p.causal ? min(t.other_len, min(t.len, t.first + S::kT) + shift) : t.other_len;
   for (int j0 = 0; j0 < last; j0 += S::kT) {
     __syncthreads();
-    load_transposed<T, kDP>(ks, k, p.k_row, j0, t.other_len, p.D);
-    load_transposed<T, kDP>(vs, v, p.v_row, j0, t.other_len, p.D);
+    load_transposed<T, kDP>(ks, k, p.k_row, j0, t.other_len, p.D, p.fours);
+    load_transposed<T, kDP>(vs, v, p.v_row, j0, t.other_len, p.D, p.fours);
     __syncthreads();
     float s[S::kR][S::kR] = {};
     products<kDP>(s, qs, ks, tx, ty);
@@ -152,9 +210,8 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const AttnDev p) {
       float add = 0.f;
 #pragma unroll
       for (int j = 0; j < S::kR; ++j) {
-        const float e = expf(s[i][j] - base);
-        add += e;
-        ps[(tx * S::kR + j) * S::kPad + ty * S::kR + i] = e;
+        s[i][j] = expf(s[i][j] - base);
+        add += s[i][j];
       }
 #pragma unroll
       for (int w = 8; w > 0; w >>= 1) add += __shfl_xor_sync(kFullMask, add, w);
@@ -162,6 +219,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const AttnDev p) {
 #pragma unroll
       for (int c = 0; c < S::kC; ++c) o[i][c] *= keep;
     }
+    store_columns_of<kDP>(ps, s, tx, ty);
     __syncthreads();
     accumulate<kDP>(o, ps, vs, tx, ty);
   }
@@ -220,24 +278,21 @@ __global__ void __launch_bounds__(kThreads) dq_kernel(const AttnDev p) {
   const float* delta = p.delta + head * p.total_q + t.begin;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const int shift = t.other_len - t.len;
-  load_transposed<T, kDP>(qs, static_cast<const T*>(p.q) + t.begin * p.q_row + head * p.q_head, p.q_row, t.first, t.len, p.D);
+  load_transposed<T, kDP>(qs, static_cast<const T*>(p.q) + t.begin * p.q_row + head * p.q_head, p.q_row, t.first, t.len, p.D, p.fours);
   load_transposed<T, kDP>(gs, static_cast<const T*>(p.grad) + t.begin * p.g_row + head * p.g_head, p.g_row, t.first, t.len,
-                          p.D);
+                          p.D, p.fours);
   float acc[S::kR][S::kC] = {};
   const int last = p.causal ? min(t.other_len, min(t.len, t.first + S::kT) + shift) : t.other_len;
   for (int j0 = 0; j0 < last; j0 += S::kT) {
     __syncthreads();
-    load_transposed<T, kDP>(ks, k, p.k_row, j0, t.other_len, p.D);
-    load_transposed<T, kDP>(vs, v, p.v_row, j0, t.other_len, p.D);
+    load_transposed<T, kDP>(ks, k, p.k_row, j0, t.other_len, p.D, p.fours);
+    load_transposed<T, kDP>(vs, v, p.v_row, j0, t.other_len, p.D, p.fours);
     __syncthreads();
     float s[S::kR][S::kR] = {}, dp[S::kR][S::kR] = {};
     products<kDP>(s, qs, ks, tx, ty);
     products<kDP>(dp, gs, vs, tx, ty);
     weights_of<kDP>(s, dp, lse, delta, t.first, j0, t.len, t.other_len, shift, p.causal, p.scale, tx, ty);
-#pragma unroll
-    for (int i = 0; i < S::kR; ++i)
-#pragma unroll
-      for (int j = 0; j < S::kR; ++j) ws[(tx * S::kR + j) * S::kPad + ty * S::kR + i] = dp[i][j];
+    store_columns_of<kDP>(ws, dp, tx, ty);
     __syncthreads();
     accumulate<kDP>(acc, ws, ks, tx, ty);
   }
@@ -267,8 +322,8 @@ __global__ void __launch_bounds__(kThreads) dkv_kernel(const AttnDev p) {
   if (!t.ok) return;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const int shift = t.len - t.other_len;
-  load_transposed<T, kDP>(ks, static_cast<const T*>(p.k) + t.begin * p.k_row + kv * p.k_head, p.k_row, t.first, t.len, p.D);
-  load_transposed<T, kDP>(vs, static_cast<const T*>(p.v) + t.begin * p.v_row + kv * p.v_head, p.v_row, t.first, t.len, p.D);
+  load_transposed<T, kDP>(ks, static_cast<const T*>(p.k) + t.begin * p.k_row + kv * p.k_head, p.k_row, t.first, t.len, p.D, p.fours);
+  load_transposed<T, kDP>(vs, static_cast<const T*>(p.v) + t.begin * p.v_row + kv * p.v_head, p.v_row, t.first, t.len, p.D, p.fours);
   float dk[S::kR][S::kC] = {}, dv[S::kR][S::kC] = {};
   const int from = p.causal ? max(0, t.first - shift) / S::kT * S::kT : 0;   // the first query that sees a key of this tile
   for (int head = kv * p.group; head < (kv + 1) * p.group; ++head) {
@@ -278,24 +333,18 @@ __global__ void __launch_bounds__(kThreads) dkv_kernel(const AttnDev p) {
     const float* delta = p.delta + head * p.total_q + t.other;
     for (int i0 = from; i0 < t.other_len; i0 += S::kT) {
       __syncthreads();
-      load_transposed<T, kDP>(qs, q, p.q_row, i0, t.other_len, p.D);
-      load_transposed<T, kDP>(gs, g, p.g_row, i0, t.other_len, p.D);
+      load_transposed<T, kDP>(qs, q, p.q_row, i0, t.other_len, p.D, p.fours);
+      load_transposed<T, kDP>(gs, g, p.g_row, i0, t.other_len, p.D, p.fours);
       __syncthreads();
       float s[S::kR][S::kR] = {}, dp[S::kR][S::kR] = {};
       products<kDP>(s, qs, ks, tx, ty);
       products<kDP>(dp, gs, vs, tx, ty);
       weights_of<kDP>(s, dp, lse, delta, i0, t.first, t.other_len, t.len, shift, p.causal, p.scale, tx, ty);
-#pragma unroll
-      for (int i = 0; i < S::kR; ++i)
-#pragma unroll
-        for (int j = 0; j < S::kR; ++j) ws[(ty * S::kR + i) * S::kPad + tx * S::kR + j] = s[i][j];
+      store_rows_of<kDP>(ws, s, tx, ty);
       __syncthreads();
       accumulate<kDP>(dv, ws, gs, tx, ty);
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < S::kR; ++i)
-#pragma unroll
-        for (int j = 0; j < S::kR; ++j) ws[(ty * S::kR + i) * S::kPad + tx * S::kR + j] = dp[i][j];
+      store_rows_of<kDP>(ws, dp, tx, ty);
       __syncthreads();
       accumulate<kDP>(dk, ws, qs, tx, ty);
     }
@@ -342,6 +391,18 @@ int backward_as(const AttnDev& p, cudaStream_t stream) {
   return st;
 }
 
+// Whether every operand can be read in fours of elements.
+AttnDev in_fours(AttnDev p, int elem_bytes, bool backward) {
+  const uint64_t size = 4 * elem_bytes;
+  uint64_t off = (reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) % size;
+  if (backward) off |= reinterpret_cast<uintptr_t>(p.grad) % size;
+  for (int64_t x : {static_cast<int64_t>(p.D), p.q_row, p.q_head, p.k_row, p.k_head, p.v_row, p.v_head, backward ? p.g_row : 0,
+                    backward ? p.g_head : 0})
+    off |= x % 4 != 0;
+  p.fours = off == 0;
+  return p;
+}
+
 template <typename T>
 int forward_of(const AttnDev& p, cudaStream_t stream) {
   if (p.D <= 32) return forward_as<T, 32>(p, stream);
@@ -361,15 +422,17 @@ int backward_of(const AttnDev& p, cudaStream_t stream) {
 }  // namespace
 
 int attention_forward_simt(const AttnDev& p, int dtype, cudaStream_t stream) {
-  if (dtype == B200TBE_FP32) return forward_of<float>(p, stream);
-  if (dtype == B200TBE_FP16) return forward_of<__half>(p, stream);
-  return forward_of<__nv_bfloat16>(p, stream);
+  const AttnDev d = in_fours(p, dtype == B200TBE_FP32 ? 4 : 2, false);
+  if (dtype == B200TBE_FP32) return forward_of<float>(d, stream);
+  if (dtype == B200TBE_FP16) return forward_of<__half>(d, stream);
+  return forward_of<__nv_bfloat16>(d, stream);
 }
 
 int attention_backward_simt(const AttnDev& p, int dtype, cudaStream_t stream) {
-  if (dtype == B200TBE_FP32) return backward_of<float>(p, stream);
-  if (dtype == B200TBE_FP16) return backward_of<__half>(p, stream);
-  return backward_of<__nv_bfloat16>(p, stream);
+  const AttnDev d = in_fours(p, dtype == B200TBE_FP32 ? 4 : 2, true);
+  if (dtype == B200TBE_FP32) return backward_of<float>(d, stream);
+  if (dtype == B200TBE_FP16) return backward_of<__half>(d, stream);
+  return backward_of<__nv_bfloat16>(d, stream);
 }
 
 }  // namespace b200tbe
