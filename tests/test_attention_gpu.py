@@ -297,6 +297,29 @@ def test_offsets_beyond_the_rows_read_and_write_nothing_outside():
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("heads,kv,D,causal", [(4, 2, 128, True), (3, 1, 64, False), (2, 2, 40, True)])
+def test_many_tiles_for_every_cta(heads, kv, D, causal):
+    """More tiles than the GPU has CTAs, of long and short sequences mixed, so that CTAs take several after one another:
+    some sequences against the reference, and the whole a second time, bit for bit."""
+    gen = torch.Generator().manual_seed(6)
+    lengths = torch.randint(100, 700, (90,), generator=gen).tolist() + [0, 1, 1500]
+    o = _offsets(lengths)
+    q, g = (_normal((o[-1], heads, D), BF16, s) for s in (181, 182))
+    k, v = (_normal((o[-1], kv, D), BF16, s) for s in (183, 184))
+    dev = torch.tensor(o, device="cuda")
+    parts = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = attention(*parts, dev, None, causal)
+    grads = torch.autograd.grad(out, parts, g)
+    for b in (0, 17, 55, 89, 91, 92):
+        s = slice(o[b], o[b + 1])
+        one = ref.one_sequence(q[s], k[s], v[s], causal, D ** -0.5, g[s])
+        for name, x in zip(("o", "dq", "dk", "dv"), (out, *grads)):
+            ref.assert_within(x[s], one[name], one[name + "_off"], "%s of sequence %d" % (name, b))
+    again = attention(*parts, dev, None, causal)
+    assert torch.equal(out, again)
+    assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(again, parts, g)))
+
+
 def test_many_short_sequences():
     """More sequences than one search step covers, single rows among them."""
     gen = torch.Generator().manual_seed(5)

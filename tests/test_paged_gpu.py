@@ -281,6 +281,42 @@ def test_repeats_bit_for_bit():
         assert torch.equal(first, answer(q, k, v, table.cuda(), n))
 
 
+def test_two_streams_at_once():
+    """The operators on two streams at the same time, several calls deep, give what they give alone."""
+    gen = torch.Generator().manual_seed(51)
+    work = []
+    for i, (dtype, D) in enumerate(((BF16, 128), (FP16, 64))):
+        lengths = torch.randint(1, 700, (40,), generator=gen).tolist()
+        table, pages = _pages(lengths, 32, 52 + i)
+        cache = [_normal((pages, 32, 2, D), dtype, 53 + i).cuda(), _normal((pages, 32, 2, D), dtype, 55 + i).cuda()]
+        n = sum(lengths)
+        offsets = torch.tensor([0] + lengths, device="cuda").cumsum(0)
+        rows = [_normal((n, h, D), dtype, 57 + i + j).cuda() for j, h in enumerate((4, 2, 2))]
+        work.append((rows, offsets, cache, table.cuda(), torch.tensor(lengths, device="cuda"), _normal((40, 4, D), dtype, 61 + i).cuda()))
+
+    def run(rows, offsets, cache, table, lengths, q):
+        parts = [t.detach().requires_grad_() for t in rows]
+        out = attention(*parts, offsets, None, True)
+        grads = torch.autograd.grad(out, parts, torch.ones_like(out))
+        got = answer(q, *cache, table, lengths)
+        append(rows[1], rows[2], offsets, *cache, table, lengths)
+        return (out.detach(), *grads, got, answer(q, *cache, table, lengths))
+
+    want = [run(*w[:2], [c.clone() for c in w[2]], *w[3:]) for w in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    for _ in range(3):
+        got = []
+        copies = [[c.clone() for c in w[2]] for w in work]
+        torch.cuda.synchronize()
+        for stream, w, cache in zip(streams, work, copies):
+            with torch.cuda.stream(stream):
+                got.append(run(*w[:2], cache, *w[3:]))
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_many_sequences():
     gen = torch.Generator().manual_seed(45)
     lengths = torch.randint(0, 40, (1500,), generator=gen).tolist()

@@ -1011,6 +1011,8 @@ extern "C" int b200tbe_paged_attention(const b200tbe_paged_cache* cache, const v
     return B200TBE_ERR_SCRATCH;
   AnswerDev p{};
   p.c = cache_dev(cache);
+  // copies of nothing still name an address
+  if (cache->num_pages == 0) p.c.k = p.c.v = static_cast<char*>(const_cast<void*>(q));
   p.q = q, p.out = out;
   p.q_row = q_stride, p.q_head = q_head_stride, p.o_row = out_stride, p.o_head = out_head_stride;
   p.heads = heads, p.group = heads / cache->kv_heads, p.per = kHeads, p.chunks = (p.group + kHeads - 1) / kHeads;

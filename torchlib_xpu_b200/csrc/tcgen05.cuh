@@ -44,8 +44,8 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   const long long begin = clock64();
   while (!mbar_try(bar, parity)) {
     if (*dead) return false;
-    if (clock64() - begin > kWaitCycles) {
-      *dead = 1;
+    if (clock64() - begin > kWaitCycles && !mbar_try(bar, parity)) {   // looked at once more: the clock ran on while
+      *dead = 1;                                                         // another process had the GPU
       return false;
     }
   }
