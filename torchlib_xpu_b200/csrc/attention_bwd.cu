@@ -697,15 +697,13 @@ int launch(const BwdDev& p, cudaStream_t stream) {
   const int64_t q_tiles = tile_slots<kRows>(a.total_q, a.batch) * a.heads;
   const int64_t k_tiles = tile_slots<kRows>(a.total_k, a.batch) * a.kv_heads;
   if (q_tiles > 0x7fffff00 || k_tiles > 0x7fffff00) return B200TBE_ERR_UNSUPPORTED;   // tickets are 32-bit
-  const auto dq = attention_dq_kernel<kBf16, kDP>;
-  const auto dkv = attention_dkv_kernel<kBf16, kDP>;
-  if (cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDqSmem) != cudaSuccess ||
-      cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDkvSmem) != cudaSuccess)
+  if (!allow_shared_memory<attention_dq_kernel<kBf16, kDP>>(L::kDqSmem) ||
+      !allow_shared_memory<attention_dkv_kernel<kBf16, kDP>>(L::kDkvSmem))
     return B200TBE_ERR_LAUNCH;
-  dkv<<<static_cast<unsigned>(k_tiles < kNumSMs ? k_tiles : kNumSMs), kThreads, L::kDkvSmem, stream>>>(p, q, k, v, g);
+  attention_dkv_kernel<kBf16, kDP><<<static_cast<unsigned>(k_tiles < kNumSMs ? k_tiles : kNumSMs), kThreads, L::kDkvSmem, stream>>>(p, q, k, v, g);
   const int st = launch_status();
   if (st != B200TBE_OK) return st;
-  dq<<<static_cast<unsigned>(q_tiles < kNumSMs ? q_tiles : kNumSMs), kThreads, L::kDqSmem, stream>>>(p, q, k, v, g);
+  attention_dq_kernel<kBf16, kDP><<<static_cast<unsigned>(q_tiles < kNumSMs ? q_tiles : kNumSMs), kThreads, L::kDqSmem, stream>>>(p, q, k, v, g);
   return launch_status();
 }
 

@@ -445,11 +445,8 @@ int launch(FwdDev p, cudaStream_t stream) {
   p.slots = kNQ == 2 && !p.pair_heads ? tile_slots<2 * kRows>(a.total_q, a.batch) : tile_slots<kRows>(a.total_q, a.batch);
   const int64_t items = p.slots * (p.pair_heads && kNQ == 2 ? a.heads / 2 : a.heads), ctas = kNumSMs * L::kCtas;
   if (items > 0x7fff0000) return B200TBE_ERR_UNSUPPORTED;   // tickets are 32-bit
-  const auto kernel = attention_fwd_kernel<kBf16, kDP, kNQ>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess ||
-      cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess)
-    return B200TBE_ERR_LAUNCH;
-  kernel<<<static_cast<unsigned>(items < ctas ? items : ctas), L::kThreads, L::kSmem, stream>>>(p, q, k, v);
+  if (!allow_shared_memory<attention_fwd_kernel<kBf16, kDP, kNQ>>(L::kSmem)) return B200TBE_ERR_LAUNCH;
+  attention_fwd_kernel<kBf16, kDP, kNQ><<<static_cast<unsigned>(items < ctas ? items : ctas), L::kThreads, L::kSmem, stream>>>(p, q, k, v);
   return launch_status();
 }
 

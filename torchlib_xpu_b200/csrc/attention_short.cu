@@ -599,12 +599,9 @@ int launch_forward(const ShortDev& p, cudaStream_t stream) {
     return B200TBE_ERR_UNSUPPORTED;
   const int64_t blocks = (static_cast<int64_t>(a.batch) + 2) * a.heads;
   if (blocks > 0x7fff0000) return B200TBE_ERR_UNSUPPORTED;   // items are counted in 32 bits
-  const auto kernel = attention_short_fwd_kernel<kBf16, kDP>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess) return B200TBE_ERR_LAUNCH;
-  // all of the SM's shared memory, or fewer CTAs fit than the launch bounds promise
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess) return B200TBE_ERR_LAUNCH;
+  if (!allow_shared_memory<attention_short_fwd_kernel<kBf16, kDP>>(L::kSmem)) return B200TBE_ERR_LAUNCH;
   const int64_t ctas = kNumSMs * L::kCtas;
-  kernel<<<static_cast<unsigned>(blocks < ctas ? blocks : ctas), 128, L::kSmem, stream>>>(p, q, k, v);
+  attention_short_fwd_kernel<kBf16, kDP><<<static_cast<unsigned>(blocks < ctas ? blocks : ctas), 128, L::kSmem, stream>>>(p, q, k, v);
   return launch_status();
 }
 
@@ -620,12 +617,9 @@ int launch_backward(const ShortDev& p, cudaStream_t stream) {
     return B200TBE_ERR_UNSUPPORTED;
   const int64_t blocks = (static_cast<int64_t>(a.batch) + 2) * a.kv_heads;
   if (blocks > 0x7fff0000) return B200TBE_ERR_UNSUPPORTED;   // items are counted in 32 bits
-  const auto kernel = attention_short_bwd_kernel<kBf16, kDP, kAlone>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess) return B200TBE_ERR_LAUNCH;
-  // all of the SM's shared memory, or fewer CTAs fit than the launch bounds promise
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess) return B200TBE_ERR_LAUNCH;
+  if (!allow_shared_memory<attention_short_bwd_kernel<kBf16, kDP, kAlone>>(L::kSmem)) return B200TBE_ERR_LAUNCH;
   const int64_t ctas = kNumSMs * L::kCtas;
-  kernel<<<static_cast<unsigned>(blocks < ctas ? blocks : ctas), 256, L::kSmem, stream>>>(p, q, k, v, g);
+  attention_short_bwd_kernel<kBf16, kDP, kAlone><<<static_cast<unsigned>(blocks < ctas ? blocks : ctas), 256, L::kSmem, stream>>>(p, q, k, v, g);
   return launch_status();
 }
 

@@ -364,19 +364,18 @@ __global__ void __launch_bounds__(kThreads) dkv_kernel(const AttnDev p) {
   }
 }
 
-template <typename K>
-int launch(K kernel, int64_t blocks, int floats, const AttnDev& p, cudaStream_t stream) {
+template <auto kKernel>
+int launch(int64_t blocks, int floats, const AttnDev& p, cudaStream_t stream) {
   if (blocks > 0x7fffffff) return B200TBE_ERR_TOO_LARGE;
   const int bytes = floats * 4;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return B200TBE_ERR_LAUNCH;
-  kernel<<<static_cast<unsigned>(blocks), kThreads, bytes, stream>>>(p);
+  if (!allow_shared_memory<kKernel>(bytes)) return B200TBE_ERR_LAUNCH;
+  kKernel<<<static_cast<unsigned>(blocks), kThreads, bytes, stream>>>(p);
   return launch_status();
 }
 
 template <typename T, int kDP>
 int forward_as(const AttnDev& p, cudaStream_t stream) {
-  return launch(forward_kernel<T, kDP>, tile_slots<Shape<kDP>::kT>(p.total_q, p.batch) * p.heads,
+  return launch<forward_kernel<T, kDP>>(tile_slots<Shape<kDP>::kT>(p.total_q, p.batch) * p.heads,
                 3 * Shape<kDP>::kOperand + Shape<kDP>::kWeights, p, stream);
 }
 
@@ -385,9 +384,9 @@ int backward_as(const AttnDev& p, cudaStream_t stream) {
   constexpr int kFloats = 4 * Shape<kDP>::kOperand + Shape<kDP>::kWeights;
   int st = B200TBE_OK;
   if (p.total_q > 0)
-    st = launch(dq_kernel<T, kDP>, tile_slots<Shape<kDP>::kT>(p.total_q, p.batch) * p.heads, kFloats, p, stream);
+    st = launch<dq_kernel<T, kDP>>(tile_slots<Shape<kDP>::kT>(p.total_q, p.batch) * p.heads, kFloats, p, stream);
   if (st == B200TBE_OK && p.total_k > 0)
-    st = launch(dkv_kernel<T, kDP>, tile_slots<Shape<kDP>::kT>(p.total_k, p.batch) * p.kv_heads, kFloats, p, stream);
+    st = launch<dkv_kernel<T, kDP>>(tile_slots<Shape<kDP>::kT>(p.total_k, p.batch) * p.kv_heads, kFloats, p, stream);
   return st;
 }
 

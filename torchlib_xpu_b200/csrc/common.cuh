@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "b200tbe.h"
 
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ < 1000)
@@ -20,6 +22,21 @@ constexpr unsigned kFullMask = 0xffffffffu;
 
 inline int launch_status() {
   return cudaGetLastError() == cudaSuccess ? B200TBE_OK : B200TBE_ERR_LAUNCH;
+}
+
+// Lets a kernel have this much dynamic shared memory, and its SM all of it (or fewer CTAs fit than its launch bounds
+// promise): once a device, since the two calls cost as much as a launch.
+template <auto kKernel>
+inline bool allow_shared_memory(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  if (device < 64 && (done.load() >> device & 1) != 0) return true;
+  if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+      cudaFuncSetAttribute(kKernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess)
+    return false;
+  if (device < 64) done.fetch_or(1ull << device);
+  return true;
 }
 
 inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }

@@ -921,17 +921,14 @@ bool answer_in_pieces(const AnswerDev& p, int elem_bytes) {
 template <int kDP, int kH>
 int launch_answer_fma(AnswerDev p, int64_t most, cudaStream_t stream) {
   using R = RingF<kDP, kH>;
-  const auto kernel = answer_fma_kernel<kDP, kH>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes) != cudaSuccess ||
-      cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess)
-    return B200TBE_ERR_LAUNCH;
+  if (!allow_shared_memory<answer_fma_kernel<kDP, kH>>(R::kBytes)) return B200TBE_ERR_LAUNCH;
   p.per = kH;
   p.chunks = (p.group + p.per - 1) / p.per;
   p.units = p.c.kv_heads * p.chunks;
   if (static_cast<int64_t>(p.units) * p.c.batch > 0x7fffffff) return B200TBE_ERR_TOO_LARGE;
   const int64_t tiles = static_cast<int64_t>(p.units) * p.c.batch * (most + kUnitCost);
   const int ctas = static_cast<int>(tiles < kNumSMs * R::kCtas ? tiles : kNumSMs * R::kCtas);
-  kernel<<<ctas, kAnswerThreads, R::kBytes, stream>>>(p);
+  answer_fma_kernel<kDP, kH><<<ctas, kAnswerThreads, R::kBytes, stream>>>(p);
   const int st = launch_status();
   return st != B200TBE_OK ? st : join<float>(p, ctas, stream);
 }
@@ -939,12 +936,9 @@ int launch_answer_fma(AnswerDev p, int64_t most, cudaStream_t stream) {
 template <typename T, bool kBf16, int kDP>
 int launch_answer_mma(const AnswerDev& p, int64_t tiles, cudaStream_t stream) {
   using R = Ring<kDP>;
-  const auto kernel = answer_mma_kernel<kBf16, kDP>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes) != cudaSuccess ||
-      cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess)
-    return B200TBE_ERR_LAUNCH;
+  if (!allow_shared_memory<answer_mma_kernel<kBf16, kDP>>(R::kBytes)) return B200TBE_ERR_LAUNCH;
   const int ctas = static_cast<int>(tiles < kNumSMs * R::kCtas ? tiles : kNumSMs * R::kCtas);
-  kernel<<<ctas, kAnswerThreads, R::kBytes, stream>>>(p);
+  answer_mma_kernel<kBf16, kDP><<<ctas, kAnswerThreads, R::kBytes, stream>>>(p);
   const int st = launch_status();
   return st != B200TBE_OK ? st : join<T>(p, ctas, stream);
 }
@@ -952,9 +946,14 @@ int launch_answer_mma(const AnswerDev& p, int64_t tiles, cudaStream_t stream) {
 template <typename T>
 int launch_answer(const AnswerDev& p, int ctas, cudaStream_t stream) {
   const int bytes = (kHeads * p.c.D + kTile * (p.c.D + 1)) * 4;
-  const auto kernel = p.c.D <= kAnswerThreads ? answer_simt_kernel<T, 1> : answer_simt_kernel<T, 2>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return B200TBE_ERR_LAUNCH;
-  kernel<<<ctas, kAnswerThreads, bytes, stream>>>(p);
+  constexpr int kMost = (kHeads * 256 + kTile * 257) * 4;   // at the largest head dimension
+  if (p.c.D <= kAnswerThreads) {
+    if (!allow_shared_memory<answer_simt_kernel<T, 1>>(kMost)) return B200TBE_ERR_LAUNCH;
+    answer_simt_kernel<T, 1><<<ctas, kAnswerThreads, bytes, stream>>>(p);
+  } else {
+    if (!allow_shared_memory<answer_simt_kernel<T, 2>>(kMost)) return B200TBE_ERR_LAUNCH;
+    answer_simt_kernel<T, 2><<<ctas, kAnswerThreads, bytes, stream>>>(p);
+  }
   const int st = launch_status();
   return st != B200TBE_OK ? st : join<T>(p, ctas, stream);
 }
