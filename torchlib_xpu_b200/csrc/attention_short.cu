@@ -427,11 +427,6 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
     const int chunks = rows_here ? max(0, min(2, (s.k - half * 64 + 31) / 32)) : 0;
     for (int g = 0; g < a.group; ++g, phase ^= 1) {
       const int head = s.head * a.group + g;
-      float lse2 = 0.f;
-      if (row < s.q) {
-        lse2 = a.lse[head * a.total_q + s.q0 + row] * kLog2e;
-        if (lse2 == -INFINITY) lse2 = INFINITY;
-      }
       if (warp == 0) {
         warp_wait(&full, phase, dead);
         if (s.k % 16 != 0 || s.q % 16 != 0) {
@@ -451,6 +446,11 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
       } else if (warp == 7 && g == 0) {
         n = finder.next();
         if (row == 127) jobs[(turn + 1) & 1] = n;
+      }
+      float lse2 = 0.f;   // under the products
+      if (row < s.q) {
+        lse2 = a.lse[head * a.total_q + s.q0 + row] * kLog2e;
+        if (lse2 == -INFINITY) lse2 = INFINITY;
       }
       warp_wait(&s_full, phase, dead);
       tc_fence_after();
@@ -554,25 +554,24 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
         }
         __syncwarp();
       }
-      if (rows_here) {
-        uint16_t* out = static_cast<uint16_t*>(a.dq) + (s.q0 + warp % 4 * 32) * a.dq_row + head * a.dq_head;
+      const bool last = g + 1 == a.group;
+      const int64_t stride = half == 0 ? a.dv_row : a.dk_row;
+      const float f = half == 0 ? 1.f : a.scale;
+      uint16_t* dq_out = static_cast<uint16_t*>(a.dq) + (s.q0 + warp % 4 * 32) * a.dq_row + head * a.dq_head;
+      uint16_t* dkv_out = static_cast<uint16_t*>(half == 0 ? a.dv : a.dk) + (s.k0 + warp % 4 * 32) * stride +
+                          s.head * (half == 0 ? a.dv_head : a.dk_head);
+      const uint32_t dkv_at = (half == 0 ? dv : dk) + lanes;
 #pragma unroll 1
-        for (int i = half * kDP / 2; i < (half + 1) * kDP / 2; i += 32) {
-          tmem_ld32(x, dq + lanes + i);
-          tmem_wait_ld();
-          store_columns<kBf16>(stage, x, a.scale, false, out, a.dq_row, s.q - warp % 4 * 32, i, a.D);
-        }
+      for (int i = half * kDP / 2; i < (half + 1) * kDP / 2 && rows_here; i += 32) {
+        tmem_ld32(x, dq + lanes + i);
+        tmem_wait_ld();
+        store_columns<kBf16>(stage, x, a.scale, false, dq_out, a.dq_row, s.q - warp % 4 * 32, i, a.D);
       }
-      if (g + 1 == a.group && keys_here) {
-        const int64_t stride = half == 0 ? a.dv_row : a.dk_row;
-        uint16_t* out = static_cast<uint16_t*>(half == 0 ? a.dv : a.dk) + (s.k0 + warp % 4 * 32) * stride +
-                        s.head * (half == 0 ? a.dv_head : a.dk_head);
 #pragma unroll 1
-        for (int i = 0; i < kDP; i += 32) {
-          tmem_ld32(x, (half == 0 ? dv : dk) + lanes + i);
-          tmem_wait_ld();
-          store_columns<kBf16>(stage, x, half == 0 ? 1.f : a.scale, false, out, stride, s.k - warp % 4 * 32, i, a.D);
-        }
+      for (int i = 0; i < kDP && last && keys_here; i += 32) {
+        tmem_ld32(x, dkv_at + i);
+        tmem_wait_ld();
+        store_columns<kBf16>(stage, x, f, false, dkv_out, stride, s.k - warp % 4 * 32, i, a.D);
       }
       fence_async_smem();
       tc_fence_before();
