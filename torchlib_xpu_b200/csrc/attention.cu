@@ -63,11 +63,12 @@ TileList list_at(char* at, const Scratch& s, int64_t total_q, int64_t total_k, i
 
 // Batches whose sequences are at most 128 long on average go through the short sequences' kernels first. There
 // the general kernels' CTAs, one or two an SM, would each spend most of a sequence's time waiting: 4096 sequences
-// of 0 to 128 positions, 4 heads of 64, forward 514 us without, and the table of measurements has what it is with.
+// of 0 to 128 positions, 4 heads of 64, take 514 us forward and 1509 backward without, 137 and 397 with.
 bool mostly_short(const AttnDev& d) {
   return d.batch > 0 && d.total_q <= static_cast<int64_t>(d.batch) * 128 && d.total_k <= static_cast<int64_t>(d.batch) * 128;
 }
-// Several waves of tiles of sequences of different lengths: sorted first, so that the longest are not the last.
+// Several waves of tiles of sequences of different lengths: sorted first (5 to 8 us), so that the longest are not the
+// last. 96 batches of up to 200 queries and 1500 keys, 6 heads of 80: 77 us unsorted, 60 with the sorting.
 bool listed_first(const AttnDev& d) {
   const bool by_rows = d.group % 2 != 0 && d.total_q > static_cast<int64_t>(d.batch) * 128;   // tiles of 256, which no list has
   return d.batch > 1 && !by_rows && (d.total_q / 128 + d.batch) * d.heads > 2 * kNumSMs;

@@ -8,6 +8,8 @@
 // row's keys in one tile the backward pass is one kernel of five products, not two of seven, and needs neither the
 // forward pass's output nor a kernel for delta: delta = rowsum(P dP), which equals rowsum(dO O).
 // What is longer is put on the list of tiles that the general kernels take afterwards.
+// 4096 sequences of 0 to 128 positions, 4 heads of 64, causal: forward 137 us (its bytes take 82 at the copy rate), backward
+// 397 us (143); the general kernels take 514 and 1509.
 #include "attention.cuh"
 #include "tcgen05.cuh"
 
