@@ -431,8 +431,8 @@ typedef struct {
   int32_t causal;
   float scale;
   int32_t* status;                  /* device word or NULL: B200TBE_DEV_WAIT_TIMEOUT */
-  void* scratch;                    /* of the forward pass, 16-byte aligned, or NULL: batches of short sequences
-                                       are slower without it */
+  void* scratch;                    /* of the forward pass, 16-byte aligned, or NULL: batches are slower
+                                       without it, beyond 128 queries and 128 keys in all */
   size_t scratch_bytes;             /* b200tbe_jagged_attention_scratch_bytes() */
 } b200tbe_attention_params;
 

@@ -100,8 +100,11 @@ extern "C" int b200tbe_jagged_attention(const b200tbe_attention_params* p, b200t
     const TileList* rest = nullptr;
     TileList list;
     int tc = B200TBE_ERR_UNSUPPORTED;
-    if (p->scratch != nullptr && mostly_short(d)) {
-      list = list_at(static_cast<char*>(p->scratch), backward_scratch(d.total_q, 0, d.batch, 0), d.total_q, 0, d.batch);
+    if ((p->scratch != nullptr || all_short(d)) && mostly_short(d)) {
+      if (p->scratch != nullptr)
+        list = list_at(static_cast<char*>(p->scratch), backward_scratch(d.total_q, 0, d.batch, 0), d.total_q, 0, d.batch);
+      else
+        list = TileList{};   // nothing goes on it
       if (!all_short(d) && cudaMemsetAsync(p->scratch, 0, 16, stream) != cudaSuccess) return B200TBE_ERR_LAUNCH;
       tc = attention_short_forward(d, list, p->dtype, p->status, stream);
       if (tc == B200TBE_OK && all_short(d)) return tc;

@@ -174,6 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t tmem_base;
   __shared__ int dead_word;
   const AttnDev& a = p.a;
+  if (p.plan.counts[0] <= 0) return;
   uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* gs = qs + L::kTileBytes;
   uint8_t* ks = gs + L::kTileBytes;
@@ -414,6 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int dead_word;
   __shared__ __align__(16) float stats[2][2][kRows];   // [stage][lse log2 e, delta][query]
   const AttnDev& a = p.a;
+  if (p.plan.counts[1] <= 0) return;
   uint8_t* ks = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* vs = ks + L::kTileBytes;
   uint8_t* qs = vs + L::kTileBytes;

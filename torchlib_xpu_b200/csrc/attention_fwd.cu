@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
   __shared__ uint32_t tmem_base;
   __shared__ int dead_word;
   const AttnDev& a = p.a;
+  if (p.listed && p.list.counts[0] <= 0) return;
   uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* ks = qs + kNQ * L::kTileBytes;
   uint8_t* vs = ks + kSt * L::kTileBytes;

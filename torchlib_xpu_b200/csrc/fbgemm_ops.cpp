@@ -502,7 +502,7 @@ std::tuple<Tensor, Tensor> jagged_attention_forward(const Tensor& q_, const Tens
   if (keep_lse) lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
   auto p = attention_params(q, k, v, q_offsets, k_offsets, causal, scale, out, lse);
   Tensor scratch;
-  if (p.dtype != B200TBE_FP32) {
+  if (p.dtype != B200TBE_FP32 && (p.total_q > 128 || p.total_k > 128)) {   // what is smaller needs none
     scratch = at::empty({static_cast<int64_t>(b200tbe_jagged_attention_scratch_bytes(p.total_q, p.batch))},
                         q.options().dtype(at::kByte));
     p.scratch = scratch.data_ptr(), p.scratch_bytes = static_cast<size_t>(scratch.numel());
