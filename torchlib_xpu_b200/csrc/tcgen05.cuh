@@ -313,6 +313,14 @@ __device__ __forceinline__ void store_columns(uint8_t* stage, const uint32_t (&o
     if (i * 8 < rows) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(from + i * 512);
 }
 
+template <bool kBf16>
+__device__ __forceinline__ float2 unpack2(uint32_t x) {
+  if constexpr (kBf16)
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  else
+    return half2_bits_to_float2(x);
+}
+
 // A tensor map over [rows][heads][D] of 16-bit elements, in boxes of 64 columns of one head x `box_rows` rows.
 // Columns past D and rows past the end read as zero. false: the driver refuses it.
 bool rows_map(CUtensorMap* map, bool bf16, const void* base, int64_t rows, int heads, int D, int64_t row_stride,
