@@ -156,11 +156,12 @@ __device__ __forceinline__ void report(const int* dead, int32_t* status) {
   }
 }
 
-// Where the queries see few keys, dS goes into the product in two parts: rounded, and what the rounding left. Such a row
-// of dQ also bears the error of its delta (from an O that was rounded) times the mean of its keys, which is large for few
-// keys and falls with their number; with the rounding of dS beside it, dQ of sequences of some hundred positions was off
-// by half as much again as its own last rounding (0.0025 against 0.0017 in bf16). In two parts for all tiles: train_long's
-// dQ 300 to 377 us.
+// Where the queries see few keys, dS goes into the products in two parts: rounded, and what the rounding left. Such a row
+// of dS also bears the error of its delta (from an O that was rounded), which dQ multiplies by the mean of its keys: large
+// for few keys, falling with their number. With the rounding of dS beside it, dQ of sequences of some hundred positions
+// was off by half as much again as its own last rounding (0.0025 against 0.0017 in bf16), and dK under a causal mask by
+// nearly as much (0.00031 against 0.00021 in fp16; now 0.00026), as its early queries see few keys. Long sequences' kernels (fp16,
+// causal, heads of 128): dQ 300 to 303 us, dK and dV 413 to 421; in two parts for all tiles dQ alone took 377.
 constexpr int kFewTiles = 2;
 __device__ __forceinline__ bool in_two_parts(int tiles) { return tiles <= kFewTiles; }
 
@@ -471,6 +472,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_base, dp_at = tmem + kRows, dv_at = dp_at + kRows, dk_at = dv_at + kDP;
   // the first tile of queries with one that sees a key of the item, and how many there are from it on, of one head
   auto from_of = [&](const Item& it) { return a.causal ? max(0, it.first - (it.len - it.other_len)) / kRows : 0; };
+  // whether the queries of an item's tile j see few keys
+  auto few_keys = [&](const Item& it, int from, int j, int per_head) {
+    const int sees = a.causal ? min(it.len, (from + j % per_head + 1) * kRows + it.len - it.other_len) : it.len;
+    return in_two_parts((sees + kRows - 1) / kRows);
+  };
   auto per_head_of = [&](const Item& it) { return max(0, (it.other_len + kRows - 1) / kRows - from_of(it)); };
 
   if (warp >= kIssue) {
@@ -596,7 +602,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!alive) break;
           tc_fence_after();
           if (elect_one()) {
-            mma_over_rows<16, 2>(dk_at, dp_at, smem_addr(qs) + stage_of(j), out_desc, steps, j > 0);
+            mma_over_rows<16, 2>(dk_at, dp_at + 16, smem_addr(qs) + stage_of(j), out_desc, steps, j > 0);
+            if (few_keys(it, from, j, per_head)) mma_over_rows<16, 2>(dk_at, dp_at, smem_addr(qs) + stage_of(j), out_desc, steps, true);
             mma_commit(&bars.q_empty[of & 1]);
             if (!more) mma_commit(&bars.done);
           }
@@ -679,10 +686,20 @@ __global__ void __launch_bounds__(kThreads, 1)
               y.x = e + 2 < low || e + 2 >= high ? 0.f : y.x;
               y.y = e + 3 < low || e + 3 >= high ? 0.f : y.y;
             }
+            s[e] = __float_as_uint(x.x), s[e + 1] = __float_as_uint(x.y);
+            s[e + 2] = __float_as_uint(y.x), s[e + 3] = __float_as_uint(y.y);
             w[e / 2] = pack2<kBf16>(x.x, x.y);
             w[e / 2 + 1] = pack2<kBf16>(y.x, y.y);
           }
-          tmem_st16(ds_at, w);
+          tmem_st16(ds_at + 16, w);
+          if (few_keys(it, from, j, per_head)) {   // and what the rounding left
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 r = unpack2<kBf16>(w[e / 2]);
+              w[e / 2] = pack2<kBf16>(__uint_as_float(s[e]) - r.x, __uint_as_float(s[e + 1]) - r.y);
+            }
+            tmem_st16(ds_at, w);
+          }
         }
         tmem_wait_st();
         tc_fence_before();
