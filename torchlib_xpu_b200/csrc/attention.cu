@@ -35,16 +35,17 @@ AttnDev device_params(const b200tbe_attention_params* p) {
 
 size_t rounded(size_t n) { return (n + 15) / 16 * 16; }
 
-// delta, then the list's tickets and counts, then the two lists
+// delta, then the list's tickets and counts, the norms (of gradients and of values), then the two lists
 struct Scratch {
-  size_t delta, words, q_tiles, k_tiles;
-  size_t total() const { return delta + words + q_tiles + k_tiles; }
+  size_t delta, words, norms, q_tiles, k_tiles;
+  size_t total() const { return delta + words + 2 * norms + q_tiles + k_tiles; }
 };
 
 Scratch backward_scratch(int64_t total_q, int64_t total_k, int64_t batch, int64_t heads) {
   Scratch s;
   s.delta = rounded(static_cast<size_t>(total_q) * heads * sizeof(float));
   s.words = 16;
+  s.norms = rounded((static_cast<size_t>(batch) + 2) * heads * sizeof(uint32_t));
   s.q_tiles = rounded(static_cast<size_t>(tile_slots<128>(total_q, batch)) * sizeof(int2));
   s.k_tiles = rounded(static_cast<size_t>(tile_slots<128>(total_k, batch)) * sizeof(int2));
   return s;
@@ -54,8 +55,10 @@ TileList list_at(char* at, const Scratch& s, int64_t total_q, int64_t total_k, i
   TileList list;
   list.tickets = reinterpret_cast<int32_t*>(at);
   list.counts = list.tickets + 2;
-  list.q_tiles = reinterpret_cast<int2*>(at + s.words);
-  list.k_tiles = reinterpret_cast<int2*>(at + s.words + s.q_tiles);
+  list.grad_norms = reinterpret_cast<uint32_t*>(at + s.words);
+  list.v_norms = reinterpret_cast<uint32_t*>(at + s.words + s.norms);
+  list.q_tiles = reinterpret_cast<int2*>(at + s.words + 2 * s.norms);
+  list.k_tiles = reinterpret_cast<int2*>(at + s.words + 2 * s.norms + s.q_tiles);
   list.q_room = static_cast<int32_t>(tile_slots<128>(total_q, batch));
   list.k_room = static_cast<int32_t>(tile_slots<128>(total_k, batch));
   return list;
@@ -145,14 +148,23 @@ extern "C" int b200tbe_jagged_attention_backward(const b200tbe_attention_backwar
   d.dk_row = p->grad_k_stride, d.dk_head = p->grad_k_head_stride, d.dv_row = p->grad_v_stride, d.dv_head = p->grad_v_head_stride;
   const TileList list = list_at(static_cast<char*>(p->scratch) + s.delta, s, f->total_q, f->total_k, f->batch);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  const bool fits = attention_backward_fits(d, f->dtype);
-  bool listed = false;   // by the short sequences' kernel
+  bool fits = attention_backward_fits(d, f->dtype);
+  const bool ranged = fits && f->dtype == B200TBE_FP16;   // the general kernels need the norms
+  const size_t cleared = s.words + (ranged ? 2 * s.norms : 0);
+  if (fits && !all_short(d) && (ranged || mostly_short(d)) && cudaMemsetAsync(list.tickets, 0, cleared, stream) != cudaSuccess)
+    return B200TBE_ERR_LAUNCH;
+  bool listed = false;
   if (fits && mostly_short(d)) {
-    if (!all_short(d) && cudaMemsetAsync(list.tickets, 0, 16, stream) != cudaSuccess) return B200TBE_ERR_LAUNCH;
     st = attention_short_backward(d, list, f->dtype, f->status, stream);
     if (st == B200TBE_OK && all_short(d)) return st;
     if (st != B200TBE_OK && st != B200TBE_ERR_UNSUPPORTED) return st;
     listed = st == B200TBE_OK;
+    fits = listed;   // the general kernels make the same tensor maps
+  }
+  if (ranged && fits && !listed) {
+    st = attention_list(d, list, stream);
+    if (st != B200TBE_OK) return st;
+    listed = true;
   }
   st = listed ? attention_delta_listed(d, list, f->dtype, stream) : attention_delta(d, list, f->dtype, stream);
   if (st != B200TBE_OK) return st;

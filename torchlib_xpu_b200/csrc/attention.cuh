@@ -38,6 +38,10 @@ struct TileList {
   int2* q_tiles;
   int2* k_tiles;
   int32_t q_room, k_room;
+  // of an fp16 backward pass, zero before: the largest |dO|^2 of a stretch's rows [batch + 2][heads], the largest |v|^2
+  // [batch + 2][kv_heads], as the bits of floats (which compare as they do)
+  uint32_t* grad_norms;
+  uint32_t* v_norms;
 };
 
 int attention_forward_simt(const AttnDev& p, int dtype, cudaStream_t stream);
@@ -51,6 +55,7 @@ int attention_short_forward(const AttnDev& p, const TileList& list, int dtype, i
 int attention_short_backward(const AttnDev& p, const TileList& list, int dtype, int32_t* status, cudaStream_t stream);
 // All tiles, the long sequences' first, as attention_delta() lists them. With k_room 0, of the queries alone.
 int attention_list(const AttnDev& p, const TileList& list, cudaStream_t stream);
+// delta of the listed tiles; in fp16 their norms too.
 int attention_delta_listed(const AttnDev& p, const TileList& list, int dtype, cudaStream_t stream);
 bool attention_backward_fits(const AttnDev& p, int dtype);
 int attention_backward_tc(const AttnDev& p, const TileList& plan, int dtype, int32_t* status, cudaStream_t stream);

@@ -9,8 +9,8 @@
 // twice (7 products instead of 5), and nothing is added in memory. Scores and dP come into tensor memory with a row for
 // each four threads; four warpgroups take a quarter of the columns each (two with half of them: dK and dV 455 instead of
 // 430 us). P and dS go back into tensor memory, each in its own columns' place, as the left operand of the next
-// product: rounded to the operands' type, since the tensor cores multiply 16-bit operands, and summed in fp32. (In fp16 a dS
-// past 65504 is infinite, as such a gradient would be.)
+// product: rounded to the operands' type, since the tensor cores multiply 16-bit operands, and summed in fp32. In fp16, dS is
+// taken in a unit of the sequence's own (unit_of(), below).
 // The CTAs take the tiles of a list, which an earlier kernel of the pass leaves, one after the other.
 //
 // What bounds them: of a tile's 128 x 128 the products take 2048 (dK, dV) and 1536 cycles (dQ) at 128 columns, those
@@ -56,7 +56,7 @@ struct DkvBarriers {
 
 // What a tile's CTA knows.
 struct Item {
-  int begin, other, first, len, other_len, head;
+  int begin, other, first, len, other_len, head, stretch;
 };
 
 // Tile and head `index` of the list of tiles of queries (kOf 0) or of keys (1).
@@ -77,7 +77,32 @@ __device__ __forceinline__ Item item_at(const BwdDev& p, int64_t index) {
   it.len = static_cast<int>(stretch_bound(mine, a.offset_bytes, a.batch, total, at.x + 1) - begin);
   it.first = at.y * kRows;
   it.head = static_cast<int>(index % heads);
+  it.stretch = at.x;
   return it;
+}
+
+// A power of two by which dS is multiplied before it is rounded, and its products divided afterwards. |dS| is at most
+// 2 max|dO| max|v| of the sequence (Cauchy and Schwarz for each dP; delta is a mean of them): output gradients of 10^4, which
+// loss scaling makes, take it past 65504 where dQ and dK fit fp16, and gradients of 10^-4 take most of it below fp16's normal range. In
+// this unit it stays at or under 2^15, and 2^-38 max|dO| max|v| is the most that its last bits are worth. A sequence's unit does not depend on
+// the rest of the batch, and results do not depend on the unit but for those last bits. bf16 has fp32's range and no unit.
+template <bool kBf16, int kOf>
+__device__ __forceinline__ float unit_of(const BwdDev& p, const Item& it) {
+  if constexpr (kBf16) {
+    return 1.f;
+  } else {
+    const AttnDev& a = p.a;
+    // what a key head's query heads add up to needs one unit; a query head's dQ has its own
+    const int kv = kOf == 0 ? it.head / a.group : it.head, heads = kOf == 0 ? 1 : a.group;
+    const uint32_t* norms = p.plan.grad_norms + static_cast<int64_t>(it.stretch) * a.heads + (kOf == 0 ? it.head : kv * a.group);
+    uint32_t largest = norms[0];
+    for (int h = 1; h < heads; ++h) largest = max(largest, norms[h]);
+    const float square =
+        __uint_as_float(largest) * __uint_as_float(p.plan.v_norms[static_cast<int64_t>(it.stretch) * a.kv_heads + kv]);
+    if (!(square > 0.f && square < INFINITY)) return 1.f;
+    const int x = static_cast<int>(__float_as_uint(square) >> 23) - 127;   // square < 2^(x + 1), its root at most 2^((x + 2) >> 1)
+    return __int_as_float((127 + 14 - ((x + 2) >> 1)) << 23);
+  }
 }
 
 // The next item nobody has taken, or -1; by a whole warp.
@@ -354,7 +379,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         delta = a.delta[it.head * a.total_q + it.begin + row];
         if (lse2 == -INFINITY) lse2 = INFINITY;
       }
-      const uint64_t minus_delta = pair(-delta, -delta);
+      const float unit = unit_of<kBf16, 0>(p, it);
+      const uint64_t unit2 = pair(unit, unit), minus_delta = pair(-delta * unit, -delta * unit);
       if (n > 0 && !brought) alive = bring();
       for (int j = 0; alive && j < n; ++j, ++tile) {
         alive = warp_wait(&bars.s_full, tile & 1, dead);
@@ -378,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool cut = __any_sync(kFullMask, left < 32);
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            float2 d = unpair(mul2(as_pair(&s[e]), add2(as_pair(&dp[e]), minus_delta)));
+            float2 d = unpair(mul2(as_pair(&s[e]), less_delta<kBf16>(as_pair(&dp[e]), unit2, minus_delta)));
             if (cut) {
               d.x = e < left ? d.x : 0.f;
               d.y = e + 1 < left ? d.y : 0.f;
@@ -412,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!alive) break;
       if (part < kDP / 32)
         store_rows<kBf16>(stage + warp * L::kStage, static_cast<uint16_t*>(a.dq) + (it.begin + static_cast<int64_t>(row - lane)) * a.dq_row + it.head * a.dq_head,
-                          a.dq_row, dq_at + lanes, part * 32, a.D, a.scale, n > 0, it.len - row + lane);
+                          a.dq_row, dq_at + lanes, part * 32, a.D, a.scale / unit, n > 0, it.len - row + lane);
     }
     tc_fence_before();
   }
@@ -435,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Queue queue;
   __shared__ uint32_t tmem_base;
   __shared__ int dead_word;
-  __shared__ __align__(16) float stats[2][2][kRows];   // [stage][lse log2 e, delta][query]
+  __shared__ __align__(16) float stats[2][2][kRows];   // [stage][lse log2 e, delta in the item's unit][query]
   const AttnDev& a = p.a;
   if (p.plan.counts[1] <= 0) return;
   uint8_t* ks = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -527,6 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (index < 0) break;
         const Item it = item_at<1>(p, index);
         const int from = from_of(it), per_head = per_head_of(it), n = per_head * a.group;
+        const float unit = unit_of<kBf16, 1>(p, it);
         for (int j = 0; j < n; ++j, ++tile) {
           const int st = tile & 1, i0 = (from + j % per_head) * kRows, head = it.head * a.group + j / per_head;
           alive = tile < 2 || warp_wait(&bars.stat_empty[st], (tile / 2 - 1) & 1, dead);
@@ -536,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int64_t at = head * a.total_q + it.other + i0 + e;
             const float lse2 = in ? a.lse[at] * kLog2e : INFINITY;
             stats[st][0][e] = lse2 == -INFINITY ? INFINITY : lse2;
-            stats[st][1][e] = in ? a.delta[at] : 0.f;
+            stats[st][1][e] = in ? a.delta[at] * unit : 0.f;
           }
           mbar_arrive(&bars.stat_full[st]);
         }
@@ -638,6 +665,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Item it = item_at<1>(p, index);
       const int from = from_of(it), per_head = per_head_of(it), n = per_head * a.group;
       const int key = it.first + local, shift = it.len - it.other_len;
+      const float unit = unit_of<kBf16, 1>(p, it);
+      const uint64_t unit2 = pair(unit, unit);
       for (int j = 0; j < n; ++j, ++tile) {
         const int st = tile & 1, i0 = (from + j % per_head) * kRows + part * 32;
         alive = warp_wait(&bars.stat_full[st], (tile / 2) & 1, dead) && warp_wait(&bars.s_full, tile & 1, dead);
@@ -678,8 +707,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
             const float4 d = *reinterpret_cast<const float4*>(&stats[st][1][part * 32 + e]);
-            float2 x = unpair(mul2(as_pair(&s[e]), add2(as_pair(&dp[e]), pair(-d.x, -d.y))));
-            float2 y = unpair(mul2(as_pair(&s[e + 2]), add2(as_pair(&dp[e + 2]), pair(-d.z, -d.w))));
+            float2 x = unpair(mul2(as_pair(&s[e]), less_delta<kBf16>(as_pair(&dp[e]), unit2, pair(-d.x, -d.y))));
+            float2 y = unpair(mul2(as_pair(&s[e + 2]), less_delta<kBf16>(as_pair(&dp[e + 2]), unit2, pair(-d.z, -d.w))));
             if (cut) {
               x.x = e < low || e >= high ? 0.f : x.x;
               x.y = e + 1 < low || e + 1 >= high ? 0.f : x.y;
@@ -718,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int i = 0; i < kDP; i += 32)
           store_rows<kBf16>(stage + (part / 2 * 4 + warp % 4) * L::kStage, out, stride, (first ? dv_at : dk_at) + lanes, i, a.D,
-                            first ? 1.f : a.scale, n > 0, it.len - key + lane);
+                            first ? 1.f : a.scale / unit, n > 0, it.len - key + lane);
       }
       tc_fence_before();
     }

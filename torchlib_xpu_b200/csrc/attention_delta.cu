@@ -99,8 +99,14 @@ __global__ void __launch_bounds__(kThreads) delta_kernel(const AttnDev p, const 
   if (in && threadIdx.x % kLanes == 0) p.delta[head * p.total_q + row] = s;
 }
 
-// The same for the rows of the listed tiles alone.
-template <typename T, int kElems, int kLanes>
+// Into the word goes the largest of the warp's numbers, none of which is below zero. Which of them comes last does not matter.
+__device__ __forceinline__ void keep_largest(uint32_t* word, float x) {
+  const uint32_t bits = __reduce_max_sync(kFullMask, __float_as_uint(x));
+  if (threadIdx.x % 32 == 0 && bits > __ldcg(word)) atomicMax(word, bits);
+}
+
+// The same for the rows of the listed tiles alone; with kNorms also the norms of their dO and of their values.
+template <typename T, int kElems, int kLanes, bool kNorms>
 __global__ void __launch_bounds__(kThreads) delta_listed_kernel(const AttnDev p, const TileList list) {
   struct __align__(sizeof(T) * kElems) Vec {
     T x[kElems];
@@ -111,21 +117,56 @@ __global__ void __launch_bounds__(kThreads) delta_listed_kernel(const AttnDev p,
     const int head = static_cast<int>(item % p.heads);
     const int64_t first = stretch_bound(p.q_offsets, p.offset_bytes, p.batch, p.total_q, tile.x) + tile.y * kRows;
     const int64_t end = stretch_bound(p.q_offsets, p.offset_bytes, p.batch, p.total_q, tile.x + 1);
+    float most = 0.f;
     for (int r = threadIdx.x / kLanes; r < kRows; r += kThreads / kLanes) {
       const int64_t row = first + r;
-      float s = 0.f;
+      float s = 0.f, norm = 0.f;
       if (row < end) {
         const T* g = static_cast<const T*>(p.grad) + row * p.g_row + head * p.g_head;
         const T* o = static_cast<const T*>(p.out) + row * p.o_row + head * p.o_head;
         for (int d = threadIdx.x % kLanes * kElems; d < p.D; d += kLanes * kElems) {
           const Vec x = *reinterpret_cast<const Vec*>(g + d), y = *reinterpret_cast<const Vec*>(o + d);
 #pragma unroll
-          for (int e = 0; e < kElems; ++e) s = fmaf(to_float<T>(x.x[e]), to_float<T>(y.x[e]), s);
+          for (int e = 0; e < kElems; ++e) {
+            s = fmaf(to_float<T>(x.x[e]), to_float<T>(y.x[e]), s);
+            if constexpr (kNorms) norm = fmaf(to_float<T>(x.x[e]), to_float<T>(x.x[e]), norm);
+          }
         }
       }
 #pragma unroll
-      for (int w = kLanes / 2; w > 0; w >>= 1) s += __shfl_xor_sync(kFullMask, s, w);
+      for (int w = kLanes / 2; w > 0; w >>= 1) {
+        s += __shfl_xor_sync(kFullMask, s, w);
+        if constexpr (kNorms) norm += __shfl_xor_sync(kFullMask, norm, w);
+      }
       if (row < end && threadIdx.x % kLanes == 0) p.delta[head * p.total_q + row] = s;
+      most = fmaxf(most, norm);
+    }
+    if constexpr (kNorms) keep_largest(list.grad_norms + static_cast<int64_t>(tile.x) * p.heads + head, most);
+  }
+  if constexpr (kNorms) {
+    const int64_t values = static_cast<int64_t>(min(list.counts[1], list.k_room)) * p.kv_heads;
+    for (int64_t item = blockIdx.x; item < values; item += gridDim.x) {
+      const int2 tile = list.k_tiles[item / p.kv_heads];
+      const int head = static_cast<int>(item % p.kv_heads);
+      const int64_t first = stretch_bound(p.k_offsets, p.offset_bytes, p.batch, p.total_k, tile.x) + tile.y * kRows;
+      const int64_t end = stretch_bound(p.k_offsets, p.offset_bytes, p.batch, p.total_k, tile.x + 1);
+      float most = 0.f;
+      for (int r = threadIdx.x / kLanes; r < kRows; r += kThreads / kLanes) {
+        const int64_t row = first + r;
+        float norm = 0.f;
+        if (row < end) {
+          const T* v = static_cast<const T*>(p.v) + row * p.v_row + head * p.v_head;
+          for (int d = threadIdx.x % kLanes * kElems; d < p.D; d += kLanes * kElems) {
+            const Vec x = *reinterpret_cast<const Vec*>(v + d);
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) norm = fmaf(to_float<T>(x.x[e]), to_float<T>(x.x[e]), norm);
+          }
+        }
+#pragma unroll
+        for (int w = kLanes / 2; w > 0; w >>= 1) norm += __shfl_xor_sync(kFullMask, norm, w);
+        most = fmaxf(most, norm);
+      }
+      keep_largest(list.v_norms + static_cast<int64_t>(tile.x) * p.kv_heads + head, most);
     }
   }
 }
@@ -162,9 +203,9 @@ int attention_delta_listed(const AttnDev& p, const TileList& list, int dtype, cu
   const int64_t most = static_cast<int64_t>(list.q_room) * p.heads;
   const unsigned blocks = static_cast<unsigned>(most < kNumSMs * 8 ? most : kNumSMs * 8);
   if (dtype == B200TBE_FP16)
-    delta_listed_kernel<__half, 8, 8><<<blocks, kThreads, 0, stream>>>(p, list);
+    delta_listed_kernel<__half, 8, 8, true><<<blocks, kThreads, 0, stream>>>(p, list);
   else
-    delta_listed_kernel<__nv_bfloat16, 8, 8><<<blocks, kThreads, 0, stream>>>(p, list);
+    delta_listed_kernel<__nv_bfloat16, 8, 8, false><<<blocks, kThreads, 0, stream>>>(p, list);
   return launch_status();
 }
 

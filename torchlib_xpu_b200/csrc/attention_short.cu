@@ -369,6 +369,7 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
   __shared__ uint32_t tmem_base;
   __shared__ int dead_word;
   __shared__ float halves[2][kRows];
+  __shared__ uint32_t tops[8];   // of the warps, the largest |dP|
   const AttnDev& a = p.a;
   uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* gs = qs + L::kTileBytes;
@@ -427,6 +428,7 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
     // a warp whose rows are all behind the last computes nothing
     const bool rows_here = warp % 4 * 32 < s.q, keys_here = warp % 4 * 32 < s.k;
     const int chunks = rows_here ? max(0, min(2, (s.k - half * 64 + 31) / 32)) : 0;
+    float unit = 1.f;
     for (int g = 0; g < a.group; ++g, phase ^= 1) {
       const int head = s.head * a.group + g;
       if (warp == 0) {
@@ -459,6 +461,7 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
       // ---- P, and the row's part of delta ----
       uint32_t w[2][32], x[32];
       uint64_t part = 0;
+      float top = 0.f;
       // a row of 64 keys is 128 bytes, its 16-byte pieces exchanged by the row's number, as the copies do it
       uint8_t* p_row = ps + half * kRows * 128 + row * 128;
       auto put = [&](int i) {
@@ -490,9 +493,17 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
           }
 #pragma unroll
           for (int e = 0; e < 32; e += 2) part = fma2(as_pair(&w[i][e]), as_pair(&x[e]), part);
+          if constexpr (!kBf16) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) top = max3(top, fabsf(__uint_as_float(x[e])), fabsf(__uint_as_float(x[e + 1])));
+          }
           put(i);   // v, whose place it is, has been read
         }
       halves[half][row] = unpair(part).x + unpair(part).y;
+      if constexpr (!kBf16) {
+        const uint32_t bits = __reduce_max_sync(kFullMask, __float_as_uint(top));
+        if (threadIdx.x % 32 == 0) tops[warp] = bits;
+      }
       fence_async_smem();
       tc_fence_before();
       __syncthreads();
@@ -505,8 +516,34 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
         __syncwarp();
       }
       // ---- dS ----
-      const float delta = halves[0][row] + halves[1][row];
-      const uint64_t minus_delta = pair(-delta, -delta);
+      // In fp16 dS, at most twice the largest |dP|, is multiplied by a power of two that keeps it under 2^15 (why: unit_of() of the
+      // general kernels). Heads that are summed share theirs: where a later one needs a smaller, the sums so far follow it.
+      if constexpr (!kBf16) {
+        uint32_t bits = tops[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) bits = max(bits, tops[i]);
+        const int x_of = static_cast<int>(bits >> 23);   // biased; 0 and 255: nothing there, or nothing finite
+        const float needs = x_of > 0 && x_of < 255 ? __int_as_float(min(127 + 60, 2 * 127 + 13 - x_of) << 23) : (x_of == 0 ? 0x1p60f : 1.f);
+        if (kAlone || g == 0) {
+          unit = needs;
+        } else if (needs < unit) {
+          const float follow = needs / unit;
+          unit = needs;
+          if (half == 1) {
+#pragma unroll 1
+            for (int i = 0; i < kDP; i += 32) {
+              tmem_ld32(x, dk + lanes + i);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * follow);
+              tmem_st32(dk + lanes + i, x);
+            }
+            tmem_wait_st();
+          }
+        }
+      }
+      const float delta = (halves[0][row] + halves[1][row]) * unit;
+      const uint64_t unit2 = pair(unit, unit), minus_delta = pair(-delta, -delta);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (i < chunks) {
@@ -519,7 +556,7 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
           }
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float2 y = unpair(mul2(as_pair(&w[i][e]), add2(as_pair(&x[e]), minus_delta)));
+            const float2 y = unpair(mul2(as_pair(&w[i][e]), less_delta<kBf16>(as_pair(&x[e]), unit2, minus_delta)));
             w[i][e] = __float_as_uint(y.x);
             w[i][e + 1] = __float_as_uint(y.y);
           }
@@ -558,7 +595,7 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
       }
       const bool last = g + 1 == a.group;
       const int64_t stride = half == 0 ? a.dv_row : a.dk_row;
-      const float f = half == 0 ? 1.f : a.scale;
+      const float f = half == 0 ? 1.f : a.scale / unit;
       uint16_t* dq_out = static_cast<uint16_t*>(a.dq) + (s.q0 + warp % 4 * 32) * a.dq_row + head * a.dq_head;
       uint16_t* dkv_out = static_cast<uint16_t*>(half == 0 ? a.dv : a.dk) + (s.k0 + warp % 4 * 32) * stride +
                           s.head * (half == 0 ? a.dv_head : a.dk_head);
@@ -567,7 +604,7 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
       for (int i = half * kDP / 2; i < (half + 1) * kDP / 2 && rows_here; i += 32) {
         tmem_ld32(x, dq + lanes + i);
         tmem_wait_ld();
-        store_columns<kBf16>(stage, x, a.scale, false, dq_out, a.dq_row, s.q - warp % 4 * 32, i, a.D);
+        store_columns<kBf16>(stage, x, a.scale / unit, false, dq_out, a.dq_row, s.q - warp % 4 * 32, i, a.D);
       }
 #pragma unroll 1
       for (int i = 0; i < kDP && last && keys_here; i += 32) {

@@ -239,6 +239,15 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// Of a backward pass: dP - delta, in fp16 in a unit, which minus_delta has already.
+template <bool kBf16>
+__device__ __forceinline__ uint64_t less_delta(uint64_t dp, uint64_t unit, uint64_t minus_delta) {
+  if constexpr (kBf16)
+    return add2(dp, minus_delta);
+  else
+    return fma2(dp, unit, minus_delta);
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
