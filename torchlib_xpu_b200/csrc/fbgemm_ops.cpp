@@ -421,6 +421,12 @@ Tensor jagged_2d_to_dense_autograd(const Tensor& values, const Tensor& offsets, 
 // Operators outside fbgemm's schema, named as b200tbe_pop_device_status is. q, k and v may be slices of one
 // projection: only the elements of a head have to lie side by side.
 
+// Dual tensors neither require gradients nor have a place for a tangent in a kernel's result, which torch would take for zero.
+void refuse_forward_mode(const char* name, at::ArrayRef<Tensor> inputs) {
+  for (const Tensor& t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name, " has no forward-mode derivative");
+}
+
 // t as the kernels read it: [rows, heads, D] with the last dimension dense.
 Tensor dense_heads(const Tensor& t) { return t.size(2) <= 1 || t.stride(2) == 1 ? t : t.contiguous(); }
 
@@ -542,6 +548,7 @@ class JaggedAttentionFunction : public torch::autograd::Function<JaggedAttention
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "b200tbe_jagged_attention is differentiable once: create_graph is not supported");
+    refuse_forward_mode("b200tbe_jagged_attention's backward pass", grads);
     at::AutoDispatchBelowADInplaceOrView below;
     const auto saved = ctx->get_saved_variables();
     const Tensor q = dense_heads(saved[0]), k = dense_heads(saved[1]), v = dense_heads(saved[2]);
@@ -570,6 +577,7 @@ class JaggedAttentionFunction : public torch::autograd::Function<JaggedAttention
 
 Tensor jagged_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets,
                                  const c10::optional<Tensor>& k_offsets, bool causal, c10::optional<double> scale) {
+  refuse_forward_mode("b200tbe_jagged_attention", {q, k, v});
   const Tensor& ko = key_offsets(q, k, q_offsets, k_offsets);
   if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad())) {
     at::AutoDispatchBelowADInplaceOrView guard;   // nothing to keep for a backward pass
