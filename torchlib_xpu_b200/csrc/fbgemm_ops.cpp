@@ -639,6 +639,30 @@ void paged_cache_append(const Tensor& k_, const Tensor& v_, const Tensor& offset
                "b200tbe_paged_cache_append");
 }
 
+// The write counts as one: a graph that saved a cache, or a view of it, raises in its backward pass instead of using what
+// came later. (Tensors of inference mode have no version.)
+void written(const Tensor& cache) {
+  if (!cache.is_inference()) torch::autograd::impl::bump_version(cache);
+}
+
+void paged_cache_append_versioned(const Tensor& k, const Tensor& v, const Tensor& offsets, Tensor k_cache, Tensor v_cache,
+                                  const Tensor& page_table, const Tensor& lengths) {
+  at::AutoDispatchBelowADInplaceOrView below;
+  paged_cache_append(k, v, offsets, k_cache, v_cache, page_table, lengths);
+  written(k_cache);
+  written(v_cache);
+}
+
+// Rows are stored as values, without the graph that they come from; a cache that is itself part of a graph is refused, since
+// its gradient would go to what was there before.
+void paged_cache_append_autograd(const Tensor& k, const Tensor& v, const Tensor& offsets, Tensor k_cache, Tensor v_cache,
+                                 const Tensor& page_table, const Tensor& lengths) {
+  refuse_forward_mode("b200tbe_paged_cache_append", {k, v, k_cache, v_cache});
+  TORCH_CHECK(!at::GradMode::is_enabled() || !(k_cache.requires_grad() || v_cache.requires_grad()),
+              "b200tbe_paged_cache_append writes values only: a cache that requires grad can be written under torch.no_grad()");
+  paged_cache_append_versioned(k, v, offsets, k_cache, v_cache, page_table, lengths);
+}
+
 Tensor paged_attention(const Tensor& q_, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
                        const Tensor& lengths, c10::optional<double> scale) {
   auto c = paged_cache(k_cache, v_cache, page_table, lengths);
@@ -1207,6 +1231,11 @@ TORCH_LIBRARY_IMPL(fbgemm, CUDA, m) {
   m.impl("b200tbe_paged_attention", TORCH_FN(paged_attention));
 }
 
+// Under inference mode a call passes the Autograd key by.
+TORCH_LIBRARY_IMPL(fbgemm, ADInplaceOrView, m) {
+  m.impl("b200tbe_paged_cache_append", TORCH_FN(paged_cache_append_versioned));
+}
+
 // The training lookups and the jagged ops carry their own autograd nodes, so they also sit on the
 // Autograd key (the jagged ops' CUDA registrations above are what those nodes call).
 TORCH_LIBRARY_IMPL(fbgemm, AutogradCUDA, m) {
@@ -1215,6 +1244,7 @@ TORCH_LIBRARY_IMPL(fbgemm, AutogradCUDA, m) {
   m.impl("jagged_dense_elementwise_add", TORCH_FN(jagged_dense_elementwise_add_autograd));
   m.impl("jagged_2d_to_dense", TORCH_FN(jagged_2d_to_dense_autograd));
   m.impl("b200tbe_jagged_attention", TORCH_FN(jagged_attention_autograd));
+  m.impl("b200tbe_paged_cache_append", TORCH_FN(paged_cache_append_autograd));
   m.impl("split_embedding_codegen_lookup_rowwise_adagrad_function",
          TORCH_FN(split_embedding_codegen_lookup_rowwise_adagrad_function));
   m.impl("split_embedding_codegen_lookup_sgd_function",
