@@ -1,4 +1,4 @@
-"""Writes to a paged cache count as writes."""
+"""Writes to a paged cache count as writes, and derivatives through it are refused."""
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -71,12 +71,37 @@ def test_rows_and_caches_that_require_gradients():
         assert trained[i]._version == 1
 
 
+def test_answers_have_no_gradient():
+    rows, offsets, caches, table, lengths, q = _arguments()
+    append(*rows, offsets, *caches, table, lengths)
+    plain = answer(q, *caches, table, lengths)
+    assert not plain.requires_grad
+    leaf = q.clone().requires_grad_()
+    got = answer(leaf, *caches, table, lengths)
+    assert torch.equal(got, plain)
+    with pytest.raises(RuntimeError, match="b200tbe_paged_attention has no gradient"):
+        got.sum().backward()
+    trained = caches[1].clone().requires_grad_()
+    got = answer(q, caches[0], trained, table, lengths)
+    with pytest.raises(RuntimeError, match="b200tbe_paged_attention has no gradient"):
+        got.sum().backward()
+    with torch.no_grad():
+        assert not answer(leaf, *caches, table, lengths).requires_grad
+
+
 def test_forward_mode_is_refused():
     rows, offsets, caches, table, lengths, q = _arguments()
     with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            answer(dual, *caches, table, lengths)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            answer(dual, *caches, table, lengths)
         for i in range(2):
             both = list(caches)
             both[i] = forward_ad.make_dual(caches[i], torch.ones_like(caches[i]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                answer(q, *both, table, lengths)
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 append(*rows, offsets, *both, table, lengths)
             moved = list(rows)

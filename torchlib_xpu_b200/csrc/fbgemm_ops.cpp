@@ -684,6 +684,29 @@ Tensor paged_attention(const Tensor& q_, const Tensor& k_cache, const Tensor& v_
   return out;
 }
 
+// A result that a graph goes through, which ends here: with an error, not with gradients that are left out.
+class PagedAttentionFunction : public torch::autograd::Function<PagedAttentionFunction> {
+ public:
+  static Variable forward(AutogradContext*, const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                          const Tensor& page_table, const Tensor& lengths, c10::optional<double> scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return paged_attention(q, k_cache, v_cache, page_table, lengths, scale);
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK_NOT_IMPLEMENTED(false, "b200tbe_paged_attention has no gradient; b200tbe_jagged_attention does");
+    return {};
+  }
+};
+
+Tensor paged_attention_autograd(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
+                                const Tensor& lengths, c10::optional<double> scale) {
+  refuse_forward_mode("b200tbe_paged_attention", {q, k_cache, v_cache});
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k_cache.requires_grad() || v_cache.requires_grad()))
+    return PagedAttentionFunction::apply(q, k_cache, v_cache, page_table, lengths, scale);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return paged_attention(q, k_cache, v_cache, page_table, lengths, scale);
+}
+
 // ---- permute_2D_sparse_data -----------------------------------------------------------------------
 // lengths is [T, B], indices (and weights) hold the T rows' ids one row after the other; row j of
 // the result is row permute[j] of the input (rows may repeat or be left out, so the result can be
@@ -1245,6 +1268,7 @@ TORCH_LIBRARY_IMPL(fbgemm, AutogradCUDA, m) {
   m.impl("jagged_2d_to_dense", TORCH_FN(jagged_2d_to_dense_autograd));
   m.impl("b200tbe_jagged_attention", TORCH_FN(jagged_attention_autograd));
   m.impl("b200tbe_paged_cache_append", TORCH_FN(paged_cache_append_autograd));
+  m.impl("b200tbe_paged_attention", TORCH_FN(paged_attention_autograd));
   m.impl("split_embedding_codegen_lookup_rowwise_adagrad_function",
          TORCH_FN(split_embedding_codegen_lookup_rowwise_adagrad_function));
   m.impl("split_embedding_codegen_lookup_sgd_function",
