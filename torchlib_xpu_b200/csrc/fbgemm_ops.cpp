@@ -207,13 +207,14 @@ TableRows table_rows_of(const Tensor& hash_size_cumsum) {
 
 // One int32 per device that the kernels OR B200TBE_DEV_* bits into (an index out of range, a row
 // shape a kernel cannot take). Nothing reads it on the hot path; fbgemm::b200tbe_pop_device_status
-// returns and clears it.
-Tensor device_status(const at::Device& device) {
+// returns and clears it. With make false, undefined where there is none yet.
+Tensor device_status(const at::Device& device, bool make = true) {
   static std::mutex mu;
   static std::unordered_map<int, Tensor> words;
   std::lock_guard<std::mutex> lock(mu);
   auto it = words.find(device.index());
   if (it != words.end()) return it->second;
+  if (!make) return Tensor();
   Tensor w = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(device));
   words.emplace(device.index(), w);
   return w;
@@ -444,21 +445,14 @@ void check_sequence_offsets(const Tensor& t, const char* name, const Tensor& lik
   TORCH_CHECK(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, name, " must be int64 or int32");
 }
 
-// The device's status word, unless this call is captured into a graph before the word exists: its memory
+// The device's status word, unless this call is captured into a graph before any operator made the word: its memory
 // would belong to the graph.
-int32_t* status_word_of(const at::Device& device, Tensor* keep) {
-  static std::mutex mu;
-  static std::unordered_map<int, bool> made;
-  std::lock_guard<std::mutex> lock(mu);
+int32_t* status_word_of(const at::Device& device) {
   cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
   TORCH_CHECK(cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream().stream(), &capturing) == cudaSuccess,
               "the stream's capture status could not be read");
-  if (!made[device.index()]) {
-    if (capturing != cudaStreamCaptureStatusNone) return nullptr;
-    made[device.index()] = true;
-  }
-  *keep = device_status(device);
-  return keep->data_ptr<int32_t>();
+  const Tensor word = device_status(device, capturing == cudaStreamCaptureStatusNone);   // the library keeps it
+  return word.defined() ? word.data_ptr<int32_t>() : nullptr;
 }
 
 b200tbe_attention_params attention_params(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_offsets,
@@ -478,8 +472,7 @@ b200tbe_attention_params attention_params(const Tensor& q, const Tensor& k, cons
   p.offset_bytes = static_cast<int32_t>(q_offsets.element_size());
   p.causal = causal;
   p.scale = static_cast<float>(scale);
-  Tensor word;   // kept by the library
-  p.status = status_word_of(q.device(), &word);
+  p.status = status_word_of(q.device());
   return p;
 }
 
@@ -631,8 +624,7 @@ void paged_cache_append(const Tensor& k_, const Tensor& v_, const Tensor& offset
   TORCH_CHECK(offsets.numel() == static_cast<int64_t>(c.batch) + 1, "offsets must have one entry more than the batch");
   c10::cuda::CUDAGuard guard(k_cache.device());
   const Tensor k = dense_heads(k_), v = dense_heads(v_);
-  Tensor status;
-  c.status = status_word_of(k_cache.device(), &status);
+  c.status = status_word_of(k_cache.device());
   check_status(b200tbe_paged_cache_append(&c, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
                                           offsets.data_ptr(), static_cast<int32_t>(offsets.element_size()), k.size(0),
                                           current_stream()),
@@ -675,8 +667,7 @@ Tensor paged_attention(const Tensor& q_, const Tensor& k_cache, const Tensor& v_
   Tensor out = at::empty(q.sizes(), q.options());
   Tensor scratch = at::empty({static_cast<int64_t>(b200tbe_paged_attention_scratch_bytes(c.head_dim))},
                              q.options().dtype(at::kByte));
-  Tensor status;
-  c.status = status_word_of(k_cache.device(), &status);
+  c.status = status_word_of(k_cache.device());
   check_status(b200tbe_paged_attention(&c, q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1),
                                        static_cast<int32_t>(q.size(1)), static_cast<float>(scale_or_default(scale, q)),
                                        scratch.data_ptr(), static_cast<size_t>(scratch.numel()), current_stream()),
