@@ -37,3 +37,23 @@ print("done")
 def test_a_first_call_under_capture(made):
     run = subprocess.run([sys.executable, "-c", PROGRAM % made], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "done" in run.stdout, run.stderr[-2000:]
+
+
+INFERENCE = """
+import torch, torchlib_xpu_b200
+torchlib_xpu_b200.load_torch_ops()
+ops = torch.ops.fbgemm
+with torch.inference_mode():
+    k = torch.zeros(4, 16, 2, 64, dtype=torch.float16, device="cuda")
+    q = torch.zeros(1, 2, 64, dtype=torch.float16, device="cuda")
+    table, lengths = torch.tensor([[1, 9]], dtype=torch.int32, device="cuda"), torch.tensor([20], device="cuda")
+    ops.b200tbe_paged_attention(q, k, k, table, lengths)   # makes the word
+assert ops.b200tbe_pop_device_status(q) == 1
+assert ops.b200tbe_pop_device_status(q) == 0
+print("done")
+"""
+
+
+def test_a_word_made_in_inference_mode_is_cleared_outside():
+    run = subprocess.run([sys.executable, "-c", INFERENCE], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "done" in run.stdout, run.stderr[-2000:]

@@ -16,6 +16,7 @@
 // value. There is no CPU implementation and no fallback: only the CUDA dispatch key is registered.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
@@ -215,6 +216,7 @@ Tensor device_status(const at::Device& device, bool make = true) {
   auto it = words.find(device.index());
   if (it != words.end()) return it->second;
   if (!make) return Tensor();
+  c10::InferenceMode normal(false);   // a tensor of inference mode could not be cleared outside of it
   Tensor w = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(device));
   words.emplace(device.index(), w);
   return w;
