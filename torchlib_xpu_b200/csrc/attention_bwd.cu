@@ -86,23 +86,29 @@ __device__ __forceinline__ Item item_at(const BwdDev& p, int64_t index) {
 // loss scaling makes, take it past 65504 where dQ and dK fit fp16, and gradients of 10^-4 take most of it below fp16's normal range. In
 // this unit it stays at or under 2^15, and 2^-38 max|dO| max|v| is the most that its last bits are worth. A sequence's unit does not depend on
 // the rest of the batch, and results do not depend on the unit but for those last bits. bf16 has fp32's range and no unit.
+// The squares of the two norms that bound the dS of an item, multiplied. What a key head's query heads add up to
+// needs one unit (here by a whole warp); a query head's dQ has its own.
 template <bool kBf16, int kOf>
-__device__ __forceinline__ float unit_of(const BwdDev& p, const Item& it) {
-  if constexpr (kBf16) {
-    return 1.f;
+__device__ __forceinline__ float norms_of(const BwdDev& p, const Item& it) {
+  if constexpr (kBf16) return 0.f;
+  const AttnDev& a = p.a;
+  const int kv = kOf == 0 ? it.head / a.group : it.head;
+  const uint32_t* norms = p.plan.grad_norms + static_cast<int64_t>(it.stretch) * a.heads;
+  uint32_t largest = 0;
+  if constexpr (kOf == 0) {
+    largest = norms[it.head];
   } else {
-    const AttnDev& a = p.a;
-    // what a key head's query heads add up to needs one unit; a query head's dQ has its own
-    const int kv = kOf == 0 ? it.head / a.group : it.head, heads = kOf == 0 ? 1 : a.group;
-    const uint32_t* norms = p.plan.grad_norms + static_cast<int64_t>(it.stretch) * a.heads + (kOf == 0 ? it.head : kv * a.group);
-    uint32_t largest = norms[0];
-    for (int h = 1; h < heads; ++h) largest = max(largest, norms[h]);
-    const float square =
-        __uint_as_float(largest) * __uint_as_float(p.plan.v_norms[static_cast<int64_t>(it.stretch) * a.kv_heads + kv]);
-    if (!(square > 0.f && square < INFINITY)) return 1.f;
-    const int x = static_cast<int>(__float_as_uint(square) >> 23) - 127;   // square < 2^(x + 1), its root at most 2^((x + 2) >> 1)
-    return __int_as_float((127 + 14 - ((x + 2) >> 1)) << 23);
+    for (int h = threadIdx.x % 32; h < a.group; h += 32) largest = max(largest, norms[kv * a.group + h]);
+    largest = __reduce_max_sync(kFullMask, largest);
   }
+  return __uint_as_float(largest) * __uint_as_float(p.plan.v_norms[static_cast<int64_t>(it.stretch) * a.kv_heads + kv]);
+}
+template <bool kBf16>
+__device__ __forceinline__ float unit_of(float squares) {
+  if constexpr (kBf16) return 1.f;
+  const int x = static_cast<int>(__float_as_uint(squares) >> 23) - 127;   // below 2^(x + 1), the root at most 2^((x + 2) >> 1)
+  const float unit = __int_as_float((127 + 14 - ((x + 2) >> 1)) << 23);
+  return squares > 0.f && squares < INFINITY ? unit : 1.f;
 }
 
 // The next item nobody has taken, or -1; by a whole warp.
@@ -373,13 +379,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Item it = item_at<0>(p, index);
       const int n = tiles_of(it), row = it.first + local, klen = it.other_len;
       const int limit = row >= it.len ? 0 : (a.causal ? min(klen, row + klen - it.len + 1) : klen);
+      const float squares = norms_of<kBf16, 0>(p, it);
       float lse2 = 0.f, delta = 0.f;
       if (row < it.len) {
         lse2 = a.lse[it.head * a.total_q + it.begin + row] * kLog2e;
         delta = a.delta[it.head * a.total_q + it.begin + row];
         if (lse2 == -INFINITY) lse2 = INFINITY;
       }
-      const float unit = unit_of<kBf16, 0>(p, it);
+      const float unit = unit_of<kBf16>(squares);
       const uint64_t unit2 = pair(unit, unit), minus_delta = pair(-delta * unit, -delta * unit);
       if (n > 0 && !brought) alive = bring();
       for (int j = 0; alive && j < n; ++j, ++tile) {
@@ -462,6 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t tmem_base;
   __shared__ int dead_word;
   __shared__ __align__(16) float stats[2][2][kRows];   // [stage][lse log2 e, delta in the item's unit][query]
+  __shared__ float units[2];                           // the unit again, for those who do not look for it themselves
   const AttnDev& a = p.a;
   if (p.plan.counts[1] <= 0) return;
   uint8_t* ks = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -553,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (index < 0) break;
         const Item it = item_at<1>(p, index);
         const int from = from_of(it), per_head = per_head_of(it), n = per_head * a.group;
-        const float unit = unit_of<kBf16, 1>(p, it);
+        const float unit = unit_of<kBf16>(norms_of<kBf16, 1>(p, it));
         for (int j = 0; j < n; ++j, ++tile) {
           const int st = tile & 1, i0 = (from + j % per_head) * kRows, head = it.head * a.group + j / per_head;
           alive = tile < 2 || warp_wait(&bars.stat_empty[st], (tile / 2 - 1) & 1, dead);
@@ -565,6 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             stats[st][0][e] = lse2 == -INFINITY ? INFINITY : lse2;
             stats[st][1][e] = in ? a.delta[at] * unit : 0.f;
           }
+          if (lane == 0) units[st] = unit;
           mbar_arrive(&bars.stat_full[st]);
         }
       }
@@ -665,8 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Item it = item_at<1>(p, index);
       const int from = from_of(it), per_head = per_head_of(it), n = per_head * a.group;
       const int key = it.first + local, shift = it.len - it.other_len;
-      const float unit = unit_of<kBf16, 1>(p, it);
-      const uint64_t unit2 = pair(unit, unit);
+      float unit = 1.f;
       for (int j = 0; j < n; ++j, ++tile) {
         const int st = tile & 1, i0 = (from + j % per_head) * kRows + part * 32;
         alive = warp_wait(&bars.stat_full[st], (tile / 2) & 1, dead) && warp_wait(&bars.s_full, tile & 1, dead);
@@ -704,6 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t dp[32];
           tmem_ld32(dp, ds_at);
           tmem_wait_ld();
+          const uint64_t unit2 = pair(units[st], units[st]);
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
             const float4 d = *reinterpret_cast<const float4*>(&stats[st][1][part * 32 + e]);
@@ -733,6 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&bars.ds_full);
+        if constexpr (!kBf16) unit = units[st];
         mbar_arrive(&bars.stat_empty[st]);
       }
       if (alive && n > 0) alive = warp_wait(&bars.done, items++ & 1, dead);

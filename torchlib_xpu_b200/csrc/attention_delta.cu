@@ -105,12 +105,16 @@ __device__ __forceinline__ void keep_largest(uint32_t* word, float x) {
   if (threadIdx.x % 32 == 0 && bits > __ldcg(word)) atomicMax(word, bits);
 }
 
-// The same for the rows of the listed tiles alone; with kNorms also the norms of their dO and of their values.
+// The same for the rows of the listed tiles alone, kLanes x kElems columns or fewer; with kNorms also the norms of their dO
+// and of their values.
 template <typename T, int kElems, int kLanes, bool kNorms>
 __global__ void __launch_bounds__(kThreads) delta_listed_kernel(const AttnDev p, const TileList list) {
   struct __align__(sizeof(T) * kElems) Vec {
     T x[kElems];
   };
+  constexpr int kEach = kThreads / kLanes, kAtOnce = 4;   // rows at once, a group of lanes' rows on their way
+  const int d = threadIdx.x % kLanes * kElems, r0 = threadIdx.x / kLanes;
+  const bool in = d < p.D;
   const int64_t all = static_cast<int64_t>(min(list.counts[0], list.q_room)) * p.heads;
   for (int64_t item = blockIdx.x; item < all; item += gridDim.x) {
     const int2 tile = list.q_tiles[item / p.heads];
@@ -118,28 +122,35 @@ __global__ void __launch_bounds__(kThreads) delta_listed_kernel(const AttnDev p,
     const int64_t first = stretch_bound(p.q_offsets, p.offset_bytes, p.batch, p.total_q, tile.x) + tile.y * kRows;
     const int64_t end = stretch_bound(p.q_offsets, p.offset_bytes, p.batch, p.total_q, tile.x + 1);
     float most = 0.f;
-    for (int r = threadIdx.x / kLanes; r < kRows; r += kThreads / kLanes) {
-      const int64_t row = first + r;
-      float s = 0.f, norm = 0.f;
-      if (row < end) {
-        const T* g = static_cast<const T*>(p.grad) + row * p.g_row + head * p.g_head;
-        const T* o = static_cast<const T*>(p.out) + row * p.o_row + head * p.o_head;
-        for (int d = threadIdx.x % kLanes * kElems; d < p.D; d += kLanes * kElems) {
-          const Vec x = *reinterpret_cast<const Vec*>(g + d), y = *reinterpret_cast<const Vec*>(o + d);
+#pragma unroll 1
+    for (int r = r0; r < kRows; r += kAtOnce * kEach) {
+      Vec x[kAtOnce], y[kAtOnce];
 #pragma unroll
-          for (int e = 0; e < kElems; ++e) {
-            s = fmaf(to_float<T>(x.x[e]), to_float<T>(y.x[e]), s);
-            if constexpr (kNorms) norm = fmaf(to_float<T>(x.x[e]), to_float<T>(x.x[e]), norm);
-          }
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int64_t row = first + r + u * kEach;
+        x[u] = y[u] = Vec{};
+        if (row < end && in) {
+          x[u] = *reinterpret_cast<const Vec*>(static_cast<const T*>(p.grad) + row * p.g_row + head * p.g_head + d);
+          y[u] = *reinterpret_cast<const Vec*>(static_cast<const T*>(p.out) + row * p.o_row + head * p.o_head + d);
         }
       }
 #pragma unroll
-      for (int w = kLanes / 2; w > 0; w >>= 1) {
-        s += __shfl_xor_sync(kFullMask, s, w);
-        if constexpr (kNorms) norm += __shfl_xor_sync(kFullMask, norm, w);
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int64_t row = first + r + u * kEach;
+        float s = 0.f, norm = 0.f;
+#pragma unroll
+        for (int e = 0; e < kElems; ++e) {
+          s = fmaf(to_float<T>(x[u].x[e]), to_float<T>(y[u].x[e]), s);
+          if constexpr (kNorms) norm = fmaf(to_float<T>(x[u].x[e]), to_float<T>(x[u].x[e]), norm);
+        }
+#pragma unroll
+        for (int w = kLanes / 2; w > 0; w >>= 1) {
+          s += __shfl_xor_sync(kFullMask, s, w);
+          if constexpr (kNorms) norm += __shfl_xor_sync(kFullMask, norm, w);
+        }
+        if (row < end && threadIdx.x % kLanes == 0) p.delta[head * p.total_q + row] = s;
+        most = fmaxf(most, norm);
       }
-      if (row < end && threadIdx.x % kLanes == 0) p.delta[head * p.total_q + row] = s;
-      most = fmaxf(most, norm);
     }
     if constexpr (kNorms) keep_largest(list.grad_norms + static_cast<int64_t>(tile.x) * p.heads + head, most);
   }
@@ -151,20 +162,24 @@ __global__ void __launch_bounds__(kThreads) delta_listed_kernel(const AttnDev p,
       const int64_t first = stretch_bound(p.k_offsets, p.offset_bytes, p.batch, p.total_k, tile.x) + tile.y * kRows;
       const int64_t end = stretch_bound(p.k_offsets, p.offset_bytes, p.batch, p.total_k, tile.x + 1);
       float most = 0.f;
-      for (int r = threadIdx.x / kLanes; r < kRows; r += kThreads / kLanes) {
-        const int64_t row = first + r;
-        float norm = 0.f;
-        if (row < end) {
-          const T* v = static_cast<const T*>(p.v) + row * p.v_row + head * p.v_head;
-          for (int d = threadIdx.x % kLanes * kElems; d < p.D; d += kLanes * kElems) {
-            const Vec x = *reinterpret_cast<const Vec*>(v + d);
+#pragma unroll 1
+      for (int r = r0; r < kRows; r += kAtOnce * kEach) {
+        Vec x[kAtOnce];
 #pragma unroll
-            for (int e = 0; e < kElems; ++e) norm = fmaf(to_float<T>(x.x[e]), to_float<T>(x.x[e]), norm);
-          }
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int64_t row = first + r + u * kEach;
+          x[u] = Vec{};
+          if (row < end && in) x[u] = *reinterpret_cast<const Vec*>(static_cast<const T*>(p.v) + row * p.v_row + head * p.v_head + d);
         }
 #pragma unroll
-        for (int w = kLanes / 2; w > 0; w >>= 1) norm += __shfl_xor_sync(kFullMask, norm, w);
-        most = fmaxf(most, norm);
+        for (int u = 0; u < kAtOnce; ++u) {
+          float norm = 0.f;
+#pragma unroll
+          for (int e = 0; e < kElems; ++e) norm = fmaf(to_float<T>(x[u].x[e]), to_float<T>(x[u].x[e]), norm);
+#pragma unroll
+          for (int w = kLanes / 2; w > 0; w >>= 1) norm += __shfl_xor_sync(kFullMask, norm, w);
+          most = fmaxf(most, norm);
+        }
       }
       keep_largest(list.v_norms + static_cast<int64_t>(tile.x) * p.kv_heads + head, most);
     }
@@ -202,10 +217,14 @@ int attention_delta_listed(const AttnDev& p, const TileList& list, int dtype, cu
   // 16-byte vectors: the tensor-core kernels that use the list have checked the strides
   const int64_t most = static_cast<int64_t>(list.q_room) * p.heads;
   const unsigned blocks = static_cast<unsigned>(most < kNumSMs * 8 ? most : kNumSMs * 8);
-  if (dtype == B200TBE_FP16)
+  if (dtype == B200TBE_FP16 && p.D <= 64)
     delta_listed_kernel<__half, 8, 8, true><<<blocks, kThreads, 0, stream>>>(p, list);
-  else
+  else if (dtype == B200TBE_FP16)
+    delta_listed_kernel<__half, 8, 16, true><<<blocks, kThreads, 0, stream>>>(p, list);
+  else if (p.D <= 64)
     delta_listed_kernel<__nv_bfloat16, 8, 8, false><<<blocks, kThreads, 0, stream>>>(p, list);
+  else
+    delta_listed_kernel<__nv_bfloat16, 8, 16, false><<<blocks, kThreads, 0, stream>>>(p, list);
   return launch_status();
 }
 
