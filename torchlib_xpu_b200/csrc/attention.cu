@@ -66,7 +66,13 @@ TileList list_at(char* at, const Scratch& s, int64_t total_q, int64_t total_k, i
 
 // Batches whose sequences are at most 128 long on average go through the short sequences' kernels first. There
 // the general kernels' CTAs, one or two an SM, would each spend most of a sequence's time waiting: 4096 sequences
-// of 0 to 128 positions, 4 heads of 64, take 514 us forward and 1509 backward without, 137 and 397 with.
+// of 0 to 128 positions, 4 heads of 64, bf16, causal, take 141 us forward and 418 backward with, 255 and 1351 without. The two
+// meet later the fewer query heads a key head has, and never far below 128 on average (forward + backward, with against without):
+//   sequences    positions   4 heads of 64           4 heads of 128          8 heads of 128 over 1 key head
+//   1024 (512)   0 to 256    136 + 544, 227 + 596    170 + 746, 249 + 845    167 + 571, 164 + 562 (half as many sequences)
+//   512          0 to 512    160 + 601, 206 + 585    175 + 802, 245 + 801    175 + 639, 165 + 553 (256)
+//   1024 (512)   128         60 + 141, 82 + 386      96 + 241, 103 + 608     85 + 194, 109 + 413
+//   2048 (1024)  0 to 128    79 + 223, 135 + 680     129 + 339, 166 + 951    126 + 295, 181 + 626
 bool mostly_short(const AttnDev& d) {
   return d.batch > 0 && d.total_q <= static_cast<int64_t>(d.batch) * 128 && d.total_k <= static_cast<int64_t>(d.batch) * 128;
 }

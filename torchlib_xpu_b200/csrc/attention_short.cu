@@ -3,13 +3,15 @@
 //
 // A batch of short sequences is bound by the chain of each of them (copy, product, softmax, product, store: some
 // microseconds) and by HBM, not by the tensor cores. So a CTA takes one sequence and head from beginning to end
-// without roles or pipelines, and small enough that several share an SM and hide one another's chain: the forward
-// pass takes 128 columns of tensor memory (P and O lie where the scores were), the backward pass 256. With all of a
+// without roles or pipelines, and as small as it goes, so that several share an SM and hide one another's chain. The forward
+// pass takes 128 columns of tensor memory for heads of up to 64 (P and O lie where the scores were; four CTAs an SM), 256 beyond
+// (two). The backward pass takes a key head with all its query heads, one after the other: 256 columns for one query head of up to 64
+// (two CTAs an SM), else 512 (one, with nothing beside it: still at least twice as fast as the general kernels up to 64 positions on average; figures in attention.cu). With all of a
 // row's keys in one tile the backward pass is one kernel of five products, not two of seven, and needs neither the
 // forward pass's output nor a kernel for delta: delta = rowsum(P dP), which equals rowsum(dO O).
 // What is longer is put on the list of tiles that the general kernels take afterwards.
 // 4096 sequences of 0 to 128 positions, 4 heads of 64, causal: forward 137 us (its bytes take 82 at the copy rate), backward
-// 397 us (143); the general kernels take 514 and 1509.
+// 397 us (143); the general kernels take 255 and 1351.
 #include "attention.cuh"
 #include "tcgen05.cuh"
 
