@@ -66,8 +66,10 @@ typedef enum { B200TBE_OPT_SGD = 0, B200TBE_OPT_ROWWISE_ADAGRAD = 1 } b200tbe_op
  * (in smaller batches such a bag only moves lookups of its table to other bags of the table). */
 #define B200TBE_DEV_OFFSETS_NOT_MONOTONE 2
 #define B200TBE_DEV_UNSUPPORTED_SHAPE 4 /* a table's row is not whole 16-byte vectors */
-#define B200TBE_DEV_WAIT_TIMEOUT 8      /* a bounded wait inside a kernel gave up: its results are not valid (no
-                                           kernel waits on anything but its own block's copies and products) */
+#define B200TBE_DEV_WAIT_TIMEOUT 8      /* a bounded wait inside a kernel gave up: its results are not valid. Such
+                                           waits are for the block's own copies and products; the others, for tensor
+                                           memory and for the launch before (one new token's joining kernel), end by
+                                           themselves */
 
 #define B200TBE_MAX_DESTS 16
 #define B200TBE_MAX_JAGGED_DIMS 4

@@ -179,14 +179,6 @@ __device__ __forceinline__ void exponentials(uint32_t (&x)[32], uint64_t c, uint
   for (int e = 0; e < 32; e += 4) exponentials4(x, e, c, m, m);
 }
 
-// After a wait gave up: report it, and let what is in flight land before its memory is given back.
-__device__ __forceinline__ void report(const int* dead, int32_t* status) {
-  if (*dead) {
-    if (threadIdx.x == 0 && status != nullptr) atomicOr(status, B200TBE_DEV_WAIT_TIMEOUT);
-    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-  }
-}
-
 // Where the queries see few keys, dS goes into the products in two parts: rounded, and what the rounding left. Such a row
 // of dS also bears the error of its delta (from an O that was rounded), which dQ multiplies by the mean of its keys: large
 // for few keys, falling with their number. With the rounding of dS beside it, dQ of sequences of some hundred positions

@@ -432,12 +432,8 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
     tc_fence_before();
   }
   __syncthreads();
-  if (dead_word) {
-    // a wait gave up: report it, and let what is in flight land before the memory is given back
-    if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, B200TBE_DEV_WAIT_TIMEOUT);
-    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-    __syncthreads();
-  }
+  report(&dead_word, p.status);
+  __syncthreads();
   tc_fence_after();
   if (warp == kNQ * 4) tmem_free(tmem, L::kColumns);
 }

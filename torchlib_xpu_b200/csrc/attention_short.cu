@@ -130,14 +130,6 @@ __device__ __forceinline__ void zero_tail(uint8_t* tile, int rows) {
 
 __device__ __forceinline__ uint32_t up16(int n) { return static_cast<uint32_t>(n + 15) & ~15u; }
 
-// A wait gave up: report it, and let what is in flight land before its memory is given back.
-__device__ __forceinline__ void report(const int* dead, int32_t* status) {
-  if (*dead) {
-    if (threadIdx.x == 0 && status != nullptr) atomicOr(status, B200TBE_DEV_WAIT_TIMEOUT);
-    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-  }
-}
-
 template <int kDP>
 struct Forward {
   static constexpr int kTileBytes = kRows * kDP * 2;

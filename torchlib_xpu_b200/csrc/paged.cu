@@ -187,7 +187,7 @@ __device__ __forceinline__ Start find_start(const AnswerDev& p, int64_t* end) {
                   static_cast<int32_t>(tiles), static_cast<int32_t>(ctas), first, all};
   }
   __syncthreads();
-  // the joining kernel may be set up meanwhile: it waits for this one's end
+  // the joining kernel may be set up meanwhile: it waits for this one's end (without a limit; nothing here waits for it)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Start s = found;
   if (at >= *end) s = Start{-1, 0, 0, static_cast<int32_t>(ctas), at, all};   // no piece

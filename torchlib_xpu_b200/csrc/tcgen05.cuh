@@ -1,5 +1,7 @@
 // The sm_100a instructions that the tensor-core attention kernels are made of: barriers, tensor copies, tensor
-// memory and its matrix instruction. Every wait is bounded.
+// memory and its matrix instruction. Every wait for a barrier is bounded. tmem_alloc() is not: it waits until CTAs on its SM,
+// of any kernel, have freed columns. It ends because a CTA allocates once, before it has anything that another could wait for,
+// and comes to tmem_free() whether its waits succeed or give up.
 #pragma once
 
 #include <cuda.h>
@@ -55,6 +57,15 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 // The same for a whole warp, which goes on together.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
   return __all_sync(kFullMask, mbar_wait(bar, parity, dead));
+}
+
+// At a kernel's end, by the whole CTA, between two barriers: if a wait gave up, report it, and let what is in flight land before
+// its memory is given back.
+__device__ __forceinline__ void report(const int* dead, int32_t* status) {
+  if (*dead) {
+    if (threadIdx.x == 0 && status != nullptr) atomicOr(status, B200TBE_DEV_WAIT_TIMEOUT);
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  }
 }
 
 // Registers of a warpgroup from here on; the block's shares must not exceed what it was launched with.
