@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kIssue) tmem_free(tmem, 512);
 }
 
-// Tensor memory: scores (transposed: a key a row; P takes their place), dP (dS takes its place), dV, dK. dV and
+// Tensor memory: scores (transposed: a key a row; P, lifted, takes their place), dP (dS takes its place), dV, dK. dV and
 // the next scores are computed under the arithmetic on dP, dK and the next dP under the exponentials.
 template <bool kBf16, int kDP>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -460,8 +460,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Queue queue;
   __shared__ uint32_t tmem_base;
   __shared__ int dead_word;
-  __shared__ __align__(16) float stats[2][2][kRows];   // [stage][lse log2 e, delta in the item's unit][query]
-  __shared__ float units[2];                           // the unit again, for those who do not look for it themselves
+  // [stage][lse log2 e less the lift of P, delta in the item's unit without the lift][query], and that unit
+  __shared__ __align__(16) float stats[2][2][kRows];
+  __shared__ float units[2];
+  constexpr float kDown = kBf16 ? 1.f : 0x1p-14f;      // 2^-kLift
   const AttnDev& a = p.a;
   if (p.plan.counts[1] <= 0) return;
   uint8_t* ks = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -553,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (index < 0) break;
         const Item it = item_at<1>(p, index);
         const int from = from_of(it), per_head = per_head_of(it), n = per_head * a.group;
-        const float unit = unit_of<kBf16>(norms_of<kBf16, 1>(p, it));
+        const float unit = unit_of<kBf16>(norms_of<kBf16, 1>(p, it)) * kDown;
         for (int j = 0; j < n; ++j, ++tile) {
           const int st = tile & 1, i0 = (from + j % per_head) * kRows, head = it.head * a.group + j / per_head;
           alive = tile < 2 || warp_wait(&bars.stat_empty[st], (tile / 2 - 1) & 1, dead);
@@ -562,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool in = i0 + e < it.other_len;
             const int64_t at = head * a.total_q + it.other + i0 + e;
             const float lse2 = in ? a.lse[at] * kLog2e : INFINITY;
-            stats[st][0][e] = lse2 == -INFINITY ? INFINITY : lse2;
+            stats[st][0][e] = lse2 == -INFINITY ? INFINITY : lse2 - kLift<kBf16>;
             stats[st][1][e] = in ? a.delta[at] * unit : 0.f;
           }
           if (lane == 0) units[st] = unit;
@@ -666,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Item it = item_at<1>(p, index);
       const int from = from_of(it), per_head = per_head_of(it), n = per_head * a.group;
       const int key = it.first + local, shift = it.len - it.other_len;
-      float unit = 1.f;
+      float unit = kDown;
       for (int j = 0; j < n; ++j, ++tile) {
         const int st = tile & 1, i0 = (from + j % per_head) * kRows + part * 32;
         alive = warp_wait(&bars.stat_full[st], (tile / 2) & 1, dead) && warp_wait(&bars.s_full, tile & 1, dead);
@@ -749,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int i = 0; i < kDP; i += 32)
           store_rows<kBf16>(stage + (part / 2 * 4 + warp % 4) * L::kStage, out, stride, (first ? dv_at : dk_at) + lanes, i, a.D,
-                            first ? 1.f : a.scale / unit, n > 0, it.len - key + lane);
+                            first ? kDown : a.scale * kDown / unit, n > 0, it.len - key + lane);
       }
       tc_fence_before();
     }

@@ -9,8 +9,8 @@
 // While one tile's softmax runs, the tensor cores work on the other's products.
 //
 // A row's maximum is not followed exactly: as long as it has not grown by more than 2^8 in P, the old one stays,
-// O needs no rescaling, and P, at most 256, keeps the same relative precision. Normalising with the same sum
-// makes the result independent of that choice. P is rounded to the operands' type, since the tensor cores multiply
+// O needs no rescaling, and P, at most 256, keeps the same relative precision. (fp16 P is lifted by another 2^6, which the
+// difference from the maximum takes along: kLift.) Normalising with the same sum makes the result independent of that choice. P is rounded to the operands' type, since the tensor cores multiply
 // 16-bit operands; it is summed, like everything, in fp32.
 //
 // What bounds it: for 128 queries and 128 keys of 128 columns the products take 1024 cycles, the exponentials 1024 at 16
@@ -299,6 +299,7 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
     const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
     const uint32_t s_at = tmem + lanes + s * kRows, o_at = tmem + lanes + kNQ * kRows + s * kDP;
     const float c = a.scale * 1.4426950408889634f;
+    constexpr float kLag = 8.f, kHere = kBf16 ? 0.f : kLift<kBf16> - kLag;   // the lift that the lag leaves
     bool alive = true;
     int scored = 0, summed = 0;   // tiles of the stream, and its items
     for (int turn = 0; alive; ++turn) {
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
       const int row = it.row0 + (pair_heads ? 0 : s * kRows) + (warp % 4) * 32 + lane;
       const int tiles = it.n[kNQ == 2 ? s : 0];
       const int limit = row >= it.qlen ? 0 : (a.causal ? min(it.klen, row + it.klen - it.qlen + 1) : it.klen);   // keys that the row sees
-      float top = -INFINITY, base = 0.f;   // the maximum in use, times c
+      float top = -INFINITY, base = 0.f;   // the maximum in use; times c, less the lift
       float sum = 0.f;
       for (int j = 0; j < tiles; ++j, ++scored) {
         alive = warp_wait(&bars.s_full[s], scored & 1, dead);
@@ -344,10 +345,10 @@ __global__ void __launch_bounds__(Layout<kDP, kNQ>::kThreads, Layout<kDP, kNQ>::
         auto follow = [&](float now) {
           if (j == 0) {
             top = now;
-            base = now == -INFINITY ? 0.f : now * c;
-          } else if (__any_sync(kFullMask, now * c > base + 8.f)) {
+            base = now == -INFINITY ? 0.f : now * c - kHere;
+          } else if (__any_sync(kFullMask, now * c > base + (kLag + kHere))) {
             top = fmaxf(top, now);
-            const float next = top == -INFINITY ? 0.f : top * c, keep = fast_exp2(base - next);
+            const float next = top == -INFINITY ? 0.f : top * c - kHere, keep = fast_exp2(base - next);
             base = next;
             sum *= keep;
             // the products up to the last tile are in O: they came before these scores

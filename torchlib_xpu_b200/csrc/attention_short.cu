@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(128, Forward<kDP>::kCtas)
       tmem_wait_ld();
       m = largest(x[0], 0, m);
       if (chunks > 1) m = largest(x[1], 1, m);
-      base = m == -INFINITY ? 0.f : m * c;
+      base = m == -INFINITY ? 0.f : m * c - kLift<kBf16>;
       weigh(x[0], 0);
       if (chunks > 1) weigh(x[1], 1);
       if (chunks > 2) {
@@ -394,6 +394,7 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
   const int d_steps = (a.D + 15) / 16;
   const uint64_t c2 = pair(a.scale * kLog2e, a.scale * kLog2e);
   uint8_t* stage = ps + L::kStage + warp * 2048;
+  constexpr float kDown = kBf16 ? 1.f : 0x1p-14f;   // 2^-kLift
 
   auto copy = [&](const Job& s, int g) {
     const int head = s.head * a.group + g;
@@ -467,7 +468,7 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
           *reinterpret_cast<uint4*>(p_row + (((i * 32 + e) / 8) ^ (row % 8)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
         }
       };
-      const uint64_t minus = pair(-lse2, -lse2);
+      const uint64_t minus = pair(kLift<kBf16> - lse2, kLift<kBf16> - lse2);   // w is P lifted
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (i < chunks) {
@@ -536,8 +537,9 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
           }
         }
       }
-      const float delta = (halves[0][row] + halves[1][row]) * unit;
-      const uint64_t unit2 = pair(unit, unit), minus_delta = pair(-delta, -delta);
+      const float here = unit * kDown;   // dS from the lifted P, and delta, which was summed with it
+      const float delta = (halves[0][row] + halves[1][row]) * kDown * here;
+      const uint64_t unit2 = pair(here, here), minus_delta = pair(-delta, -delta);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (i < chunks) {
@@ -589,7 +591,7 @@ __global__ void __launch_bounds__(256, Backward<kDP, kAlone>::kCtas)
       }
       const bool last = g + 1 == a.group;
       const int64_t stride = half == 0 ? a.dv_row : a.dk_row;
-      const float f = half == 0 ? 1.f : a.scale / unit;
+      const float f = half == 0 ? kDown : a.scale / unit;
       uint16_t* dq_out = static_cast<uint16_t*>(a.dq) + (s.q0 + warp % 4 * 32) * a.dq_row + head * a.dq_head;
       uint16_t* dkv_out = static_cast<uint16_t*>(half == 0 ? a.dv : a.dk) + (s.k0 + warp % 4 * 32) * stride +
                           s.head * (half == 0 ? a.dv_head : a.dk_head);

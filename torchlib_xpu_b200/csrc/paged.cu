@@ -370,6 +370,7 @@ template <bool kBf16, int kDP>
 __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_kernel(const AnswerDev p) {
   using R = Ring<kDP>;
   constexpr int kKC = R::kKC, kVC = R::kVC, kStages = R::kStages, kTiles = R::kTiles, kL = R::kLanes;
+  constexpr float kLag = 8.f, kHere = kBf16 ? 0.f : kLift<kBf16> - kLag;   // all sums of a call are lifted alike, until they are divided
   extern __shared__ uint4 ring[];
   __shared__ float stats[kAnswerThreads / 32][kHeads][2];
   __shared__ longlong2 places[kAnswerThreads / 32][32];   // where the positions' keys and values begin
@@ -482,7 +483,7 @@ __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_k
           x[j][i] = (in >> (j * 16 + g + i / 2 * 8) & 1) != 0 ? x[j][i] * p.scale_log2 : -INFINITY;
           most[i & 1] = fmaxf(most[i & 1], x[j][i]);
         }
-      if (__any_sync(kFullMask, most[0] > top[0] + 8.f || most[1] > top[1] + 8.f)) {
+      if (__any_sync(kFullMask, most[0] > top[0] + kLag || most[1] > top[1] + kLag)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float m = fmaxf(top[i], most[i]);
@@ -499,11 +500,12 @@ __global__ void __launch_bounds__(kAnswerThreads, Ring<kDP>::kCtas) answer_mma_k
         }
       }
       uint32_t w[kTiles][2];
+      const float base[2] = {top[0] == -INFINITY ? 0.f : top[0] - kHere, top[1] == -INFINITY ? 0.f : top[1] - kHere};
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[j][i] = fast_exp2(x[j][i] - (top[i & 1] == -INFINITY ? 0.f : top[i & 1]));
+          x[j][i] = fast_exp2(x[j][i] - base[i & 1]);
           sum[i & 1] += x[j][i];
         }
         w[j][0] = transpose8x8(pack2<kBf16>(x[j][0], x[j][1]));

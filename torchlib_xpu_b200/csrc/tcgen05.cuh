@@ -250,6 +250,12 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// Binary places by which weights of at most 1 are lifted before they are rounded to 16 bits. fp16 holds what is below 2^-14
+// with ever fewer bits, and many small weights may be what a result is made of; its upper half, unused otherwise, takes them down to
+// 2^-28 (and leaves a factor of four for a score's rounding). bf16 has fp32's range.
+template <bool kBf16>
+constexpr float kLift = kBf16 ? 0.f : 14.f;
+
 // Of a backward pass: dP - delta, in fp16 in a unit, which minus_delta has already.
 template <bool kBf16>
 __device__ __forceinline__ uint64_t less_delta(uint64_t dp, uint64_t unit, uint64_t minus_delta) {
