@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import torchlib_xpu_b200
+from tests.test_attention_gpu import CASES, CROSS
 from torchlib_xpu_b200 import _build
 
 WAIT_TIMEOUT = 8
@@ -56,4 +57,19 @@ def test_a_wait_that_nothing_ends(waits):
     want = torch.einsum("hij,jhd->ihd", want, q.double())
     # the weights and the result are rounded to bf16 (by 2^-8 each of at most max|v| < 8), all else is far smaller
     assert (out.double() - want).abs().max() < 2 * 2.0 ** -8 * 8
+    assert torch.ops.fbgemm.b200tbe_pop_device_status(q) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,q_lengths,k_lengths,heads,kv,D,causal",
+                         [(c[0], c[1], c[1], *c[2:]) for c in CASES] + [c[:7] for c in CROSS])
+def test_no_wait_of_the_attention_gives_up(dtype, q_lengths, k_lengths, heads, kv, D, causal):
+    torchlib_xpu_b200.load_torch_ops()
+    offsets = [torch.tensor([0] + n, device="cuda").cumsum(0) for n in (q_lengths, k_lengths)]
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v = (torch.randn(n, h, D, generator=gen, device="cuda").to(dtype).requires_grad_()
+               for n, h in ((sum(q_lengths), heads), (sum(k_lengths), kv), (sum(k_lengths), kv)))
+    torch.ops.fbgemm.b200tbe_pop_device_status(q)
+    out = torch.ops.fbgemm.b200tbe_jagged_attention(q, k, v, *offsets, causal)
+    torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
     assert torch.ops.fbgemm.b200tbe_pop_device_status(q) == 0
