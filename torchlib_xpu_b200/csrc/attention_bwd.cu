@@ -16,7 +16,7 @@
 // What bounds them: of a tile's 128 x 128 the products take 2048 (dK, dV) and 1536 cycles (dQ) at 128 columns, those
 // from shared memory longer, since its bandwidth feeds just one operand pair at that rate; the exponentials take 1024
 // more under some of them, and the handing over between the warps that multiply and those that weigh does the rest. 7
-// sequences of 301 to 4099 positions, 16 heads of 128 over 4 key heads, causal, fp16: dK and dV 425 us, dQ 300 us, the tensor
+// sequences of 301 to 4099 positions, 16 heads of 128 over 4 key heads, causal, fp16: dK and dV 415 us, dQ 309 us, the tensor
 // cores 48 and 50 % busy.
 #include "attention.cuh"
 #include "tcgen05.cuh"

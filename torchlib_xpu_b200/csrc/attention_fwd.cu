@@ -16,9 +16,9 @@
 // What bounds it: for 128 queries and 128 keys of 128 columns the products take 1024 cycles, the exponentials 1024 at 16
 // a clock and SM, and the two operands of the scores, from shared memory, its whole bandwidth. A query tile's chain
 // is 2540 cycles of softmax and 1520 of waiting for its own two products; the two tiles' chains overlap. Five prompts
-// of 611 to 8192 positions, 32 heads of 128 over 8 key heads, causal: 1044 us, 1042 TFLOP/s, the tensor cores 45 to 50 %
-// busy. Not better: weights handed over in two halves (1176 against 1138 us), a quarter of the exponentials by a
-// polynomial on the FMA pipe (1426).
+// of 611 to 8192 positions, 32 heads of 128 over 8 key heads, causal: 1165 us a pass in a loop, which the power cap slows
+// down (935 TFLOP/s; 1020 us in a short run), the tensor cores 45 to 50 % busy. Not better, as measured before the CTAs stayed (1138 us
+// then): weights handed over in two halves (1176 us), a quarter of the exponentials by a polynomial on the FMA pipe (1426).
 #include "attention.cuh"
 #include "tcgen05.cuh"
 
