@@ -108,3 +108,32 @@ def test_no_gradient_at_all():
         out = attention(parts[0], parts[1], zero, o, None, True)
         dq, dk = torch.autograd.grad(out, parts[:2], torch.ones_like(out))
         assert (dq == 0).all() and (dk == 0).all()
+
+
+@pytest.mark.parametrize("lengths", [[150, 64], [300, 200, 1000]])
+def test_a_replayed_graph_finds_its_units_again(lengths):
+    """One captured backward pass, replayed with output gradients of 10^4, of 10^-4 and of 10^4 again: nothing is left of
+    the pass before, and each is what an eager call gives."""
+    o = [0]
+    for n in lengths:
+        o.append(o[-1] + n)
+    dev = torch.tensor(o, device="cuda")
+    q, k, v = (_normal((o[-1], h, 64), s, 0.25) for h, s in ((4, 31), (2, 32), (2, 33)))
+    sizes = [_normal((o[-1], 4, 64), 34, x) for x in (1e4, 1e-4, 1e4)]
+
+    def run(g):
+        parts = [t.detach().requires_grad_() for t in (q, k, v)]
+        return torch.autograd.grad(attention(*parts, dev, None, True), parts, g)
+
+    want = [run(g) for g in sizes]
+    held = sizes[1].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(held)
+    for g, w in zip(sizes, want):
+        held.copy_(g)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(w, got))
+    assert all(torch.isfinite(t).all() for w in want for t in w)

@@ -81,11 +81,6 @@ __device__ __forceinline__ Item item_at(const BwdDev& p, int64_t index) {
   return it;
 }
 
-// A power of two by which dS is multiplied before it is rounded, and its products divided afterwards. |dS| is at most
-// 2 max|dO| max|v| of the sequence (Cauchy and Schwarz for each dP; delta is a mean of them): output gradients of 10^4, which
-// loss scaling makes, take it past 65504 where dQ and dK fit fp16, and gradients of 10^-4 take most of it below fp16's normal range. In
-// this unit it stays at or under 2^15, and 2^-38 max|dO| max|v| is the most that its last bits are worth. A sequence's unit does not depend on
-// the rest of the batch, and results do not depend on the unit but for those last bits. bf16 has fp32's range and no unit.
 // The squares of the two norms that bound the dS of an item, multiplied. What a key head's query heads add up to
 // needs one unit (here by a whole warp); a query head's dQ has its own.
 template <bool kBf16, int kOf>
@@ -103,6 +98,11 @@ __device__ __forceinline__ float norms_of(const BwdDev& p, const Item& it) {
   }
   return __uint_as_float(largest) * __uint_as_float(p.plan.v_norms[static_cast<int64_t>(it.stretch) * a.kv_heads + kv]);
 }
+// A power of two by which dS is multiplied before it is rounded, and its products divided afterwards. |dS| is at most
+// 2 max|dO| max|v| of the sequence (Cauchy and Schwarz for each dP; delta is a mean of them): output gradients of 10^4, which
+// loss scaling makes, take it past 65504 where dQ and dK fit fp16, and gradients of 10^-4 take most of it below fp16's normal range. In
+// this unit it stays at or under 2^15, and 2^-38 max|dO| max|v| is the most that its last bits are worth. A sequence's unit does not depend on
+// the rest of the batch, and results do not depend on the unit but for those last bits. bf16 has fp32's range and no unit.
 template <bool kBf16>
 __device__ __forceinline__ float unit_of(float squares) {
   if constexpr (kBf16) return 1.f;
